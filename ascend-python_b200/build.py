@@ -108,7 +108,7 @@ def build_plugin(force=False, verbose=False) -> Path:
         from codegen import gen_backend_stubs
     finally:
         sys.path.pop(0)
-    gen_backend_stubs.run(OPP / "config" / "op_plugin_functions.yaml", OPP)
+    gen_backend_stubs.run([OPP / "config" / "op_plugin_functions.yaml", OPP / "config" / "op_plugin_cache_functions.yaml"], OPP)
 
     BUILD.mkdir(exist_ok=True)
     LIB.mkdir(exist_ok=True)

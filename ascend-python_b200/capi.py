@@ -17,7 +17,7 @@ _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "lib" / "libqmm_b200.so"
 
 QMM_OK = 0
-DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_I32, DTYPE_NONE = 0, 1, 2, 3, -1
+DTYPE_BF16, DTYPE_F16, DTYPE_F32, DTYPE_I32, DTYPE_I64, DTYPE_NONE = 0, 1, 2, 3, 4, -1
 ALGO_AUTO, ALGO_TILE, ALGO_STREAMK, ALGO_SIMT, ALGO_PAIR, ALGO_SPLITK, ALGO_CLUSTER = 0, 1, 2, 3, 4, 5, 6
 UNIQUE_ID_BYTES = 128
 
@@ -35,6 +35,8 @@ EXPORTED_SYMBOLS = (
     "qmm_rms_norm", "qmm_rms_norm_dynamic_quant", "qmm_comm_stats", "qmm_int8_mma_peak", "qmm_noalloc_status",
     "qmm_mm_reduce_scatter_workspace_size", "qmm_mm_reduce_scatter", "qmm_all_gather_mm_workspace_size",
     "qmm_all_gather_mm", "qmm_quant_matmul_int8_workspace_size", "qmm_quant_matmul_int8",
+    "qmm_rotary_axes", "qmm_rotary_axes_cache", "qmm_paged_attention_workspace_size", "qmm_paged_attention",
+    "qmm_paged_prompt_attention_workspace_size", "qmm_paged_prompt_attention",
 )
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
@@ -46,6 +48,13 @@ _lib = None
 
 class QmmError(RuntimeError):
     pass
+
+
+class KvCache(ctypes.Structure):
+    """``qmm_kv_cache``: a paged key-value cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("key", "value")] + \
+        [(n, ctypes.c_int64) for n in ("pages", "page_size", "kv_heads", "dim", "key_stride_page", "key_stride_place",
+                                       "key_stride_head", "value_stride_page", "value_stride_place", "value_stride_head")]
 
 
 def _export_nccl_path() -> None:
@@ -155,6 +164,21 @@ def lib() -> ctypes.CDLL:
                                         c.c_int64, c.c_void_p, c.c_void_p, c.c_int, c.c_void_p, c.c_int, c.c_int64,
                                         c.c_int64, c.c_int64, c.c_int64, c.c_char_p, c.c_char_p, c.c_int64,
                                         c.c_void_p, c.c_size_t, c.c_void_p]
+        p, i64, i = c.c_void_p, c.c_int64, c.c_int
+        cache = c.POINTER(KvCache)
+        L.qmm_rotary_axes.argtypes = [p, i64, i64, p, i64, i64, i, i64, i64, i64, i64, p, i, i64, i64, p, i64, c.POINTER(i64), i64,
+                                      i, i, p, p, p]
+        L.qmm_rotary_axes_cache.argtypes = [p, i64, i64, p, i64, i64, p, i64, i64, i, i64, i64, p, i, i64, i64, p, i64,
+                                            c.POINTER(i64), i64, i, i, cache, p, i, i64, p, p]
+        L.qmm_paged_attention_workspace_size.argtypes = [i64] * 5 + [c.POINTER(c.c_size_t)]
+        L.qmm_paged_attention.argtypes = [p, i, i64, i64, i64, i64, cache, p, i64, i64, p, c.c_double, i64, i64, p, p, p,
+                                          c.c_size_t, p]
+        L.qmm_paged_prompt_attention_workspace_size.argtypes = [i64] * 6 + [c.POINTER(c.c_size_t)]
+        L.qmm_paged_prompt_attention.argtypes = [p, i, i64, i64, i64, i64, cache, p, i64, i64, p, p, i64, c.c_double, i64, i64, p,
+                                                 p, p, c.c_size_t, p]
+        for name in ("qmm_rotary_axes", "qmm_rotary_axes_cache", "qmm_paged_attention_workspace_size", "qmm_paged_attention",
+                     "qmm_paged_prompt_attention_workspace_size", "qmm_paged_prompt_attention"):
+            getattr(L, name).restype = c.c_int
         for name in ("qmm_dynamic_quant", "qmm_quant_matmul_workspace_size", "qmm_quant_matmul",
                      "qmm_weight_quant_batchmatmul", "qmm_comm_unique_id", "qmm_comm_init_rank",
                      "qmm_comm_register", "qmm_comm_info", "qmm_comm_destroy", "qmm_mm_all_reduce",
@@ -407,3 +431,61 @@ def quant_matmul_int8(x1, x2, scale, offset=None, pertoken_scale=None, bias=None
                                           _ptr(pertoken_scale), _ptr(bias), _ptr(out), max(N, 1), M, N, K, _ptr(ws),
                                           int(n.value), _stream()), "qmm_quant_matmul_int8")
     return out
+
+
+def kv_cache(key_cache, value_cache) -> KvCache:
+    """[pages, page size, heads, dim] keys and values, any strides with a dense last dimension."""
+    assert key_cache.shape == value_cache.shape and key_cache.stride(-1) == 1 and value_cache.stride(-1) == 1
+    return KvCache(key_cache.data_ptr(), value_cache.data_ptr(), *key_cache.shape, *key_cache.stride()[:3], *value_cache.stride()[:3])
+
+
+def _rotary_arguments(positions, inv_freq, sections, interleaved, cyclic):
+    positions = positions.reshape(-1, positions.shape[-1])
+    sections = list(sections) if sections else [inv_freq.numel()]
+    code = DTYPE_I64 if positions.dtype == torch.int64 else DTYPE_I32
+    return (_ptr(positions), code, *positions.stride(), _ptr(inv_freq), inv_freq.numel(),
+            (ctypes.c_int64 * len(sections))(*sections), len(sections), int(interleaved), int(cyclic))
+
+
+def rotary_axes(query, key, positions, inv_freq, sections=(), interleaved=False, cyclic=False):
+    """query [T, H, D], key [T, KV, D], positions [axes, T] or [T] -> both turned (see qmm_rotary_axes)."""
+    T, H, D = query.shape
+    q, k = torch.empty(query.shape, dtype=query.dtype, device=query.device), torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    with torch.cuda.device(query.device):
+        check(lib().qmm_rotary_axes(_ptr(query), *query.stride()[:2], _ptr(key), *key.stride()[:2], dtype_code(query.dtype), T, H,
+                                    key.shape[1], D, *_rotary_arguments(positions, inv_freq, sections, interleaved, cyclic), _ptr(q),
+                                    _ptr(k), _stream()), "qmm_rotary_axes")
+    return q, k
+
+
+def rotary_axes_cache(query, key, value, positions, inv_freq, key_cache, value_cache, slots, sections=(), interleaved=False,
+                      cyclic=False):
+    """rotary_axes whose keys go to their slots of the cache, with the values; returns the query turned."""
+    T, H, D = query.shape
+    q = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    with torch.cuda.device(query.device):
+        check(lib().qmm_rotary_axes_cache(
+            _ptr(query), *query.stride()[:2], _ptr(key), *key.stride()[:2], _ptr(value), *value.stride()[:2], dtype_code(query.dtype),
+            T, H, *_rotary_arguments(positions, inv_freq, sections, interleaved, cyclic), kv_cache(key_cache, value_cache), _ptr(slots),
+            DTYPE_I64 if slots.dtype == torch.int64 else DTYPE_I32, slots.stride(0), _ptr(q), _stream()), "qmm_rotary_axes_cache")
+    return q
+
+
+def paged_attention(query, key_cache, value_cache, block_table, seq_lens, query_start=None, scale_value=None, window=0, sinks=0):
+    """(out, lse); query_start None: one token a sequence (qmm_paged_attention), else qmm_paged_prompt_attention."""
+    T, H, D = query.shape
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    lse = torch.empty((T, H), dtype=torch.float32, device=query.device)
+    name = "qmm_paged_attention" if query_start is None else "qmm_paged_prompt_attention"
+    B, n = seq_lens.numel(), ctypes.c_size_t(0)
+    places = block_table.shape[1] * key_cache.shape[1]
+    sizes = (B,) if query_start is None else (T, B)
+    check(getattr(lib(), name + "_workspace_size")(*sizes, H, key_cache.shape[2], D, places, ctypes.byref(n)), name)
+    scratch = torch.empty(int(n.value), dtype=torch.uint8, device=query.device)
+    starts = () if query_start is None else (_ptr(query_start), B)
+    with torch.cuda.device(query.device):
+        check(getattr(lib(), name)(_ptr(query), dtype_code(query.dtype), T, H, *query.stride()[:2], kv_cache(key_cache, value_cache),
+                                   _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(seq_lens), *starts,
+                                   D ** -0.5 if scale_value is None else scale_value, window, sinks, _ptr(out), _ptr(lse),
+                                   _ptr(scratch), int(n.value), _stream()), name)
+    return out, lse

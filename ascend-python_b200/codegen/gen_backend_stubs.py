@@ -15,10 +15,11 @@ and — the step the reference leaves to its host framework — a
 in ``TorchLibrary.cpp`` so that ``torch.ops.npu.<name>`` resolves.
 
 The schema grammar handled is the subset these operators use:
-``Tensor``, ``Tensor?``, ``str``, ``int``, ``float``, ``bool``, ``ScalarType?``,
-keyword-only marker ``*``, defaults, and ``Tensor`` / tuple-of-``Tensor`` returns.
+``Tensor``, ``Tensor(a!)`` (written in place), ``Tensor?``, ``str``, ``int``, ``int[]``,
+``float``, ``float?``, ``bool``, ``ScalarType?``, keyword-only marker ``*``, defaults, and
+``Tensor`` / tuple-of-``Tensor`` returns.
 
-Usage: ``python -m codegen.gen_backend_stubs --source_yaml <yaml> --output_dir <dir>``
+Usage: ``python -m codegen.gen_backend_stubs --source_yaml <yaml> [<yaml> ...] --output_dir <dir>``
 """
 from __future__ import annotations
 
@@ -35,7 +36,9 @@ CPP_ARG_TYPES = {
     "Tensor?": "const c10::optional<at::Tensor> &",
     "str": "c10::string_view",
     "int": "int64_t",
+    "int[]": "at::IntArrayRef",
     "float": "double",
+    "float?": "c10::optional<double>",
     "bool": "bool",
     "ScalarType?": "c10::optional<at::ScalarType>",
     "ScalarType": "at::ScalarType",
@@ -57,6 +60,8 @@ class Argument:
             return "c10::nullopt"
         if d in ("True", "False"):
             return d.lower()
+        if d == "[]":
+            return "{}"
         if self.type == "str":
             return '"' + d.strip("'\"") + '"'
         return d
@@ -112,6 +117,7 @@ def parse_schema(func: str, impl_ns) -> OpSchema:
         if len(parts) != 2:
             raise ValueError(f"cannot parse argument '{raw}' in: {func}")
         typ, name = parts
+        typ = re.sub(r"^Tensor\([a-z]!\)$", "Tensor", typ)
         if typ not in CPP_ARG_TYPES:
             raise ValueError(f"unsupported argument type '{typ}' in: {func}")
         args.append(Argument(typ, name, default, kwarg_only))
@@ -212,7 +218,9 @@ def _write_if_changed(path: Path, text: str) -> None:
 
 
 def run(source_yaml, output_dir) -> List[OpSchema]:
-    ops = parse_native_yaml(source_yaml)
+    """``source_yaml``: one registry or a list of them."""
+    sources = source_yaml if isinstance(source_yaml, (list, tuple)) else [source_yaml]
+    ops = [op for source in sources for op in parse_native_yaml(source)]
     out = Path(output_dir)
     _write_if_changed(out / "OpApiInterface.h", gen_interface_header(ops, "op_api", "OP_PLUGIN_OPAPI_INTERFACE_H_"))
     _write_if_changed(out / "OpInterface.h", gen_interface_header(ops, "op_plugin", "OP_PLUGIN_OP_INTERFACE_H_"))
@@ -223,7 +231,7 @@ def run(source_yaml, output_dir) -> List[OpSchema]:
 
 def main() -> None:
     parser = argparse.ArgumentParser(description="Generate op_plugin dispatch stubs")
-    parser.add_argument("-s", "--source_yaml", required=True)
+    parser.add_argument("-s", "--source_yaml", required=True, nargs="+")
     parser.add_argument("-o", "--output_dir", required=True)
     opts = parser.parse_args()
     run(opts.source_yaml, opts.output_dir)

@@ -1,0 +1,175 @@
+// C entries of the attention over a paged key-value cache (npu_paged_attention, npu_paged_prompt_attention): argument checks
+// and the simplest kernel that is right, one warp a row.
+#include "paged_common.cuh"
+
+namespace qmm {
+namespace paged {
+
+namespace {
+
+// The sequence of a token and the token's place in it; false: the token belongs to no sequence.
+__device__ __forceinline__ bool find_token(const Problem &p, int64_t token, int *b, int *place) {
+    if (p.start == nullptr) {
+        *b = static_cast<int>(token);
+        *place = p.lens[token] <= 0 ? -1 : p.lens[token] - 1;
+        return true;
+    }
+    for (int i = 0; i < p.batch; ++i) {
+        const int64_t first = p.start[i], end = p.start[i + 1];
+        if (token >= first && token < end) {
+            *b = i;
+            const int64_t at = p.lens[i] - (end - token);
+            *place = at < 0 ? -1 : static_cast<int>(at);
+            return true;
+        }
+    }
+    return false;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(128) plain_kernel(const __grid_constant__ Problem p) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (row >= p.tokens * p.heads) return;
+    const int64_t token = row / p.heads;
+    const int head = static_cast<int>(row - token * p.heads);
+    int b = 0, place = 0;
+    if (find_token(p, token, &b, &place))
+        plain_row<T>(p, b, token, head, place);
+    else
+        empty_row<T>(p, token, head);
+}
+
+int launch_plain(const Problem &p, int dtype, cudaStream_t stream) {
+    const int64_t ctas = (p.tokens * p.heads + 3) / 4;
+    if (ctas > 0x7fffffff) return fail(QMM_ERR_UNSUPPORTED, "paged attention: too many tokens");
+    if (dtype == QMM_DTYPE_BF16)
+        plain_kernel<__nv_bfloat16><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(p);
+    else
+        plain_kernel<__half><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(p);
+    QMM_CUDA_OK(cudaGetLastError());
+    return QMM_OK;
+}
+
+}  // namespace
+
+int launch_decode(const Problem &p, int dtype, void *, size_t, cudaStream_t stream) { return launch_plain(p, dtype, stream); }
+int launch_prompt(const Problem &p, int dtype, void *, size_t, cudaStream_t stream) { return launch_plain(p, dtype, stream); }
+
+static bool vectors(const void *base, int64_t a, int64_t b, int64_t c) {
+    return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ((a | b | c) & 7) == 0;
+}
+
+// The arguments of both entries as a Problem.
+static int describe(Problem *p, const char *op, const void *query, int dtype, int64_t tokens, int64_t heads, int64_t stride_token,
+                    int64_t stride_head, const qmm_kv_cache *cache, const int32_t *block_table, int64_t table_stride,
+                    int64_t max_pages, const int32_t *seq_lens, int64_t batch, double scale, int64_t window, int64_t sinks,
+                    void *out, float *lse) {
+    const std::string name(op);
+    QMM_REQUIRE(dtype == QMM_DTYPE_BF16 || dtype == QMM_DTYPE_F16, name + ": the query must be bf16 or f16");
+    QMM_REQUIRE(cache != nullptr, name + ": no cache given");
+    QMM_REQUIRE(tokens >= 0 && heads >= 0 && batch >= 0 && max_pages >= 0 && cache->pages >= 0,
+                name + ": sizes must be non-negative");
+    QMM_REQUIRE(window >= 0 && sinks >= 0, name + ": window and sinks must be non-negative");
+    QMM_REQUIRE(window > 0 || sinks == 0, name + ": sinks have a meaning with a window only");
+    QMM_REQUIRE(cache->dim >= 8 && cache->dim <= 256 && cache->dim % 8 == 0,
+                name + ": the head dimension must be a multiple of 8 up to 256");
+    QMM_REQUIRE(cache->page_size >= 1 && cache->page_size <= 0x7fffffff, name + ": the page size must be positive");
+    QMM_REQUIRE(cache->kv_heads >= 1 && heads % cache->kv_heads == 0,
+                name + ": the query's heads must be a multiple of the cache's");
+    QMM_REQUIRE(tokens < 0x7fffffff && batch < 0x7fffffff && heads <= 65535 && max_pages <= 0x7fffffff && cache->pages <= 0x7fffffff,
+                name + ": sizes out of range");
+    QMM_REQUIRE(scale == scale && scale - scale == 0.0, name + ": scale_value must be finite");
+    QMM_REQUIRE(vectors(query, stride_token, stride_head, 0) &&
+                    vectors(cache->key, cache->key_stride_page, cache->key_stride_place, cache->key_stride_head) &&
+                    vectors(cache->value, cache->value_stride_page, cache->value_stride_place, cache->value_stride_head),
+                name + ": query and caches must begin at 16-byte boundaries, with strides of multiples of 8 elements");
+    p->q = query;
+    p->q_st = stride_token;
+    p->q_sh = stride_head;
+    p->k = cache->key;
+    p->v = cache->value;
+    p->k_sb = cache->key_stride_page;
+    p->k_st = cache->key_stride_place;
+    p->k_sh = cache->key_stride_head;
+    p->v_sb = cache->value_stride_page;
+    p->v_st = cache->value_stride_place;
+    p->v_sh = cache->value_stride_head;
+    p->table = block_table;
+    p->table_st = table_stride;
+    p->lens = seq_lens;
+    p->start = nullptr;
+    p->out = out;
+    p->lse = lse;
+    p->batch = static_cast<int>(batch);
+    p->heads = static_cast<int>(heads);
+    p->kv_heads = static_cast<int>(cache->kv_heads);
+    p->group = static_cast<int>(heads / cache->kv_heads);
+    p->dim = static_cast<int>(cache->dim);
+    p->page = static_cast<int>(cache->page_size);
+    p->page_shift = -1;
+    for (int s = 0; s < 31; ++s)
+        if (p->page == 1 << s) p->page_shift = s;
+    p->max_pages = static_cast<int>(max_pages);
+    p->window = static_cast<int>(window < 0x7fffffff ? window : 0x7fffffff);
+    p->sinks = static_cast<int>(sinks < 0x7fffffff ? sinks : 0x7fffffff);
+    p->tokens = tokens;
+    p->pages = cache->pages;
+    const int64_t capacity = cache->pages == 0 ? 0 : max_pages * cache->page_size;
+    p->capacity = static_cast<int>(capacity < 0x7fffffff ? capacity : 0x7fffffff);
+    p->scale = static_cast<float>(scale);
+    return QMM_OK;
+}
+
+}  // namespace paged
+}  // namespace qmm
+
+using qmm::fail;
+
+extern "C" {
+
+int qmm_paged_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_places,
+                                       size_t *bytes) {
+    QMM_REQUIRE(bytes != nullptr, "qmm_paged_attention_workspace_size: no result given");
+    QMM_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 1 && dim >= 0 && max_places >= 0,
+                "qmm_paged_attention_workspace_size: sizes must be non-negative");
+    *bytes = 0;
+    return QMM_OK;
+}
+
+int qmm_paged_attention(const void *query, int dtype, int64_t batch, int64_t heads, int64_t query_stride_token,
+                        int64_t query_stride_head, const qmm_kv_cache *cache, const int32_t *block_table, int64_t table_stride,
+                        int64_t max_pages, const int32_t *seq_lens, double scale_value, int64_t window, int64_t sinks, void *out,
+                        float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    qmm::paged::Problem p;
+    const int rc = qmm::paged::describe(&p, "qmm_paged_attention", query, dtype, batch, heads, query_stride_token,
+                                        query_stride_head, cache, block_table, table_stride, max_pages, seq_lens, batch,
+                                        scale_value, window, sinks, out, lse);
+    if (rc != QMM_OK) return rc;
+    if (batch == 0 || heads == 0) return QMM_OK;
+    return qmm::paged::launch_decode(p, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int qmm_paged_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                                              int64_t max_places, size_t *bytes) {
+    QMM_REQUIRE(bytes != nullptr, "qmm_paged_prompt_attention_workspace_size: no result given");
+    QMM_REQUIRE(tokens >= 0 && batch >= 0 && heads >= 0 && kv_heads >= 1 && dim >= 0 && max_places >= 0,
+                "qmm_paged_prompt_attention_workspace_size: sizes must be non-negative");
+    *bytes = 0;
+    return QMM_OK;
+}
+
+int qmm_paged_prompt_attention(const void *query, int dtype, int64_t tokens, int64_t heads, int64_t query_stride_token,
+                               int64_t query_stride_head, const qmm_kv_cache *cache, const int32_t *block_table,
+                               int64_t table_stride, int64_t max_pages, const int32_t *seq_lens, const int32_t *query_start,
+                               int64_t batch, double scale_value, int64_t window, int64_t sinks, void *out, float *lse,
+                               void *workspace, size_t workspace_bytes, void *stream) {
+    qmm::paged::Problem p;
+    const int rc = qmm::paged::describe(&p, "qmm_paged_prompt_attention", query, dtype, tokens, heads, query_stride_token,
+                                        query_stride_head, cache, block_table, table_stride, max_pages, seq_lens, batch,
+                                        scale_value, window, sinks, out, lse);
+    if (rc != QMM_OK) return rc;
+    p.start = query_start;
+    if (tokens == 0 || heads == 0) return QMM_OK;
+    return qmm::paged::launch_prompt(p, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+}

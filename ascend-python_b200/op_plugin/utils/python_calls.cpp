@@ -16,6 +16,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <vector>
+
 #include "op_plugin/utils/Export.h"
 
 namespace {
@@ -50,6 +52,35 @@ struct Arguments {
     {
         ok = ok && PyFloat_CheckExact(args[i]);
         return ok ? PyFloat_AS_DOUBLE(args[i]) : 0.0;
+    }
+    c10::optional<double> optional_number(int i)
+    {
+        if (!ok || args[i] == Py_None) return c10::nullopt;
+        return number(i);
+    }
+    std::vector<int64_t> integers(int i)
+    {
+        std::vector<int64_t> out;
+        ok = ok && (PyList_CheckExact(args[i]) || PyTuple_CheckExact(args[i]));
+        const Py_ssize_t n = ok ? PySequence_Fast_GET_SIZE(args[i]) : 0;
+        for (Py_ssize_t j = 0; j < n && ok; ++j) {
+            PyObject *item = PySequence_Fast_GET_ITEM(args[i], j);
+            ok = PyLong_CheckExact(item);
+            if (!ok) break;
+            int overflow = 0;
+            out.push_back(PyLong_AsLongLongAndOverflow(item, &overflow));
+            ok = overflow == 0;
+        }
+        return out;
+    }
+    c10::string_view text(int i)
+    {
+        ok = ok && PyUnicode_CheckExact(args[i]);
+        if (!ok) return "";
+        Py_ssize_t n = 0;
+        const char *s = PyUnicode_AsUTF8AndSize(args[i], &n);
+        if (s == nullptr) throw python_error();
+        return c10::string_view(s, static_cast<size_t>(n));
     }
     c10::optional<at::ScalarType> dtype(int i)
     {
@@ -156,6 +187,67 @@ PyObject *weight_quant_batchmatmul(PyObject *, PyObject *const *args, Py_ssize_t
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *rotary_axes(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<std::tuple<at::Tensor, at::Tensor>(const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                                   const at::Tensor &, at::IntArrayRef, c10::string_view,
+                                                                   c10::string_view)>("npu::npu_rotary_axes");
+    Arguments a(args, n, 7);
+    if (!a.ok) return not_here();
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &positions = a.tensor(2), &inv_freq = a.tensor(3);
+    const std::vector<int64_t> sections = a.integers(4);
+    const c10::string_view mode = a.text(5), order = a.text(6);
+    return a.ok ? call(op, q, k, positions, inv_freq, at::IntArrayRef(sections), mode, order) : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *rotary_axes_cache(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<at::Tensor(const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                           const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                           at::IntArrayRef, c10::string_view, c10::string_view)>("npu::npu_rotary_axes_cache");
+    Arguments a(args, n, 11);
+    if (!a.ok) return not_here();
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &positions = a.tensor(3), &inv_freq = a.tensor(4);
+    const at::Tensor &k_cache = a.tensor(5), &v_cache = a.tensor(6), &slots = a.tensor(7);
+    const std::vector<int64_t> sections = a.integers(8);
+    const c10::string_view mode = a.text(9), order = a.text(10);
+    return a.ok ? call(op, q, k, v, positions, inv_freq, k_cache, v_cache, slots, at::IntArrayRef(sections), mode, order) : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<std::tuple<at::Tensor, at::Tensor>(const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                                   const at::Tensor &, const at::Tensor &, c10::optional<double>,
+                                                                   int64_t, int64_t)>("npu::npu_paged_attention");
+    Arguments a(args, n, 8);
+    if (!a.ok) return not_here();
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &table = a.tensor(3), &lens = a.tensor(4);
+    const c10::optional<double> scale = a.optional_number(5);
+    const int64_t window = a.integer(6), sinks = a.integer(7);
+    return a.ok ? call(op, q, k, v, table, lens, scale, window, sinks) : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *paged_prompt_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<std::tuple<at::Tensor, at::Tensor>(const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                                   const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                                   c10::optional<double>, int64_t, int64_t)>("npu::npu_paged_prompt_attention");
+    Arguments a(args, n, 9);
+    if (!a.ok) return not_here();
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &table = a.tensor(3), &lens = a.tensor(4), &start = a.tensor(5);
+    const c10::optional<double> scale = a.optional_number(6);
+    const int64_t window = a.integer(7), sinks = a.integer(8);
+    return a.ok ? call(op, q, k, v, table, lens, start, scale, window, sinks) : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyMethodDef method(const char *name)
 {
@@ -167,6 +259,10 @@ PyMethodDef methods[] = {method<dynamic_quant>("dynamic_quant"),
                          method<rms_norm_dynamic_quant>("rms_norm_dynamic_quant"),
                          method<quant_matmul>("quant_matmul"),
                          method<weight_quant_batchmatmul>("weight_quant_batchmatmul"),
+                         method<rotary_axes>("rotary_axes"),
+                         method<rotary_axes_cache>("rotary_axes_cache"),
+                         method<paged_attention>("paged_attention"),
+                         method<paged_prompt_attention>("paged_prompt_attention"),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_op_plugin_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -88,6 +88,66 @@ def npu_weight_quant_batchmatmul(x, weight, antiquant_scale, antiquant_offset=No
                                              bias, antiquant_group_size)
 
 
+def npu_rotary_axes(query, key, positions, inv_freq, *, sections=(), rotary_mode="half", axis_order="blocked"):
+    """Rotary positions on one or several axes: (query, key) turned.
+
+    query [tokens, heads, dim], key [tokens, kv heads, dim]; positions [axes, tokens], or [tokens] for one axis; inv_freq fp32,
+    one frequency a pair; sections: frequencies of each axis (may be left out for one axis); rotary_mode "half" or
+    "interleave"; axis_order "blocked" or "cyclic".
+    """
+    if not _compiling():
+        out = _calls.rotary_axes(query, key, positions, inv_freq, sections, rotary_mode, axis_order)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_rotary_axes(query, key, positions, inv_freq, sections=sections, rotary_mode=rotary_mode, axis_order=axis_order)
+
+
+def npu_rotary_axes_cache(query, key, value, positions, inv_freq, key_cache, value_cache, slots, *, sections=(), rotary_mode="half",
+                          axis_order="blocked"):
+    """npu_rotary_axes whose keys go to the paged cache, with the values: the query turned.
+
+    key_cache, value_cache [pages, page size, kv heads, dim]; slots [tokens]: page * page size + place; a slot outside the cache
+    (-1: padding) writes nothing.
+    """
+    if not _compiling():
+        out = _calls.rotary_axes_cache(query, key, value, positions, inv_freq, key_cache, value_cache, slots, sections, rotary_mode,
+                                       axis_order)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_rotary_axes_cache(query, key, value, positions, inv_freq, key_cache, value_cache, slots, sections=sections,
+                                      rotary_mode=rotary_mode, axis_order=axis_order)
+
+
+def npu_paged_attention(query, key_cache, value_cache, block_table, seq_lens, *, scale_value=None, window=0, sinks=0):
+    """Attention of one new token a sequence over the paged cache: (out [batch, heads, dim], lse [batch, heads] fp32).
+
+    The token's own key and value are in the cache, at place seq_lens[b] - 1.  window > 0: it sees the last `window` places and
+    the first `sinks`.  scale_value: 1 / sqrt(dim) if left out.
+    """
+    if not _compiling():
+        out = _calls.paged_attention(query, key_cache, value_cache, block_table, seq_lens, scale_value, window, sinks)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_paged_attention(query, key_cache, value_cache, block_table, seq_lens, scale_value=scale_value, window=window,
+                                    sinks=sinks)
+
+
+def npu_paged_prompt_attention(query, key_cache, value_cache, block_table, seq_lens, query_start, *, scale_value=None, window=0,
+                               sinks=0):
+    """npu_paged_attention for the last tokens of each sequence: prompts, chunks of them, drafted tokens.
+
+    query [tokens, heads, dim]; sequence b has its rows query_start[b] ... query_start[b + 1] - 1, which end at place
+    seq_lens[b] - 1; each sees the places up to its own.
+    """
+    if not _compiling():
+        out = _calls.paged_prompt_attention(query, key_cache, value_cache, block_table, seq_lens, query_start, scale_value, window,
+                                            sinks)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_paged_prompt_attention(query, key_cache, value_cache, block_table, seq_lens, query_start,
+                                           scale_value=scale_value, window=window, sinks=sinks)
+
+
 def npu_mm_all_reduce_base(x1, x2, hcom, *, reduce_op="sum", bias=None, antiquant_scale=None, antiquant_offset=None,
                            x3=None, dequant_scale=None, pertoken_scale=None, antiquant_group_size=0, comm_turn=0):
     if comm_turn == 0 and x1.is_cuda:

@@ -49,6 +49,7 @@ enum {
     QMM_DTYPE_F16 = 1,
     QMM_DTYPE_F32 = 2,
     QMM_DTYPE_I32 = 3,
+    QMM_DTYPE_I64 = 4, /* positions and slots only */
     QMM_DTYPE_NONE = -1
 };
 
@@ -358,6 +359,88 @@ QMM_API int qmm_all_gather_mm(const void *x1, int dtype, int64_t ld_x1, const vo
                               int64_t ld_gather, int64_t M, int64_t N, int64_t K, const char *hcom,
                               int64_t gather_index, int64_t comm_turn, void *workspace, size_t workspace_bytes,
                               void *stream);
+
+/*
+ * A paged key-value cache: `pages` pages of `page_size` places, at each place kv_heads rows of `dim` elements for the keys and as
+ * many for the values.  Element (page, place, head, d) of the keys lies at key[page * key_stride_page + place *
+ * key_stride_place + head * key_stride_head + d]; strides are in elements and may put heads in front of places.
+ */
+typedef struct qmm_kv_cache {
+    const void *key;
+    const void *value;
+    int64_t pages, page_size, kv_heads, dim;
+    int64_t key_stride_page, key_stride_place, key_stride_head;
+    int64_t value_stride_page, value_stride_place, value_stride_head;
+} qmm_kv_cache;
+
+/*
+ * Rotary positions on several axes (torch op `npu_rotary_axes`; no counterpart in the reference).  The first 2 * pairs elements
+ * of every head are pairs, (i, i + pairs) or, `interleaved`, (2i, 2i + 1); pair i turns by the angle
+ *   positions[axis(i)][token] * inv_freq[i]
+ * made in 64 bits; the rotation is fp32, rounded once.  Elements behind the pairs are copied.  The sections (one for each axis)
+ * add up to `pairs`; axis(i): blocked, sections[0] pairs on axis 0, the next sections[1] on axis 1, ...; `cyclic`, a = i mod
+ * axes while i < axes * sections[a], else 0.
+ * query [tokens, heads, dim] and key [tokens, kv_heads, dim] of bf16, f16 or f32 with the given strides (innermost: 1), any
+ * alignment; positions int32 or int64, any sign; query_out, key_out: dense; dim <= 256, at most 8 axes.
+ */
+QMM_API int qmm_rotary_axes(const void *query, int64_t query_stride_token, int64_t query_stride_head, const void *key,
+                            int64_t key_stride_token, int64_t key_stride_head, int dtype, int64_t tokens, int64_t heads,
+                            int64_t kv_heads, int64_t dim, const void *positions, int position_dtype,
+                            int64_t position_stride_axis, int64_t position_stride_token, const float *inv_freq, int64_t pairs,
+                            const int64_t *sections, int64_t axes, int interleaved, int cyclic, void *query_out, void *key_out,
+                            void *stream);
+
+/*
+ * qmm_rotary_axes whose keys go to the cache instead of an output, together with the values (torch op `npu_rotary_axes_cache`).
+ * Token t is written to place slots[t] % page_size of page slots[t] / page_size; a slot outside [0, pages * page_size) writes
+ * nothing (padding; its query row is turned all the same).  Slots inside are to differ: of two tokens with the same slot either
+ * may remain, in part.  All other places of the cache keep what they held.
+ */
+QMM_API int qmm_rotary_axes_cache(const void *query, int64_t query_stride_token, int64_t query_stride_head, const void *key,
+                                  int64_t key_stride_token, int64_t key_stride_head, const void *value,
+                                  int64_t value_stride_token, int64_t value_stride_head, int dtype, int64_t tokens, int64_t heads,
+                                  const void *positions, int position_dtype, int64_t position_stride_axis,
+                                  int64_t position_stride_token, const float *inv_freq, int64_t pairs, const int64_t *sections,
+                                  int64_t axes, int interleaved, int cyclic, const qmm_kv_cache *cache, const void *slots,
+                                  int slot_dtype, int64_t slot_stride, void *query_out, void *stream);
+
+/*
+ * Attention of one new token a sequence over the paged cache (torch op `npu_paged_attention`; the reference reads dense caches
+ * only, test/test_custom_ops/test_incre_flash_attention.py).  The token of sequence
+ * b is at place p = seq_lens[b] - 1, its key and value are in the cache already; it sees the places j <= p with
+ *   j < max_pages * page_size,  0 <= block_table[b][j / page_size] < pages,  and  window == 0 or p - j < window or j < sinks.
+ *   out[b,h] = sum_j softmax_j(scale_value * query[b,h] . key[j, h / group]) * value[j, h / group],  group = heads / kv_heads
+ *   lse[b,h] = log(sum_j exp(scale_value * query[b,h] . key[j, h / group]))
+ * A row that sees nothing (seq_lens[b] <= 0: padding) has out 0 and lse -inf.  Entries of the table for places that are not
+ * seen are not followed, and the places not read.  Scores, softmax and sums are fp32.
+ * query: bf16 or f16 like the cache, [batch, heads, dim]; out: dense; lse: [batch, heads]; block_table: int32 [batch, max_pages],
+ * rows table_stride apart; dim: a multiple of 8 up to 256; query and caches begin at 16-byte boundaries, their strides are
+ * multiples of 8 elements.  The workspace (16-byte aligned, of the size that the first function gives for max_places =
+ * max_pages * page_size) holds nothing between calls; calls that may run at the same time need one each.
+ */
+QMM_API int qmm_paged_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_places,
+                                               size_t *bytes);
+QMM_API int qmm_paged_attention(const void *query, int dtype, int64_t batch, int64_t heads, int64_t query_stride_token,
+                                int64_t query_stride_head, const qmm_kv_cache *cache, const int32_t *block_table,
+                                int64_t table_stride, int64_t max_pages, const int32_t *seq_lens, double scale_value,
+                                int64_t window, int64_t sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                                void *stream);
+
+/*
+ * The same for the last tokens of each sequence (torch op `npu_paged_prompt_attention`; cf. the reference's dense
+ * form, test/test_custom_ops/test_prompt_flash_attention.py): whole prompts, later chunks of them, a few
+ * drafted tokens.  Sequence b has the tokens query_start[b] ... query_start[b + 1] - 1 of `query` ([tokens, heads, dim]), n of
+ * them; its i-th is at place p = seq_lens[b] - n + i and sees what qmm_paged_attention says.  query_start: int32 [batch + 1], not
+ * decreasing.  Tokens of no sequence have out 0 and lse -inf.
+ */
+QMM_API int qmm_paged_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
+                                                      int64_t max_places, size_t *bytes);
+QMM_API int qmm_paged_prompt_attention(const void *query, int dtype, int64_t tokens, int64_t heads, int64_t query_stride_token,
+                                       int64_t query_stride_head, const qmm_kv_cache *cache, const int32_t *block_table,
+                                       int64_t table_stride, int64_t max_pages, const int32_t *seq_lens,
+                                       const int32_t *query_start, int64_t batch, double scale_value, int64_t window,
+                                       int64_t sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
+                                       void *stream);
 
 #ifdef __cplusplus
 }
