@@ -52,7 +52,6 @@ int launch_plain(const Problem &p, int dtype, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_decode(const Problem &p, int dtype, void *, size_t, cudaStream_t stream) { return launch_plain(p, dtype, stream); }
 int launch_prompt(const Problem &p, int dtype, void *, size_t, cudaStream_t stream) { return launch_plain(p, dtype, stream); }
 
 static bool vectors(const void *base, int64_t a, int64_t b, int64_t c) {
@@ -132,7 +131,7 @@ int qmm_paged_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_
     QMM_REQUIRE(bytes != nullptr, "qmm_paged_attention_workspace_size: no result given");
     QMM_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 1 && dim >= 0 && max_places >= 0,
                 "qmm_paged_attention_workspace_size: sizes must be non-negative");
-    *bytes = 0;
+    *bytes = qmm::paged::decode_workspace(batch, heads, kv_heads, dim);
     return QMM_OK;
 }
 

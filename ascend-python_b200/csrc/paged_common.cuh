@@ -128,6 +128,7 @@ __device__ __forceinline__ void empty_row(const Problem &p, int64_t token, int h
     if (lane == 0) p.lse[token * p.heads + head] = -INFINITY;
 }
 
+size_t decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
 int launch_decode(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 

@@ -11,8 +11,8 @@
 // made in 64 bits, in half turns, reduced to [-1, 1] there, and only then rounded for sincospif (off by 2^-25 half turns).
 // The rotation is fp32 with one rounding to the tensors' type at the end.
 //
-// Every element is read and written once.  One CTA a token: n of its threads make the token's sines and cosines, which all heads
-// share, in shared memory.
+// Bound by HBM: every element is read and written once.  One CTA a token: its threads have their first loads under way while n
+// of them make the token's sines and cosines, which all heads share, in shared memory.
 #include "qmm_common.cuh"
 
 namespace qmm {
@@ -55,61 +55,189 @@ __device__ __forceinline__ int64_t load_index(const void *base, int64_t at, int 
     return wide ? __ldg(static_cast<const long long *>(base) + at) : __ldg(static_cast<const int *>(base) + at);
 }
 
+// The token's sines and cosines, made by the CTA's first threads.
+__device__ __forceinline__ void make_turns(const RotaryParams &p, int64_t token, float *s_cos, float *s_sin) {
+    for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
+        const int64_t place = load_index(p.positions, axis_of(p, i) * p.pos_sa + token * p.pos_st, p.wide_positions);
+        const double half_turns = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.31830988618379067154;
+        sincospif(static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns)), s_sin + i, s_cos + i);
+    }
+}
+
+// Where the token goes in the cache; false: nowhere.
+__device__ __forceinline__ bool find_slot(const RotaryParams &p, int64_t token, int64_t *block, int64_t *at) {
+    const int64_t slot = load_index(p.slots, token * p.slot_st, p.wide_slots);
+    if (slot < 0 || slot >= p.places) return false;
+    *block = slot / p.page;
+    *at = slot - *block * p.page;
+    return true;
+}
+
+// Row `row` of a token: first the query's heads, then the key's, then the value's.
+template <typename T>
+__device__ __forceinline__ void find_row(const RotaryParams &p, int64_t token, int row, int64_t block, int64_t at, const T **src, T **dst) {
+    if (row < p.heads) {
+        *src = static_cast<const T *>(p.q) + token * p.q_st + row * p.q_sh;
+        *dst = static_cast<T *>(p.q_out) + (token * p.heads + row) * p.dim;
+    } else if (row < p.heads + p.kv_heads) {
+        const int head = row - p.heads;
+        *src = static_cast<const T *>(p.k) + token * p.k_st + head * p.k_sh;
+        *dst = p.cached ? static_cast<T *>(p.k_cache) + block * p.kc_sb + at * p.kc_st + head * p.kc_sh
+                        : static_cast<T *>(p.k_out) + (token * p.kv_heads + head) * p.dim;
+    } else {
+        const int head = row - p.heads - p.kv_heads;
+        *src = static_cast<const T *>(p.v) + token * p.v_st + head * p.v_sh;
+        *dst = static_cast<T *>(p.v_cache) + block * p.vc_sb + at * p.vc_st + head * p.vc_sh;
+    }
+}
+
+__device__ __forceinline__ float turned_first(float a, float b, float c, float s) { return fmaf(a, c, -(b * s)); }
+__device__ __forceinline__ float turned_second(float a, float b, float c, float s) { return fmaf(b, c, a * s); }
+
+// An element a thread: any alignment.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
     __shared__ float s_cos[kMostPairs], s_sin[kMostPairs];
     pdl_launch_dependents();
     pdl_wait();
     const int64_t token = blockIdx.x;
-    for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
-        const int64_t place = load_index(p.positions, axis_of(p, i) * p.pos_sa + token * p.pos_st, p.wide_positions);
-        const double half_turns = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.31830988618379067154;
-        float s, c;
-        sincospif(static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns)), &s, &c);
-        s_sin[i] = s;
-        s_cos[i] = c;
-    }
+    make_turns(p, token, s_cos, s_sin);
     __syncthreads();
-    int64_t slot = 0, block = 0, at = 0;
-    bool write = true;
-    if (p.cached) {
-        slot = load_index(p.slots, token * p.slot_st, p.wide_slots);
-        write = slot >= 0 && slot < p.places;
-        block = write ? slot / p.page : 0;
-        at = write ? slot - block * p.page : 0;
-    }
-    const int total = (p.heads + p.kv_heads * (p.cached ? 2 : 1)) * p.dim;
-    for (int item = threadIdx.x; item < total; item += kThreads) {
+    int64_t block = 0, at = 0;
+    const bool write = !p.cached || find_slot(p, token, &block, &at);
+    const int rows = p.heads + (write ? p.kv_heads * (p.cached ? 2 : 1) : 0);
+    for (int item = threadIdx.x; item < rows * p.dim; item += kThreads) {
         const int row = item / p.dim, e = item - row * p.dim;
-        const int kind = row < p.heads ? 0 : row < p.heads + p.kv_heads ? 1 : 2;
-        const int head = kind == 0 ? row : kind == 1 ? row - p.heads : row - p.heads - p.kv_heads;
-        if (kind > 0 && !write) break;
-        const T *src = kind == 0   ? static_cast<const T *>(p.q) + token * p.q_st + head * p.q_sh
-                       : kind == 1 ? static_cast<const T *>(p.k) + token * p.k_st + head * p.k_sh
-                                   : static_cast<const T *>(p.v) + token * p.v_st + head * p.v_sh;
+        const T *src;
         T *dst;
-        if (kind == 0)
-            dst = static_cast<T *>(p.q_out) + (token * p.heads + head) * p.dim;
-        else if (!p.cached)
-            dst = static_cast<T *>(p.k_out) + (token * p.kv_heads + head) * p.dim;
-        else if (kind == 1)
-            dst = static_cast<T *>(p.k_cache) + block * p.kc_sb + at * p.kc_st + head * p.kc_sh;
-        else
-            dst = static_cast<T *>(p.v_cache) + block * p.vc_sb + at * p.vc_st + head * p.vc_sh;
-        if (kind == 2 || e >= 2 * p.pairs) {
+        find_row(p, token, row, block, at, &src, &dst);
+        if (row >= p.heads + p.kv_heads || e >= 2 * p.pairs) {
             dst[e] = src[e];
             continue;
         }
         const int i = p.interleaved ? e >> 1 : e < p.pairs ? e : e - p.pairs;
         const bool second = p.interleaved ? (e & 1) != 0 : e >= p.pairs;
         const float a = to_float(src[p.interleaved ? 2 * i : i]), b = to_float(src[p.interleaved ? 2 * i + 1 : i + p.pairs]);
-        dst[e] = from_float<T>(second ? fmaf(b, s_cos[i], a * s_sin[i]) : fmaf(a, s_cos[i], -(b * s_sin[i])));
+        dst[e] = from_float<T>(second ? turned_second(a, b, s_cos[i], s_sin[i]) : turned_first(a, b, s_cos[i], s_sin[i]));
     }
 }
 
 template <typename T>
+struct Vec {
+    static constexpr int kElems = 16 / sizeof(T);
+    static __device__ __forceinline__ void unpack(const uint4 &w, float (&f)[kElems]) {
+        const T *x = reinterpret_cast<const T *>(&w);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) f[i] = to_float(x[i]);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[kElems]) {
+        uint4 w;
+        T *x = reinterpret_cast<T *>(&w);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) x[i] = from_float<T>(f[i]);
+        return w;
+    }
+};
+
+// 16-byte vectors.  A thread has the same part of every row it comes to: with halves, the vector of the first elements of its
+// pairs and that of the second ones, or one vector behind the pairs; interleaved, one vector.  The first kAhead rows are under
+// way while the sines and cosines are made.
+constexpr int kAhead = 3;
+template <typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p, int shift) {
+    constexpr int E = Vec<T>::kElems;
+    __shared__ __align__(16) float s_cos[kMostPairs], s_sin[kMostPairs];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t token = blockIdx.x;
+    const int part = threadIdx.x & ((1 << shift) - 1);  // 1 << shift: a row's parts, rounded up
+    const int turning = INTERLEAVED ? 2 * p.pairs / E : p.pairs / E;
+    const int parts = INTERLEAVED ? p.dim / E : turning + (p.dim - 2 * p.pairs) / E;
+    const bool turns = part < turning;
+    const int e0 = (INTERLEAVED || turns ? part : part + turning) * E;  // first vector
+    const int e1 = e0 + p.pairs;                                        // second one
+    const bool two = !INTERLEAVED && turns;
+    int64_t block = 0, at = 0;
+    const bool write = !p.cached || find_slot(p, token, &block, &at);
+    const int rows = part < parts ? p.heads + (write ? p.kv_heads * (p.cached ? 2 : 1) : 0) : 0;
+    const int stride = kThreads >> shift;
+    bool made = false;
+    for (int row0 = threadIdx.x >> shift; !made || row0 < rows; row0 += kAhead * stride) {
+        uint4 x[kAhead], y[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int row = row0 + i * stride;
+            if (row >= rows) break;
+            const T *src;
+            T *dst;
+            find_row(p, token, row, block, at, &src, &dst);
+            x[i] = __ldg(reinterpret_cast<const uint4 *>(src + e0));
+            if (two) y[i] = __ldg(reinterpret_cast<const uint4 *>(src + e1));
+        }
+        if (!made) {
+            make_turns(p, token, s_cos, s_sin);
+            __syncthreads();
+            made = true;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int row = row0 + i * stride;
+            if (row >= rows) break;
+            const T *src;
+            T *dst;
+            find_row(p, token, row, block, at, &src, &dst);
+            if (turns && row < p.heads + p.kv_heads) {
+                float a[E], b[E];
+                Vec<T>::unpack(x[i], a);
+                if (INTERLEAVED) {
+#pragma unroll
+                    for (int j = 0; j < E; j += 2) {
+                        const float c = s_cos[(e0 + j) >> 1], s = s_sin[(e0 + j) >> 1];
+                        b[j] = turned_first(a[j], a[j + 1], c, s);
+                        b[j + 1] = turned_second(a[j], a[j + 1], c, s);
+                    }
+                    x[i] = Vec<T>::pack(b);
+                } else {
+                    Vec<T>::unpack(y[i], b);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) {
+                        const float c = s_cos[e0 + j], s = s_sin[e0 + j], first = a[j];
+                        a[j] = turned_first(first, b[j], c, s);
+                        b[j] = turned_second(first, b[j], c, s);
+                    }
+                    x[i] = Vec<T>::pack(a);
+                    y[i] = Vec<T>::pack(b);
+                }
+            }
+            *reinterpret_cast<uint4 *>(dst + e0) = x[i];
+            if (two) *reinterpret_cast<uint4 *>(dst + e1) = y[i];
+        }
+    }
+}
+
+// Whether rows `stride` elements apart begin at 16-byte boundaries.
+template <typename T>
+bool aligned(const void *base, int64_t a, int64_t b, int64_t c = 0) {
+    return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ((a | b | c) & (Vec<T>::kElems - 1)) == 0;
+}
+
+template <typename T>
 int launch_rotary(const RotaryParams &p, int64_t tokens, cudaStream_t stream) {
-    QMM_CUDA_OK(launch_pdl(rotary_kernel<T>, dim3(static_cast<unsigned>(tokens)), dim3(kThreads), 0, stream, p));
+    constexpr int E = Vec<T>::kElems;
+    const dim3 grid(static_cast<unsigned>(tokens));
+    const bool vectors = p.dim % E == 0 && (p.interleaved ? 2 * p.pairs : p.pairs) % E == 0 && aligned<T>(p.q, p.q_st, p.q_sh) &&
+                         aligned<T>(p.k, p.k_st, p.k_sh) && aligned<T>(p.q_out, 0, 0) && aligned<T>(p.k_out, 0, 0) &&
+                         aligned<T>(p.v, p.v_st, p.v_sh) && aligned<T>(p.k_cache, p.kc_sb, p.kc_st, p.kc_sh) &&
+                         aligned<T>(p.v_cache, p.vc_sb, p.vc_st, p.vc_sh);
+    if (!vectors) {
+        QMM_CUDA_OK(launch_pdl(rotary_kernel<T>, grid, dim3(kThreads), 0, stream, p));
+        return QMM_OK;
+    }
+    const int parts = p.interleaved ? p.dim / E : (p.dim - p.pairs) / E;
+    int shift = 0;
+    while (1 << shift < parts) ++shift;
+    QMM_CUDA_OK(launch_pdl(p.interleaved ? rotary_vec_kernel<T, true> : rotary_vec_kernel<T, false>, grid, dim3(kThreads), 0, stream,
+                           p, shift));
     return QMM_OK;
 }
 
