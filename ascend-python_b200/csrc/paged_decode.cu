@@ -4,15 +4,17 @@
 // time) are the rows of mma.sync m16n8k16, so a key costs the tensor pipe the same for one head as for sixteen, about a fifth of
 // the time its bytes take (tcgen05 would need 64 rows at least and a hand-off through tensor memory for every few keys).
 //
-// One warp is one worker and never waits for another: it has a private ring of stages of 16 keys and values in shared memory,
-// filled by cp.async with the rows' page looked up one stage ahead.  Places that are not seen are not read but zero-filled, so
-// what lies there has no part in any product.  The softmax is one pass: running maximum and sum a row, sums rescaled only
-// when a maximum moved.
+// A warp has a private ring of tiles of 32 keys or values in shared memory, filled by cp.async with the tiles' pages looked up
+// one tile ahead, and never waits for another warp's loads.  Places that are not seen are not read but zero-filled, so what lies
+// there has no part in any product.  The softmax is one pass: running maximum and sum a row, sums rescaled only when a maximum
+// moved.
 //
-// The work of a call is the list of all (sequence, head tile, 16 keys), cut into equal contiguous ranges, one for each worker,
-// wherever sequences begin and end; so a batch of ragged lengths and one long sequence load the GPU alike.  A sequence's heads
-// that one worker has whole are written from registers; of a cut one each worker leaves its sums, and a second kernel joins
-// them in the workers' order.  Nothing depends on timing, and nothing has to be zero before a call.
+// The work of a call is the list of all (sequence, head tile, 32 places), cut into equal contiguous ranges, one for each CTA,
+// wherever sequences begin and end; so a batch of ragged lengths and one long sequence load the GPU alike.  The warps of a CTA
+// take the tiles of a piece (what a CTA has of one sequence's head tile) in turn and add their sums in shared memory, while the
+// tiles of the next piece are under way.  A piece that is the whole is written at once; of a cut one the sums go to the
+// workspace, and a second kernel joins them in the order of the CTAs.  Where every sequence is short, whole head tiles go to
+// the CTAs in turn and nothing is cut.  Nothing depends on timing, and nothing has to be zero before a call.
 #include "paged_common.cuh"
 
 namespace qmm {
@@ -20,22 +22,28 @@ namespace paged {
 
 namespace {
 
-constexpr int kKeys = 16;       // keys of a stage
-constexpr int kRows = 16;       // query heads of a tile
-constexpr int kMinRange = 4;    // stages of a worker at least, where there are as many
+constexpr int kRows = 16;   // query heads of a tile
+constexpr int kShort = 16;  // tiles of a sequence that is not cut while all are this short
 
-// DP: the head dimension rounded up to 64, 128 or 256.  Shared memory of a CTA: 128, 192 and 192 KiB.
+// DP: the head dimension rounded up to 64, 128 or 256.  Shared memory of a CTA: the rings, 192 KiB, eight rows of sums of half
+// the warps, and a query tile.
 template <int DP>
 struct Shape {
-    static constexpr int kStages = DP == 64 ? 4 : DP == 128 ? 3 : 2;
-    static constexpr int kWarps = DP == 256 ? 6 : 8;
+    static constexpr int kKeys = DP == 256 ? 16 : 32;  // keys of a tile: 256 columns of sums leave no registers for 32 scores
+    static constexpr int kWarps = DP == 256 ? 4 : 8;
+    static constexpr int kSlots = DP == 256 ? 6 : DP == 128 ? 3 : 6;  // tiles of a warp's ring, keys and values in turn
     static constexpr int kTileBytes = kKeys * DP * 2;
-    static constexpr int kStageBytes = 2 * kTileBytes;
-    static constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kStageBytes;
+    static constexpr int kHalf = kWarps / 2;
+    static constexpr int kPitch = DP + 8;  // floats of a row of sums: rows 8 banks apart
+    static constexpr int kRing = kWarps * kSlots * kTileBytes;
+    static constexpr int kSums = kHalf * 8 * kPitch * 4;
+    static constexpr int kQuery = kRows * DP * 2;
+    static constexpr int kStats = kHalf * 8 * 8;
+    static constexpr size_t kSmem = kRing + kSums + kQuery + kStats;
 };
 
-// Workspace: part[worker][2][rows][dim] sums, stat[worker][2][rows] (maximum, sum), cut[index]: the first and last worker
-// of a cut item (first < 0: not cut), by item where there are no more items than workers, else by the item's first worker.
+// Workspace: part[CTA][2][rows][dim] sums, stat[CTA][2][rows] (maximum, sum), cut[index]: first and last CTA of a cut item, its
+// sequence and head tile (first < 0: not cut); by item where there are no more items than CTAs, else by the item's first CTA.
 struct Scratch {
     float *part;
     float2 *stat;
@@ -44,7 +52,7 @@ struct Scratch {
 };
 
 struct Plan {
-    int sms, warps, workers, rows, tiles;
+    int workers, rows, tiles;
     int64_t items;
     size_t part_bytes, stat_bytes, bytes;
 };
@@ -52,9 +60,7 @@ struct Plan {
 Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
     Plan plan;
     const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
-    plan.sms = sm_count();
-    plan.warps = dim > 128 ? Shape<256>::kWarps : Shape<128>::kWarps;
-    plan.workers = plan.sms * plan.warps;
+    plan.workers = sm_count();
     plan.rows = static_cast<int>(group < kRows ? group : kRows);
     plan.tiles = static_cast<int>((group + kRows - 1) / kRows);
     plan.items = batch * kv_heads * plan.tiles;
@@ -64,39 +70,65 @@ Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
     return plan;
 }
 
-// What a sequence's token sees, as stages of 16 places: those of the sinks, then those of the window.
+// What a sequence's token sees, as tiles of KEYS places: those of the sinks, then those of the window.
 struct Sequence {
-    int sink_end, lo, hi, sink_stages, first, stages;
+    int sink_end, lo, hi, sink_tiles, first, tiles;
 };
+template <int KEYS>
 __device__ __forceinline__ Sequence sequence_of(const Problem &p, int b) {
-    const int len = p.lens[b];
+    const int len = __ldg(p.lens + b);
     const Range r = visible_range(p, len <= 0 ? -1 : len - 1);
     Sequence s;
     s.sink_end = r.sink_end;
     s.lo = r.lo;
     s.hi = r.hi;
-    s.sink_stages = (r.sink_end + kKeys - 1) / kKeys;
-    s.first = max(r.lo / kKeys, s.sink_stages);
-    const int end = r.hi / kKeys + (r.hi % kKeys != 0);
-    s.stages = s.sink_stages + max(0, end - s.first);
+    s.sink_tiles = (r.sink_end + KEYS - 1) / KEYS;
+    s.first = max(r.lo / KEYS, s.sink_tiles);
+    const int end = r.hi / KEYS + (r.hi % KEYS != 0);
+    s.tiles = s.sink_tiles + max(0, end - s.first);
     return s;
 }
 
-struct Cursor {
-    int b, item, at;  // sequence, head tile of it, stage of that
+// A CTA's part of the list.
+struct Share {
+    int64_t end;    // whole: number of items; else: where the CTA's range ends
+    int64_t range;  // length of a range
+    int items;      // of a sequence
+    bool whole;     // items are not cut, CTA c has c, c + workers, ...
+};
+
+// What a CTA has of one item: tiles [from, to) of sequence b's item.
+struct Piece {
+    int64_t at;  // whole: the item's number; else: where the piece begins in the list
+    int b, item, from, to;
     Sequence s;
 };
 
-// Steps to the next stage of the list; `left`: how many there are from here on (at least 1).
-__device__ __forceinline__ void step(const Problem &p, Cursor &c, int items, bool more) {
-    if (++c.at < c.s.stages) return;
-    c.at = 0;
-    if (++c.item < items) return;
-    c.item = 0;
-    if (!more) return;
-    do {
-        c.s = sequence_of(p, ++c.b);
-    } while (c.s.stages == 0);
+// Steps to the CTA's next piece; false: there is none.
+template <int KEYS>
+__device__ __forceinline__ bool next_piece(const Problem &p, const Share &share, int workers, Piece &piece) {
+    if (share.whole) {
+        piece.at += workers;
+        if (piece.at >= share.end) return false;
+        const int b = static_cast<int>(piece.at / share.items);
+        piece.item = static_cast<int>(piece.at - static_cast<int64_t>(b) * share.items);
+        piece.b = b;
+        piece.s = sequence_of<KEYS>(p, b);
+        piece.from = 0;
+        piece.to = piece.s.tiles;
+        return true;
+    }
+    piece.at += piece.to - piece.from;
+    if (piece.at >= share.end) return false;
+    if (++piece.item == share.items) {
+        piece.item = 0;
+        do {
+            piece.s = sequence_of<KEYS>(p, ++piece.b);
+        } while (piece.s.tiles == 0);
+    }
+    piece.from = 0;
+    piece.to = static_cast<int>(min(static_cast<int64_t>(piece.s.tiles), share.end - piece.at));
+    return true;
 }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
@@ -145,50 +177,69 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
 decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
     using S = Shape<DP>;
-    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int KEYS = S::kKeys, kThreads = S::kWarps * 32;
     constexpr int kChunks = DP / 8;  // 16-byte chunks of a row in shared memory
+    extern __shared__ __align__(128) uint8_t smem[];
+    float *sums = reinterpret_cast<float *>(smem + S::kRing);
+    uint8_t *query = smem + S::kRing + S::kSums;
+    float2 *stats = reinterpret_cast<float2 *>(query + S::kQuery);
     const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
-    // neighbours of the list go to different SMs
-    const int worker = warp * gridDim.x + blockIdx.x;
-    const uint32_t ring = smem_u32(smem) + warp * (S::kStages * S::kStageBytes);
+    const int worker = blockIdx.x;
+    const uint32_t ring = smem_u32(smem) + warp * (S::kSlots * S::kTileBytes);
     pdl_launch_dependents();
     pdl_wait();
 
     const int tiles = (p.group + kRows - 1) / kRows;
-    const int items = p.kv_heads * tiles;
     const int ksteps = (p.dim + 15) / 16;
     const int row_chunks = p.dim / 8;
+    Share share;
+    share.items = p.kv_heads * tiles;
 
-    // sequences that see nothing, and the list's length
+    // the list's length, and whether all sequences are short
     int64_t total = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int b = b0 + lane;
-        const int n = b < p.batch ? sequence_of(p, b).stages : 1;
-        if (b < p.batch) total += n;
-        for (uint32_t none = __ballot_sync(0xffffffffu, n == 0); none != 0; none &= none - 1) {
-            const int e = b0 + __ffs(none) - 1;
-            if (e % scratch.workers != worker) continue;
-            for (int h = 0; h < p.heads; ++h) empty_row<T>(p, e, h);
-            if (scratch.by_item)
-                for (int i = lane; i < items; i += 32) scratch.cut[static_cast<int64_t>(e) * items + i] = make_int4(-1, 0, 0, 0);
-        }
+    int longest = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+        const int n = sequence_of<KEYS>(p, b).tiles;
+        total += n;
+        longest = max(longest, n);
     }
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= items;
-    const int64_t range = max(static_cast<int64_t>(kMinRange), (total + scratch.workers - 1) / scratch.workers);
-    const int64_t begin = worker * range;
-    const int64_t end = min(total, begin + range);
-    if (!scratch.by_item && lane == 0) scratch.cut[worker] = make_int4(-1, 0, 0, 0);
-    if (begin >= end) return;
-
-    // where this worker's range begins
-    Cursor load;
-    {
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    }
+    total *= share.items;
+    share.whole = longest <= kShort;
+    Piece load;
+    load.b = load.item = load.from = load.to = 0;
+    if (!scratch.by_item && threadIdx.x == 0) scratch.cut[worker] = make_int4(-1, 0, 0, 0);
+    if (share.whole) {
+        share.end = static_cast<int64_t>(p.batch) * share.items;
+        share.range = 1;
+        load.at = worker - scratch.workers;
+        if (!next_piece<KEYS>(p, share, scratch.workers, load)) return;
+    } else {
+        share.range = max(static_cast<int64_t>(S::kWarps), (total + scratch.workers - 1) / scratch.workers);
+        const int64_t begin = worker * share.range;
+        share.end = min(total, begin + share.range);
         int64_t before = 0;
-        for (int b0 = 0;; b0 += 32) {
+        bool found = false;
+        // sequences that see nothing, and where this CTA's range begins
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
             const int b = b0 + lane;
-            const int64_t n = b < p.batch ? static_cast<int64_t>(sequence_of(p, b).stages) * items : 0;
-            int64_t sum = n;
+            const int n = b < p.batch ? sequence_of<KEYS>(p, b).tiles : 1;
+            if (warp == 0) {
+                for (uint32_t none = __ballot_sync(0xffffffffu, n == 0); none != 0; none &= none - 1) {
+                    const int e = b0 + __ffs(none) - 1;
+                    if (e % scratch.workers != worker) continue;
+                    for (int h = 0; h < p.heads; ++h) empty_row<T>(p, e, h);
+                    if (scratch.by_item)
+                        for (int i = lane; i < share.items; i += 32)
+                            scratch.cut[static_cast<int64_t>(e) * share.items + i] = make_int4(-1, 0, 0, 0);
+                }
+            }
+            if (found || begin >= share.end) continue;
+            const int64_t mine = b < p.batch ? static_cast<int64_t>(n) * share.items : 0;
+            int64_t sum = mine;
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t left = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += left;
@@ -198,219 +249,326 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 before += __shfl_sync(0xffffffffu, sum, 31);
                 continue;
             }
-            const int which = __ffs(past) - 1;
-            load.b = b0 + which;
-            before += __shfl_sync(0xffffffffu, sum - n, which);
-            break;
+            found = true;
+            load.b = b0 + __ffs(past) - 1;
+            before += __shfl_sync(0xffffffffu, sum - mine, __ffs(past) - 1);
         }
-        load.s = sequence_of(p, load.b);
+        if (!found) return;
+        load.s = sequence_of<KEYS>(p, load.b);
         const int64_t in = begin - before;
-        load.item = static_cast<int>(in / load.s.stages);
-        load.at = static_cast<int>(in - static_cast<int64_t>(load.item) * load.s.stages);
+        load.at = begin;
+        load.item = static_cast<int>(in / load.s.tiles);
+        load.from = static_cast<int>(in - static_cast<int64_t>(load.item) * load.s.tiles);
+        load.to = static_cast<int>(min(static_cast<int64_t>(load.s.tiles), load.from + share.end - begin));
     }
-    Cursor use = load;
+    Piece piece = load;
 
-    // ---- loads: lanes 0..15 look up the stage's keys, lanes 16..31 its values ----
-    int64_t loads_left = end - begin;
-    int at_place = 0, entry = 0;
-    bool at_seen = false;
-    auto look_up = [&] {
-        const int first = load.at < load.s.sink_stages ? load.at * kKeys : (load.s.first + load.at - load.s.sink_stages) * kKeys;
-        const int j = first + (lane & 15);
-        at_seen = j < load.s.hi && (j < load.s.sink_end || j >= load.s.lo);
-        const int page = at_seen ? page_of(p, j) : 0;
-        at_place = j - page * p.page;
-        entry = at_seen ? __ldg(p.table + load.b * p.table_st + page) : -1;
-    };
-    uint64_t seen_queue = 0;  // 16 bits for each stage under way
-    int under_way = 0, load_slot = 0;
-    auto produce = [&] {
-        if (loads_left > 0) {
-            const bool ok = at_seen && entry >= 0 && entry < p.pages;
-            const uint32_t seen = __ballot_sync(0xffffffffu, ok);
-            seen_queue |= static_cast<uint64_t>(seen & 0xffffu) << (16 * under_way);
-            const int kvh = load.item / tiles;
-            const bool keys = lane < 16;
-            const int64_t offset = ok ? entry * (keys ? p.k_sb : p.v_sb) + at_place * (keys ? p.k_st : p.v_st) + kvh * (keys ? p.k_sh : p.v_sh) : 0;
-            const uint32_t stage = ring + load_slot * S::kStageBytes;
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                const T *base = static_cast<const T *>(part == 0 ? p.k : p.v);
-#pragma unroll
-                for (int i = 0; i < kChunks / 2; ++i) {
-                    const int idx = i * 32 + lane, key = idx / kChunks, chunk = idx % kChunks;
-                    const T *row = base + __shfl_sync(0xffffffffu, offset, key + 16 * part);
-                    if (chunk < 2 * ksteps)
-                        cp_async_16(stage + part * S::kTileBytes + key * (DP * 2) + ((chunk ^ (key & 7)) << 4),
-                                    row + (chunk < row_chunks ? chunk * 8 : 0), chunk < row_chunks && (seen >> key & 1) ? 16 : 0);
-                }
-            }
-            --loads_left;
-            step(p, load, items, loads_left > 0);
-            if (loads_left > 0) look_up();
+    // ---- loads: one place of the tile a lane (16 keys: lanes 16..31 the same again), keys and values of a tile apart ----
+    int at = load.from + warp;  // this warp's next tile of the piece that is being loaded
+    bool more = true;
+    auto settle = [&] {  // on to a piece that has a tile for this warp
+        while (more && at >= load.to) {
+            more = next_piece<KEYS>(p, share, scratch.workers, load);
+            at = load.from + warp;
         }
-        cp_async_commit();
-        ++under_way;
-        load_slot = load_slot + 1 == S::kStages ? 0 : load_slot + 1;
+    };
+    settle();
+    int at_place = 0, entry = -1;
+    auto look_up = [&] {
+        entry = -1;
+        if (!more) return;
+        const int first = at < load.s.sink_tiles ? at * KEYS : (load.s.first + at - load.s.sink_tiles) * KEYS;
+        const int j = first + (lane & (KEYS - 1));
+        if (j < load.s.hi && (j < load.s.sink_end || j >= load.s.lo)) {
+            const int page = page_of(p, j);
+            at_place = j - page * p.page;
+            entry = __ldg(p.table + load.b * p.table_st + page);
+        }
     };
     look_up();
+    // every load of keys is followed by that of their values, so the lookup and the mask are kept for it
+    constexpr int kMasks = S::kSlots / 2 + 1;
+    uint32_t masks[kMasks];  // of the tiles under way, oldest first
 #pragma unroll
-    for (int i = 0; i < S::kStages - 1; ++i) produce();
+    for (int i = 0; i < kMasks; ++i) masks[i] = 0;
+    int under_way = 0, slot = 0, value_place = 0, value_entry = 0, value_head = 0;
+    uint32_t value_seen = 0;
+    auto copy_tile = [&](const void *cache, int64_t sb, int64_t st, int64_t sh, int id, int place, int kvh, uint32_t seen) {
+        const uint32_t dst = ring + slot * S::kTileBytes;
+        const int64_t offset = seen >> lane & 1 ? id * sb + place * st + kvh * sh : 0;
+        const T *base = static_cast<const T *>(cache);
+#pragma unroll
+        for (int i = 0; i < KEYS * kChunks / 32; ++i) {
+            const int idx = i * 32 + lane, key = idx / kChunks, chunk = idx % kChunks;
+            const T *row = base + __shfl_sync(0xffffffffu, offset, key);
+            if (chunk < 2 * ksteps)
+                cp_async_16(dst + key * (DP * 2) + ((chunk ^ (key & 7)) << 4), row + (chunk < row_chunks ? chunk * 8 : 0),
+                            chunk < row_chunks && (seen >> key & 1) ? 16 : 0);
+        }
+    };
+    auto load_keys = [&] {
+        if (more) {
+            value_seen = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.pages);
+            value_place = at_place;
+            value_entry = entry;
+            value_head = load.item / tiles;
+#pragma unroll
+            for (int i = 0; i < kMasks; ++i)
+                if (i == under_way) masks[i] = value_seen;
+            ++under_way;
+            copy_tile(p.k, p.k_sb, p.k_st, p.k_sh, value_entry, value_place, value_head, value_seen);
+            at += S::kWarps;
+            settle();
+            look_up();
+        } else {
+            value_head = -1;
+        }
+        cp_async_commit();
+        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+    };
+    auto load_values = [&] {
+        if (value_head >= 0) copy_tile(p.v, p.v_sb, p.v_st, p.v_sh, value_entry, value_place, value_head, value_seen);
+        cp_async_commit();
+        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+    };
+    static_assert(S::kSlots >= 3, "keys, values and the next keys");
+#pragma unroll
+    for (int i = 0; i < S::kSlots - 1; ++i) {
+        if (i % 2 == 0)
+            load_keys();
+        else
+            load_values();
+    }
+    // steps of one load each, in the order of the ring: the load that a step of the products makes room for
+    constexpr bool kKeysNext = (S::kSlots - 1) % 2 == 0;
+
+    // ---- the query tile of the piece to come: loaded a piece ahead, stored when the warps meet ----
+    constexpr int kQueryChunks = kRows * kChunks / kThreads > 0 ? kRows * kChunks / kThreads : 1;
+    uint4 ahead[kQueryChunks];
+    auto load_query = [&](const Piece &of) {
+        const int kvh = of.item / tiles, tile = of.item - kvh * tiles;
+        const int rows = min(kRows, p.group - tile * kRows);
+        const T *base = static_cast<const T *>(p.q) + of.b * p.q_st + (kvh * p.group + tile * kRows) * p.q_sh;
+#pragma unroll
+        for (int i = 0; i < kQueryChunks; ++i) {
+            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, chunk = idx % kChunks;
+            ahead[i] = row < rows && chunk < row_chunks ? __ldg(reinterpret_cast<const uint4 *>(base + row * p.q_sh + chunk * 8))
+                                                        : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto store_query = [&] {
+#pragma unroll
+        for (int i = 0; i < kQueryChunks; ++i) {
+            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, chunk = idx % kChunks;
+            if (row < kRows) *reinterpret_cast<uint4 *>(query + row * (DP * 2) + ((chunk ^ (row & 7)) << 4)) = ahead[i];
+        }
+    };
+    load_query(piece);
+    store_query();
+    __syncthreads();
 
     // ---- products ----
     const float scale = p.scale * kLog2e;
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-    uint32_t q[DP / 16][4];
-    float o[DP / 8][4];
-    float top[2], sum[2];
-    bool fresh = true;
     int use_slot = 0;
-    bool whole = use.at == 0;  // this worker has the item from its first stage on
-    for (int64_t u = begin; u < end; ++u) {
-        const int kvh = use.item / tiles, tile = use.item - kvh * tiles;
-        const int head0 = kvh * p.group + tile * kRows;
-        const int rows = min(kRows, p.group - tile * kRows);
-        if (fresh) {
-            fresh = false;
-            const T *base = static_cast<const T *>(p.q) + use.b * p.q_st + head0 * p.q_sh;
+    while (true) {
+        Piece next = piece;
+        const bool another = next_piece<KEYS>(p, share, scratch.workers, next);
+        if (another) load_query(next);
+        auto query_part = [&](uint32_t (&r)[4], int ks) {
+            const int row = lane & 15, chunk = ks * 2 + (lane >> 4);
+            ldmatrix_x4(r, smem_u32(query) + row * (DP * 2) + ((chunk ^ (row & 7)) << 4));
+        };
+        constexpr bool kKept = DP < 256;  // in registers; 256 columns of sums leave none
+        uint32_t q[kKept ? DP / 16 : 1][4];
+        if (kKept) {
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) query_part(q[kKept ? ks : 0], ks);
+        }
+        float o[DP / 8][4];
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+
+        for (int g = piece.from + warp; g < piece.to; g += S::kWarps) {
+            // scores of 16 rows x KEYS keys: accumulators of 8 keys
+            float s[KEYS / 8][4];
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            cp_async_wait<S::kSlots - 2>();
+            __syncwarp();
+            const uint32_t seen = masks[0];
+#pragma unroll
+            for (int i = 0; i + 1 < kMasks; ++i) masks[i] = masks[i + 1];
+            --under_way;
+            // into the slot that the step before this one used
+            if (kKeysNext) load_keys(); else load_values();
+            const uint32_t keys = ring + use_slot * S::kTileBytes;
+            use_slot = use_slot + 1 == S::kSlots ? 0 : use_slot + 1;
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
+                if (ks >= ksteps) break;
+                uint32_t(&qk)[4] = q[kKept ? ks : 0];
+                if (!kKept) query_part(qk, ks);
+#pragma unroll
+                for (int n = 0; n < KEYS / 16; ++n) {
+                    uint32_t b[4];
+                    const int key = n * 16 + ((lane >> 4) << 3) + (lane & 7), chunk = ks * 2 + ((lane >> 3) & 1);
+                    ldmatrix_x4(b, keys + key * (DP * 2) + ((chunk ^ (key & 7)) << 4));
+                    mma_16816<T>(s[2 * n], qk, b[0], b[1]);
+                    mma_16816<T>(s[2 * n + 1], qk, b[2], b[3]);
+                }
+            }
+            float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int row = r0 + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + c0;
-                    q[ks][i] = row < rows && col < p.dim ? __ldg(reinterpret_cast<const uint32_t *>(base + row * p.q_sh + col)) : 0;
+                    // hidden behind the scaling, whose sign and zero a hidden score must not meet
+                    s[n][i] = seen >> (n * 8 + c0 + (i & 1)) & 1 ? s[n][i] * scale : -INFINITY;
+                    most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
                 }
             }
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-            top[0] = top[1] = -INFINITY;
-            sum[0] = sum[1] = 0.0f;
-        }
-        cp_async_wait<S::kStages - 2>();
-        __syncwarp();
-        const uint32_t seen = static_cast<uint32_t>(seen_queue) & 0xffffu;
-        seen_queue >>= 16;
-        --under_way;
-        produce();  // into the stage that the step before this one used
-        const uint32_t keys = ring + use_slot * S::kStageBytes, values = keys + S::kTileBytes;
-        use_slot = use_slot + 1 == S::kStages ? 0 : use_slot + 1;
-
-        // scores of 16 rows x 16 keys: two accumulators of 8 keys
-        float s[2][4] = {};
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            if (ks >= ksteps) break;
-            uint32_t b[4];
-            const int key = ((lane >> 4) << 3) + (lane & 7), chunk = ks * 2 + ((lane >> 3) & 1);
-            ldmatrix_x4(b, keys + key * (DP * 2) + ((chunk ^ (key & 7)) << 4));
-            mma_16816<T>(s[0], q[ks], b[0], b[1]);
-            mma_16816<T>(s[1], q[ks], b[2], b[3]);
-        }
-        float most[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = n * 8 + c0 + (i & 1);
-                // hidden behind the scaling, whose sign and zero a hidden score must not meet
-                s[n][i] = seen >> key & 1 ? s[n][i] * scale : -INFINITY;
-                most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
-            }
-        }
-        bool moved = false;
-        float base[2], keep[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
-            most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
-            const float now = fmaxf(top[r], most[r]);
-            base[r] = now == -INFINITY ? 0.0f : now;
-            keep[r] = exp2_fast(top[r] - base[r]);
-            moved |= now != top[r];
-            top[r] = now;
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-                o[n][0] *= keep[0];
-                o[n][1] *= keep[0];
-                o[n][2] *= keep[1];
-                o[n][3] *= keep[1];
-            }
-            sum[0] *= keep[0];
-            sum[1] *= keep[1];
-        }
-        float e[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[n][i] = exp2_fast(s[n][i] - base[i >> 1]);
-                sum[i >> 1] += e[n][i];
-            }
-        }
-        // the weights, rounded to the type of the values (the sum above takes them unrounded: 2^-9 or 2^-12 of each weight,
-        // independent of one another), as they lie are the second product's first operand
-        const uint32_t a[4] = {pack2<T>(e[0][0], e[0][1]), pack2<T>(e[0][2], e[0][3]), pack2<T>(e[1][0], e[1][1]),
-                               pack2<T>(e[1][2], e[1][3])};
-#pragma unroll
-        for (int n = 0; n < DP / 16; ++n) {
-            if (n >= ksteps) break;
-            uint32_t b[4];
-            const int key = (((lane >> 3) & 1) << 3) + (lane & 7), chunk = n * 2 + (lane >> 4);
-            ldmatrix_x4_trans(b, values + key * (DP * 2) + ((chunk ^ (key & 7)) << 4));
-            mma_16816<T>(o[2 * n], a, b[0], b[1]);
-            mma_16816<T>(o[2 * n + 1], a, b[2], b[3]);
-        }
-
-        const bool item_ends = use.at + 1 == use.s.stages;
-        if (item_ends || u + 1 == end) {
+            bool moved = false;
+            float base[2], keep[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+                most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
+                most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
+                const float now = fmaxf(top[r], most[r]);
+                base[r] = now == -INFINITY ? 0.0f : now;
+                keep[r] = exp2_fast(top[r] - base[r]);
+                moved |= now != top[r];
+                top[r] = now;
             }
-            const int64_t index = static_cast<int64_t>(use.b) * items + use.item;
-            if (whole && item_ends) {
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n) {
+                    o[n][0] *= keep[0];
+                    o[n][1] *= keep[0];
+                    o[n][2] *= keep[1];
+                    o[n][3] *= keep[1];
+                }
+                sum[0] *= keep[0];
+                sum[1] *= keep[1];
+            }
+            // the weights, rounded to the type of the values (the sum takes them unrounded: 2^-9 or 2^-12 of each weight,
+            // independent of one another), as they lie are the second product's first operand
+            uint32_t a[KEYS / 16][4];
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int row = r0 + r * 8;
-                    if (row >= rows) continue;
-                    const int64_t at = static_cast<int64_t>(use.b) * p.heads + head0 + row;
-                    const float inv = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
-                    T *dst = static_cast<T *>(p.out) + at * p.dim;
-#pragma unroll
-                    for (int n = 0; n < DP / 8; ++n)
-                        if (n * 8 < p.dim)
-                            *reinterpret_cast<uint32_t *>(dst + n * 8 + c0) = pack2<T>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
-                    if ((lane & 3) == 0) p.lse[at] = sum[r] == 0.0f ? -INFINITY : top[r] * kLn2 + logf(sum[r]);
-                }
-                if (scratch.by_item && lane == 0) scratch.cut[index] = make_int4(-1, 0, 0, 0);
-            } else {
-                const int64_t slot = worker * 2 + (whole ? 1 : 0);
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int row = r0 + r * 8;
-                    if (row >= rows) continue;
-                    float *dst = scratch.part + (slot * scratch.rows + row) * p.dim;
-#pragma unroll
-                    for (int n = 0; n < DP / 8; ++n)
-                        if (n * 8 < p.dim) *reinterpret_cast<float2 *>(dst + n * 8 + c0) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
-                    if ((lane & 3) == 0) scratch.stat[slot * scratch.rows + row] = make_float2(top[r], sum[r]);
-                }
-                if (whole && lane == 0) {
-                    const int last = static_cast<int>((u - use.at + use.s.stages - 1) / range);
-                    scratch.cut[scratch.by_item ? index : worker] = make_int4(worker, last, use.b, use.item);
+                    const float e0 = exp2_fast(s[n][2 * r] - base[r]), e1 = exp2_fast(s[n][2 * r + 1] - base[r]);
+                    sum[r] += e0 + e1;
+                    a[n >> 1][(n & 1) * 2 + r] = pack2<T>(e0, e1);
                 }
             }
-            fresh = whole = true;
+            cp_async_wait<S::kSlots - 2>();
+            __syncwarp();
+            if (kKeysNext) load_values(); else load_keys();
+            const uint32_t values = ring + use_slot * S::kTileBytes;
+            use_slot = use_slot + 1 == S::kSlots ? 0 : use_slot + 1;
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n) {
+                if (n >= ksteps) break;
+#pragma unroll
+                for (int k = 0; k < KEYS / 16; ++k) {
+                    uint32_t b[4];
+                    const int key = k * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), chunk = n * 2 + (lane >> 4);
+                    ldmatrix_x4_trans(b, values + key * (DP * 2) + ((chunk ^ (key & 7)) << 4));
+                    mma_16816<T>(o[2 * n], a[k], b[0], b[1]);
+                    mma_16816<T>(o[2 * n + 1], a[k], b[2], b[3]);
+                }
+            }
         }
-        step(p, use, items, u + 1 < end);
+
+        // ---- the warps' sums, eight rows at a time: the upper half's to the lower half's, then what is left by all threads ----
+        const int kvh = piece.item / tiles, tile = piece.item - kvh * tiles;
+        const int head0 = kvh * p.group + tile * kRows;
+        const int rows = min(kRows, p.group - tile * kRows);
+        const bool begins = piece.from == 0, ends = piece.to == piece.s.tiles;
+        const int64_t slot_row = (worker * 2 + (begins ? 1 : 0)) * static_cast<int64_t>(scratch.rows);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (r * 8 >= rows) break;
+            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+            const int buffer = warp < S::kHalf ? warp : warp - S::kHalf;
+            float *mine = sums + (buffer * 8 + r0) * S::kPitch + c0;
+            float2 *my_stat = stats + buffer * 8 + r0;
+            auto put = [&] {
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float2 *>(mine + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                if ((lane & 3) == 0) *my_stat = make_float2(top[r], sum[r]);
+            };
+            if (warp >= S::kHalf) put();
+            __syncthreads();
+            if (r == 0 && another) store_query();
+            if (warp < S::kHalf) {
+                const float2 other = *my_stat;
+                const float now = fmaxf(top[r], other.x), base = now == -INFINITY ? 0.0f : now;
+                const float keep = exp2_fast(top[r] - base), add = exp2_fast(other.x - base);
+#pragma unroll
+                for (int n = 0; n < DP / 8; ++n) {
+                    const float2 v = *reinterpret_cast<const float2 *>(mine + n * 8);
+                    o[n][2 * r] = fmaf(v.x, add, o[n][2 * r] * keep);
+                    o[n][2 * r + 1] = fmaf(v.y, add, o[n][2 * r + 1] * keep);
+                }
+                sum[r] = fmaf(other.y, add, sum[r] * keep);
+                top[r] = now;
+                __syncwarp();  // a row's four lanes have read its statistics
+                put();
+            }
+            __syncthreads();
+            for (int idx = threadIdx.x; idx < min(8, rows - r * 8) * (DP / 4); idx += kThreads) {
+                const int at_row = idx / (DP / 4), row = r * 8 + at_row, d = idx % (DP / 4) * 4;
+                if (d >= p.dim) continue;
+                float2 stat[S::kHalf];
+                float now = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < S::kHalf; ++w) {
+                    stat[w] = stats[w * 8 + at_row];
+                    now = fmaxf(now, stat[w].x);
+                }
+                const float base = now == -INFINITY ? 0.0f : now;
+                float all = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < S::kHalf; ++w) {
+                    const float weight = exp2_fast(stat[w].x - base);
+                    const float4 x = *reinterpret_cast<const float4 *>(sums + (w * 8 + at_row) * S::kPitch + d);
+                    all = fmaf(stat[w].y, weight, all);
+                    v.x = fmaf(x.x, weight, v.x);
+                    v.y = fmaf(x.y, weight, v.y);
+                    v.z = fmaf(x.z, weight, v.z);
+                    v.w = fmaf(x.w, weight, v.w);
+                }
+                if (begins && ends) {
+                    const int64_t to = static_cast<int64_t>(piece.b) * p.heads + head0 + row;
+                    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+                    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to * p.dim + d) =
+                        make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+                    if (d == 0) p.lse[to] = all == 0.0f ? -INFINITY : now * kLn2 + logf(all);
+                } else {
+                    *reinterpret_cast<float4 *>(scratch.part + (slot_row + row) * p.dim + d) = v;
+                    if (d == 0) scratch.stat[slot_row + row] = make_float2(now, all);
+                }
+            }
+            __syncthreads();  // before the buffers are written again
+        }
+        if (threadIdx.x == 0 && begins && (scratch.by_item || !ends)) {
+            const int last = ends ? 0 : static_cast<int>((piece.at + piece.s.tiles - 1) / share.range);
+            scratch.cut[scratch.by_item ? static_cast<int64_t>(piece.b) * share.items + piece.item : worker] =
+                make_int4(ends ? -1 : worker, last, piece.b, piece.item);
+        }
+        if (!another) break;
+        piece = next;
     }
     cp_async_wait<0>();
 }
 
-// Joins the parts of the cut items, in the order of the workers.  share_parts (few items): a CTA has one row of an item and its
+// Joins the parts of the cut items, in the order of the CTAs.  share_parts (few items): a CTA has one row of an item and its
 // warps share the parts; else its warps share the rows.
 constexpr int kJoinWarps = 8;
 template <typename T>
@@ -502,9 +660,9 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch s
 template <typename T, int DP>
 int launch(const Problem &p, const Plan &plan, Scratch scratch, cudaStream_t stream) {
     QMM_CUDA_OK(cudaFuncSetAttribute(decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<DP>::kSmem)));
-    QMM_CUDA_OK(launch_pdl(decode_kernel<T, DP>, dim3(plan.sms), dim3(Shape<DP>::kWarps * 32), Shape<DP>::kSmem, stream, p, scratch));
+    QMM_CUDA_OK(launch_pdl(decode_kernel<T, DP>, dim3(plan.workers), dim3(Shape<DP>::kWarps * 32), Shape<DP>::kSmem, stream, p, scratch));
     const int64_t indices = scratch.by_item ? plan.items : plan.workers;
-    const bool share_parts = indices * plan.rows <= 2 * plan.sms;
+    const bool share_parts = indices * plan.rows <= 4 * plan.workers;
     QMM_CUDA_OK(launch_pdl(join_kernel<T>, dim3(static_cast<unsigned>(indices), share_parts ? plan.rows : 1), dim3(kJoinWarps * 32), 0,
                            stream, p, scratch, share_parts));
     return QMM_OK;
