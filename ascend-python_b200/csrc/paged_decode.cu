@@ -30,13 +30,13 @@ constexpr int kShort = 16;  // tiles of a sequence that is not cut while all are
 template <int DP>
 struct Shape {
     static constexpr int kKeys = DP == 256 ? 16 : 32;  // keys of a tile: 256 columns of sums leave no registers for 32 scores
-    static constexpr int kWarps = DP == 256 ? 4 : 8;
+    static constexpr int kWarps = DP == 256 ? 2 : 4;
     static constexpr int kSlots = DP == 256 ? 6 : DP == 128 ? 3 : 6;  // tiles of a warp's ring, keys and values in turn
     static constexpr int kTileBytes = kKeys * DP * 2;
     static constexpr int kHalf = kWarps / 2;
     static constexpr int kPitch = DP + 8;  // floats of a row of sums: rows 8 banks apart
     static constexpr int kRing = kWarps * kSlots * kTileBytes;
-    static constexpr int kSums = kHalf * 8 * kPitch * 4;
+    static constexpr int kSums = (kHalf * 8 * kPitch * 4 + 511) / 512 * 512;  // the query tile begins at a multiple of its rows
     static constexpr int kQuery = kRows * DP * 2;
     static constexpr int kStats = kHalf * 8 * 8;
     static constexpr size_t kSmem = kRing + kSums + kQuery + kStats;
@@ -60,7 +60,7 @@ struct Plan {
 Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
     Plan plan;
     const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
-    plan.workers = sm_count();
+    plan.workers = 2 * sm_count();
     plan.rows = static_cast<int>(group < kRows ? group : kRows);
     plan.tiles = static_cast<int>((group + kRows - 1) / kRows);
     plan.items = batch * kv_heads * plan.tiles;
@@ -174,12 +174,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1)
+__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 2)
 decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
     using S = Shape<DP>;
     constexpr int KEYS = S::kKeys, kThreads = S::kWarps * 32;
     constexpr int kChunks = DP / 8;  // 16-byte chunks of a row in shared memory
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(512) uint8_t smem[];  // rows of up to 512 bytes, stepped through by exclusive or
     float *sums = reinterpret_cast<float *>(smem + S::kRing);
     uint8_t *query = smem + S::kRing + S::kSums;
     float2 *stats = reinterpret_cast<float2 *>(query + S::kQuery);
@@ -293,17 +293,40 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
     for (int i = 0; i < kMasks; ++i) masks[i] = 0;
     int under_way = 0, slot = 0, value_place = 0, value_entry = 0, value_head = 0;
     uint32_t value_seen = 0;
+    // A lane always has the same chunk, of rows kStep apart.  Rows of 16 places lie evenly apart where a page holds a multiple of
+    // 16 (tiles begin at multiples of 16), so a tile that is seen whole takes one address for 16 places; else each row its own.
+    constexpr int kStep = 32 / kChunks;
+    const int my_key = lane / kChunks, my_chunk = lane % kChunks;
+    const bool my_part = my_chunk < 2 * ksteps;
+    const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
+    const bool even = p.page % 16 == 0 && row_chunks == 2 * ksteps;
+    // the swizzled place of key kStep * i + my_key: chunk ^ key % 8, where the key's parts have no bits in common
+    const uint32_t my_dst = my_key * (DP * 2) + ((my_chunk ^ my_key) << 4);
     auto copy_tile = [&](const void *cache, int64_t sb, int64_t st, int64_t sh, int id, int place, int kvh, uint32_t seen) {
-        const uint32_t dst = ring + slot * S::kTileBytes;
-        const int64_t offset = seen >> lane & 1 ? id * sb + place * st + kvh * sh : 0;
-        const T *base = static_cast<const T *>(cache);
+        const uint32_t dst = ring + slot * S::kTileBytes + my_dst;
+        const bool ok = seen >> lane & 1;
+        const int64_t offset = ok ? id * sb + place * st + kvh * sh : 0;
+        const T *base = static_cast<const T *>(cache) + my_offset;
+        if (even && seen == 0xffffffffu) {
+            const T *row[KEYS / 16];
 #pragma unroll
-        for (int i = 0; i < KEYS * kChunks / 32; ++i) {
-            const int idx = i * 32 + lane, key = idx / kChunks, chunk = idx % kChunks;
+            for (int h = 0; h < KEYS / 16; ++h) row[h] = base + __shfl_sync(0xffffffffu, offset, 16 * h) + my_key * st;
+            if (my_part) {
+#pragma unroll
+                for (int i = 0; i < KEYS / kStep; ++i) {
+                    const int first = kStep * i;
+                    cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row[first / 16], 16);
+                    row[first / 16] += kStep * st;
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < KEYS / kStep; ++i) {
+            const int first = kStep * i, key = first + my_key;
             const T *row = base + __shfl_sync(0xffffffffu, offset, key);
-            if (chunk < 2 * ksteps)
-                cp_async_16(dst + key * (DP * 2) + ((chunk ^ (key & 7)) << 4), row + (chunk < row_chunks ? chunk * 8 : 0),
-                            chunk < row_chunks && (seen >> key & 1) ? 16 : 0);
+            if (my_part)
+                cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row, my_chunk < row_chunks && (seen >> key & 1) ? 16 : 0);
         }
     };
     auto load_keys = [&] {
@@ -342,6 +365,12 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
     // steps of one load each, in the order of the ring: the load that a step of the products makes room for
     constexpr bool kKeysNext = (S::kSlots - 1) % 2 == 0;
 
+    // The running maximum is one of unscaled scores, which takes a positive scale: a negative one's sign goes to the query, and
+    // for a scale of 0 the query is 0.
+    const float factor = p.scale * kLog2e;
+    const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
+    const uint32_t query_and = factor == 0.0f ? 0u : 0xffffffffu, query_xor = factor < 0.0f ? 0x80008000u : 0u;
+
     // ---- the query tile of the piece to come: loaded a piece ahead, stored when the warps meet ----
     constexpr int kQueryChunks = kRows * kChunks / kThreads > 0 ? kRows * kChunks / kThreads : 1;
     uint4 ahead[kQueryChunks];
@@ -360,7 +389,10 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 #pragma unroll
         for (int i = 0; i < kQueryChunks; ++i) {
             const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, chunk = idx % kChunks;
-            if (row < kRows) *reinterpret_cast<uint4 *>(query + row * (DP * 2) + ((chunk ^ (row & 7)) << 4)) = ahead[i];
+            if (row < kRows)
+                *reinterpret_cast<uint4 *>(query + row * (DP * 2) + ((chunk ^ (row & 7)) << 4)) =
+                    make_uint4((ahead[i].x & query_and) ^ query_xor, (ahead[i].y & query_and) ^ query_xor,
+                               (ahead[i].z & query_and) ^ query_xor, (ahead[i].w & query_and) ^ query_xor);
         }
     };
     load_query(piece);
@@ -368,16 +400,15 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
     __syncthreads();
 
     // ---- products ----
-    const float scale = p.scale * kLog2e;
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;
     int use_slot = 0;
     while (true) {
         Piece next = piece;
         const bool another = next_piece<KEYS>(p, share, scratch.workers, next);
         if (another) load_query(next);
+        // ldmatrix addresses: chunk 2 i + c of a row swizzled by r is (2 i) ^ (c ^ r), so a step is one exclusive or
         auto query_part = [&](uint32_t (&r)[4], int ks) {
-            const int row = lane & 15, chunk = ks * 2 + (lane >> 4);
-            ldmatrix_x4(r, smem_u32(query) + row * (DP * 2) + ((chunk ^ (row & 7)) << 4));
+            ldmatrix_x4(r, (smem_u32(query) + (lane & 15) * (DP * 2) + (((lane >> 4) ^ (lane & 7)) << 4)) ^ (ks << 5));
         };
         constexpr bool kKept = DP < 256;  // in registers; 256 columns of sums leave none
         uint32_t q[kKept ? DP / 16 : 1][4];
@@ -403,7 +434,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             --under_way;
             // into the slot that the step before this one used
             if (kKeysNext) load_keys(); else load_values();
-            const uint32_t keys = ring + use_slot * S::kTileBytes;
+            const uint32_t keys = ring + use_slot * S::kTileBytes + (((lane >> 4) << 3) + (lane & 7)) * (DP * 2) +
+                                  ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
             use_slot = use_slot + 1 == S::kSlots ? 0 : use_slot + 1;
 #pragma unroll
             for (int ks = 0; ks < DP / 16; ++ks) {
@@ -413,21 +445,24 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 #pragma unroll
                 for (int n = 0; n < KEYS / 16; ++n) {
                     uint32_t b[4];
-                    const int key = n * 16 + ((lane >> 4) << 3) + (lane & 7), chunk = ks * 2 + ((lane >> 3) & 1);
-                    ldmatrix_x4(b, keys + key * (DP * 2) + ((chunk ^ (key & 7)) << 4));
+                    ldmatrix_x4(b, (keys ^ (ks << 5)) + n * 16 * (DP * 2));
                     mma_16816<T>(s[2 * n], qk, b[0], b[1]);
                     mma_16816<T>(s[2 * n + 1], qk, b[2], b[3]);
+                }
+            }
+            if (seen != 0xffffffffu) {
+#pragma unroll
+                for (int n = 0; n < KEYS / 8; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(seen >> (n * 8 + c0 + (i & 1)) & 1)) s[n][i] = -INFINITY;
                 }
             }
             float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // hidden behind the scaling, whose sign and zero a hidden score must not meet
-                    s[n][i] = seen >> (n * 8 + c0 + (i & 1)) & 1 ? s[n][i] * scale : -INFINITY;
-                    most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
-                }
+                for (int i = 0; i < 4; ++i) most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
             }
             bool moved = false;
             float base[2], keep[2];
@@ -436,8 +471,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
                 most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
                 const float now = fmaxf(top[r], most[r]);
-                base[r] = now == -INFINITY ? 0.0f : now;
-                keep[r] = exp2_fast(top[r] - base[r]);
+                base[r] = now == -INFINITY ? 0.0f : now * scale;
+                keep[r] = exp2_fast(fmaf(top[r], scale, -base[r]));
                 moved |= now != top[r];
                 top[r] = now;
             }
@@ -459,7 +494,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float e0 = exp2_fast(s[n][2 * r] - base[r]), e1 = exp2_fast(s[n][2 * r + 1] - base[r]);
+                    const float e0 = exp2_fast(fmaf(s[n][2 * r], scale, -base[r])), e1 = exp2_fast(fmaf(s[n][2 * r + 1], scale, -base[r]));
                     sum[r] += e0 + e1;
                     a[n >> 1][(n & 1) * 2 + r] = pack2<T>(e0, e1);
                 }
@@ -467,7 +502,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             cp_async_wait<S::kSlots - 2>();
             __syncwarp();
             if (kKeysNext) load_values(); else load_keys();
-            const uint32_t values = ring + use_slot * S::kTileBytes;
+            const uint32_t values = ring + use_slot * S::kTileBytes + ((((lane >> 3) & 1) << 3) + (lane & 7)) * (DP * 2) +
+                                    (((lane >> 4) ^ (lane & 7)) << 4);
             use_slot = use_slot + 1 == S::kSlots ? 0 : use_slot + 1;
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n) {
@@ -475,8 +511,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 #pragma unroll
                 for (int k = 0; k < KEYS / 16; ++k) {
                     uint32_t b[4];
-                    const int key = k * 16 + (((lane >> 3) & 1) << 3) + (lane & 7), chunk = n * 2 + (lane >> 4);
-                    ldmatrix_x4_trans(b, values + key * (DP * 2) + ((chunk ^ (key & 7)) << 4));
+                    ldmatrix_x4_trans(b, (values ^ (n << 5)) + k * 16 * (DP * 2));
                     mma_16816<T>(o[2 * n], a[k], b[0], b[1]);
                     mma_16816<T>(o[2 * n + 1], a[k], b[2], b[3]);
                 }
@@ -494,6 +529,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             if (r * 8 >= rows) break;
             sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
             sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+            top[r] *= scale;
             const int buffer = warp < S::kHalf ? warp : warp - S::kHalf;
             float *mine = sums + (buffer * 8 + r0) * S::kPitch + c0;
             float2 *my_stat = stats + buffer * 8 + r0;
