@@ -4,17 +4,18 @@
 // time) are the rows of mma.sync m16n8k16, so a key costs the tensor pipe the same for one head as for sixteen, about a fifth of
 // the time its bytes take (tcgen05 would need 64 rows at least and a hand-off through tensor memory for every few keys).
 //
-// A warp has a private ring of tiles of 32 keys or values in shared memory, filled by cp.async with the tiles' pages looked up
+// A warp has a private ring of 8 KiB tiles of keys or values in shared memory, filled by cp.async with a tile's pages looked up
 // one tile ahead, and never waits for another warp's loads.  Places that are not seen are not read but zero-filled, so what lies
 // there has no part in any product.  The softmax is one pass: running maximum and sum a row, sums rescaled only when a maximum
 // moved.
 //
-// The work of a call is the list of all (sequence, head tile, 32 places), cut into equal contiguous ranges, one for each CTA,
-// wherever sequences begin and end; so a batch of ragged lengths and one long sequence load the GPU alike.  The warps of a CTA
-// take the tiles of a piece (what a CTA has of one sequence's head tile) in turn and add their sums in shared memory, while the
-// tiles of the next piece are under way.  A piece that is the whole is written at once; of a cut one the sums go to the
-// workspace, and a second kernel joins them in the order of the CTAs.  Where every sequence is short, whole head tiles go to
-// the CTAs in turn and nothing is cut.  Nothing depends on timing, and nothing has to be zero before a call.
+// The work of a call is the list of all (sequence, head tile, tile of places), cut into equal contiguous ranges, one for each
+// warp, wherever sequences begin and end; so a batch of ragged lengths and one long sequence load the GPU alike, and no warp
+// waits for another until its range is done.  Head tiles that a warp has whole are written from registers.  Of cut ones it
+// leaves its sums in the workspace; the CTA adds those of its warps when all are done, and a second kernel those of the CTAs, in
+// their order.  (The warps of a CTA taking the tiles of one sequence in turn, with a join at its end, cost about 3 us a sequence:
+// 64 sequences of 500 to 8000 places, 64/8 heads of 128, 131 us.)  Where every sequence is short and head tiles are few, CTAs
+// have whole ones in turn, cut for their warps alone.  Nothing depends on timing, and nothing has to be zero before a call.
 #include "paged_common.cuh"
 
 namespace qmm {
@@ -22,38 +23,35 @@ namespace paged {
 
 namespace {
 
-constexpr int kRows = 16;   // query heads of a tile
-constexpr int kShort = 16;  // tiles of a sequence that is not cut while all are this short
+constexpr int kRows = 16;     // query heads of a tile
+constexpr int kShort = 512;   // places that a CTA's warps share rather than several CTAs
+constexpr int kSlots = 3;     // of a warp's ring: keys, values, the next keys
+constexpr int kTileBytes = 8192;
 
-// DP: the head dimension rounded up to 64, 128 or 256.  Shared memory of a CTA: the rings, 192 KiB, eight rows of sums of half
-// the warps, and a query tile.
+// DP: the head dimension rounded up to 64, 128 or 256.  Two CTAs an SM: 112, 112 and 96 KiB of shared memory each.
 template <int DP>
 struct Shape {
-    static constexpr int kKeys = DP == 256 ? 16 : 32;  // keys of a tile: 256 columns of sums leave no registers for 32 scores
-    static constexpr int kWarps = DP == 256 ? 2 : 4;
-    static constexpr int kSlots = DP == 256 ? 6 : DP == 128 ? 3 : 6;  // tiles of a warp's ring, keys and values in turn
-    static constexpr int kTileBytes = kKeys * DP * 2;
-    static constexpr int kHalf = kWarps / 2;
-    static constexpr int kPitch = DP + 8;  // floats of a row of sums: rows 8 banks apart
-    static constexpr int kRing = kWarps * kSlots * kTileBytes;
-    static constexpr int kSums = (kHalf * 8 * kPitch * 4 + 511) / 512 * 512;  // the query tile begins at a multiple of its rows
+    static constexpr int kKeys = kTileBytes / (2 * DP);  // of a tile
+    static constexpr int kWarps = DP == 256 ? 3 : 4;
     static constexpr int kQuery = kRows * DP * 2;
-    static constexpr int kStats = kHalf * 8 * 8;
-    static constexpr size_t kSmem = kRing + kSums + kQuery + kStats;
+    static constexpr size_t kSmem = kWarps * (kSlots * kTileBytes + kQuery);
 };
 
-// Workspace: part[CTA][2][rows][dim] sums, stat[CTA][2][rows] (maximum, sum), cut[index]: first and last CTA of a cut item, its
-// sequence and head tile (first < 0: not cut); by item where there are no more items than CTAs, else by the item's first CTA.
+// Workspace.  part[2 * warp + begins][rows][dim], stat[..][rows] (maximum, sum): what a warp has of a head tile that it has not
+// whole; `begins`: from its first place on.  Behind those of all warps, the same for the CTAs.  cut[index]: first and last CTA
+// of a head tile that no CTA has whole, its sequence and number (first < 0: none); by head tile where there are no more of them
+// than CTAs, else by the first CTA.
 struct Scratch {
     float *part;
     float2 *stat;
     int4 *cut;
     int rows, workers, by_item;
+    int64_t cta_parts;  // index of the first CTA's parts
 };
 
 struct Plan {
     int workers, rows, tiles;
-    int64_t items;
+    int64_t items, cta_parts;
     size_t part_bytes, stat_bytes, bytes;
 };
 
@@ -64,8 +62,10 @@ Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
     plan.rows = static_cast<int>(group < kRows ? group : kRows);
     plan.tiles = static_cast<int>((group + kRows - 1) / kRows);
     plan.items = batch * kv_heads * plan.tiles;
-    plan.part_bytes = static_cast<size_t>(plan.workers) * 2 * plan.rows * dim * sizeof(float);
-    plan.stat_bytes = (static_cast<size_t>(plan.workers) * 2 * plan.rows * sizeof(float2) + 15) / 16 * 16;
+    plan.cta_parts = 2ll * plan.workers * (dim > 128 ? Shape<256>::kWarps : Shape<128>::kWarps);
+    const size_t rows = static_cast<size_t>(plan.cta_parts + 2 * plan.workers) * plan.rows;
+    plan.part_bytes = rows * dim * sizeof(float);
+    plan.stat_bytes = (rows * sizeof(float2) + 15) / 16 * 16;
     plan.bytes = plan.part_bytes + plan.stat_bytes + static_cast<size_t>(plan.workers) * sizeof(int4);
     return plan;
 }
@@ -89,45 +89,26 @@ __device__ __forceinline__ Sequence sequence_of(const Problem &p, int b) {
     return s;
 }
 
-// A CTA's part of the list.
-struct Share {
-    int64_t end;    // whole: number of items; else: where the CTA's range ends
-    int64_t range;  // length of a range
-    int items;      // of a sequence
-    bool whole;     // items are not cut, CTA c has c, c + workers, ...
-};
-
-// What a CTA has of one item: tiles [from, to) of sequence b's item.
+// What a warp has of one head tile: tiles [from, to) of sequence b's item.
 struct Piece {
-    int64_t at;  // whole: the item's number; else: where the piece begins in the list
+    int64_t at;  // where the piece begins in the list
     int b, item, from, to;
     Sequence s;
 };
 
-// Steps to the CTA's next piece; false: there is none.
+// Steps to the next piece of a range that ends at `end`; false: there is none.
 template <int KEYS>
-__device__ __forceinline__ bool next_piece(const Problem &p, const Share &share, int workers, Piece &piece) {
-    if (share.whole) {
-        piece.at += workers;
-        if (piece.at >= share.end) return false;
-        const int b = static_cast<int>(piece.at / share.items);
-        piece.item = static_cast<int>(piece.at - static_cast<int64_t>(b) * share.items);
-        piece.b = b;
-        piece.s = sequence_of<KEYS>(p, b);
-        piece.from = 0;
-        piece.to = piece.s.tiles;
-        return true;
-    }
+__device__ __forceinline__ bool next_piece(const Problem &p, int64_t end, int items, Piece &piece) {
     piece.at += piece.to - piece.from;
-    if (piece.at >= share.end) return false;
-    if (++piece.item == share.items) {
+    if (piece.at >= end) return false;
+    if (++piece.item == items) {
         piece.item = 0;
         do {
             piece.s = sequence_of<KEYS>(p, ++piece.b);
         } while (piece.s.tiles == 0);
     }
     piece.from = 0;
-    piece.to = static_cast<int>(min(static_cast<int64_t>(piece.s.tiles), share.end - piece.at));
+    piece.to = static_cast<int>(min(static_cast<int64_t>(piece.s.tiles), end - piece.at));
     return true;
 }
 
@@ -173,27 +154,37 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// What a warp left of a head tile, for the CTA to add up.
+struct Part {
+    int valid, b, item, begins, ends, last;  // last: the CTA that has the head tile's last place
+};
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 2)
 decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
     using S = Shape<DP>;
     constexpr int KEYS = S::kKeys, kThreads = S::kWarps * 32;
-    constexpr int kChunks = DP / 8;  // 16-byte chunks of a row in shared memory
+    constexpr int kChunks = DP / 8;                    // 16-byte chunks of a row in shared memory
+    constexpr int kLooks = KEYS > 32 ? KEYS / 32 : 1;  // places of a tile that a lane looks up (16 keys: every place twice)
+    constexpr bool kKept = DP < 256;  // the query in registers; 256 columns of sums leave none
     extern __shared__ __align__(512) uint8_t smem[];  // rows of up to 512 bytes, stepped through by exclusive or
-    float *sums = reinterpret_cast<float *>(smem + S::kRing);
-    uint8_t *query = smem + S::kRing + S::kSums;
-    float2 *stats = reinterpret_cast<float2 *>(query + S::kQuery);
+    __shared__ Part s_parts[2 * S::kWarps];
     const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
     const int worker = blockIdx.x;
-    const uint32_t ring = smem_u32(smem) + warp * (S::kSlots * S::kTileBytes);
+    const uint32_t ring = smem_u32(smem) + warp * (kSlots * kTileBytes);
+    const uint32_t query = smem_u32(smem) + S::kWarps * (kSlots * kTileBytes) + warp * S::kQuery;
     pdl_launch_dependents();
     pdl_wait();
 
     const int tiles = (p.group + kRows - 1) / kRows;
+    const int items = p.kv_heads * tiles;
     const int ksteps = (p.dim + 15) / 16;
     const int row_chunks = p.dim / 8;
-    Share share;
-    share.items = p.kv_heads * tiles;
+    // The running maximum is one of unscaled scores, which takes a positive scale: a negative one's sign goes to the query, and
+    // for a scale of 0 the query is 0.
+    const float factor = p.scale * kLog2e;
+    const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
+    const uint32_t query_and = factor == 0.0f ? 0u : 0xffffffffu, query_xor = factor < 0.0f ? 0x80008000u : 0u;
 
     // the list's length, and whether all sequences are short
     int64_t total = 0;
@@ -207,401 +198,410 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         total += __shfl_xor_sync(0xffffffffu, total, o);
         longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
     }
-    total *= share.items;
-    share.whole = longest <= kShort;
-    Piece load;
-    load.b = load.item = load.from = load.to = 0;
+    total *= items;
+    const int64_t all_items = static_cast<int64_t>(p.batch) * items;
+    const bool whole = longest <= kShort / KEYS && all_items <= 2 * scratch.workers;
+    const int64_t range = (total + scratch.workers - 1) / scratch.workers;  // of a CTA
     if (!scratch.by_item && threadIdx.x == 0) scratch.cut[worker] = make_int4(-1, 0, 0, 0);
-    if (share.whole) {
-        share.end = static_cast<int64_t>(p.batch) * share.items;
-        share.range = 1;
-        load.at = worker - scratch.workers;
-        if (!next_piece<KEYS>(p, share, scratch.workers, load)) return;
-    } else {
-        share.range = max(static_cast<int64_t>(S::kWarps), (total + scratch.workers - 1) / scratch.workers);
-        const int64_t begin = worker * share.range;
-        share.end = min(total, begin + share.range);
-        int64_t before = 0;
-        bool found = false;
-        // sequences that see nothing, and where this CTA's range begins
-        for (int b0 = 0; b0 < p.batch; b0 += 32) {
-            const int b = b0 + lane;
-            const int n = b < p.batch ? sequence_of<KEYS>(p, b).tiles : 1;
-            if (warp == 0) {
-                for (uint32_t none = __ballot_sync(0xffffffffu, n == 0); none != 0; none &= none - 1) {
-                    const int e = b0 + __ffs(none) - 1;
-                    if (e % scratch.workers != worker) continue;
-                    for (int h = 0; h < p.heads; ++h) empty_row<T>(p, e, h);
-                    if (scratch.by_item)
-                        for (int i = lane; i < share.items; i += 32)
-                            scratch.cut[static_cast<int64_t>(e) * share.items + i] = make_int4(-1, 0, 0, 0);
-                }
-            }
-            if (found || begin >= share.end) continue;
-            const int64_t mine = b < p.batch ? static_cast<int64_t>(n) * share.items : 0;
-            int64_t sum = mine;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t left = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += left;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + sum > begin);
-            if (past == 0) {
-                before += __shfl_sync(0xffffffffu, sum, 31);
-                continue;
-            }
-            found = true;
-            load.b = b0 + __ffs(past) - 1;
-            before += __shfl_sync(0xffffffffu, sum - mine, __ffs(past) - 1);
-        }
-        if (!found) return;
-        load.s = sequence_of<KEYS>(p, load.b);
-        const int64_t in = begin - before;
-        load.at = begin;
-        load.item = static_cast<int>(in / load.s.tiles);
-        load.from = static_cast<int>(in - static_cast<int64_t>(load.item) * load.s.tiles);
-        load.to = static_cast<int>(min(static_cast<int64_t>(load.s.tiles), load.from + share.end - begin));
-    }
-    Piece piece = load;
 
-    // ---- loads: one place of the tile a lane (16 keys: lanes 16..31 the same again), keys and values of a tile apart ----
-    int at = load.from + warp;  // this warp's next tile of the piece that is being loaded
-    bool more = true;
-    auto settle = [&] {  // on to a piece that has a tile for this warp
-        while (more && at >= load.to) {
-            more = next_piece<KEYS>(p, share, scratch.workers, load);
-            at = load.from + warp;
-        }
-    };
-    settle();
-    int at_place = 0, entry = -1;
-    auto look_up = [&] {
-        entry = -1;
-        if (!more) return;
-        const int first = at < load.s.sink_tiles ? at * KEYS : (load.s.first + at - load.s.sink_tiles) * KEYS;
-        const int j = first + (lane & (KEYS - 1));
-        if (j < load.s.hi && (j < load.s.sink_end || j >= load.s.lo)) {
-            const int page = page_of(p, j);
-            at_place = j - page * p.page;
-            entry = __ldg(p.table + load.b * p.table_st + page);
-        }
-    };
-    look_up();
-    // every load of keys is followed by that of their values, so the lookup and the mask are kept for it
-    constexpr int kMasks = S::kSlots / 2 + 1;
-    uint32_t masks[kMasks];  // of the tiles under way, oldest first
-#pragma unroll
-    for (int i = 0; i < kMasks; ++i) masks[i] = 0;
-    int under_way = 0, slot = 0, value_place = 0, value_entry = 0, value_head = 0;
-    uint32_t value_seen = 0;
-    // A lane always has the same chunk, of rows kStep apart.  Rows of 16 places lie evenly apart where a page holds a multiple of
-    // 16 (tiles begin at multiples of 16), so a tile that is seen whole takes one address for 16 places; else each row its own.
-    constexpr int kStep = 32 / kChunks;
-    const int my_key = lane / kChunks, my_chunk = lane % kChunks;
-    const bool my_part = my_chunk < 2 * ksteps;
-    const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
-    const bool even = p.page % 16 == 0 && row_chunks == 2 * ksteps;
-    // the swizzled place of key kStep * i + my_key: chunk ^ key % 8, where the key's parts have no bits in common
-    const uint32_t my_dst = my_key * (DP * 2) + ((my_chunk ^ my_key) << 4);
-    auto copy_tile = [&](const void *cache, int64_t sb, int64_t st, int64_t sh, int id, int place, int kvh, uint32_t seen) {
-        const uint32_t dst = ring + slot * S::kTileBytes + my_dst;
-        const bool ok = seen >> lane & 1;
-        const int64_t offset = ok ? id * sb + place * st + kvh * sh : 0;
-        const T *base = static_cast<const T *>(cache) + my_offset;
-        if (even && seen == 0xffffffffu) {
-            const T *row[KEYS / 16];
-#pragma unroll
-            for (int h = 0; h < KEYS / 16; ++h) row[h] = base + __shfl_sync(0xffffffffu, offset, 16 * h) + my_key * st;
-            if (my_part) {
-#pragma unroll
-                for (int i = 0; i < KEYS / kStep; ++i) {
-                    const int first = kStep * i;
-                    cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row[first / 16], 16);
-                    row[first / 16] += kStep * st;
-                }
+    // one round for the CTA's range; where head tiles are whole, one for each that the CTA has
+    for (int64_t round = worker; round < (whole ? all_items : worker + 1); round += scratch.workers) {
+        if (threadIdx.x < 2 * S::kWarps) s_parts[threadIdx.x].valid = 0;
+        Piece load;
+        int64_t begin = 0, end = 0;
+        load.at = 0;
+        load.b = load.item = load.from = load.to = 0;
+        if (whole) {
+            load.b = static_cast<int>(round / items);
+            load.item = static_cast<int>(round - static_cast<int64_t>(load.b) * items);
+            load.s = sequence_of<KEYS>(p, load.b);
+            load.from = load.s.tiles * warp / S::kWarps;
+            load.to = load.s.tiles * (warp + 1) / S::kWarps;
+            end = load.to - load.from;
+            if (load.s.tiles == 0 && warp == 0) {
+                const int kvh = load.item / tiles, first = (load.item - kvh * tiles) * kRows;
+                for (int h = first; h < min(first + kRows, p.group); ++h) empty_row<T>(p, load.b, kvh * p.group + h);
             }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < KEYS / kStep; ++i) {
-            const int first = kStep * i, key = first + my_key;
-            const T *row = base + __shfl_sync(0xffffffffu, offset, key);
-            if (my_part)
-                cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row, my_chunk < row_chunks && (seen >> key & 1) ? 16 : 0);
-        }
-    };
-    auto load_keys = [&] {
-        if (more) {
-            value_seen = __ballot_sync(0xffffffffu, entry >= 0 && entry < p.pages);
-            value_place = at_place;
-            value_entry = entry;
-            value_head = load.item / tiles;
-#pragma unroll
-            for (int i = 0; i < kMasks; ++i)
-                if (i == under_way) masks[i] = value_seen;
-            ++under_way;
-            copy_tile(p.k, p.k_sb, p.k_st, p.k_sh, value_entry, value_place, value_head, value_seen);
-            at += S::kWarps;
-            settle();
-            look_up();
+            if (scratch.by_item && threadIdx.x == 0) scratch.cut[round] = make_int4(-1, 0, 0, 0);
         } else {
+            const int64_t cta_begin = min(total, worker * range), cta_end = min(total, cta_begin + range);
+            begin = cta_begin + (cta_end - cta_begin) * warp / S::kWarps;
+            end = cta_begin + (cta_end - cta_begin) * (warp + 1) / S::kWarps;
+            int64_t before = 0;
+            bool found = false;
+            // sequences that see nothing, and where this warp's range begins
+            for (int b0 = 0; b0 < p.batch; b0 += 32) {
+                const int b = b0 + lane;
+                const int n = b < p.batch ? sequence_of<KEYS>(p, b).tiles : 1;
+                if (warp == 0) {
+                    for (uint32_t none = __ballot_sync(0xffffffffu, n == 0); none != 0; none &= none - 1) {
+                        const int e = b0 + __ffs(none) - 1;
+                        if (e % scratch.workers != worker) continue;
+                        for (int h = 0; h < p.heads; ++h) empty_row<T>(p, e, h);
+                        if (scratch.by_item)
+                            for (int i = lane; i < items; i += 32) scratch.cut[static_cast<int64_t>(e) * items + i] = make_int4(-1, 0, 0, 0);
+                    }
+                }
+                if (found || begin >= end) continue;
+                const int64_t mine = b < p.batch ? static_cast<int64_t>(n) * items : 0;
+                int64_t sum = mine;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t left = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) sum += left;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, before + sum > begin);
+                if (past == 0) {
+                    before += __shfl_sync(0xffffffffu, sum, 31);
+                    continue;
+                }
+                found = true;
+                load.b = b0 + __ffs(past) - 1;
+                before += __shfl_sync(0xffffffffu, sum - mine, __ffs(past) - 1);
+            }
+            if (found) {
+                load.s = sequence_of<KEYS>(p, load.b);
+                const int64_t in = begin - before;
+                load.at = begin;
+                load.item = static_cast<int>(in / load.s.tiles);
+                load.from = static_cast<int>(in - static_cast<int64_t>(load.item) * load.s.tiles);
+                load.to = static_cast<int>(min(static_cast<int64_t>(load.s.tiles), load.from + end - begin));
+            }
+        }
+        Piece piece = load;
+        bool more = load.to > load.from;
+        bool working = more;
+        __syncthreads();  // the parts' flags are clear
+
+        // ---- loads: the query with a piece's first keys, then keys and values of a tile in turn ----
+        int at = load.from;
+        int at_place[kLooks], entry[kLooks];
+        auto look_up = [&] {
+            const int first = at < load.s.sink_tiles ? at * KEYS : (load.s.first + at - load.s.sink_tiles) * KEYS;
+#pragma unroll
+            for (int i = 0; i < kLooks; ++i) {
+                const int j = first + 32 * i + (lane & (KEYS - 1));
+                entry[i] = -1;
+                if (more && j < load.s.hi && (j < load.s.sink_end || j >= load.s.lo)) {
+                    const int page = page_of(p, j);
+                    at_place[i] = j - page * p.page;
+                    entry[i] = __ldg(p.table + load.b * p.table_st + page);
+                }
+            }
+        };
+        if (more) look_up();
+        int slot = 0, value_place[kLooks], value_entry[kLooks], value_head = -1;
+        uint32_t value_seen[kLooks], seen[kLooks];
+        // A lane always has the same chunk, of rows kStep apart.  Rows of 16 places lie evenly apart where a page holds a
+        // multiple of 16 (tiles begin at multiples of 16), so a tile that is seen whole takes one address for 16 places; else
+        // each row its own.
+        constexpr int kStep = 32 / kChunks;
+        const int my_key = lane / kChunks, my_chunk = lane % kChunks;
+        const bool my_part = my_chunk < 2 * ksteps;
+        const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
+        const bool even = p.page % 16 == 0 && row_chunks == 2 * ksteps;
+        // the swizzled place of key kStep * i + my_key: chunk ^ key % 8, where the key's parts have no bits in common
+        const uint32_t my_dst = my_key * (DP * 2) + ((my_chunk ^ my_key) << 4);
+        auto copy_tile = [&](const void *cache, int64_t sb, int64_t st, int64_t sh) {
+            const uint32_t dst = ring + slot * kTileBytes + my_dst;
+            int64_t offset[kLooks];
+            bool full = even;
+#pragma unroll
+            for (int l = 0; l < kLooks; ++l) {
+                offset[l] = value_seen[l] >> lane & 1 ? value_entry[l] * sb + value_place[l] * st + value_head * sh : 0;
+                full = full && value_seen[l] == 0xffffffffu;
+            }
+            const T *base = static_cast<const T *>(cache) + my_offset;
+            if (full) {
+                const T *row[KEYS / 16];
+#pragma unroll
+                for (int h = 0; h < KEYS / 16; ++h) row[h] = base + __shfl_sync(0xffffffffu, offset[h / 2], 16 * (h % 2)) + my_key * st;
+                if (my_part) {
+#pragma unroll
+                    for (int i = 0; i < KEYS / kStep; ++i) {
+                        const int first = kStep * i;
+                        cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row[first / 16], 16);
+                        row[first / 16] += kStep * st;
+                    }
+                }
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < KEYS / kStep; ++i) {
+                const int first = kStep * i, key = (first & 31) + my_key;
+                const T *row = base + __shfl_sync(0xffffffffu, offset[first / 32], key);
+                if (my_part)
+                    cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row,
+                                my_chunk < row_chunks && (value_seen[first / 32] >> key & 1) ? 16 : 0);
+            }
+        };
+        auto copy_query = [&] {
+            const int kvh = load.item / tiles, tile = load.item - kvh * tiles;
+            const int rows = min(kRows, p.group - tile * kRows);
+            const T *base = static_cast<const T *>(p.q) + load.b * p.q_st + (kvh * p.group + tile * kRows) * p.q_sh + my_offset;
+#pragma unroll
+            for (int i = 0; i < kRows / kStep; ++i) {
+                const int first = kStep * i, row = first + my_key;
+                if (my_part)
+                    cp_async_16(((query + my_dst) ^ ((first & 7) << 4)) + first * (DP * 2), base + (row < rows ? row * p.q_sh : 0),
+                                row < rows && my_chunk < row_chunks ? 16 : 0);
+            }
+        };
+        auto load_keys = [&] {
             value_head = -1;
-        }
-        cp_async_commit();
-        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-    };
-    auto load_values = [&] {
-        if (value_head >= 0) copy_tile(p.v, p.v_sb, p.v_st, p.v_sh, value_entry, value_place, value_head, value_seen);
-        cp_async_commit();
-        slot = slot + 1 == S::kSlots ? 0 : slot + 1;
-    };
-    static_assert(S::kSlots >= 3, "keys, values and the next keys");
+            if (more) {
+                if (at == load.from) copy_query();
 #pragma unroll
-    for (int i = 0; i < S::kSlots - 1; ++i) {
-        if (i % 2 == 0)
+                for (int l = 0; l < kLooks; ++l) {
+                    value_seen[l] = __ballot_sync(0xffffffffu, entry[l] >= 0 && entry[l] < p.pages);
+                    value_place[l] = at_place[l];
+                    value_entry[l] = entry[l];
+                }
+                value_head = load.item / tiles;
+                copy_tile(p.k, p.k_sb, p.k_st, p.k_sh);
+                if (++at == load.to) {
+                    more = next_piece<KEYS>(p, end, items, load);
+                    at = load.from;
+                }
+                look_up();
+            }
+            cp_async_commit();
+            slot = slot + 1 == kSlots ? 0 : slot + 1;
+        };
+        auto load_values = [&] {
+            if (value_head >= 0) copy_tile(p.v, p.v_sb, p.v_st, p.v_sh);
+            cp_async_commit();
+            slot = slot + 1 == kSlots ? 0 : slot + 1;
+        };
+        if (working) {
             load_keys();
-        else
             load_values();
-    }
-    // steps of one load each, in the order of the ring: the load that a step of the products makes room for
-    constexpr bool kKeysNext = (S::kSlots - 1) % 2 == 0;
-
-    // The running maximum is one of unscaled scores, which takes a positive scale: a negative one's sign goes to the query, and
-    // for a scale of 0 the query is 0.
-    const float factor = p.scale * kLog2e;
-    const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
-    const uint32_t query_and = factor == 0.0f ? 0u : 0xffffffffu, query_xor = factor < 0.0f ? 0x80008000u : 0u;
-
-    // ---- the query tile of the piece to come: loaded a piece ahead, stored when the warps meet ----
-    constexpr int kQueryChunks = kRows * kChunks / kThreads > 0 ? kRows * kChunks / kThreads : 1;
-    uint4 ahead[kQueryChunks];
-    auto load_query = [&](const Piece &of) {
-        const int kvh = of.item / tiles, tile = of.item - kvh * tiles;
-        const int rows = min(kRows, p.group - tile * kRows);
-        const T *base = static_cast<const T *>(p.q) + of.b * p.q_st + (kvh * p.group + tile * kRows) * p.q_sh;
-#pragma unroll
-        for (int i = 0; i < kQueryChunks; ++i) {
-            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, chunk = idx % kChunks;
-            ahead[i] = row < rows && chunk < row_chunks ? __ldg(reinterpret_cast<const uint4 *>(base + row * p.q_sh + chunk * 8))
-                                                        : make_uint4(0, 0, 0, 0);
         }
-    };
-    auto store_query = [&] {
-#pragma unroll
-        for (int i = 0; i < kQueryChunks; ++i) {
-            const int idx = i * kThreads + threadIdx.x, row = idx / kChunks, chunk = idx % kChunks;
-            if (row < kRows)
-                *reinterpret_cast<uint4 *>(query + row * (DP * 2) + ((chunk ^ (row & 7)) << 4)) =
-                    make_uint4((ahead[i].x & query_and) ^ query_xor, (ahead[i].y & query_and) ^ query_xor,
-                               (ahead[i].z & query_and) ^ query_xor, (ahead[i].w & query_and) ^ query_xor);
-        }
-    };
-    load_query(piece);
-    store_query();
-    __syncthreads();
 
-    // ---- products ----
-    const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-    int use_slot = 0;
-    while (true) {
-        Piece next = piece;
-        const bool another = next_piece<KEYS>(p, share, scratch.workers, next);
-        if (another) load_query(next);
+        // ---- products ----
+        const int r0 = lane >> 2, c0 = (lane & 3) * 2;
+        int use_slot = 0;
+        uint32_t q[kKept ? DP / 16 : 1][4];
         // ldmatrix addresses: chunk 2 i + c of a row swizzled by r is (2 i) ^ (c ^ r), so a step is one exclusive or
         auto query_part = [&](uint32_t (&r)[4], int ks) {
-            ldmatrix_x4(r, (smem_u32(query) + (lane & 15) * (DP * 2) + (((lane >> 4) ^ (lane & 7)) << 4)) ^ (ks << 5));
+            ldmatrix_x4(r, (query + (lane & 15) * (DP * 2) + (((lane >> 4) ^ (lane & 7)) << 4)) ^ (ks << 5));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = (r[i] & query_and) ^ query_xor;
         };
-        constexpr bool kKept = DP < 256;  // in registers; 256 columns of sums leave none
-        uint32_t q[kKept ? DP / 16 : 1][4];
-        if (kKept) {
+        while (working) {
+            float o[DP / 8][4];
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) query_part(q[kKept ? ks : 0], ks);
-        }
-        float o[DP / 8][4];
+            for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+            for (int g = piece.from; g < piece.to; ++g) {
+                // scores of 16 rows x KEYS keys: accumulators of 8 keys
+                float s[KEYS / 8][4];
 #pragma unroll
-        for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-
-        for (int g = piece.from + warp; g < piece.to; g += S::kWarps) {
-            // scores of 16 rows x KEYS keys: accumulators of 8 keys
-            float s[KEYS / 8][4];
+                for (int n = 0; n < KEYS / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+                cp_async_wait<kSlots - 2>();
+                __syncwarp();
+                bool all_seen = true;
 #pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            cp_async_wait<S::kSlots - 2>();
-            __syncwarp();
-            const uint32_t seen = masks[0];
-#pragma unroll
-            for (int i = 0; i + 1 < kMasks; ++i) masks[i] = masks[i + 1];
-            --under_way;
-            // into the slot that the step before this one used
-            if (kKeysNext) load_keys(); else load_values();
-            const uint32_t keys = ring + use_slot * S::kTileBytes + (((lane >> 4) << 3) + (lane & 7)) * (DP * 2) +
-                                  ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
-            use_slot = use_slot + 1 == S::kSlots ? 0 : use_slot + 1;
-#pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                if (ks >= ksteps) break;
-                uint32_t(&qk)[4] = q[kKept ? ks : 0];
-                if (!kKept) query_part(qk, ks);
-#pragma unroll
-                for (int n = 0; n < KEYS / 16; ++n) {
-                    uint32_t b[4];
-                    ldmatrix_x4(b, (keys ^ (ks << 5)) + n * 16 * (DP * 2));
-                    mma_16816<T>(s[2 * n], qk, b[0], b[1]);
-                    mma_16816<T>(s[2 * n + 1], qk, b[2], b[3]);
+                for (int l = 0; l < kLooks; ++l) {
+                    seen[l] = value_seen[l];
+                    all_seen = all_seen && seen[l] == 0xffffffffu;
                 }
-            }
-            if (seen != 0xffffffffu) {
+                if (kKept) {
+                    if (g == piece.from) {
+#pragma unroll
+                        for (int ks = 0; ks < DP / 16; ++ks) query_part(q[kKept ? ks : 0], ks);
+                    }
+                    load_keys();  // into the slot of the values before
+                }
+                const uint32_t keys = ring + use_slot * kTileBytes + (((lane >> 4) << 3) + (lane & 7)) * (DP * 2) +
+                                      ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+                use_slot = use_slot + 1 == kSlots ? 0 : use_slot + 1;
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ++ks) {
+                    if (ks >= ksteps) break;
+                    uint32_t(&qk)[4] = q[kKept ? ks : 0];
+                    if (!kKept) query_part(qk, ks);
+#pragma unroll
+                    for (int n = 0; n < KEYS / 16; ++n) {
+                        uint32_t b[4];
+                        ldmatrix_x4(b, (keys ^ (ks << 5)) + n * 16 * (DP * 2));
+                        mma_16816<T>(s[2 * n], qk, b[0], b[1]);
+                        mma_16816<T>(s[2 * n + 1], qk, b[2], b[3]);
+                    }
+                }
+                if (!kKept) {
+                    __syncwarp();  // the query may be overwritten
+                    load_keys();
+                }
+                if (!all_seen) {
+#pragma unroll
+                    for (int n = 0; n < KEYS / 8; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!(seen[n / 4] >> (n % 4 * 8 + c0 + (i & 1)) & 1)) s[n][i] = -INFINITY;
+                    }
+                }
+                float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(seen >> (n * 8 + c0 + (i & 1)) & 1)) s[n][i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i) most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
                 }
-            }
-            float most[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
-            }
-            bool moved = false;
-            float base[2], keep[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
-                most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
-                const float now = fmaxf(top[r], most[r]);
-                base[r] = now == -INFINITY ? 0.0f : now * scale;
-                keep[r] = exp2_fast(fmaf(top[r], scale, -base[r]));
-                moved |= now != top[r];
-                top[r] = now;
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int n = 0; n < DP / 8; ++n) {
-                    o[n][0] *= keep[0];
-                    o[n][1] *= keep[0];
-                    o[n][2] *= keep[1];
-                    o[n][3] *= keep[1];
-                }
-                sum[0] *= keep[0];
-                sum[1] *= keep[1];
-            }
-            // the weights, rounded to the type of the values (the sum takes them unrounded: 2^-9 or 2^-12 of each weight,
-            // independent of one another), as they lie are the second product's first operand
-            uint32_t a[KEYS / 16][4];
-#pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n) {
+                bool moved = false;
+                float base[2], keep[2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float e0 = exp2_fast(fmaf(s[n][2 * r], scale, -base[r])), e1 = exp2_fast(fmaf(s[n][2 * r + 1], scale, -base[r]));
-                    sum[r] += e0 + e1;
-                    a[n >> 1][(n & 1) * 2 + r] = pack2<T>(e0, e1);
+                    most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 1));
+                    most[r] = fmaxf(most[r], __shfl_xor_sync(0xffffffffu, most[r], 2));
+                    const float now = fmaxf(top[r], most[r]);
+                    base[r] = now == -INFINITY ? 0.0f : now * scale;
+                    keep[r] = exp2_fast(fmaf(top[r], scale, -base[r]));
+                    moved |= now != top[r];
+                    top[r] = now;
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n) {
+                        o[n][0] *= keep[0];
+                        o[n][1] *= keep[0];
+                        o[n][2] *= keep[1];
+                        o[n][3] *= keep[1];
+                    }
+                    sum[0] *= keep[0];
+                    sum[1] *= keep[1];
+                }
+                // the weights, rounded to the type of the values (the sum takes them unrounded: 2^-9 or 2^-12 of each weight,
+                // independent of one another), as they lie are the second product's first operand
+                uint32_t a[KEYS / 16][4];
+#pragma unroll
+                for (int n = 0; n < KEYS / 8; ++n) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float e0 = exp2_fast(fmaf(s[n][2 * r], scale, -base[r])), e1 = exp2_fast(fmaf(s[n][2 * r + 1], scale, -base[r]));
+                        sum[r] += e0 + e1;
+                        a[n >> 1][(n & 1) * 2 + r] = pack2<T>(e0, e1);
+                    }
+                }
+                cp_async_wait<kSlots - 2>();
+                __syncwarp();
+                load_values();  // into the slot of the keys
+                const uint32_t values = ring + use_slot * kTileBytes + ((((lane >> 3) & 1) << 3) + (lane & 7)) * (DP * 2) +
+                                        (((lane >> 4) ^ (lane & 7)) << 4);
+                use_slot = use_slot + 1 == kSlots ? 0 : use_slot + 1;
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n) {
+                    if (n >= ksteps) break;
+#pragma unroll
+                    for (int k = 0; k < KEYS / 16; ++k) {
+                        uint32_t b[4];
+                        ldmatrix_x4_trans(b, (values ^ (n << 5)) + k * 16 * (DP * 2));
+                        mma_16816<T>(o[2 * n], a[k], b[0], b[1]);
+                        mma_16816<T>(o[2 * n + 1], a[k], b[2], b[3]);
+                    }
                 }
             }
-            cp_async_wait<S::kSlots - 2>();
-            __syncwarp();
-            if (kKeysNext) load_values(); else load_keys();
-            const uint32_t values = ring + use_slot * S::kTileBytes + ((((lane >> 3) & 1) << 3) + (lane & 7)) * (DP * 2) +
-                                    (((lane >> 4) ^ (lane & 7)) << 4);
-            use_slot = use_slot + 1 == S::kSlots ? 0 : use_slot + 1;
-#pragma unroll
-            for (int n = 0; n < DP / 16; ++n) {
-                if (n >= ksteps) break;
-#pragma unroll
-                for (int k = 0; k < KEYS / 16; ++k) {
-                    uint32_t b[4];
-                    ldmatrix_x4_trans(b, (values ^ (n << 5)) + k * 16 * (DP * 2));
-                    mma_16816<T>(o[2 * n], a[k], b[0], b[1]);
-                    mma_16816<T>(o[2 * n + 1], a[k], b[2], b[3]);
-                }
-            }
-        }
 
-        // ---- the warps' sums, eight rows at a time: the upper half's to the lower half's, then what is left by all threads ----
-        const int kvh = piece.item / tiles, tile = piece.item - kvh * tiles;
-        const int head0 = kvh * p.group + tile * kRows;
-        const int rows = min(kRows, p.group - tile * kRows);
-        const bool begins = piece.from == 0, ends = piece.to == piece.s.tiles;
-        const int64_t slot_row = (worker * 2 + (begins ? 1 : 0)) * static_cast<int64_t>(scratch.rows);
+            // ---- the piece's end: rows to the outputs, or sums to the workspace ----
+            const int kvh = piece.item / tiles, tile = piece.item - kvh * tiles;
+            const int rows = min(kRows, p.group - tile * kRows);
+            const bool begins = piece.from == 0, ends = piece.to == piece.s.tiles;
+            const int64_t row0 = static_cast<int64_t>(piece.b) * p.heads + kvh * p.group + tile * kRows;
+            const int64_t part0 = ((static_cast<int64_t>(worker) * S::kWarps + warp) * 2 + begins) * scratch.rows;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (r * 8 >= rows) break;
-            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-            top[r] *= scale;
-            const int buffer = warp < S::kHalf ? warp : warp - S::kHalf;
-            float *mine = sums + (buffer * 8 + r0) * S::kPitch + c0;
-            float2 *my_stat = stats + buffer * 8 + r0;
-            auto put = [&] {
+            for (int r = 0; r < 2; ++r) {
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+                top[r] *= scale;
+                const int row = r0 + r * 8;
+                if (row >= rows) continue;
+                if (begins && ends) {
+                    const float inv = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+                    T *dst = static_cast<T *>(p.out) + (row0 + row) * p.dim;
 #pragma unroll
-                for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float2 *>(mine + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
-                if ((lane & 3) == 0) *my_stat = make_float2(top[r], sum[r]);
-            };
-            if (warp >= S::kHalf) put();
-            __syncthreads();
-            if (r == 0 && another) store_query();
-            if (warp < S::kHalf) {
-                const float2 other = *my_stat;
-                const float now = fmaxf(top[r], other.x), base = now == -INFINITY ? 0.0f : now;
-                const float keep = exp2_fast(top[r] - base), add = exp2_fast(other.x - base);
+                    for (int n = 0; n < DP / 8; ++n)
+                        if (n * 8 < p.dim)
+                            *reinterpret_cast<uint32_t *>(dst + n * 8 + c0) = pack2<T>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
+                    if ((lane & 3) == 0) p.lse[row0 + row] = sum[r] == 0.0f ? -INFINITY : top[r] * kLn2 + logf(sum[r]);
+                } else {
+                    float *dst = scratch.part + (part0 + row) * p.dim;
 #pragma unroll
-                for (int n = 0; n < DP / 8; ++n) {
-                    const float2 v = *reinterpret_cast<const float2 *>(mine + n * 8);
-                    o[n][2 * r] = fmaf(v.x, add, o[n][2 * r] * keep);
-                    o[n][2 * r + 1] = fmaf(v.y, add, o[n][2 * r + 1] * keep);
+                    for (int n = 0; n < DP / 8; ++n)
+                        if (n * 8 < p.dim) *reinterpret_cast<float2 *>(dst + n * 8 + c0) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+                    if ((lane & 3) == 0) scratch.stat[part0 + row] = make_float2(top[r], sum[r]);
                 }
-                sum[r] = fmaf(other.y, add, sum[r] * keep);
-                top[r] = now;
-                __syncwarp();  // a row's four lanes have read its statistics
-                put();
             }
-            __syncthreads();
-            for (int idx = threadIdx.x; idx < min(8, rows - r * 8) * (DP / 4); idx += kThreads) {
-                const int at_row = idx / (DP / 4), row = r * 8 + at_row, d = idx % (DP / 4) * 4;
-                if (d >= p.dim) continue;
-                float2 stat[S::kHalf];
+            if (lane == 0) {
+                if (!(begins && ends))
+                    s_parts[2 * warp + begins] = {1, piece.b, piece.item, begins, ends, whole ? worker : static_cast<int>((piece.at - piece.from + piece.s.tiles - 1) / range)};
+                else if (scratch.by_item && !whole)
+                    scratch.cut[static_cast<int64_t>(piece.b) * items + piece.item] = make_int4(-1, 0, 0, 0);
+            }
+            working = next_piece<KEYS>(p, end, items, piece);
+        }
+        cp_async_wait<0>();
+        __syncthreads();
+
+        // ---- the warps' parts: neighbours of one head tile are added in their order (a warp's second part is its last) ----
+        for (int i = 0; i < 2 * S::kWarps;) {
+            if (!s_parts[i].valid) {
+                ++i;
+                continue;
+            }
+            const Part head = s_parts[i];
+            int n = i;
+            bool ends = head.ends;
+            while (!ends && ++n < 2 * S::kWarps)
+                if (s_parts[n].valid) ends = s_parts[n].ends;
+            n = min(n + 1, 2 * S::kWarps);
+            const int kvh = head.item / tiles, tile = head.item - kvh * tiles;
+            const int rows = min(kRows, p.group - tile * kRows);
+            const int64_t first = static_cast<int64_t>(worker) * S::kWarps * 2;
+            const int64_t to_part = (scratch.cta_parts + 2 * worker + head.begins) * scratch.rows;
+            for (int idx = threadIdx.x; idx < rows * (p.dim / 4); idx += kThreads) {
+                const int row = idx / (p.dim / 4), d = (idx - row * (p.dim / 4)) * 4;
+                float2 stat[2 * S::kWarps];
+                float4 x[2 * S::kWarps];
                 float now = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < S::kHalf; ++w) {
-                    stat[w] = stats[w * 8 + at_row];
+                for (int w = 0; w < 2 * S::kWarps; ++w) {
+                    stat[w] = make_float2(-INFINITY, 0.0f);
+                    x[w] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (w >= i && w < n && s_parts[w].valid) {
+                        stat[w] = __ldcg(scratch.stat + (first + w) * scratch.rows + row);
+                        x[w] = __ldcg(reinterpret_cast<const float4 *>(scratch.part + ((first + w) * scratch.rows + row) * p.dim + d));
+                    }
                     now = fmaxf(now, stat[w].x);
                 }
                 const float base = now == -INFINITY ? 0.0f : now;
                 float all = 0.0f;
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int w = 0; w < S::kHalf; ++w) {
+                for (int w = 0; w < 2 * S::kWarps; ++w) {
                     const float weight = exp2_fast(stat[w].x - base);
-                    const float4 x = *reinterpret_cast<const float4 *>(sums + (w * 8 + at_row) * S::kPitch + d);
                     all = fmaf(stat[w].y, weight, all);
-                    v.x = fmaf(x.x, weight, v.x);
-                    v.y = fmaf(x.y, weight, v.y);
-                    v.z = fmaf(x.z, weight, v.z);
-                    v.w = fmaf(x.w, weight, v.w);
+                    v.x = fmaf(x[w].x, weight, v.x);
+                    v.y = fmaf(x[w].y, weight, v.y);
+                    v.z = fmaf(x[w].z, weight, v.z);
+                    v.w = fmaf(x[w].w, weight, v.w);
                 }
-                if (begins && ends) {
-                    const int64_t to = static_cast<int64_t>(piece.b) * p.heads + head0 + row;
+                if (head.begins && ends) {
+                    const int64_t to = static_cast<int64_t>(head.b) * p.heads + kvh * p.group + tile * kRows + row;
                     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
                     *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to * p.dim + d) =
                         make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
                     if (d == 0) p.lse[to] = all == 0.0f ? -INFINITY : now * kLn2 + logf(all);
                 } else {
-                    *reinterpret_cast<float4 *>(scratch.part + (slot_row + row) * p.dim + d) = v;
-                    if (d == 0) scratch.stat[slot_row + row] = make_float2(now, all);
+                    *reinterpret_cast<float4 *>(scratch.part + (to_part + row) * p.dim + d) = v;
+                    if (d == 0) scratch.stat[to_part + row] = make_float2(now, all);
                 }
             }
-            __syncthreads();  // before the buffers are written again
+            if (threadIdx.x == 0 && head.begins && !whole && (scratch.by_item || !ends)) {
+                scratch.cut[scratch.by_item ? static_cast<int64_t>(head.b) * items + head.item : worker] =
+                    make_int4(ends ? -1 : worker, head.last, head.b, head.item);
+            }
+            i = n;
         }
-        if (threadIdx.x == 0 && begins && (scratch.by_item || !ends)) {
-            const int last = ends ? 0 : static_cast<int>((piece.at + piece.s.tiles - 1) / share.range);
-            scratch.cut[scratch.by_item ? static_cast<int64_t>(piece.b) * share.items + piece.item : worker] =
-                make_int4(ends ? -1 : worker, last, piece.b, piece.item);
-        }
-        if (!another) break;
-        piece = next;
+        __syncthreads();
     }
-    cp_async_wait<0>();
 }
 
 // Joins the parts of the cut items, in the order of the CTAs.  share_parts (few items): a CTA has one row of an item and its
@@ -624,7 +624,7 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch s
     for (int row = share_parts ? static_cast<int>(blockIdx.y) : warp; row < rows; row += share_parts ? static_cast<int>(gridDim.y) : kJoinWarps) {
         const int from = share_parts ? static_cast<int>(static_cast<int64_t>(parts) * warp / kJoinWarps) : 0;
         const int to = share_parts ? static_cast<int>(static_cast<int64_t>(parts) * (warp + 1) / kJoinWarps) : parts;
-        auto place = [&](int i) { return (static_cast<int64_t>(cut.x + i) * 2 + (i == 0)) * scratch.rows + row; };
+        auto place = [&](int i) { return (scratch.cta_parts + static_cast<int64_t>(cut.x + i) * 2 + (i == 0)) * scratch.rows + row; };
         float top = -INFINITY;
         for (int i = from + lane; i < to; i += 32) top = fmaxf(top, scratch.stat[place(i)].x);
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -697,6 +697,8 @@ template <typename T, int DP>
 int launch(const Problem &p, const Plan &plan, Scratch scratch, cudaStream_t stream) {
     QMM_CUDA_OK(cudaFuncSetAttribute(decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<DP>::kSmem)));
     QMM_CUDA_OK(launch_pdl(decode_kernel<T, DP>, dim3(plan.workers), dim3(Shape<DP>::kWarps * 32), Shape<DP>::kSmem, stream, p, scratch));
+    // all sequences are short whatever their lengths are, and no head tile is cut
+    if (p.capacity <= kShort && plan.items <= 2 * plan.workers) return QMM_OK;
     const int64_t indices = scratch.by_item ? plan.items : plan.workers;
     const bool share_parts = indices * plan.rows <= 4 * plan.workers;
     QMM_CUDA_OK(launch_pdl(join_kernel<T>, dim3(static_cast<unsigned>(indices), share_parts ? plan.rows : 1), dim3(kJoinWarps * 32), 0,
@@ -729,6 +731,7 @@ int launch_decode(const Problem &p, int dtype, void *workspace, size_t workspace
     scratch.rows = plan.rows;
     scratch.workers = plan.workers;
     scratch.by_item = plan.items <= plan.workers;
+    scratch.cta_parts = plan.cta_parts;
     return dtype == QMM_DTYPE_BF16 ? launch_t<__nv_bfloat16>(p, plan, scratch, stream) : launch_t<__half>(p, plan, scratch, stream);
 }
 
