@@ -1,58 +1,8 @@
-// C entries of the attention over a paged key-value cache (npu_paged_attention, npu_paged_prompt_attention): argument checks
-// and the simplest kernel that is right, one warp a row.
+// C entries of the attention over a paged key-value cache (npu_paged_attention, npu_paged_prompt_attention): argument checks.
 #include "paged_common.cuh"
 
 namespace qmm {
 namespace paged {
-
-namespace {
-
-// The sequence of a token and the token's place in it; false: the token belongs to no sequence.
-__device__ __forceinline__ bool find_token(const Problem &p, int64_t token, int *b, int *place) {
-    if (p.start == nullptr) {
-        *b = static_cast<int>(token);
-        *place = p.lens[token] <= 0 ? -1 : p.lens[token] - 1;
-        return true;
-    }
-    for (int i = 0; i < p.batch; ++i) {
-        const int64_t first = p.start[i], end = p.start[i + 1];
-        if (token >= first && token < end) {
-            *b = i;
-            const int64_t at = p.lens[i] - (end - token);
-            *place = at < 0 ? -1 : static_cast<int>(at);
-            return true;
-        }
-    }
-    return false;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(128) plain_kernel(const __grid_constant__ Problem p) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= p.tokens * p.heads) return;
-    const int64_t token = row / p.heads;
-    const int head = static_cast<int>(row - token * p.heads);
-    int b = 0, place = 0;
-    if (find_token(p, token, &b, &place))
-        plain_row<T>(p, b, token, head, place);
-    else
-        empty_row<T>(p, token, head);
-}
-
-int launch_plain(const Problem &p, int dtype, cudaStream_t stream) {
-    const int64_t ctas = (p.tokens * p.heads + 3) / 4;
-    if (ctas > 0x7fffffff) return fail(QMM_ERR_UNSUPPORTED, "paged attention: too many tokens");
-    if (dtype == QMM_DTYPE_BF16)
-        plain_kernel<__nv_bfloat16><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(p);
-    else
-        plain_kernel<__half><<<static_cast<unsigned>(ctas), 128, 0, stream>>>(p);
-    QMM_CUDA_OK(cudaGetLastError());
-    return QMM_OK;
-}
-
-}  // namespace
-
-int launch_prompt(const Problem &p, int dtype, void *, size_t, cudaStream_t stream) { return launch_plain(p, dtype, stream); }
 
 static bool vectors(const void *base, int64_t a, int64_t b, int64_t c) {
     return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ((a | b | c) & 7) == 0;
@@ -153,7 +103,7 @@ int qmm_paged_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int
     QMM_REQUIRE(bytes != nullptr, "qmm_paged_prompt_attention_workspace_size: no result given");
     QMM_REQUIRE(tokens >= 0 && batch >= 0 && heads >= 0 && kv_heads >= 1 && dim >= 0 && max_places >= 0,
                 "qmm_paged_prompt_attention_workspace_size: sizes must be non-negative");
-    *bytes = 0;
+    *bytes = qmm::paged::prompt_workspace(tokens, batch, heads, kv_heads, dim, max_places);
     return QMM_OK;
 }
 

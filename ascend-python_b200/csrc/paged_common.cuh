@@ -59,8 +59,8 @@ __device__ __forceinline__ bool find_place(const Problem &p, int b, int j, int64
     return id >= 0 && id < p.pages;
 }
 
-// One row (token, head) by one warp, in fp32: the lanes take 32 keys at a time and their whole products, then all lanes add
-// the keys' values for the columns lane, lane + 32, ...  Reads visible keys alone.
+// The output of one row (token, head) by one warp, in fp32: the lanes take 32 keys at a time and their whole products, then all
+// lanes add the keys' values for the columns lane, lane + 32, ...  Reads visible keys alone.
 template <typename T>
 __device__ __noinline__ void plain_row(const Problem &p, int b, int64_t token, int head, int place) {
     constexpr int kMost = 8;  // columns a lane, dim <= 256
@@ -116,7 +116,6 @@ __device__ __noinline__ void plain_row(const Problem &p, int b, int64_t token, i
 #pragma unroll
     for (int i = 0; i < kMost; ++i)
         if (lane + 32 * i < p.dim) out[lane + 32 * i] = from_float<T>(acc[i] * inv);
-    if (lane == 0) p.lse[token * p.heads + head] = total == 0.0f ? -INFINITY : top + logf(total);
 }
 
 // A row that sees nothing, by one warp.
@@ -130,6 +129,7 @@ __device__ __forceinline__ void empty_row(const Problem &p, int64_t token, int h
 
 size_t decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
 int launch_decode(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+size_t prompt_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places);
 int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 
 }  // namespace paged

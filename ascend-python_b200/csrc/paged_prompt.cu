@@ -1,0 +1,750 @@
+// Attention of the last tokens of each sequence over a paged key-value cache (npu_paged_prompt_attention).
+//
+// Rows: the tokens of one sequence times the query heads of one key-value head, token by token, in tiles of 128; so a few tokens
+// of a wide group fill a tile as well as many of a narrow one, and every key that is read serves the whole group.
+//
+// For a block of BN keys, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory.  P, rounded to the
+// values' type, lies in the first half of the columns of its S, as the second product's operand in tensor memory.  The softmax
+// is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
+// maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.  Two row tiles share the keys
+// (dimensions up to 128): the tensor pipe works on one while the softmax works on the other.
+//
+// Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warp 8: MMA.  Warps 10 and 11: keys and values by cp.async,
+// half a tile each, whatever the pages' size and the strides; rows that no row of the CTA sees are zero-filled.  A key that
+// some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
+// come out not finite are looked at again (see mended).
+#include <type_traits>
+
+#include "paged_common.cuh"
+
+namespace qmm {
+namespace paged {
+
+namespace {
+
+constexpr int kThreads = 384;  // 168 registers each: the softmax has a row of 128 scores
+constexpr int kLoaders = 2;  // warps
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
+
+// DP: the head dimension rounded up to 64, 128 or 256.  256 columns of O leave room for one row tile; S is double-buffered then.
+template <int DP>
+struct Shape {
+    static constexpr int kTiles = DP == 256 ? 1 : 2;
+    static constexpr int kBN = DP == 256 ? 64 : 128;
+    static constexpr int kStages = DP == 64 ? 6 : 4;
+    static constexpr int kBoxes = DP / 64;                    // of 64 columns: 128-byte rows
+    static constexpr int kQueryBox = 128 * 128;               // bytes
+    static constexpr int kQuery = kTiles * kBoxes * kQueryBox;
+    static constexpr int kBox = kBN * 128;
+    static constexpr int kStage = kBoxes * kBox;
+    static constexpr int kS = DP == 256 ? 64 : 128;           // columns between the two S
+    static constexpr int kO = 256;                            // first column of O
+    static constexpr int kRows = kTiles * 128;
+};
+
+constexpr int kValid = 8;  // blocks whose masks are kept: more than may be under way
+struct Tail {
+    uint64_t full[6], empty[6];
+    uint64_t q_full, s_full[2], p_full[2], o_done[2];
+    uint32_t valid[kValid][4];
+    uint32_t tmem_base, abort_flag;
+};
+template <int DP>
+constexpr size_t smem_bytes() {
+    return 1024 + Shape<DP>::kQuery + Shape<DP>::kStages * Shape<DP>::kStage + sizeof(Tail);
+}
+
+// Workspace (splits > 1): part[split][token * heads + head][dim], stat[split][..] (base, sum).
+struct Scratch {
+    float *part;
+    float2 *stat;
+    int splits;
+    uint32_t *status;
+};
+
+struct Plan {
+    int64_t pairs;  // at most
+    int splits;
+    size_t part_bytes, bytes;
+};
+
+// The tiles of a call are known on the device alone; what the host knows bounds them.  Few tiles are split over the cache.
+Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places) {
+    Plan plan;
+    const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
+    const int rows = dim > 128 ? Shape<256>::kRows : Shape<128>::kRows;
+    plan.pairs = tokens * group / rows + (batch < tokens ? batch : tokens);
+    plan.splits = 1;
+    const int64_t ctas = plan.pairs * kv_heads, sms = sm_count();
+    if (ctas > 0 && ctas < 2 * sms) {
+        const int64_t most = places / 512;
+        int64_t s = (4 * sms + ctas - 1) / ctas;
+        s = s < most ? s : most;
+        plan.splits = static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+    }
+    const size_t all = plan.splits > 1 ? static_cast<size_t>(plan.splits) * tokens * heads : 0;
+    plan.part_bytes = all * dim * sizeof(float);
+    plan.bytes = plan.part_bytes + all * sizeof(float2);
+    return plan;
+}
+
+// A sequence's new tokens: their first row in the query, how many, and the place of the first.
+struct Tokens {
+    int64_t first;
+    int count, place;
+};
+__device__ __forceinline__ Tokens tokens_of(const Problem &p, int b) {
+    const int64_t from = min(max(static_cast<int64_t>(__ldg(p.start + b)), static_cast<int64_t>(0)), p.tokens);
+    const int64_t to = min(max(static_cast<int64_t>(__ldg(p.start + b + 1)), static_cast<int64_t>(0)), p.tokens);
+    Tokens t;
+    t.first = from;
+    t.count = static_cast<int>(max(to - from, static_cast<int64_t>(0)));
+    const int64_t place = static_cast<int64_t>(__ldg(p.lens + b)) - t.count;
+    t.place = static_cast<int>(max(place, -static_cast<int64_t>(0x7fffffff)));
+    return t;
+}
+
+// A CTA's rows: `first` + i, token first / group and so on; the places that any of them sees, as blocks.
+struct Item {
+    Tokens tokens;
+    int b, kvh;
+    int64_t first, rows;  // of the sequence's rows: this CTA's first, and all
+    int sink_end, lo, hi;
+    int sink_blocks, first_block, blocks;
+};
+
+__device__ __forceinline__ int place_of(const Problem &p, const Tokens &t, int64_t row) {
+    const int64_t at = t.place + row / p.group;
+    return at < 0 ? -1 : static_cast<int>(at);
+}
+
+template <int BN, int ROWS>
+__device__ __forceinline__ void cover(const Problem &p, Item &it) {
+    const int64_t last = min(it.rows, it.first + ROWS) - 1;
+    const Range a = visible_range(p, place_of(p, it.tokens, it.first)), z = visible_range(p, place_of(p, it.tokens, last));
+    it.sink_end = z.sink_end;
+    it.lo = a.lo;
+    it.hi = z.hi;
+    it.sink_blocks = (z.sink_end + BN - 1) / BN;
+    it.first_block = max(a.lo / BN, it.sink_blocks);
+    it.blocks = it.sink_blocks + max(0, z.hi / BN + (z.hi % BN != 0) - it.first_block);
+}
+
+// The `pair`-th tile (pair) of the call, by one warp: sequences in order, a sequence's last tile, which sees most, first.
+template <int BN, int ROWS>
+__device__ __forceinline__ bool find_item(const Problem &p, int64_t pair, Item &it) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int b = b0 + lane;
+        int64_t n = 0;
+        if (b < p.batch) n = (static_cast<int64_t>(tokens_of(p, b).count) * p.group + ROWS - 1) / ROWS;
+        int64_t sum = n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t left = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += left;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + sum > pair);
+        if (past == 0) {
+            before += __shfl_sync(0xffffffffu, sum, 31);
+            continue;
+        }
+        const int which = __ffs(past) - 1;
+        it.b = b0 + which;
+        it.tokens = tokens_of(p, it.b);
+        it.rows = static_cast<int64_t>(it.tokens.count) * p.group;
+        const int64_t end = before + __shfl_sync(0xffffffffu, sum, which);
+        it.first = (end - 1 - pair) * ROWS;
+        cover<BN, ROWS>(p, it);
+        return true;
+    }
+    return false;
+}
+
+template <int BN>
+__device__ __forceinline__ int block_start(const Item &it, int i) {
+    return (i < it.sink_blocks ? i : it.first_block + i - it.sink_blocks) * BN;
+}
+
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(const uint4 &v) {
+    const uint32_t mask = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (w[i] & mask) == mask || (w[i] >> 16 & mask) == mask;
+    return bad;
+}
+
+// Whether a value of places [from, to) of the sequence is not finite, by one warp.
+template <typename T>
+__device__ __noinline__ bool holds_not_finite(const Problem &p, int b, int kvh, int from, int to) {
+    const int lane = threadIdx.x & 31;
+    bool bad = false;
+    for (int j = from; j < to; ++j) {
+        int64_t block;
+        int at;
+        if (!find_place(p, b, j, &block, &at)) continue;
+        const T *row = static_cast<const T *>(p.v) + block * p.v_sb + at * p.v_st + kvh * p.v_sh;
+        for (int c = lane * 8; c < p.dim; c += 256) bad |= any_not_finite<T>(__ldg(reinterpret_cast<const uint4 *>(row + c)));
+    }
+    return __any_sync(0xffffffffu, bad);
+}
+
+// Whether rows whose places are `low` to `high` may have met a value that is not finite at a place that they do not see but that
+// the CTA's other rows do.
+template <typename T>
+__device__ __forceinline__ bool met_not_finite(const Problem &p, const Item &it, int low, int high) {
+    const Range a = visible_range(p, low), z = visible_range(p, high);
+    if (holds_not_finite<T>(p, it.b, it.kvh, a.hi, it.hi)) return true;
+    if (holds_not_finite<T>(p, it.b, it.kvh, a.sink_end, min(it.sink_end, it.hi))) return true;
+    return holds_not_finite<T>(p, it.b, it.kvh, max(it.lo, a.sink_end), min(z.lo, it.hi));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Bits [from, to) of a word, the bounds being any numbers.
+__device__ __forceinline__ uint32_t bits(int from, int to) {
+    const uint32_t low = to <= 0 ? 0u : to >= 32 ? 0xffffffffu : (1u << to) - 1;
+    return from <= 0 ? low : from >= 32 ? 0u : low & (0xffffffffu << from);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
+    using S = Shape<DP>;
+    constexpr int BN = S::kBN;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
+    Tail *tail = reinterpret_cast<Tail *>(smem + S::kQuery + S::kStages * S::kStage);
+    volatile uint32_t *abort_flag = &tail->abort_flag;
+    const uint32_t ring = smem_base + S::kQuery;
+    const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(smem_u32(&tail->full[s]), kLoaders);
+            mbar_init(smem_u32(&tail->empty[s]), 1);
+        }
+        mbar_init(smem_u32(&tail->q_full), 4 * S::kTiles);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&tail->s_full[i]), 1);
+            mbar_init(smem_u32(&tail->p_full[i]), 4);
+            mbar_init(smem_u32(&tail->o_done[i]), 1);
+        }
+        tail->abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(smem_u32(&tail->tmem_base), 512);
+        tmem_relinquish();
+        pdl_launch_dependents();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = warp_uniform(tail->tmem_base);
+    pdl_wait();
+
+    // tokens of no sequence
+    {
+        const int64_t head = p.batch > 0 ? min(max(static_cast<int64_t>(__ldg(p.start)), static_cast<int64_t>(0)), p.tokens) : p.tokens;
+        const int64_t end = p.batch > 0 ? min(max(static_cast<int64_t>(__ldg(p.start + p.batch)), head), p.tokens) : p.tokens;
+        const int64_t none = head + p.tokens - end;
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp; i < none; i += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+            const int64_t token = i < head ? i : end + i - head;
+            for (int h = 0; h < p.heads; ++h) empty_row<T>(p, token, h);
+            if (scratch.splits > 1)
+                for (int64_t h = lane; h < static_cast<int64_t>(p.heads) * scratch.splits; h += 32)
+                    scratch.stat[h / p.heads * p.tokens * p.heads + token * p.heads + h % p.heads] = make_float2(-INFINITY, 0.0f);
+        }
+    }
+
+    const int split = blockIdx.x % scratch.splits;
+    Item it;
+    it.kvh = blockIdx.x / scratch.splits % p.kv_heads;
+    const bool found = find_item<BN, S::kRows>(p, blockIdx.x / scratch.splits / p.kv_heads, it);
+    const int begin = found ? static_cast<int>(static_cast<int64_t>(it.blocks) * split / scratch.splits) : 0;
+    const int end = found ? static_cast<int>(static_cast<int64_t>(it.blocks) * (split + 1) / scratch.splits) : 0;
+    const bool two = S::kTiles == 2 && found && it.first + 128 < it.rows;  // the second row tile has rows
+    const int ksteps = (p.dim + 15) / 16;
+    const float factor = p.scale * kLog2e;
+
+    if (!found) {
+        // nothing to do
+    } else if (warp >= 10) {
+        // ---------------- keys and values ----------------
+        const int loader = warp - 10;
+        constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
+        constexpr int kMine = BN / kLoaders, kLooks = kMine / 32;  // rows of a tile, places a lane looks up
+        const int my_key = lane / kChunks, my_chunk = lane % kChunks;
+        const int row_chunks = p.dim / 8;
+        const bool my_part = my_chunk < 2 * ksteps;
+        const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
+        const uint32_t my_box = (my_chunk / 8) * S::kBox;
+        uint32_t stage = 0, phase = 0, waiting = 0, signal = 0;  // `waiting` stages from `signal` on are under way
+        bool ok = true;
+        auto arrive = [&] {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tail->full[signal]));
+            signal = signal + 1 == S::kStages ? 0 : signal + 1;
+            --waiting;
+        };
+        for (int i = begin; i < end && ok; ++i) {
+            const int first = block_start<BN>(it, i) + loader * kMine;
+            uint32_t mask[kLooks];
+            int64_t k_offset[kLooks], v_offset[kLooks];
+#pragma unroll
+            for (int l = 0; l < kLooks; ++l) {
+                const int j = first + 32 * l + lane;
+                int64_t block = 0;
+                int at = 0;
+                const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at);
+                mask[l] = __ballot_sync(0xffffffffu, seen);
+                k_offset[l] = seen ? block * p.k_sb + at * p.k_st + it.kvh * p.k_sh : 0;
+                v_offset[l] = seen ? block * p.v_sb + at * p.v_st + it.kvh * p.v_sh : 0;
+            }
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                if (!mbar_try_wait(smem_u32(&tail->empty[stage]), phase ^ 1)) {
+                    // the MMA may wait for a tile that is under way
+                    cp_async_wait<0>();
+                    while (waiting > 0) arrive();
+                    ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
+                    if (!ok) break;
+                }
+                if (part == 0 && lane == 0) {
+#pragma unroll
+                    for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][loader * kLooks + l] = mask[l];
+                }
+                const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
+                const uint32_t dst = ring + stage * S::kStage + my_box + loader * (kMine * 128);
+#pragma unroll
+                for (int r = 0; r < kMine / kStep; ++r) {
+                    const int l = r * kStep / 32, key = r * kStep % 32 + my_key;
+                    const T *row = base + __shfl_sync(0xffffffffu, part == 0 ? k_offset[l] : v_offset[l], key);
+                    if (my_part)
+                        cp_async_16(dst + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
+                                    my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
+                }
+                cp_async_commit();
+                ++waiting;
+                if (++stage == S::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+                if (waiting == 3) {
+                    cp_async_wait<2>();
+                    arrive();
+                }
+            }
+        }
+        cp_async_wait<0>();
+        while (waiting > 0) arrive();
+    } else if (warp == 8) {
+        // ---------------- MMA ----------------
+        constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        constexpr uint32_t kHi = smem_desc_hi_sw128(1024);
+        constexpr uint32_t s_desc = make_idesc(1, kFmt, kFmt, 0, 0, 128, BN);
+        const uint32_t o_desc = make_idesc(1, kFmt, kFmt, 0, 1, 128, ksteps * 16);
+        const int blocks = end - begin;
+        uint32_t k_stage = 0, k_phase = 0;  // stages: keys, values, keys, ...
+        auto product_s = [&](int tile, int buffer, uint32_t stage) {
+            const uint32_t a = smem_desc_lo(smem_base + tile * (S::kBoxes * S::kQueryBox), 16), b = smem_desc_lo(ring + stage * S::kStage, 16);
+            for (int k = 0; k < ksteps; ++k)
+                mma_f16_ss_warp(tmem_base + buffer * S::kS, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
+                                desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
+        };
+        // 16 keys a step: eight columns of P; 16 rows of 128 bytes of V, its next 64 columns a box further
+        auto product_o = [&](int tile, int buffer, uint32_t stage, bool first) {
+            const uint32_t b = smem_desc_lo(ring + stage * S::kStage, S::kBox);
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+                mma_f16_ts_warp(tmem_base + S::kO + tile * 128, tmem_base + buffer * S::kS + k * 8, desc64(b + k * (2048 >> 4), kHi), o_desc,
+                                !first || k > 0);
+        };
+        bool ok = blocks > 0 && mbar_wait(smem_u32(&tail->q_full), 0, abort_flag, 0x91);
+        if (S::kTiles == 2) {
+            for (int i = 0; i <= blocks && ok; ++i) {
+                const uint32_t v_stage = (2 * i + S::kStages - 1) % S::kStages;  // of the block before
+                const uint32_t v_phase = ((2 * i - 1) / S::kStages) & 1;
+                if (i < blocks) ok = mbar_wait(smem_u32(&tail->full[k_stage]), k_phase, abort_flag, 0x92);
+                if (ok && i > 0) ok = mbar_wait(smem_u32(&tail->full[v_stage]), v_phase, abort_flag, 0x93);
+                for (int tile = 0; tile < 2 && ok; ++tile) {
+                    if (tile == 1 && !two) break;
+                    if (i > 0) {
+                        ok = mbar_wait(smem_u32(&tail->p_full[tile]), (i - 1) & 1, abort_flag, 0x94);
+                        if (!ok) break;
+                        tc_fence_after();
+                        product_o(tile, tile, v_stage, i == 1);
+                        if (i == blocks) tc_commit_warp(smem_u32(&tail->o_done[tile]));
+                    }
+                    if (i < blocks) {
+                        tc_fence_after();
+                        product_s(tile, tile, k_stage);
+                        tc_commit_warp(smem_u32(&tail->s_full[tile]));
+                    }
+                }
+                if (ok && i > 0) tc_commit_warp(smem_u32(&tail->empty[v_stage]));
+                if (ok && i < blocks) tc_commit_warp(smem_u32(&tail->empty[k_stage]));
+                k_stage += 2;
+                if (k_stage >= S::kStages) {
+                    k_stage -= S::kStages;
+                    k_phase ^= 1;
+                }
+            }
+        } else {
+            for (int i = 0; i <= blocks && ok; ++i) {
+                if (i < blocks) {
+                    ok = mbar_wait(smem_u32(&tail->full[k_stage]), k_phase, abort_flag, 0x95);
+                    if (!ok) break;
+                    tc_fence_after();
+                    product_s(0, i & 1, k_stage);
+                    tc_commit_warp(smem_u32(&tail->s_full[i & 1]));
+                    tc_commit_warp(smem_u32(&tail->empty[k_stage]));
+                }
+                if (i > 0) {
+                    const uint32_t v_stage = (2 * i + S::kStages - 1) % S::kStages, v_phase = ((2 * i - 1) / S::kStages) & 1;
+                    ok = mbar_wait(smem_u32(&tail->full[v_stage]), v_phase, abort_flag, 0x96) &&
+                         mbar_wait(smem_u32(&tail->p_full[0]), (i - 1) & 1, abort_flag, 0x97);
+                    if (!ok) break;
+                    tc_fence_after();
+                    product_o(0, (i - 1) & 1, v_stage, i == 1);
+                    tc_commit_warp(smem_u32(&tail->o_done[(i - 1) & 1]));
+                    tc_commit_warp(smem_u32(&tail->empty[v_stage]));
+                }
+                k_stage += 2;
+                if (k_stage >= S::kStages) {
+                    k_stage -= S::kStages;
+                    k_phase ^= 1;
+                }
+            }
+        }
+    } else if (warp < 4 * S::kTiles) {
+        // ---------------- softmax and epilogue: a row a thread ----------------
+        const int tile = warp >> 2;
+        const int64_t row0 = it.first + warp * 32;  // this warp's first row
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        if (end > begin) {
+            // the warp's rows of the query: 16-byte chunks into 128-byte rows, swizzled; the scale's sign and zero go with them
+            const uint32_t with = factor == 0.0f ? 0u : 0xffffffffu, flip = factor < 0.0f ? 0x80008000u : 0u;
+            constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
+            const int chunk = lane % kChunks;
+            uint8_t *dst = smem + (tile * S::kBoxes + chunk / 8) * S::kQueryBox;
+#pragma unroll 4
+            for (int r = 0; r < 32 / kStep; ++r) {
+                const int local = r * kStep + lane / kChunks, row = (warp & 3) * 32 + local;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row0 + local < it.rows && chunk * 8 < p.dim) {
+                    const int64_t token = (row0 + local) / p.group;
+                    const int head = it.kvh * p.group + static_cast<int>(row0 + local - token * p.group);
+                    v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (it.tokens.first + token) * p.q_st + head * p.q_sh + chunk * 8));
+                }
+                if (chunk < 2 * ksteps)
+                    *reinterpret_cast<uint4 *>(dst + row * 128 + (((chunk ^ row) & 7) << 4)) =
+                        make_uint4((v.x & with) ^ flip, (v.y & with) ^ flip, (v.z & with) ^ flip, (v.w & with) ^ flip);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tail->q_full));
+        }
+        const int64_t my_row = row0 + lane;
+        const bool mine = my_row < it.rows;
+        const int place = mine ? place_of(p, it.tokens, my_row) : -1;
+        const Range range = visible_range(p, place);
+        // what all rows of the warp see: below `common_sink`, and from `common_lo` to `common_hi`
+        const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
+        const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
+        const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
+        float base = -INFINITY;  // unscaled
+        float2 sum2 = make_float2(0.0f, 0.0f);
+        bool ok = true;
+        const bool works = end > begin && (tile == 0 || two);
+        for (int i = begin; i < end && works && ok; ++i) {
+            const int n = i - begin;
+            const int buffer = S::kTiles == 2 ? tile : n & 1;
+            ok = mbar_wait(smem_u32(&tail->s_full[buffer]), S::kTiles == 2 ? n & 1 : (n >> 1) & 1, abort_flag, 0x98);
+            if (!ok) break;
+            tc_fence_after();
+            // one row tile: a barrier for even and one for odd blocks, each waited for in every phase, so that a phase's parity
+            // is its own
+            if (S::kTiles == 1 && n > 1) ok = mbar_wait(smem_u32(&tail->o_done[n & 1]), ((n - 2) >> 1) & 1, abort_flag, 0x9b);
+            if (!ok) break;
+            const uint32_t s_addr = tmem_base + lanes + buffer * S::kS;
+            uint32_t s[BN / 32][32];
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_addr + c * 32, s[c]);
+            tmem_ld_wait();
+            const int start = block_start<BN>(it, i);
+            uint32_t valid[BN / 32];
+            bool all = start + BN <= first_range.sink_end || (start >= last_range.lo && start + BN <= first_range.hi);
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) {
+                valid[c] = tail->valid[i % kValid][c];
+                all = all && valid[c] == 0xffffffffu;
+            }
+            if (!all) {
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) {
+                    const int at = start + c * 32;
+                    const uint32_t see = valid[c] & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (!(see >> j & 1)) s[c][j] = 0xff800000u;  // -inf
+                }
+            }
+            float most = -INFINITY, most2 = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < BN; j += 2) {
+                most = fmaxf(most, __uint_as_float(s[j / 32][j % 32]));
+                most2 = fmaxf(most2, __uint_as_float(s[j / 32][j % 32 + 1]));
+            }
+            most = fmaxf(most, most2);
+            const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+            if (__any_sync(0xffffffffu, move)) {
+                const float now = move ? most : base;
+                const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                sum2.x *= keep;
+                sum2.y *= keep;
+                if (n > 0) {
+                    if (S::kTiles == 1) {  // the other tiles' S are behind their O in order
+                        ok = mbar_wait(smem_u32(&tail->o_done[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, 0x99);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    for (int c = 0; c < ksteps; ++c) {
+                        uint32_t o[16];
+                        const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
+                        tmem_ld_32x16(addr, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                        tmem_st_32x16(addr, o);
+                    }
+                }
+                base = now;
+            }
+            const float offset = base == -INFINITY ? 0.0f : -base * scale;
+            const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+            // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another; the sum
+            // takes the weights unrounded
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
+                    const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                    sum2 = add2(sum2, e);
+                    w[j] = pack2<T>(e.x, e.y);
+                }
+                tmem_st_32x16(s_addr + c * 16, w);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile]));
+        }
+        const float sum = sum2.x + sum2.y;
+        const float top = base * scale;
+        const int64_t token = my_row / p.group;
+        const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
+        const int64_t out_row = (it.tokens.first + token) * p.heads + head;
+        if (works && ok) {
+            const int last = end - begin - 1;
+            ok = mbar_wait(smem_u32(&tail->o_done[S::kTiles == 2 ? tile : last & 1]), S::kTiles == 2 ? 0 : (last >> 1) & 1, abort_flag, 0x9a);
+            tc_fence_after();
+        }
+        if (scratch.splits > 1) {
+            const int64_t at = (static_cast<int64_t>(split) * p.tokens * p.heads) + out_row;
+            if (mine) scratch.stat[at] = make_float2(top, sum);
+            for (int c = 0; c < ksteps && works && ok; ++c) {
+                uint32_t o[16];
+                tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
+                tmem_ld_wait();
+                if (mine) {
+                    float *dst = scratch.part + at * p.dim + c * 16;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4)
+                        if (c * 16 + j < p.dim) *reinterpret_cast<uint4 *>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
+                __syncwarp();
+            }
+        } else {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            bool bad = false;
+            for (int c = 0; c < ksteps; ++c) {
+                uint32_t o[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] = 0;
+                if (works && ok) {
+                    tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
+                    tmem_ld_wait();
+                }
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float a = __uint_as_float(o[2 * j]), b = __uint_as_float(o[2 * j + 1]);
+                    bad |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
+                    w[j] = pack2<T>(a * inv, b * inv);
+                }
+                if (mine) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + out_row * p.dim + c * 16);
+                    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (c * 16 + 8 < p.dim) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+                __syncwarp();
+            }
+            if (mine) p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+            // rows that are not finite although their weights are
+            uint32_t again = __ballot_sync(0xffffffffu, mine && bad && sum == sum);
+            if (again != 0 && met_not_finite<T>(p, it, low, high)) {
+                __syncwarp();
+                for (; again != 0; again &= again - 1) {
+                    const int64_t row = row0 + __ffs(again) - 1, t = row / p.group;
+                    plain_row<T>(p, it.b, it.tokens.first + t, it.kvh * p.group + static_cast<int>(row - t * p.group),
+                                 place_of(p, it.tokens, row));
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && tail->abort_flag != 0 && scratch.status != nullptr) atomicMax(scratch.status, tail->abort_flag);
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// Joins the splits of a row, in their order: a warp a row.
+template <typename T, int BN, int ROWS>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), rows = p.tokens * p.heads;
+    if (row >= rows) return;
+    float top = -INFINITY;
+    for (int i = lane; i < scratch.splits; i += 32) top = fmaxf(top, scratch.stat[i * rows + row].x);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, acc[8] = {};
+    for (int i0 = 0; i0 < scratch.splits; i0 += 32) {
+        float weight = 0.0f;
+        bool any = false;
+        if (i0 + lane < scratch.splits) {
+            const float2 st = scratch.stat[(i0 + lane) * rows + row];
+            weight = exp2_fast(st.x - base);
+            sum = fmaf(st.y, weight, sum);
+            any = st.y != 0.0f;  // a split without blocks has written no part
+        }
+        const uint32_t has = __ballot_sync(0xffffffffu, any);
+#pragma unroll 4
+        for (int i = 0; i < min(32, scratch.splits - i0); ++i) {
+            const float w = __shfl_sync(0xffffffffu, weight, i);
+            if (!(has >> i & 1)) continue;
+            const float *src = scratch.part + ((i0 + i) * rows + row) * p.dim;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int d = c * 128 + lane * 4;
+                if (d < p.dim) {
+                    const float4 v = *reinterpret_cast<const float4 *>(src + d);
+                    acc[4 * c] = fmaf(v.x, w, acc[4 * c]);
+                    acc[4 * c + 1] = fmaf(v.y, w, acc[4 * c + 1]);
+                    acc[4 * c + 2] = fmaf(v.z, w, acc[4 * c + 2]);
+                    acc[4 * c + 3] = fmaf(v.w, w, acc[4 * c + 3]);
+                }
+            }
+        }
+    }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T *dst = static_cast<T *>(p.out) + row * p.dim;
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int d = c * 128 + lane * 4;
+        if (d < p.dim)
+            *reinterpret_cast<uint2 *>(dst + d) = make_uint2(pack2<T>(acc[4 * c] * inv, acc[4 * c + 1] * inv),
+                                                             pack2<T>(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= !(fabsf(acc[4 * c + j]) < INFINITY);
+    }
+    if (lane == 0) p.lse[row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+    if (__any_sync(0xffffffffu, bad) && sum == sum) {
+        const int64_t token = row / p.heads;
+        const int head = static_cast<int>(row - token * p.heads);
+        Item it;
+        it.kvh = head / p.group;
+        for (it.b = 0; it.b < p.batch; ++it.b) {
+            it.tokens = tokens_of(p, it.b);
+            if (token >= it.tokens.first && token < it.tokens.first + it.tokens.count) break;
+        }
+        if (it.b == p.batch) return;
+        it.rows = static_cast<int64_t>(it.tokens.count) * p.group;
+        const int64_t at = (token - it.tokens.first) * p.group + head - it.kvh * p.group;
+        it.first = at / ROWS * ROWS;
+        cover<BN, ROWS>(p, it);
+        const int place = place_of(p, it.tokens, at);
+        if (met_not_finite<T>(p, it, place, place)) {
+            __syncwarp();
+            plain_row<T>(p, it.b, token, head, place);
+        }
+    }
+}
+
+template <typename T, int DP>
+int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStream_t stream) {
+    const int64_t ctas = plan.pairs * p.kv_heads * plan.splits;
+    if (ctas > 0x7fffffff) return fail(QMM_ERR_UNSUPPORTED, "qmm_paged_prompt_attention: too many tokens");
+    QMM_CUDA_OK(cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<DP>())));
+    QMM_CUDA_OK(launch_pdl(prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch));
+    if (plan.splits > 1) {
+        const int64_t joins = (p.tokens * p.heads + 7) / 8;
+        QMM_CUDA_OK(launch_pdl(prompt_join_kernel<T, Shape<DP>::kBN, Shape<DP>::kRows>, dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, p, scratch));
+    }
+    return QMM_OK;
+}
+
+template <typename T>
+int launch_t(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStream_t stream) {
+    if (p.dim <= 64) return launch<T, 64>(p, plan, scratch, stream);
+    if (p.dim <= 128) return launch<T, 128>(p, plan, scratch, stream);
+    return launch<T, 256>(p, plan, scratch, stream);
+}
+
+}  // namespace
+
+size_t prompt_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places) {
+    return tokens == 0 || heads == 0 ? 0 : make_plan(tokens, batch, heads, kv_heads, dim, places).bytes;
+}
+
+int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    const Plan plan = make_plan(p.tokens, p.batch, p.heads, p.kv_heads, p.dim, static_cast<int64_t>(p.max_pages) * p.page);
+    if (plan.bytes > 0 && (workspace_bytes < plan.bytes || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
+        return fail(QMM_ERR_WORKSPACE, "qmm_paged_prompt_attention: needs a workspace of " + std::to_string(plan.bytes) + " bytes, 16-byte aligned");
+    Scratch scratch;
+    scratch.part = static_cast<float *>(workspace);
+    scratch.stat = reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + plan.part_bytes);
+    scratch.splits = plan.splits;
+    scratch.status = device_status_word();
+    return dtype == QMM_DTYPE_BF16 ? launch_t<__nv_bfloat16>(p, plan, scratch, stream) : launch_t<__half>(p, plan, scratch, stream);
+}
+
+}  // namespace paged
+}  // namespace qmm
