@@ -9,9 +9,10 @@
 // maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.  Two row tiles share the keys
 // (dimensions up to 128): the tensor pipe works on one while the softmax works on the other.
 //
-// Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warp 8: MMA.  Warps 10 and 11: keys and values by cp.async,
-// half a tile each, whatever the pages' size and the strides; rows that no row of the CTA sees are zero-filled.  A key that
-// some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
+// Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warp 8: MMA.  Warps 9 to 11: keys and values.  Where a page
+// holds a multiple of 16 places, a tile that is seen whole comes by TMA, a box of 16 places and 64 columns a lane of warp 9 (by
+// cp.async two warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
+// and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
 // come out not finite are looked at again (see mended).
 #include <type_traits>
 
@@ -23,7 +24,7 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 384;  // 168 registers each: the softmax has a row of 128 scores
-constexpr int kLoaders = 2;  // warps
+constexpr int kLoaders = 3;  // warps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
@@ -210,10 +211,81 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives on the barrier when this thread's copies so far are done.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Four K=16 MMAs under one election: both operands K-major in 128-byte rows (32 bytes, +2, a step).
+__device__ __forceinline__ void mma_ss_x4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, e, t;\n\t"
+        ".reg .b64 ad, bd;\n\t"
+        ".reg .b32 al, bl;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "setp.eq.b32 t, 0, 0;\n\t"
+        "mov.b64 ad, {%1, %3};\n\t"
+        "mov.b64 bd, {%2, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, p;\n\t"
+        "add.u32 al, %1, 2;\n\t"
+        "add.u32 bl, %2, 2;\n\t"
+        "mov.b64 ad, {al, %3};\n\t"
+        "mov.b64 bd, {bl, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, t;\n\t"
+        "add.u32 al, %1, 4;\n\t"
+        "add.u32 bl, %2, 4;\n\t"
+        "mov.b64 ad, {al, %3};\n\t"
+        "mov.b64 bd, {bl, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, t;\n\t"
+        "add.u32 al, %1, 6;\n\t"
+        "add.u32 bl, %2, 6;\n\t"
+        "mov.b64 ad, {al, %3};\n\t"
+        "mov.b64 bd, {bl, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, t;\n\t"
+        "}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Four K=16 MMAs under one election: A in tensor memory (eight columns a step), B MN-major (16 rows of 128 bytes, +128, a step).
+__device__ __forceinline__ void mma_ts_x4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, e, t;\n\t"
+        ".reg .b64 bd;\n\t"
+        ".reg .b32 a, bl;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "setp.eq.b32 t, 0, 0;\n\t"
+        "mov.b64 bd, {%2, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %4, p;\n\t"
+        "add.u32 a, %1, 8;\n\t"
+        "add.u32 bl, %2, 128;\n\t"
+        "mov.b64 bd, {bl, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], bd, %4, t;\n\t"
+        "add.u32 a, %1, 16;\n\t"
+        "add.u32 bl, %2, 256;\n\t"
+        "mov.b64 bd, {bl, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], bd, %4, t;\n\t"
+        "add.u32 a, %1, 24;\n\t"
+        "add.u32 bl, %2, 384;\n\t"
+        "mov.b64 bd, {bl, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], bd, %4, t;\n\t"
+        "}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 4-D tiled load global -> shared: columns, places of a page, heads, pages.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *m, int32_t column, int32_t place, int32_t head, int32_t page,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(column), "r"(place), "r"(head), "r"(page)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 // Bits [from, to) of a word, the bounds being any numbers.
 __device__ __forceinline__ uint32_t bits(int from, int to) {
@@ -222,7 +294,8 @@ __device__ __forceinline__ uint32_t bits(int from, int to) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, const __grid_constant__ CUtensorMap tmap_k,
+              const __grid_constant__ CUtensorMap tmap_v, bool tma) {
     using S = Shape<DP>;
     constexpr int BN = S::kBN;
     extern __shared__ uint8_t smem_raw[];
@@ -235,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(smem_u32(&tail->full[s]), kLoaders);
+            mbar_init(smem_u32(&tail->full[s]), kLoaders * 33);  // every lane's copies, and the lookup
             mbar_init(smem_u32(&tail->empty[s]), 1);
         }
         mbar_init(smem_u32(&tail->q_full), 4 * S::kTiles);
@@ -246,6 +319,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         tail->abort_flag = 0;
         mbar_fence_init();
+        if (tma) {
+            tma_prefetch_desc(&tmap_k);
+            tma_prefetch_desc(&tmap_v);
+        }
     }
     if (warp == 8) {
         tmem_alloc(smem_u32(&tail->tmem_base), 512);
@@ -284,76 +361,88 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (!found) {
         // nothing to do
-    } else if (warp >= 10) {
+    } else if (warp >= 9) {
         // ---------------- keys and values ----------------
-        const int loader = warp - 10;
+        const int loader = warp - 9;
         constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
-        constexpr int kMine = BN / kLoaders, kLooks = kMine / 32;  // rows of a tile, places a lane looks up
+        constexpr int kLooks = BN / 32;  // places that a lane looks up; every loader all of them
         const int my_key = lane / kChunks, my_chunk = lane % kChunks;
         const int row_chunks = p.dim / 8;
         const bool my_part = my_chunk < 2 * ksteps;
-        const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
-        uint32_t stage = 0, phase = 0, waiting = 0, signal = 0;  // `waiting` stages from `signal` on are under way
+        const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
+        uint32_t stage = 0, phase = 0;
         bool ok = true;
-        auto arrive = [&] {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&tail->full[signal]));
-            signal = signal + 1 == S::kStages ? 0 : signal + 1;
-            --waiting;
-        };
         for (int i = begin; i < end && ok; ++i) {
-            const int first = block_start<BN>(it, i) + loader * kMine;
+            const int first = block_start<BN>(it, i);
+            bool full = true;
             uint32_t mask[kLooks];
-            int64_t k_offset[kLooks], v_offset[kLooks];
+            int id[kLooks], at[kLooks];
 #pragma unroll
             for (int l = 0; l < kLooks; ++l) {
                 const int j = first + 32 * l + lane;
                 int64_t block = 0;
-                int at = 0;
-                const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at);
+                at[l] = 0;
+                const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at[l]);
+                id[l] = static_cast<int>(block);
                 mask[l] = __ballot_sync(0xffffffffu, seen);
-                k_offset[l] = seen ? block * p.k_sb + at * p.k_st + it.kvh * p.k_sh : 0;
-                v_offset[l] = seen ? block * p.v_sb + at * p.v_st + it.kvh * p.v_sh : 0;
+                full = full && mask[l] == 0xffffffffu;
             }
-#pragma unroll
             for (int part = 0; part < 2; ++part) {
-                if (!mbar_try_wait(smem_u32(&tail->empty[stage]), phase ^ 1)) {
-                    // the MMA may wait for a tile that is under way
-                    cp_async_wait<0>();
-                    while (waiting > 0) arrive();
-                    ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
-                    if (!ok) break;
-                }
-                if (part == 0 && lane == 0) {
+                ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
+                if (part == 0 && loader == 0 && lane == 0) {
 #pragma unroll
-                    for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][loader * kLooks + l] = mask[l];
+                    for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
                 }
-                const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
-                const uint32_t dst = ring + stage * S::kStage + my_box + loader * (kMine * 128);
+                if (full && tma) {
+                    if (loader == 0) {
+                        if (lane == 0) mbar_expect_tx(bar, S::kStage);
+                        // lane: group of 16 places, box of 64 columns; the group's page from the lane that looked its first place up
+                        const int group = lane / S::kBoxes, box = lane % S::kBoxes;
+                        int page = 0, place = 0;
 #pragma unroll
-                for (int r = 0; r < kMine / kStep; ++r) {
-                    const int l = r * kStep / 32, key = r * kStep % 32 + my_key;
-                    const T *row = base + __shfl_sync(0xffffffffu, part == 0 ? k_offset[l] : v_offset[l], key);
-                    if (my_part)
-                        cp_async_16(dst + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
-                                    my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
+                        for (int l = 0; l < kLooks; ++l) {
+                            const int x = __shfl_sync(0xffffffffu, id[l], group * 16 % 32), y = __shfl_sync(0xffffffffu, at[l], group * 16 % 32);
+                            if (group / 2 == l) {
+                                page = x;
+                                place = y;
+                            }
+                        }
+                        if (group < BN / 16)
+                            tma_load_4d(dst + box * S::kBox + group * 2048, part == 0 ? &tmap_k : &tmap_v, box * 64, place, it.kvh, page, bar);
+                        if (lane == 0) mbar_arrive_n(bar, 32);
+                    } else if (lane == 0) {
+                        mbar_arrive_n(bar, 33);
+                    }
+                } else {
+                    const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
+                    const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
+#pragma unroll
+                    for (int group = 0; group < BN / 16; ++group) {
+                        if (group % kLoaders != loader) continue;
+                        const int l = group / 2;
+                        const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
+#pragma unroll
+                        for (int r = 0; r < 16; r += kStep) {
+                            const int key = group * 16 % 32 + r + my_key;
+                            const T *row = base + __shfl_sync(0xffffffffu, offset, key);
+                            if (my_part)
+                                cp_async_16(dst + my_box + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
+                                            my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
+                        }
+                    }
+                    cp_async_arrive(bar);
+                    if (lane == 0) mbar_arrive(bar);
                 }
-                cp_async_commit();
-                ++waiting;
                 if (++stage == S::kStages) {
                     stage = 0;
                     phase ^= 1;
                 }
-                if (waiting == 3) {
-                    cp_async_wait<2>();
-                    arrive();
-                }
             }
         }
-        cp_async_wait<0>();
-        while (waiting > 0) arrive();
+        cp_async_wait_all();
     } else if (warp == 8) {
         // ---------------- MMA ----------------
         constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -364,7 +453,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         uint32_t k_stage = 0, k_phase = 0;  // stages: keys, values, keys, ...
         auto product_s = [&](int tile, int buffer, uint32_t stage) {
             const uint32_t a = smem_desc_lo(smem_base + tile * (S::kBoxes * S::kQueryBox), 16), b = smem_desc_lo(ring + stage * S::kStage, 16);
-            for (int k = 0; k < ksteps; ++k)
+#pragma unroll
+            for (int box = 0; box < S::kBoxes; ++box)
+                if (box * 4 + 4 <= ksteps)
+                    mma_ss_x4(tmem_base + buffer * S::kS, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
+            for (int k = ksteps & ~3; k < ksteps; ++k)
                 mma_f16_ss_warp(tmem_base + buffer * S::kS, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
                                 desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
         };
@@ -372,17 +465,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         auto product_o = [&](int tile, int buffer, uint32_t stage, bool first) {
             const uint32_t b = smem_desc_lo(ring + stage * S::kStage, S::kBox);
 #pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-                mma_f16_ts_warp(tmem_base + S::kO + tile * 128, tmem_base + buffer * S::kS + k * 8, desc64(b + k * (2048 >> 4), kHi), o_desc,
-                                !first || k > 0);
+            for (int k = 0; k < BN / 16; k += 4)
+                mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + buffer * S::kS + k * 8, b + k * (2048 >> 4), kHi, o_desc, !first || k > 0);
+        };
+        // The loaders' copies are writes of the generic proxy, which their barrier makes visible here; the fence hands them to the
+        // MMA's.
+        auto landed = [&](uint32_t stage, uint32_t phase, uint32_t where) {
+            const bool there = mbar_wait(smem_u32(&tail->full[stage]), phase, abort_flag, where);
+            fence_proxy_async_smem();
+            return there;
         };
         bool ok = blocks > 0 && mbar_wait(smem_u32(&tail->q_full), 0, abort_flag, 0x91);
         if (S::kTiles == 2) {
             for (int i = 0; i <= blocks && ok; ++i) {
                 const uint32_t v_stage = (2 * i + S::kStages - 1) % S::kStages;  // of the block before
                 const uint32_t v_phase = ((2 * i - 1) / S::kStages) & 1;
-                if (i < blocks) ok = mbar_wait(smem_u32(&tail->full[k_stage]), k_phase, abort_flag, 0x92);
-                if (ok && i > 0) ok = mbar_wait(smem_u32(&tail->full[v_stage]), v_phase, abort_flag, 0x93);
+                if (i < blocks) ok = landed(k_stage, k_phase, 0x92);
+                if (ok && i > 0) ok = landed(v_stage, v_phase, 0x93);
                 for (int tile = 0; tile < 2 && ok; ++tile) {
                     if (tile == 1 && !two) break;
                     if (i > 0) {
@@ -409,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         } else {
             for (int i = 0; i <= blocks && ok; ++i) {
                 if (i < blocks) {
-                    ok = mbar_wait(smem_u32(&tail->full[k_stage]), k_phase, abort_flag, 0x95);
+                    ok = landed(k_stage, k_phase, 0x95);
                     if (!ok) break;
                     tc_fence_after();
                     product_s(0, i & 1, k_stage);
@@ -418,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 if (i > 0) {
                     const uint32_t v_stage = (2 * i + S::kStages - 1) % S::kStages, v_phase = ((2 * i - 1) / S::kStages) & 1;
-                    ok = mbar_wait(smem_u32(&tail->full[v_stage]), v_phase, abort_flag, 0x96) &&
+                    ok = landed(v_stage, v_phase, 0x96) &&
                          mbar_wait(smem_u32(&tail->p_full[0]), (i - 1) & 1, abort_flag, 0x97);
                     if (!ok) break;
                     tc_fence_after();
@@ -708,12 +807,27 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
     }
 }
 
+// A cache as TMA sees it: boxes of 16 places of one page and head by 64 columns (zeros behind the head dimension).  False: its
+// strides are none that TMA takes, cp.async loads it.
+bool cache_map(CUtensorMap *map, const Problem &p, const void *base, int64_t sb, int64_t st, int64_t sh) {
+    const int64_t sizes[4] = {p.dim, p.page, p.kv_heads, p.pages};
+    int64_t strides[3] = {st, sh, sb};
+    for (int i = 0; i < 3; ++i) {
+        if (sizes[i + 1] == 1) strides[i] = p.dim;  // takes no step
+        if (strides[i] <= 0 || strides[i] >= 1ll << 38) return false;
+    }
+    return make_tmap_4d(map, base, sizes, strides, 64, 16);
+}
+
 template <typename T, int DP>
 int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStream_t stream) {
     const int64_t ctas = plan.pairs * p.kv_heads * plan.splits;
     if (ctas > 0x7fffffff) return fail(QMM_ERR_UNSUPPORTED, "qmm_paged_prompt_attention: too many tokens");
     QMM_CUDA_OK(cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<DP>())));
-    QMM_CUDA_OK(launch_pdl(prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch));
+    CUtensorMap tmap_k = {}, tmap_v = {};
+    const bool tma = p.page % 16 == 0 && p.pages > 0 && cache_map(&tmap_k, p, p.k, p.k_sb, p.k_st, p.k_sh) && cache_map(&tmap_v, p, p.v, p.v_sb, p.v_st, p.v_sh);
+    QMM_CUDA_OK(launch_pdl(prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch,
+                           tmap_k, tmap_v, tma));
     if (plan.splits > 1) {
         const int64_t joins = (p.tokens * p.heads + 7) / 8;
         QMM_CUDA_OK(launch_pdl(prompt_join_kernel<T, Shape<DP>::kBN, Shape<DP>::kRows>, dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, p, scratch));
