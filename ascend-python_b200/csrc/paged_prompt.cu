@@ -10,8 +10,8 @@
 // (dimensions up to 128): the tensor pipe works on one while the softmax works on the other.
 //
 // Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warp 8: MMA.  Warps 9 to 11: keys and values.  Where a page
-// holds a multiple of 16 places, a tile that is seen whole comes by TMA, a box of 16 places and 64 columns a lane of warp 9 (by
-// cp.async two warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
+// holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
+// warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
 // and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
 // come out not finite are looked at again (see mended).
 #include <type_traits>
@@ -48,7 +48,7 @@ constexpr int kValid = 8;  // blocks whose masks are kept: more than may be unde
 struct Tail {
     uint64_t full[6], empty[6];
     uint64_t q_full, s_full[2], p_full[2], o_done[2];
-    uint32_t valid[kValid][4];
+    alignas(16) uint32_t valid[kValid][4];
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -208,6 +208,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -276,11 +281,16 @@ __device__ __forceinline__ void mma_ts_x4(uint32_t d, uint32_t a, uint32_t b_lo,
         "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 4-D tiled load global -> shared: columns, places of a page, heads, pages.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *m, int32_t column, int32_t place, int32_t head, int32_t page,
+// 4-D tiled load global -> shared: columns, places of a page, heads, pages; by one lane of a converged warp.  (16 lanes with a box
+// each took 90 clocks a box: the instruction takes uniform operands, so lanes that differ go one by one.)
+__device__ __forceinline__ void tma_load_4d_warp(uint32_t dst, const CUtensorMap *m, int32_t column, int32_t place, int32_t head, int32_t page,
                                             uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t"
+        "}\n" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(column), "r"(place), "r"(head), "r"(page)
         : "memory");
 }
@@ -295,7 +305,7 @@ __device__ __forceinline__ uint32_t bits(int from, int to) {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, const __grid_constant__ CUtensorMap tmap_k,
-              const __grid_constant__ CUtensorMap tmap_v, bool tma) {
+              const __grid_constant__ CUtensorMap tmap_v, int box_rows) {
     using S = Shape<DP>;
     constexpr int BN = S::kBN;
     extern __shared__ uint8_t smem_raw[];
@@ -319,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         tail->abort_flag = 0;
         mbar_fence_init();
-        if (tma) {
+        if (box_rows > 0) {
             tma_prefetch_desc(&tmap_k);
             tma_prefetch_desc(&tmap_v);
         }
@@ -373,21 +383,36 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
         uint32_t stage = 0, phase = 0;
         bool ok = true;
-        for (int i = begin; i < end && ok; ++i) {
+        // the groups of 16 places whose boxes this warp fetches, and their bytes
+        uint32_t my_groups = 0;
+        for (int group = 0, n = 0; box_rows > 0 && group < BN / 16; group += box_rows / 16, ++n)
+            if (n % kLoaders == loader) my_groups |= 1u << group;
+        const uint32_t my_bytes = __popc(my_groups) * S::kBoxes * box_rows * 128;
+        int next_id[kLooks], next_at[kLooks];  // looked up a block ahead
+        auto look_up = [&](int i) {
             const int first = block_start<BN>(it, i);
+#pragma unroll
+            for (int l = 0; l < kLooks; ++l) {
+                const int j = first + 32 * l + lane;
+                const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo);
+                const int page = seen ? page_of(p, j) : 0;
+                next_at[l] = j - page * p.page;
+                next_id[l] = seen ? __ldg(p.table + it.b * p.table_st + page) : -1;
+            }
+        };
+        if (begin < end) look_up(begin);
+        for (int i = begin; i < end && ok; ++i) {
             bool full = true;
             uint32_t mask[kLooks];
             int id[kLooks], at[kLooks];
 #pragma unroll
             for (int l = 0; l < kLooks; ++l) {
-                const int j = first + 32 * l + lane;
-                int64_t block = 0;
-                at[l] = 0;
-                const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at[l]);
-                id[l] = static_cast<int>(block);
-                mask[l] = __ballot_sync(0xffffffffu, seen);
+                id[l] = next_id[l];
+                at[l] = next_at[l];
+                mask[l] = __ballot_sync(0xffffffffu, id[l] >= 0 && id[l] < p.pages);
                 full = full && mask[l] == 0xffffffffu;
             }
+            if (i + 1 < end) look_up(i + 1);
             for (int part = 0; part < 2; ++part) {
                 ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
                 if (!ok) break;
@@ -396,25 +421,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
                     for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
                 }
-                if (full && tma) {
-                    if (loader == 0) {
-                        if (lane == 0) mbar_expect_tx(bar, S::kStage);
-                        // lane: group of 16 places, box of 64 columns; the group's page from the lane that looked its first place up
-                        const int group = lane / S::kBoxes, box = lane % S::kBoxes;
-                        int page = 0, place = 0;
+                if (full && box_rows > 0) {
+                    const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
+                    if (lane == 0) {
+                        mbar_expect_tx(bar, my_bytes);
+                        mbar_arrive_n(bar, 32);
+                    }
+                    __syncwarp();
 #pragma unroll
-                        for (int l = 0; l < kLooks; ++l) {
-                            const int x = __shfl_sync(0xffffffffu, id[l], group * 16 % 32), y = __shfl_sync(0xffffffffu, at[l], group * 16 % 32);
-                            if (group / 2 == l) {
-                                page = x;
-                                place = y;
-                            }
-                        }
-                        if (group < BN / 16)
-                            tma_load_4d(dst + box * S::kBox + group * 2048, part == 0 ? &tmap_k : &tmap_v, box * 64, place, it.kvh, page, bar);
-                        if (lane == 0) mbar_arrive_n(bar, 32);
-                    } else if (lane == 0) {
-                        mbar_arrive_n(bar, 33);
+                    for (int group = 0; group < BN / 16; ++group) {
+                        if (!(my_groups >> group & 1)) continue;
+                        // its page from the lane that looked its first place up
+                        const int page = __shfl_sync(0xffffffffu, id[group / 2], group * 16 % 32);
+                        const int place = __shfl_sync(0xffffffffu, at[group / 2], group * 16 % 32);
+#pragma unroll
+                        for (int box = 0; box < S::kBoxes; ++box)
+                            tma_load_4d_warp(dst + box * S::kBox + group * 2048, map, box * 64, place, it.kvh, page, bar);
                     }
                 } else {
                     const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
@@ -588,14 +610,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_addr + c * 32, s[c]);
             tmem_ld_wait();
             const int start = block_start<BN>(it, i);
-            uint32_t valid[BN / 32];
-            bool all = start + BN <= first_range.sink_end || (start >= last_range.lo && start + BN <= first_range.hi);
-#pragma unroll
-            for (int c = 0; c < BN / 32; ++c) {
-                valid[c] = tail->valid[i % kValid][c];
-                all = all && valid[c] == 0xffffffffu;
-            }
-            if (!all) {
+            const uint4 valid4 = *reinterpret_cast<const uint4 *>(tail->valid[i % kValid]);
+            const uint32_t valid[4] = {valid4.x, valid4.y, BN == 128 ? valid4.z : 0xffffffffu, BN == 128 ? valid4.w : 0xffffffffu};
+            const bool all = start + BN <= first_range.sink_end || (start >= last_range.lo && start + BN <= first_range.hi);
+            if (!all || (valid[0] & valid[1] & valid[2] & valid[3]) != 0xffffffffu) {
 #pragma unroll
                 for (int c = 0; c < BN / 32; ++c) {
                     const int at = start + c * 32;
@@ -605,13 +623,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         if (!(see >> j & 1)) s[c][j] = 0xff800000u;  // -inf
                 }
             }
-            float most = -INFINITY, most2 = -INFINITY;
+            float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < BN; j += 2) {
-                most = fmaxf(most, __uint_as_float(s[j / 32][j % 32]));
-                most2 = fmaxf(most2, __uint_as_float(s[j / 32][j % 32 + 1]));
+            for (int j = 0; j < BN; j += 8) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    most4[c] = max3(most4[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
             }
-            most = fmaxf(most, most2);
+            const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
             const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
             if (__any_sync(0xffffffffu, move)) {
                 const float now = move ? most : base;
@@ -807,16 +826,16 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
     }
 }
 
-// A cache as TMA sees it: boxes of 16 places of one page and head by 64 columns (zeros behind the head dimension).  False: its
+// A cache as TMA sees it: boxes of `rows` places of one page and head by 64 columns (zeros behind the head dimension).  False: its
 // strides are none that TMA takes, cp.async loads it.
-bool cache_map(CUtensorMap *map, const Problem &p, const void *base, int64_t sb, int64_t st, int64_t sh) {
+bool cache_map(CUtensorMap *map, const Problem &p, const void *base, int64_t sb, int64_t st, int64_t sh, int rows) {
     const int64_t sizes[4] = {p.dim, p.page, p.kv_heads, p.pages};
     int64_t strides[3] = {st, sh, sb};
     for (int i = 0; i < 3; ++i) {
         if (sizes[i + 1] == 1) strides[i] = p.dim;  // takes no step
         if (strides[i] <= 0 || strides[i] >= 1ll << 38) return false;
     }
-    return make_tmap_4d(map, base, sizes, strides, 64, 16);
+    return make_tmap_4d(map, base, sizes, strides, 64, rows);
 }
 
 template <typename T, int DP>
@@ -825,9 +844,14 @@ int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStrea
     if (ctas > 0x7fffffff) return fail(QMM_ERR_UNSUPPORTED, "qmm_paged_prompt_attention: too many tokens");
     QMM_CUDA_OK(cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<DP>())));
     CUtensorMap tmap_k = {}, tmap_v = {};
-    const bool tma = p.page % 16 == 0 && p.pages > 0 && cache_map(&tmap_k, p, p.k, p.k_sb, p.k_st, p.k_sh) && cache_map(&tmap_v, p, p.v, p.v_sb, p.v_st, p.v_sh);
+    // as many places a box as begin together in any page and any tile
+    int box_rows = 16;
+    while (2 * box_rows <= Shape<DP>::kBN && p.page % (2 * box_rows) == 0) box_rows *= 2;
+    if (p.page % 16 != 0 || p.pages == 0 || !cache_map(&tmap_k, p, p.k, p.k_sb, p.k_st, p.k_sh, box_rows) ||
+        !cache_map(&tmap_v, p, p.v, p.v_sb, p.v_st, p.v_sh, box_rows))
+        box_rows = 0;
     QMM_CUDA_OK(launch_pdl(prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch,
-                           tmap_k, tmap_v, tma));
+                           tmap_k, tmap_v, box_rows));
     if (plan.splits > 1) {
         const int64_t joins = (p.tokens * p.heads + 7) / 8;
         QMM_CUDA_OK(launch_pdl(prompt_join_kernel<T, Shape<DP>::kBN, Shape<DP>::kRows>, dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, p, scratch));
