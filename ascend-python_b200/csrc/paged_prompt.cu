@@ -3,11 +3,13 @@
 // Rows: the tokens of one sequence times the query heads of one key-value head, token by token, in tiles of 128; so a few tokens
 // of a wide group fill a tile as well as many of a narrow one, and every key that is read serves the whole group.
 //
-// For a block of BN keys, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory.  P, rounded to the
+// For 64 keys at a time, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory.  P, rounded to the
 // values' type, lies in the first half of the columns of its S, as the second product's operand in tensor memory.  The softmax
 // is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
-// maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.  Two row tiles share the keys
-// (dimensions up to 128): the tensor pipe works on one while the softmax works on the other.
+// maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.
+//
+// S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
+// one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
 // Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warp 8: MMA.  Warps 9 to 11: keys and values.  Where a page
 // holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
@@ -26,20 +28,22 @@ namespace {
 constexpr int kThreads = 384;  // 168 registers each: the softmax has a row of 128 scores
 constexpr int kLoaders = 3;  // warps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMix = 2;  // every second pair of weights comes from the FMA pipe: the special-function unit alone takes as long as the products
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
-// DP: the head dimension rounded up to 64, 128 or 256.  256 columns of O leave room for one row tile; S is double-buffered then.
+// DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: two S of 64 for each row tile, then O; 256
+// columns of O leave room for one row tile.
 template <int DP>
 struct Shape {
     static constexpr int kTiles = DP == 256 ? 1 : 2;
-    static constexpr int kBN = DP == 256 ? 64 : 128;
+    static constexpr int kBN = DP == 256 ? 64 : 128;          // keys of a tile in shared memory
+    static constexpr int kSub = kBN / 64;                     // steps of a tile
     static constexpr int kStages = DP == 64 ? 6 : 4;
     static constexpr int kBoxes = DP / 64;                    // of 64 columns: 128-byte rows
     static constexpr int kQueryBox = 128 * 128;               // bytes
     static constexpr int kQuery = kTiles * kBoxes * kQueryBox;
     static constexpr int kBox = kBN * 128;
     static constexpr int kStage = kBoxes * kBox;
-    static constexpr int kS = DP == 256 ? 64 : 128;           // columns between the two S
     static constexpr int kO = 256;                            // first column of O
     static constexpr int kRows = kTiles * 128;
 };
@@ -47,7 +51,7 @@ struct Shape {
 constexpr int kValid = 8;  // blocks whose masks are kept: more than may be under way
 struct Tail {
     uint64_t full[6], empty[6];
-    uint64_t q_full, s_full[2], p_full[2], o_done[2];
+    uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][step % 2]
     alignas(16) uint32_t valid[kValid][4];
     uint32_t tmem_base, abort_flag;
 };
@@ -208,10 +212,27 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+// 2^x of two numbers, not infinite and not NaN, on the FMA pipe: x = n + f with n whole and f in [-1/2, 1/2], a polynomial of degree 5
+// for 2^f (the coefficients are a least-maximum fit of the relative error, 2^-23.6), and n added to its exponent.  Below -125
+// the result is 2^-125.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which is then in the low bits
+    x.x = fmaxf(x.x, -125.0f);
+    x.y = fmaxf(x.y, -125.0f);
+    const float2 n = add2(x, make_float2(kRound, kRound));
+    const float2 f = fma2(add2(n, make_float2(-kRound, -kRound)), make_float2(-1.0f, -1.0f), x);
+    float2 y = fma2(f, make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f), make_float2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
+    y = fma2(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+    y = fma2(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+    y = fma2(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
+    y = fma2(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -322,10 +343,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             mbar_init(smem_u32(&tail->empty[s]), 1);
         }
         mbar_init(smem_u32(&tail->q_full), 4 * S::kTiles);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&tail->s_full[i]), 1);
-            mbar_init(smem_u32(&tail->p_full[i]), 4);
-            mbar_init(smem_u32(&tail->o_done[i]), 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&tail->s_full[i >> 1][i & 1]), 1);
+            mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 4);
+            mbar_init(smem_u32(&tail->o_done[i >> 1][i & 1]), 1);
         }
         tail->abort_flag = 0;
         mbar_fence_init();
@@ -366,6 +387,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const int begin = found ? static_cast<int>(static_cast<int64_t>(it.blocks) * split / scratch.splits) : 0;
     const int end = found ? static_cast<int>(static_cast<int64_t>(it.blocks) * (split + 1) / scratch.splits) : 0;
     const bool two = S::kTiles == 2 && found && it.first + 128 < it.rows;  // the second row tile has rows
+    // steps of 64 keys; the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
+    int steps = (end - begin) * S::kSub;
+    if (S::kSub == 2 && end > begin) {
+        const int last = block_start<BN>(it, end - 1);
+        if (last + 64 >= (end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --steps;
+    }
     const int ksteps = (p.dim + 15) / 16;
     const float factor = p.scale * kLog2e;
 
@@ -469,90 +496,64 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         // ---------------- MMA ----------------
         constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t kHi = smem_desc_hi_sw128(1024);
-        constexpr uint32_t s_desc = make_idesc(1, kFmt, kFmt, 0, 0, 128, BN);
+        constexpr uint32_t s_desc = make_idesc(1, kFmt, kFmt, 0, 0, 128, 64);
         const uint32_t o_desc = make_idesc(1, kFmt, kFmt, 0, 1, 128, ksteps * 16);
-        const int blocks = end - begin;
-        uint32_t k_stage = 0, k_phase = 0;  // stages: keys, values, keys, ...
-        auto product_s = [&](int tile, int buffer, uint32_t stage) {
-            const uint32_t a = smem_desc_lo(smem_base + tile * (S::kBoxes * S::kQueryBox), 16), b = smem_desc_lo(ring + stage * S::kStage, 16);
+        constexpr uint32_t kSubStep = 64 * 128 >> 4;  // 64 rows of a box
+        const int row_tiles = two ? 2 : 1;
+        // tile of keys 2 * block, of values 2 * block + 1
+        auto stage_of = [](int load) { return static_cast<uint32_t>(load % S::kStages); };
+        // The loaders' copies are writes of the generic proxy, which their barrier makes visible here; the fence hands them to the
+        // MMA's.
+        auto landed = [&](int load, uint32_t where) {
+            const bool there = mbar_wait(smem_u32(&tail->full[stage_of(load)]), load / S::kStages & 1, abort_flag, where);
+            fence_proxy_async_smem();
+            tc_fence_after();
+            return there;
+        };
+        auto product_s = [&](int tile, int step) {
+            const uint32_t a = smem_desc_lo(smem_base + tile * (S::kBoxes * S::kQueryBox), 16);
+            const uint32_t b = smem_desc_lo(ring + stage_of(step / S::kSub * 2) * S::kStage, 16) + step % S::kSub * kSubStep;
+            const uint32_t d = tmem_base + tile * 128 + (step & 1) * 64;
 #pragma unroll
             for (int box = 0; box < S::kBoxes; ++box)
                 if (box * 4 + 4 <= ksteps)
-                    mma_ss_x4(tmem_base + buffer * S::kS, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
+                    mma_ss_x4(d, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
             for (int k = ksteps & ~3; k < ksteps; ++k)
-                mma_f16_ss_warp(tmem_base + buffer * S::kS, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
+                mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
                                 desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
+            tc_commit_warp(smem_u32(&tail->s_full[tile][step & 1]));
         };
-        // 16 keys a step: eight columns of P; 16 rows of 128 bytes of V, its next 64 columns a box further
-        auto product_o = [&](int tile, int buffer, uint32_t stage, bool first) {
-            const uint32_t b = smem_desc_lo(ring + stage * S::kStage, S::kBox);
-#pragma unroll
-            for (int k = 0; k < BN / 16; k += 4)
-                mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + buffer * S::kS + k * 8, b + k * (2048 >> 4), kHi, o_desc, !first || k > 0);
+        // 16 keys a MMA: eight columns of P; 16 rows of 128 bytes of V, its next 64 columns a box further
+        auto product_o = [&](int tile, int step) {
+            mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + tile * 128 + (step & 1) * 64,
+                      smem_desc_lo(ring + stage_of(step / S::kSub * 2 + 1) * S::kStage, S::kBox) + step % S::kSub * kSubStep, kHi, o_desc, step > 0);
+            tc_commit_warp(smem_u32(&tail->o_done[tile][step & 1]));
         };
-        // The loaders' copies are writes of the generic proxy, which their barrier makes visible here; the fence hands them to the
-        // MMA's.
-        auto landed = [&](uint32_t stage, uint32_t phase, uint32_t where) {
-            const bool there = mbar_wait(smem_u32(&tail->full[stage]), phase, abort_flag, where);
-            fence_proxy_async_smem();
-            return there;
+        // the step is its tile's last: the tile's stage is free when the MMAs so far are done
+        auto release = [&](int step, int load) {
+            if (step % S::kSub == S::kSub - 1) tc_commit_warp(smem_u32(&tail->empty[stage_of(load)]));
         };
-        bool ok = blocks > 0 && mbar_wait(smem_u32(&tail->q_full), 0, abort_flag, 0x91);
-        if (S::kTiles == 2) {
-            for (int i = 0; i <= blocks && ok; ++i) {
-                const uint32_t v_stage = (2 * i + S::kStages - 1) % S::kStages;  // of the block before
-                const uint32_t v_phase = ((2 * i - 1) / S::kStages) & 1;
-                if (i < blocks) ok = landed(k_stage, k_phase, 0x92);
-                if (ok && i > 0) ok = landed(v_stage, v_phase, 0x93);
-                for (int tile = 0; tile < 2 && ok; ++tile) {
-                    if (tile == 1 && !two) break;
-                    if (i > 0) {
-                        ok = mbar_wait(smem_u32(&tail->p_full[tile]), (i - 1) & 1, abort_flag, 0x94);
-                        if (!ok) break;
-                        tc_fence_after();
-                        product_o(tile, tile, v_stage, i == 1);
-                        if (i == blocks) tc_commit_warp(smem_u32(&tail->o_done[tile]));
-                    }
-                    if (i < blocks) {
-                        tc_fence_after();
-                        product_s(tile, tile, k_stage);
-                        tc_commit_warp(smem_u32(&tail->s_full[tile]));
-                    }
-                }
-                if (ok && i > 0) tc_commit_warp(smem_u32(&tail->empty[v_stage]));
-                if (ok && i < blocks) tc_commit_warp(smem_u32(&tail->empty[k_stage]));
-                k_stage += 2;
-                if (k_stage >= S::kStages) {
-                    k_stage -= S::kStages;
-                    k_phase ^= 1;
-                }
+        bool ok = steps > 0 && mbar_wait(smem_u32(&tail->q_full), 0, abort_flag, 0x91);
+        for (int step = 0; step < min(2, steps) && ok; ++step) {
+            if (step % S::kSub == 0) ok = landed(step / S::kSub * 2, 0x92);
+            if (!ok) break;
+            for (int tile = 0; tile < row_tiles; ++tile) product_s(tile, step);
+            release(step, step / S::kSub * 2);
+        }
+        for (int step = 0; step < steps && ok; ++step) {
+            const int block = step / S::kSub, ahead = step + 2;
+            if (step % S::kSub == 0) ok = landed(block * 2 + 1, 0x93);
+            if (ok && ahead < steps && ahead % S::kSub == 0) ok = landed(ahead / S::kSub * 2, 0x94);
+            for (int tile = 0; tile < row_tiles && ok; ++tile) {
+                ok = mbar_wait(smem_u32(&tail->p_full[tile][step & 1]), (step >> 1) & 1, abort_flag, 0x95);
+                if (!ok) break;
+                tc_fence_after();
+                product_o(tile, step);
+                if (ahead < steps) product_s(tile, ahead);
             }
-        } else {
-            for (int i = 0; i <= blocks && ok; ++i) {
-                if (i < blocks) {
-                    ok = landed(k_stage, k_phase, 0x95);
-                    if (!ok) break;
-                    tc_fence_after();
-                    product_s(0, i & 1, k_stage);
-                    tc_commit_warp(smem_u32(&tail->s_full[i & 1]));
-                    tc_commit_warp(smem_u32(&tail->empty[k_stage]));
-                }
-                if (i > 0) {
-                    const uint32_t v_stage = (2 * i + S::kStages - 1) % S::kStages, v_phase = ((2 * i - 1) / S::kStages) & 1;
-                    ok = landed(v_stage, v_phase, 0x96) &&
-                         mbar_wait(smem_u32(&tail->p_full[0]), (i - 1) & 1, abort_flag, 0x97);
-                    if (!ok) break;
-                    tc_fence_after();
-                    product_o(0, (i - 1) & 1, v_stage, i == 1);
-                    tc_commit_warp(smem_u32(&tail->o_done[(i - 1) & 1]));
-                    tc_commit_warp(smem_u32(&tail->empty[v_stage]));
-                }
-                k_stage += 2;
-                if (k_stage >= S::kStages) {
-                    k_stage -= S::kStages;
-                    k_phase ^= 1;
-                }
-            }
+            if (!ok) break;
+            release(step, block * 2 + 1);
+            if (ahead < steps) release(ahead, ahead / S::kSub * 2);
         }
     } else if (warp < 4 * S::kTiles) {
         // ---------------- softmax and epilogue: a row a thread ----------------
@@ -586,104 +587,119 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const bool mine = my_row < it.rows;
         const int place = mine ? place_of(p, it.tokens, my_row) : -1;
         const Range range = visible_range(p, place);
-        // what all rows of the warp see: below `common_sink`, and from `common_lo` to `common_hi`
         const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
         const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
         const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
         float base = -INFINITY;  // unscaled
-        float2 sum2 = make_float2(0.0f, 0.0f);
+        float2 sum2 = make_float2(0.0f, 0.0f), more2 = sum2;
         bool ok = true;
         const bool works = end > begin && (tile == 0 || two);
-        for (int i = begin; i < end && works && ok; ++i) {
-            const int n = i - begin;
-            const int buffer = S::kTiles == 2 ? tile : n & 1;
-            ok = mbar_wait(smem_u32(&tail->s_full[buffer]), S::kTiles == 2 ? n & 1 : (n >> 1) & 1, abort_flag, 0x98);
+        for (int n = 0; n < steps && works && ok; ++n) {
+            const int i = begin + n / S::kSub, half = n % S::kSub;
+            ok = mbar_wait(smem_u32(&tail->s_full[tile][n & 1]), (n >> 1) & 1, abort_flag, 0x98);
+            // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
+            if (n > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][n & 1]), ((n - 2) >> 1) & 1, abort_flag, 0x9b);
             if (!ok) break;
             tc_fence_after();
-            // one row tile: a barrier for even and one for odd blocks, each waited for in every phase, so that a phase's parity
-            // is its own
-            if (S::kTiles == 1 && n > 1) ok = mbar_wait(smem_u32(&tail->o_done[n & 1]), ((n - 2) >> 1) & 1, abort_flag, 0x9b);
-            if (!ok) break;
-            const uint32_t s_addr = tmem_base + lanes + buffer * S::kS;
-            uint32_t s[BN / 32][32];
-#pragma unroll
-            for (int c = 0; c < BN / 32; ++c) tmem_ld_32x32(s_addr + c * 32, s[c]);
+            const uint32_t s_addr = tmem_base + lanes + tile * 128 + (n & 1) * 64;
+            uint32_t s[2][32];
+            tmem_ld_32x32(s_addr, s[0]);
+            tmem_ld_32x32(s_addr + 32, s[1]);
+            const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[i % kValid][half * 2]);
+            const int start = block_start<BN>(it, i) + half * 64;
+            const bool whole = (start + 64 <= first_range.sink_end || (start >= last_range.lo && start + 64 <= first_range.hi)) &&
+                               (valid.x & valid.y) == 0xffffffffu;
             tmem_ld_wait();
-            const int start = block_start<BN>(it, i);
-            const uint4 valid4 = *reinterpret_cast<const uint4 *>(tail->valid[i % kValid]);
-            const uint32_t valid[4] = {valid4.x, valid4.y, BN == 128 ? valid4.z : 0xffffffffu, BN == 128 ? valid4.w : 0xffffffffu};
-            const bool all = start + BN <= first_range.sink_end || (start >= last_range.lo && start + BN <= first_range.hi);
-            if (!all || (valid[0] & valid[1] & valid[2] & valid[3]) != 0xffffffffu) {
+            auto maximum = [&] {
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c) {
-                    const int at = start + c * 32;
-                    const uint32_t see = valid[c] & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
+                for (int j = 0; j < 64; j += 8) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (!(see >> j & 1)) s[c][j] = 0xff800000u;  // -inf
+                    for (int c = 0; c < 4; ++c)
+                        m[c] = max3_nan(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
                 }
-            }
-            float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < BN; j += 8) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    most4[c] = max3(most4[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
-            }
-            const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-            const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
-            if (__any_sync(0xffffffffu, move)) {
-                const float now = move ? most : base;
-                const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
-                sum2.x *= keep;
-                sum2.y *= keep;
-                if (n > 0) {
-                    if (S::kTiles == 1) {  // the other tiles' S are behind their O in order
-                        ok = mbar_wait(smem_u32(&tail->o_done[(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, 0x99);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    for (int c = 0; c < ksteps; ++c) {
-                        uint32_t o[16];
-                        const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
-                        tmem_ld_32x16(addr, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                        tmem_st_32x16(addr, o);
-                    }
-                }
-                base = now;
-            }
-            const float offset = base == -INFINITY ? 0.0f : -base * scale;
-            const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+                return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+            };
+            float most = maximum();
             // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another; the sum
             // takes the weights unrounded
+            auto weights = [&](auto mixed, float offset) {
+                const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
 #pragma unroll
-            for (int c = 0; c < BN / 32; ++c) {
-                uint32_t w[16];
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
-                    const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                    sum2 = add2(sum2, e);
-                    w[j] = pack2<T>(e.x, e.y);
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
+                        float2 e;
+                        if (decltype(mixed)::value && j % kMix == kMix - 1)
+                            e = exp2_poly(x);
+                        else
+                            e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                        if (j % 2 == 0)
+                            sum2 = add2(sum2, e);
+                        else
+                            more2 = add2(more2, e);
+                        w[j] = pack2<T>(e.x, e.y);
+                    }
+                    tmem_st_32x16(s_addr + c * 16, w);
                 }
-                tmem_st_32x16(s_addr + c * 16, w);
+            };
+            // A block that all rows see whole and that moves no base: most are.  (A maximum that is not finite counts as one that
+            // moves: exp2_poly takes finite numbers alone.)
+            const bool settled = (most - base) * scale <= kGrowth && most < INFINITY;
+            if (whole && __all_sync(0xffffffffu, settled)) {
+                weights(std::true_type{}, -base * scale);
+            } else {
+                if (!whole) {
+                    const uint32_t word[2] = {valid.x, valid.y};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = start + c * 32;
+                        const uint32_t see = word[c] & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!(see >> j & 1)) s[c][j] = 0xff800000u;  // -inf
+                    }
+                    most = maximum();
+                }
+                const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+                if (__any_sync(0xffffffffu, move)) {
+                    const float now = move ? most : base;
+                    const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                    sum2 = mul2(sum2, make_float2(keep, keep));
+                    more2 = mul2(more2, make_float2(keep, keep));
+                    if (n > 0) {
+                        ok = mbar_wait(smem_u32(&tail->o_done[tile][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, 0x99);
+                        if (!ok) break;
+                        tc_fence_after();
+                        for (int c = 0; c < ksteps; ++c) {
+                            uint32_t o[16];
+                            const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
+                            tmem_ld_32x16(addr, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_st_32x16(addr, o);
+                        }
+                    }
+                    base = now;
+                }
+                weights(std::false_type{}, base == -INFINITY ? 0.0f : -base * scale);
             }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile]));
+            if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile][n & 1]));
         }
-        const float sum = sum2.x + sum2.y;
+        const float sum = (sum2.x + sum2.y) + (more2.x + more2.y);
         const float top = base * scale;
         const int64_t token = my_row / p.group;
         const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
         const int64_t out_row = (it.tokens.first + token) * p.heads + head;
         if (works && ok) {
-            const int last = end - begin - 1;
-            ok = mbar_wait(smem_u32(&tail->o_done[S::kTiles == 2 ? tile : last & 1]), S::kTiles == 2 ? 0 : (last >> 1) & 1, abort_flag, 0x9a);
+            const int last = steps - 1;
+            ok = mbar_wait(smem_u32(&tail->o_done[tile][last & 1]), (last >> 1) & 1, abort_flag, 0x9a);
             tc_fence_after();
         }
         if (scratch.splits > 1) {
