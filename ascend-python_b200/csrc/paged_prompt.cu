@@ -410,62 +410,74 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
         uint32_t stage = 0, phase = 0;
         bool ok = true;
-        // the groups of 16 places whose boxes this warp fetches, and their bytes
-        uint32_t my_groups = 0;
-        for (int group = 0, n = 0; box_rows > 0 && group < BN / 16; group += box_rows / 16, ++n)
-            if (n % kLoaders == loader) my_groups |= 1u << group;
-        const uint32_t my_bytes = __popc(my_groups) * S::kBoxes * box_rows * 128;
-        int next_id[kLooks], next_at[kLooks];  // looked up a block ahead
+        // Boxes: a warp fetches every third.  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
+        const int boxes = box_rows > 0 ? BN / box_rows : 0;
+        constexpr int kMost = (BN / 16 + kLoaders - 1) / kLoaders;
+        int mine = 0;
+        for (int n = loader; n < boxes; n += kLoaders) ++mine;
+        const uint32_t my_bytes = mine * S::kBoxes * box_rows * 128;
+        int next_id = -1, next_at = 0;
         auto look_up = [&](int i) {
-            const int first = block_start<BN>(it, i);
-#pragma unroll
-            for (int l = 0; l < kLooks; ++l) {
-                const int j = first + 32 * l + lane;
-                const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo);
-                const int page = seen ? page_of(p, j) : 0;
-                next_at[l] = j - page * p.page;
-                next_id[l] = seen ? __ldg(p.table + it.b * p.table_st + page) : -1;
+            if (lane >= boxes) return;
+            const int j = block_start<BN>(it, i) + lane * box_rows;
+            next_id = -1;
+            if (j < p.capacity) {
+                const int page = page_of(p, j);
+                next_at = j - page * p.page;
+                next_id = __ldg(p.table + it.b * p.table_st + page);
             }
         };
         if (begin < end) look_up(begin);
         for (int i = begin; i < end && ok; ++i) {
-            bool full = true;
+            const int first = block_start<BN>(it, i);
+            const bool whole = boxes > 0 && (first + BN <= it.sink_end || (first >= it.lo && first + BN <= it.hi)) &&
+                               __all_sync(0xffffffffu, lane >= boxes || (next_id >= 0 && next_id < p.pages));
             uint32_t mask[kLooks];
-            int id[kLooks], at[kLooks];
+            int id[kLooks], at[kLooks], box_page[kMost], box_place[kMost];
+            if (whole) {
 #pragma unroll
-            for (int l = 0; l < kLooks; ++l) {
-                id[l] = next_id[l];
-                at[l] = next_at[l];
-                mask[l] = __ballot_sync(0xffffffffu, id[l] >= 0 && id[l] < p.pages);
-                full = full && mask[l] == 0xffffffffu;
+                for (int n = 0; n < kMost; ++n) {
+                    const int box = loader + n * kLoaders;
+                    box_page[n] = __shfl_sync(0xffffffffu, next_id, box);
+                    box_place[n] = __shfl_sync(0xffffffffu, next_at, box);
+                }
+            } else {
+#pragma unroll
+                for (int l = 0; l < kLooks; ++l) {
+                    const int j = first + 32 * l + lane;
+                    int64_t block = 0;
+                    at[l] = 0;
+                    const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at[l]);
+                    id[l] = static_cast<int>(block);
+                    mask[l] = __ballot_sync(0xffffffffu, seen);
+                }
             }
             if (i + 1 < end) look_up(i + 1);
             for (int part = 0; part < 2; ++part) {
                 ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
                 if (!ok) break;
                 const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
-                if (part == 0 && loader == 0 && lane == 0) {
-#pragma unroll
-                    for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
-                }
-                if (full && box_rows > 0) {
-                    const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
+                if (whole) {
                     if (lane == 0) {
+                        if (part == 0 && loader == 0) *reinterpret_cast<uint4 *>(tail->valid[i % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
                         mbar_expect_tx(bar, my_bytes);
                         mbar_arrive_n(bar, 32);
                     }
                     __syncwarp();
+                    const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
 #pragma unroll
-                    for (int group = 0; group < BN / 16; ++group) {
-                        if (!(my_groups >> group & 1)) continue;
-                        // its page from the lane that looked its first place up
-                        const int page = __shfl_sync(0xffffffffu, id[group / 2], group * 16 % 32);
-                        const int place = __shfl_sync(0xffffffffu, at[group / 2], group * 16 % 32);
+                    for (int n = 0; n < kMost; ++n) {
+                        const int box = loader + n * kLoaders;
+                        if (box >= boxes) break;
 #pragma unroll
-                        for (int box = 0; box < S::kBoxes; ++box)
-                            tma_load_4d_warp(dst + box * S::kBox + group * 2048, map, box * 64, place, it.kvh, page, bar);
+                        for (int column = 0; column < S::kBoxes; ++column)
+                            tma_load_4d_warp(dst + column * S::kBox + box * box_rows * 128, map, column * 64, box_place[n], it.kvh, box_page[n], bar);
                     }
                 } else {
+                    if (part == 0 && loader == 0 && lane == 0) {
+#pragma unroll
+                        for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
+                    }
                     const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
                     const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
 #pragma unroll
