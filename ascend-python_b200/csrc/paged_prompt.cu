@@ -8,10 +8,12 @@
 // is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
 // maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.
 //
+// Two threads have a row, half of the 64 keys each, and tell each other their maxima through shared memory: four softmax warps a
+// scheduler keep its units busier than two with a whole row a thread (8192 tokens, 32/8 heads of 128: TIMES).
 // S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
 // one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
-// Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warp 8: MMA.  Warps 9 to 11: keys and values.  Where a page
+// Warps 0..7 and 8..15: softmax and epilogue of the two row tiles.  Warp 16: MMA.  Warps 17 to 19: keys and values.  Where a page
 // holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
 // and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
@@ -25,10 +27,10 @@ namespace paged {
 
 namespace {
 
-constexpr int kThreads = 384;  // 168 registers each: the softmax has a row of 128 scores
+constexpr int kSoftmax = 16;   // warps
+constexpr int kThreads = 640;
 constexpr int kLoaders = 3;  // warps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMix = 2;  // every second pair of weights comes from the FMA pipe: the special-function unit alone takes as long as the products
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
 // DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: two S of 64 for each row tile, then O; 256
@@ -53,6 +55,8 @@ struct Tail {
     uint64_t full[6], empty[6];
     uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][step % 2]
     alignas(16) uint32_t valid[kValid][4];
+    uint32_t copied[6];           // stage: by cp.async
+    float half[2][2][2][128];     // [row tile][step % 2][half]: maxima; then sums
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -212,27 +216,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
-}
-// 2^x of two numbers, not infinite and not NaN, on the FMA pipe: x = n + f with n whole and f in [-1/2, 1/2], a polynomial of degree 5
-// for 2^f (the coefficients are a least-maximum fit of the relative error, 2^-23.6), and n added to its exponent.  Below -125
-// the result is 2^-125.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which is then in the low bits
-    x.x = fmaxf(x.x, -125.0f);
-    x.y = fmaxf(x.y, -125.0f);
-    const float2 n = add2(x, make_float2(kRound, kRound));
-    const float2 f = fma2(add2(n, make_float2(-kRound, -kRound)), make_float2(-1.0f, -1.0f), x);
-    float2 y = fma2(f, make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f), make_float2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
-    y = fma2(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
-    y = fma2(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
-    y = fma2(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
-    y = fma2(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
-    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -342,10 +329,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             mbar_init(smem_u32(&tail->full[s]), kLoaders * 33);  // every lane's copies, and the lookup
             mbar_init(smem_u32(&tail->empty[s]), 1);
         }
-        mbar_init(smem_u32(&tail->q_full), 4 * S::kTiles);
+        mbar_init(smem_u32(&tail->q_full), 8 * S::kTiles);
         for (int i = 0; i < 4; ++i) {
             mbar_init(smem_u32(&tail->s_full[i >> 1][i & 1]), 1);
-            mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 4);
+            mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 8);
             mbar_init(smem_u32(&tail->o_done[i >> 1][i & 1]), 1);
         }
         tail->abort_flag = 0;
@@ -355,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             tma_prefetch_desc(&tmap_v);
         }
     }
-    if (warp == 8) {
+    if (warp == kSoftmax) {
         tmem_alloc(smem_u32(&tail->tmem_base), 512);
         tmem_relinquish();
         pdl_launch_dependents();
@@ -398,9 +385,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (!found) {
         // nothing to do
-    } else if (warp >= 9) {
+    } else if (warp > kSoftmax) {
         // ---------------- keys and values ----------------
-        const int loader = warp - 9;
+        const int loader = warp - kSoftmax - 1;
         constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
         constexpr int kLooks = BN / 32;  // places that a lane looks up; every loader all of them
         const int my_key = lane / kChunks, my_chunk = lane % kChunks;
@@ -459,7 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
                 if (whole) {
                     if (lane == 0) {
-                        if (part == 0 && loader == 0) *reinterpret_cast<uint4 *>(tail->valid[i % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
+                        if (loader == 0) {
+                            if (part == 0) *reinterpret_cast<uint4 *>(tail->valid[i % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
+                            tail->copied[stage] = 0;
+                        }
                         mbar_expect_tx(bar, my_bytes);
                         mbar_arrive_n(bar, 32);
                     }
@@ -474,9 +464,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             tma_load_4d_warp(dst + column * S::kBox + box * box_rows * 128, map, column * 64, box_place[n], it.kvh, box_page[n], bar);
                     }
                 } else {
-                    if (part == 0 && loader == 0 && lane == 0) {
+                    if (loader == 0 && lane == 0) {
+                        tail->copied[stage] = 1;
 #pragma unroll
-                        for (int l = 0; l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
+                        for (int l = 0; part == 0 && l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
                     }
                     const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
                     const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
@@ -504,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         }
         cp_async_wait_all();
-    } else if (warp == 8) {
+    } else if (warp == kSoftmax) {
         // ---------------- MMA ----------------
         constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t kHi = smem_desc_hi_sw128(1024);
@@ -518,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         // MMA's.
         auto landed = [&](int load, uint32_t where) {
             const bool there = mbar_wait(smem_u32(&tail->full[stage_of(load)]), load / S::kStages & 1, abort_flag, where);
-            fence_proxy_async_smem();
+            if (tail->copied[stage_of(load)] != 0) fence_proxy_async_smem();
             tc_fence_after();
             return there;
         };
@@ -567,10 +558,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             release(step, block * 2 + 1);
             if (ahead < steps) release(ahead, ahead / S::kSub * 2);
         }
-    } else if (warp < 4 * S::kTiles) {
-        // ---------------- softmax and epilogue: a row a thread ----------------
-        const int tile = warp >> 2;
-        const int64_t row0 = it.first + warp * 32;  // this warp's first row
+    } else if (warp < 8 * S::kTiles) {
+        // ---------------- softmax and epilogue: half a row a thread ----------------
+        const int tile = warp >> 3, half = (warp >> 2) & 1;
+        const int64_t row0 = it.first + tile * 128 + (warp & 3) * 32;  // this warp's first row
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         if (end > begin) {
             // the warp's rows of the query: 16-byte chunks into 128-byte rows, swizzled; the scale's sign and zero go with them
@@ -579,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int chunk = lane % kChunks;
             uint8_t *dst = smem + (tile * S::kBoxes + chunk / 8) * S::kQueryBox;
 #pragma unroll 4
-            for (int r = 0; r < 32 / kStep; ++r) {
+            for (int r = half; r < 32 / kStep; r += 2) {
                 const int local = r * kStep + lane / kChunks, row = (warp & 3) * 32 + local;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (row0 + local < it.rows && chunk * 8 < p.dim) {
@@ -603,121 +594,102 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
         const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
         float base = -INFINITY;  // unscaled
-        float2 sum2 = make_float2(0.0f, 0.0f), more2 = sum2;
+        float2 sum2 = make_float2(0.0f, 0.0f);
         bool ok = true;
         const bool works = end > begin && (tile == 0 || two);
-        for (int n = 0; n < steps && works && ok; ++n) {
-            const int i = begin + n / S::kSub, half = n % S::kSub;
-            ok = mbar_wait(smem_u32(&tail->s_full[tile][n & 1]), (n >> 1) & 1, abort_flag, 0x98);
+        const int my_lane = (warp & 3) * 32 + lane;
+        // the two warps that share rows
+        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + (warp & 3)) : "memory"); };
+        const int o_from = half == 0 ? 0 : (ksteps + 1) / 2, o_to = half == 0 ? (ksteps + 1) / 2 : ksteps;  // 16 columns of O each
+        for (int n = 0; n < steps && works; ++n) {
+            const int i = begin + n / S::kSub;
+            // a wait that gave up ends the waits, not the steps: the warps of a row meet in every one
+            ok = ok && mbar_wait(smem_u32(&tail->s_full[tile][n & 1]), (n >> 1) & 1, abort_flag, 0x98);
             // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
             if (n > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][n & 1]), ((n - 2) >> 1) & 1, abort_flag, 0x9b);
-            if (!ok) break;
             tc_fence_after();
             const uint32_t s_addr = tmem_base + lanes + tile * 128 + (n & 1) * 64;
-            uint32_t s[2][32];
-            tmem_ld_32x32(s_addr, s[0]);
-            tmem_ld_32x32(s_addr + 32, s[1]);
-            const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[i % kValid][half * 2]);
-            const int start = block_start<BN>(it, i) + half * 64;
+            uint32_t s[32];
+            tmem_ld_32x32(s_addr + half * 32, s);
+            const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[i % kValid][n % S::kSub * 2]);
+            const int start = block_start<BN>(it, i) + n % S::kSub * 64;
             const bool whole = (start + 64 <= first_range.sink_end || (start >= last_range.lo && start + 64 <= first_range.hi)) &&
                                (valid.x & valid.y) == 0xffffffffu;
             tmem_ld_wait();
-            auto maximum = [&] {
-                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (!whole) {
+                const int at = start + half * 32;
+                const uint32_t see = (half == 0 ? valid.x : valid.y) & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
 #pragma unroll
-                for (int j = 0; j < 64; j += 8) {
+                for (int j = 0; j < 32; ++j)
+                    if (!(see >> j & 1)) s[j] = 0xff800000u;  // -inf
+            }
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        m[c] = max3_nan(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
+            for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) m[c] = max3(m[c], __uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1]));
+            }
+            float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+            tail->half[tile][n & 1][half][my_lane] = most;
+            tc_fence_before();  // the other half's P comes where this one's S was
+            meet();
+            tc_fence_after();
+            most = fmaxf(most, tail->half[tile][n & 1][half ^ 1][my_lane]);
+            const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+            if (__any_sync(0xffffffffu, move)) {
+                const float now = move ? most : base;
+                const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                sum2 = mul2(sum2, make_float2(keep, keep));
+                if (n > 0) {
+                    ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, 0x99);
+                    tc_fence_after();
+                    for (int c = o_from; c < o_to; ++c) {
+                        uint32_t o[16];
+                        const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
+                        tmem_ld_32x16(addr, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                        tmem_st_32x16(addr, o);
+                    }
                 }
-                return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
-            };
-            float most = maximum();
+                base = now;
+            }
+            const float offset = base == -INFINITY ? 0.0f : -base * scale;
+            const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
             // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another; the sum
             // takes the weights unrounded
-            auto weights = [&](auto mixed, float offset) {
-                const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+            uint32_t w[16];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
-                        float2 e;
-                        if (decltype(mixed)::value && j % kMix == kMix - 1)
-                            e = exp2_poly(x);
-                        else
-                            e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                        if (j % 2 == 0)
-                            sum2 = add2(sum2, e);
-                        else
-                            more2 = add2(more2, e);
-                        w[j] = pack2<T>(e.x, e.y);
-                    }
-                    tmem_st_32x16(s_addr + c * 16, w);
-                }
-            };
-            // A block that all rows see whole and that moves no base: most are.  (A maximum that is not finite counts as one that
-            // moves: exp2_poly takes finite numbers alone.)
-            const bool settled = (most - base) * scale <= kGrowth && most < INFINITY;
-            if (whole && __all_sync(0xffffffffu, settled)) {
-                weights(std::true_type{}, -base * scale);
-            } else {
-                if (!whole) {
-                    const uint32_t word[2] = {valid.x, valid.y};
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int at = start + c * 32;
-                        const uint32_t see = word[c] & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!(see >> j & 1)) s[c][j] = 0xff800000u;  // -inf
-                    }
-                    most = maximum();
-                }
-                const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
-                if (__any_sync(0xffffffffu, move)) {
-                    const float now = move ? most : base;
-                    const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
-                    sum2 = mul2(sum2, make_float2(keep, keep));
-                    more2 = mul2(more2, make_float2(keep, keep));
-                    if (n > 0) {
-                        ok = mbar_wait(smem_u32(&tail->o_done[tile][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, 0x99);
-                        if (!ok) break;
-                        tc_fence_after();
-                        for (int c = 0; c < ksteps; ++c) {
-                            uint32_t o[16];
-                            const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
-                            tmem_ld_32x16(addr, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                            tmem_st_32x16(addr, o);
-                        }
-                    }
-                    base = now;
-                }
-                weights(std::false_type{}, base == -INFINITY ? 0.0f : -base * scale);
+            for (int j = 0; j < 16; ++j) {
+                const float2 x = fma2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, offset2);
+                const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                sum2 = add2(sum2, e);
+                w[j] = pack2<T>(e.x, e.y);
             }
+            tmem_st_32x16(s_addr + half * 16, w);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile][n & 1]));
         }
-        const float sum = (sum2.x + sum2.y) + (more2.x + more2.y);
+        // the places of the step before the last, which both warps have read
+        tail->half[tile][steps & 1][half][my_lane] = sum2.x + sum2.y;
+        meet();
+        const float sum = tail->half[tile][steps & 1][0][my_lane] + tail->half[tile][steps & 1][1][my_lane];
         const float top = base * scale;
         const int64_t token = my_row / p.group;
         const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
         const int64_t out_row = (it.tokens.first + token) * p.heads + head;
-        if (works && ok) {
+        if (works) {
             const int last = steps - 1;
-            ok = mbar_wait(smem_u32(&tail->o_done[tile][last & 1]), (last >> 1) & 1, abort_flag, 0x9a);
+            ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][last & 1]), (last >> 1) & 1, abort_flag, 0x9a);
             tc_fence_after();
         }
         if (scratch.splits > 1) {
             const int64_t at = (static_cast<int64_t>(split) * p.tokens * p.heads) + out_row;
-            if (mine) scratch.stat[at] = make_float2(top, sum);
-            for (int c = 0; c < ksteps && works && ok; ++c) {
+            if (mine && half == 0) scratch.stat[at] = make_float2(top, sum);
+            for (int c = o_from; c < o_to && works; ++c) {
                 uint32_t o[16];
                 tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
                 tmem_ld_wait();
@@ -732,11 +704,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         } else {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             bool bad = false;
-            for (int c = 0; c < ksteps; ++c) {
+            for (int c = o_from; c < o_to; ++c) {
                 uint32_t o[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = 0;
-                if (works && ok) {
+                if (works) {
                     tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
                     tmem_ld_wait();
                 }
@@ -754,9 +726,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 __syncwarp();
             }
-            if (mine) p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
-            // rows that are not finite although their weights are
-            uint32_t again = __ballot_sync(0xffffffffu, mine && bad && sum == sum);
+            if (mine && half == 0) p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+            // rows that are not finite although their weights are, when both halves are written
+            tail->half[tile][(steps + 1) & 1][half][my_lane] = bad ? 1.0f : 0.0f;
+            meet();
+            bad = bad || tail->half[tile][(steps + 1) & 1][half ^ 1][my_lane] != 0.0f;
+            uint32_t again = __ballot_sync(0xffffffffu, half == 0 && mine && bad && sum == sum);
             if (again != 0 && met_not_finite<T>(p, it, low, high)) {
                 __syncwarp();
                 for (; again != 0; again &= again - 1) {
@@ -771,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && tail->abort_flag != 0 && scratch.status != nullptr) atomicMax(scratch.status, tail->abort_flag);
-    if (warp == 8) {
+    if (warp == kSoftmax) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
