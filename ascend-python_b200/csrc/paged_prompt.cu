@@ -13,7 +13,8 @@
 // S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
 // one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
-// Warps 0..7 and 8..15: softmax and epilogue of the two row tiles.  Warp 16: MMA.  Warps 17 to 19: keys and values.  Where a page
+// Warps 0..7 and 8..15: softmax and epilogue of the two row tiles.  Warps 16 and 17: MMA, one for each row tile, so
+// that the tensor pipe has the one's products while the other waits at its barriers.  Warps 18 and 19: keys and values.  Where a page
 // holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
 // and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
@@ -29,7 +30,7 @@ namespace {
 
 constexpr int kSoftmax = 16;   // warps
 constexpr int kThreads = 640;
-constexpr int kLoaders = 3;  // warps
+constexpr int kLoaders = 2;  // warps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
@@ -261,6 +262,56 @@ __device__ __forceinline__ void mma_ss_x4(uint32_t d, uint32_t a_lo, uint32_t b_
         "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// Eight K=16 MMAs under one election: both operands two boxes of 128-byte rows; the first one begins the accumulator.
+__device__ __forceinline__ void mma_ss_x8(uint32_t d, uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, uint32_t hi, uint32_t idesc) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred e, f, t;\n\t"
+        ".reg .b64 ad, bd;\n\t"
+        ".reg .b32 al, bl;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 f, 0, 0;\n\t"
+        "setp.eq.b32 t, 0, 0;\n\t"
+        "mov.b64 ad, {%1, %5};\n\t"
+        "mov.b64 bd, {%3, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, f;\n\t"
+        "add.u32 al, %1, 2;\n\t"
+        "add.u32 bl, %3, 2;\n\t"
+        "mov.b64 ad, {al, %5};\n\t"
+        "mov.b64 bd, {bl, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "add.u32 al, %1, 4;\n\t"
+        "add.u32 bl, %3, 4;\n\t"
+        "mov.b64 ad, {al, %5};\n\t"
+        "mov.b64 bd, {bl, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "add.u32 al, %1, 6;\n\t"
+        "add.u32 bl, %3, 6;\n\t"
+        "mov.b64 ad, {al, %5};\n\t"
+        "mov.b64 bd, {bl, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "mov.b64 ad, {%2, %5};\n\t"
+        "mov.b64 bd, {%4, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "add.u32 al, %2, 2;\n\t"
+        "add.u32 bl, %4, 2;\n\t"
+        "mov.b64 ad, {al, %5};\n\t"
+        "mov.b64 bd, {bl, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "add.u32 al, %2, 4;\n\t"
+        "add.u32 bl, %4, 4;\n\t"
+        "mov.b64 ad, {al, %5};\n\t"
+        "mov.b64 bd, {bl, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "add.u32 al, %2, 6;\n\t"
+        "add.u32 bl, %4, 6;\n\t"
+        "mov.b64 ad, {al, %5};\n\t"
+        "mov.b64 bd, {bl, %5};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %6, t;\n\t"
+        "}\n" ::"r"(d),
+        "r"(a0), "r"(a1), "r"(b0), "r"(b1), "r"(hi), "r"(idesc)
+        : "memory");
+}
 // Four K=16 MMAs under one election: A in tensor memory (eight columns a step), B MN-major (16 rows of 128 bytes, +128, a step).
 __device__ __forceinline__ void mma_ts_x4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -327,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(smem_u32(&tail->full[s]), kLoaders * 33);  // every lane's copies, and the lookup
-            mbar_init(smem_u32(&tail->empty[s]), 1);
+            mbar_init(smem_u32(&tail->empty[s]), S::kTiles);  // every row tile's products
         }
         mbar_init(smem_u32(&tail->q_full), 8 * S::kTiles);
         for (int i = 0; i < 4; ++i) {
@@ -385,9 +436,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (!found) {
         // nothing to do
-    } else if (warp > kSoftmax) {
+    } else if (warp >= kSoftmax + 2) {
         // ---------------- keys and values ----------------
-        const int loader = warp - kSoftmax - 1;
+        const int loader = warp - kSoftmax - 2;
         constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
         constexpr int kLooks = BN / 32;  // places that a lane looks up; every loader all of them
         const int my_key = lane / kChunks, my_chunk = lane % kChunks;
@@ -495,68 +546,85 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         }
         cp_async_wait_all();
-    } else if (warp == kSoftmax) {
+    } else if (warp == kSoftmax || (S::kTiles == 2 && warp == kSoftmax + 1 && two)) {
         // ---------------- MMA ----------------
+        const uint32_t tile = warp_uniform(warp - kSoftmax);
         constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         constexpr uint32_t kHi = smem_desc_hi_sw128(1024);
         constexpr uint32_t s_desc = make_idesc(1, kFmt, kFmt, 0, 0, 128, 64);
         const uint32_t o_desc = make_idesc(1, kFmt, kFmt, 0, 1, 128, ksteps * 16);
         constexpr uint32_t kSubStep = 64 * 128 >> 4;  // 64 rows of a box
-        const int row_tiles = two ? 2 : 1;
-        // tile of keys 2 * block, of values 2 * block + 1
-        auto stage_of = [](int load) { return static_cast<uint32_t>(load % S::kStages); };
+        // Counters and descriptors in a form that the compiler knows to be the same in all lanes; with others an MMA takes 60 clocks
+        // to issue, as long as it runs.
+        const int all = static_cast<int>(warp_uniform(steps));
+        const bool alone = warp_uniform(S::kTiles == 2 && !two) != 0;  // frees stages for the row tile that is not there, too
+        const uint32_t q_lo = warp_uniform(smem_desc_lo(smem_base, 16));
+        const uint32_t k_lo = warp_uniform(smem_desc_lo(ring, 16)), v_lo = warp_uniform(smem_desc_lo(ring, S::kBox));
+        const uint32_t bars = warp_uniform(smem_u32(tail));
+        auto bar_of = [&](const uint64_t *bar) { return bars + static_cast<uint32_t>(reinterpret_cast<const uint8_t *>(bar) - reinterpret_cast<const uint8_t *>(tail)); };
+        constexpr uint32_t kStageStep = S::kStage >> 4;
         // The loaders' copies are writes of the generic proxy, which their barrier makes visible here; the fence hands them to the
         // MMA's.
-        auto landed = [&](int load, uint32_t where) {
-            const bool there = mbar_wait(smem_u32(&tail->full[stage_of(load)]), load / S::kStages & 1, abort_flag, where);
-            if (tail->copied[stage_of(load)] != 0) fence_proxy_async_smem();
-            tc_fence_after();
+        auto landed = [&](uint32_t stage, uint32_t phase, uint32_t where) {
+            const bool there = mbar_wait(bar_of(tail->full) + stage * 8, phase, abort_flag, where);
+            if (tail->copied[stage] != 0) fence_proxy_async_smem();
             return there;
         };
-        auto product_s = [&](int tile, int step) {
-            const uint32_t a = smem_desc_lo(smem_base + tile * (S::kBoxes * S::kQueryBox), 16);
-            const uint32_t b = smem_desc_lo(ring + stage_of(step / S::kSub * 2) * S::kStage, 16) + step % S::kSub * kSubStep;
-            const uint32_t d = tmem_base + tile * 128 + (step & 1) * 64;
+        auto product_s = [&](uint32_t odd, uint32_t b) {
+            const uint32_t a = q_lo + tile * (S::kBoxes * S::kQueryBox >> 4);
+            const uint32_t d = tmem_base + tile * 128 + odd * 64;
+            if (S::kBoxes == 2 && ksteps == 8) {
+                mma_ss_x8(d, a, a + (S::kQueryBox >> 4), b, b + (S::kBox >> 4), kHi, s_desc);
+            } else {
 #pragma unroll
-            for (int box = 0; box < S::kBoxes; ++box)
-                if (box * 4 + 4 <= ksteps)
-                    mma_ss_x4(d, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
-            for (int k = ksteps & ~3; k < ksteps; ++k)
-                mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
-                                desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
-            tc_commit_warp(smem_u32(&tail->s_full[tile][step & 1]));
+                for (int box = 0; box < S::kBoxes; ++box)
+                    if (box * 4 + 4 <= ksteps)
+                        mma_ss_x4(d, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
+                for (int k = ksteps & ~3; k < ksteps; ++k)
+                    mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
+                                    desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
+            }
+            tc_commit_warp(bar_of(tail->s_full[0]) + (tile * 2 + odd) * 8);
         };
         // 16 keys a MMA: eight columns of P; 16 rows of 128 bytes of V, its next 64 columns a box further
-        auto product_o = [&](int tile, int step) {
-            mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + tile * 128 + (step & 1) * 64,
-                      smem_desc_lo(ring + stage_of(step / S::kSub * 2 + 1) * S::kStage, S::kBox) + step % S::kSub * kSubStep, kHi, o_desc, step > 0);
-            tc_commit_warp(smem_u32(&tail->o_done[tile][step & 1]));
+        auto product_o = [&](uint32_t odd, uint32_t b, uint32_t accumulate) {
+            mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + tile * 128 + odd * 64, b, kHi, o_desc, accumulate);
+            tc_commit_warp(bar_of(tail->o_done[0]) + (tile * 2 + odd) * 8);
         };
-        // the step is its tile's last: the tile's stage is free when the MMAs so far are done
-        auto release = [&](int step, int load) {
-            if (step % S::kSub == S::kSub - 1) tc_commit_warp(smem_u32(&tail->empty[stage_of(load)]));
-        };
-        bool ok = steps > 0 && mbar_wait(smem_u32(&tail->q_full), 0, abort_flag, 0x91);
-        for (int step = 0; step < min(2, steps) && ok; ++step) {
-            if (step % S::kSub == 0) ok = landed(step / S::kSub * 2, 0x92);
-            if (!ok) break;
-            for (int tile = 0; tile < row_tiles; ++tile) product_s(tile, step);
-            release(step, step / S::kSub * 2);
-        }
-        for (int step = 0; step < steps && ok; ++step) {
-            const int block = step / S::kSub, ahead = step + 2;
-            if (step % S::kSub == 0) ok = landed(block * 2 + 1, 0x93);
-            if (ok && ahead < steps && ahead % S::kSub == 0) ok = landed(ahead / S::kSub * 2, 0x94);
-            for (int tile = 0; tile < row_tiles && ok; ++tile) {
-                ok = mbar_wait(smem_u32(&tail->p_full[tile][step & 1]), (step >> 1) & 1, abort_flag, 0x95);
-                if (!ok) break;
-                tc_fence_after();
-                product_o(tile, step);
-                if (ahead < steps) product_s(tile, ahead);
+        // the tiles of keys and values that the next product takes, and its half of them: keys in the even stages' order
+        uint32_t k_stage = 0, k_phase = 0, k_half = 0, v_stage = 1, v_phase = 0, v_half = 0;
+        auto advance = [&](uint32_t &stage, uint32_t &phase, uint32_t &half) {
+            if (++half < S::kSub) return;
+            half = 0;
+            // its last step: the stage is free when the MMAs so far are done
+            tc_commit_warp(bar_of(tail->empty) + stage * 8);
+            if (alone) tc_commit_warp(bar_of(tail->empty) + stage * 8);
+            stage += 2;
+            if (stage >= S::kStages) {
+                stage -= S::kStages;
+                phase ^= 1;
             }
+        };
+        bool ok = all > 0 && mbar_wait(bar_of(&tail->q_full), 0, abort_flag, 0x91);
+        for (int step = 0; step < 2 && step < all && ok; ++step) {
+            if (k_half == 0) ok = landed(k_stage, k_phase, 0x92);
             if (!ok) break;
-            release(step, block * 2 + 1);
-            if (ahead < steps) release(ahead, ahead / S::kSub * 2);
+            tc_fence_after();
+            product_s(step, k_lo + k_stage * kStageStep + k_half * kSubStep);
+            advance(k_stage, k_phase, k_half);
+        }
+        for (int step = 0; step < all && ok; ++step) {
+            const uint32_t odd = step & 1;
+            const bool ahead = step + 2 < all;
+            if (v_half == 0) ok = landed(v_stage, v_phase, 0x93);
+            if (ok && ahead && k_half == 0) ok = landed(k_stage, k_phase, 0x94);
+            ok = ok && mbar_wait(bar_of(tail->p_full[0]) + (tile * 2 + odd) * 8, (step >> 1) & 1, abort_flag, 0x95);
+            if (!ok) break;
+            tc_fence_after();
+            product_o(odd, v_lo + v_stage * kStageStep + v_half * kSubStep, step > 0);
+            if (ahead) product_s(odd, k_lo + k_stage * kStageStep + k_half * kSubStep);
+            advance(v_stage, v_phase, v_half);
+            if (ahead) advance(k_stage, k_phase, k_half);
         }
     } else if (warp < 8 * S::kTiles) {
         // ---------------- softmax and epilogue: half a row a thread ----------------
