@@ -8,13 +8,17 @@
 // is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
 // maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.
 //
+// A CTA goes on to a further block of the grid, as long as there are blocks that have not begun (cluster launch control), so the
+// hardware's order of the blocks balances the work as it does without; the next item's keys, values and query are fetched, and
+// its first S made, while the softmax ends the present one.  (A CTA an item cost 7 us for each.)
+//
 // Two threads have a row, half of the 64 keys each, and tell each other their maxima through shared memory: four softmax warps a
 // scheduler keep its units busier than two with a whole row a thread (8192 tokens, 32/8 heads of 128: TIMES).
 // S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
 // one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
 // Warps 0..7 and 8..15: softmax and epilogue of the two row tiles.  Warps 16 and 17: MMA, one for each row tile, so
-// that the tensor pipe has the one's products while the other waits at its barriers.  Warps 18 and 19: keys and values.  Where a page
+// that the tensor pipe has the one's products while the other waits at its barriers.  Warps 18 and 19: keys and values.  Warp 20: items, and the query.  Where a page
 // holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
 // and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
@@ -29,7 +33,7 @@ namespace paged {
 namespace {
 
 constexpr int kSoftmax = 16;   // warps
-constexpr int kThreads = 640;
+constexpr int kThreads = 672;
 constexpr int kLoaders = 2;  // warps
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
@@ -51,13 +55,34 @@ struct Shape {
     static constexpr int kRows = kTiles * 128;
 };
 
-constexpr int kValid = 8;  // blocks whose masks are kept: more than may be under way
+// A CTA's rows: `first` + i of a sequence's rows (tokens times heads of a group), and the places that any of them sees.
+struct Tokens {
+    int64_t first;     // a sequence's new tokens: their first row in the query, how many, and the place of the first
+    int count, place;
+};
+struct Item {
+    Tokens tokens;
+    int64_t first, rows;  // this item's first row, and all of the sequence's
+    int b, kvh;
+    int sink_end, lo, hi;
+    int sink_blocks, first_block, blocks;  // tiles of keys that hold places that are seen
+    int split, begin, end;                 // the tiles of this item
+    int steps;                             // of 64 keys
+    int two;                               // the second row tile has rows
+    int none;                              // there is no further item
+};
+
+constexpr int kValid = 8;  // tiles of keys whose masks are kept: more than may be under way
 struct Tail {
     uint64_t full[6], empty[6];
-    uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][step % 2]
+    uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][step % 2]
+    uint64_t o_free[2], q_full, q_empty, item_full[2], item_empty[2], next_full;
     alignas(16) uint32_t valid[kValid][4];
-    uint32_t copied[6];           // stage: by cp.async
-    float half[2][2][2][128];     // [row tile][step % 2][half]: maxima; then sums
+    alignas(16) uint32_t next[4];  // the answer to the request for a further block
+    Item item[2];
+    uint32_t copied[6];            // stage: by cp.async
+    float half[2][2][2][128];      // [row tile][step % 2][half]: maxima; then sums
+    uint32_t going[2][4][2];       // [row tile][quarter][half]: the warp has an item
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -99,11 +124,7 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
     return plan;
 }
 
-// A sequence's new tokens: their first row in the query, how many, and the place of the first.
-struct Tokens {
-    int64_t first;
-    int count, place;
-};
+// A sequence's new tokens.
 __device__ __forceinline__ Tokens tokens_of(const Problem &p, int b) {
     const int64_t from = min(max(static_cast<int64_t>(__ldg(p.start + b)), static_cast<int64_t>(0)), p.tokens);
     const int64_t to = min(max(static_cast<int64_t>(__ldg(p.start + b + 1)), static_cast<int64_t>(0)), p.tokens);
@@ -114,15 +135,6 @@ __device__ __forceinline__ Tokens tokens_of(const Problem &p, int b) {
     t.place = static_cast<int>(max(place, -static_cast<int64_t>(0x7fffffff)));
     return t;
 }
-
-// A CTA's rows: `first` + i, token first / group and so on; the places that any of them sees, as blocks.
-struct Item {
-    Tokens tokens;
-    int b, kvh;
-    int64_t first, rows;  // of the sequence's rows: this CTA's first, and all
-    int sink_end, lo, hi;
-    int sink_blocks, first_block, blocks;
-};
 
 __device__ __forceinline__ int place_of(const Problem &p, const Tokens &t, int64_t row) {
     const int64_t at = t.place + row / p.group;
@@ -353,6 +365,29 @@ __device__ __forceinline__ void tma_load_4d_warp(uint32_t dst, const CUtensorMap
         "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(column), "r"(place), "r"(head), "r"(page)
         : "memory");
 }
+// Asks for a block of the grid that has not begun, in its place; the answer, 16 bytes, is counted on the barrier.
+__device__ __forceinline__ void ask_next_block(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ bool next_block(uint32_t answer, uint32_t *block) {
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b128 a;\n\t"
+        "ld.shared.b128 a, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t"
+        "}\n"
+        : "=r"(got), "=r"(x)
+        : "r"(answer)
+        : "memory");
+    *block = x;
+    return got != 0;
+}
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -362,9 +397,26 @@ __device__ __forceinline__ uint32_t bits(int from, int to) {
     return from <= 0 ? low : from >= 32 ? 0u : low & (0xffffffffu << from);
 }
 
+// Tokens of no sequence: block `id`'s part of them.
+template <typename T>
+__device__ __noinline__ void clear_rest(const Problem &p, const Scratch &scratch, int64_t id, int64_t blocks) {
+    const int lane = threadIdx.x & 31;
+    const int64_t head = p.batch > 0 ? min(max(static_cast<int64_t>(__ldg(p.start)), static_cast<int64_t>(0)), p.tokens) : p.tokens;
+    const int64_t end = p.batch > 0 ? min(max(static_cast<int64_t>(__ldg(p.start + p.batch)), head), p.tokens) : p.tokens;
+    const int64_t none = head + p.tokens - end;
+    for (int64_t i = id; i < none; i += blocks) {
+        const int64_t token = i < head ? i : end + i - head;
+        for (int h = 0; h < p.heads; ++h) empty_row<T>(p, token, h);
+        if (scratch.splits > 1)
+            for (int64_t h = lane; h < static_cast<int64_t>(p.heads) * scratch.splits; h += 32)
+                scratch.stat[h / p.heads * p.tokens * p.heads + token * p.heads + h % p.heads] = make_float2(-INFINITY, 0.0f);
+    }
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, const __grid_constant__ CUtensorMap tmap_k,
-              const __grid_constant__ CUtensorMap tmap_v, int box_rows) {
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, const __grid_constant__ CUtensorMap tmap_k,
+              const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_q, int box_rows, bool box_query) {
     using S = Shape<DP>;
     constexpr int BN = S::kBN;
     extern __shared__ uint8_t smem_raw[];
@@ -378,20 +430,28 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(smem_u32(&tail->full[s]), kLoaders * 33);  // every lane's copies, and the lookup
-            mbar_init(smem_u32(&tail->empty[s]), S::kTiles);  // every row tile's products
+            mbar_init(smem_u32(&tail->empty[s]), S::kTiles);     // every row tile's products
         }
-        mbar_init(smem_u32(&tail->q_full), 8 * S::kTiles);
         for (int i = 0; i < 4; ++i) {
             mbar_init(smem_u32(&tail->s_full[i >> 1][i & 1]), 1);
             mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 8);
             mbar_init(smem_u32(&tail->o_done[i >> 1][i & 1]), 1);
         }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&tail->o_free[i]), 8);
+            mbar_init(smem_u32(&tail->item_full[i]), 1);
+            mbar_init(smem_u32(&tail->item_empty[i]), 9 * S::kTiles + kLoaders);  // the warps that take items
+        }
+        mbar_init(smem_u32(&tail->q_full), 33);
+        mbar_init(smem_u32(&tail->q_empty), S::kTiles);
+        mbar_init(smem_u32(&tail->next_full), 1);
         tail->abort_flag = 0;
         mbar_fence_init();
         if (box_rows > 0) {
             tma_prefetch_desc(&tmap_k);
             tma_prefetch_desc(&tmap_v);
         }
+        if (box_query) tma_prefetch_desc(&tmap_q);
     }
     if (warp == kSoftmax) {
         tmem_alloc(smem_u32(&tail->tmem_base), 512);
@@ -404,38 +464,103 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const uint32_t tmem_base = warp_uniform(tail->tmem_base);
     pdl_wait();
 
-    // tokens of no sequence
-    {
-        const int64_t head = p.batch > 0 ? min(max(static_cast<int64_t>(__ldg(p.start)), static_cast<int64_t>(0)), p.tokens) : p.tokens;
-        const int64_t end = p.batch > 0 ? min(max(static_cast<int64_t>(__ldg(p.start + p.batch)), head), p.tokens) : p.tokens;
-        const int64_t none = head + p.tokens - end;
-        for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + warp; i < none; i += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
-            const int64_t token = i < head ? i : end + i - head;
-            for (int h = 0; h < p.heads; ++h) empty_row<T>(p, token, h);
-            if (scratch.splits > 1)
-                for (int64_t h = lane; h < static_cast<int64_t>(p.heads) * scratch.splits; h += 32)
-                    scratch.stat[h / p.heads * p.tokens * p.heads + token * p.heads + h % p.heads] = make_float2(-INFINITY, 0.0f);
-        }
-    }
-
-    const int split = blockIdx.x % scratch.splits;
-    Item it;
-    it.kvh = blockIdx.x / scratch.splits % p.kv_heads;
-    const bool found = find_item<BN, S::kRows>(p, blockIdx.x / scratch.splits / p.kv_heads, it);
-    const int begin = found ? static_cast<int>(static_cast<int64_t>(it.blocks) * split / scratch.splits) : 0;
-    const int end = found ? static_cast<int>(static_cast<int64_t>(it.blocks) * (split + 1) / scratch.splits) : 0;
-    const bool two = S::kTiles == 2 && found && it.first + 128 < it.rows;  // the second row tile has rows
-    // steps of 64 keys; the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
-    int steps = (end - begin) * S::kSub;
-    if (S::kSub == 2 && end > begin) {
-        const int last = block_start<BN>(it, end - 1);
-        if (last + 64 >= (end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --steps;
-    }
     const int ksteps = (p.dim + 15) / 16;
     const float factor = p.scale * kLog2e;
+    // the `n`-th item of this CTA; and its slot free again
+    auto take = [&](int n) { return mbar_wait(smem_u32(&tail->item_full[n & 1]), (n >> 1) & 1, abort_flag, 0x9d); };
+    auto release = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&tail->item_empty[n & 1]));
+    };
 
-    if (!found) {
-        // nothing to do
+    if (warp == kSoftmax + 4) {
+        // ---------------- items, and the query ----------------
+        uint32_t id = blockIdx.x;
+        bool have = true, ok = true;
+        uint32_t asked = 0, queries = 0;
+        int n = 0;
+        while (ok) {
+            if (have && lane == 0) {
+                mbar_expect_tx(smem_u32(&tail->next_full), 16);
+                ask_next_block(smem_u32(tail->next), smem_u32(&tail->next_full));
+            }
+            __syncwarp();
+            Item it;
+            bool found = false;
+            if (have) {
+                clear_rest<T>(p, scratch, id, gridDim.x);
+                it.split = id % scratch.splits;
+                it.kvh = id / scratch.splits % p.kv_heads;
+                found = find_item<BN, S::kRows>(p, id / scratch.splits / p.kv_heads, it);
+            }
+            if (found || !have) {
+                ok = mbar_wait(smem_u32(&tail->item_empty[n & 1]), (n >> 1 & 1) ^ 1, abort_flag, 0x9e);
+                if (!ok) break;
+                if (found) {
+                    it.begin = static_cast<int>(static_cast<int64_t>(it.blocks) * it.split / scratch.splits);
+                    it.end = static_cast<int>(static_cast<int64_t>(it.blocks) * (it.split + 1) / scratch.splits);
+                    it.two = S::kTiles == 2 && it.first + 128 < it.rows;
+                    // the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
+                    it.steps = (it.end - it.begin) * S::kSub;
+                    if (S::kSub == 2 && it.end > it.begin) {
+                        const int last = block_start<BN>(it, it.end - 1);
+                        if (last + 64 >= (it.end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --it.steps;
+                    }
+                }
+                it.none = !found;
+                if (lane == 0) {
+                    tail->item[n & 1] = it;
+                    mbar_arrive(smem_u32(&tail->item_full[n & 1]));
+                }
+                __syncwarp();
+                ++n;
+            }
+            if (!have) break;
+            if (found && it.steps > 0) {
+                ok = mbar_wait(smem_u32(&tail->q_empty), (queries & 1) ^ 1, abort_flag, 0x9f);
+                if (!ok) break;
+                ++queries;
+                const uint32_t bar = smem_u32(&tail->q_full);
+                const int tiles = it.two ? 2 : 1;
+                if (box_query) {
+                    if (lane == 0) {
+                        mbar_expect_tx(bar, tiles * S::kBoxes * S::kQueryBox);
+                        mbar_arrive_n(bar, 32);
+                    }
+                    __syncwarp();
+                    for (int tile = 0; tile < tiles; ++tile) {
+                        const int token = static_cast<int>(it.tokens.first + (it.first + tile * 128) / p.group);
+#pragma unroll
+                        for (int column = 0; column < S::kBoxes; ++column)
+                            tma_load_4d_warp(smem_base + (tile * S::kBoxes + column) * S::kQueryBox, &tmap_q, column * 64, 0, it.kvh, token, bar);
+                    }
+                } else {
+                    // row by row: 16-byte chunks into 128-byte rows, swizzled; zeros behind the sequence's rows
+                    constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
+                    const int chunk = lane % kChunks;
+                    const bool mine = chunk < 2 * ksteps, there = chunk * 8 < p.dim;
+                    const T *q = static_cast<const T *>(p.q) + it.kvh * p.group * p.q_sh + (there ? chunk * 8 : 0);
+                    int64_t token = (it.first + lane / kChunks) / p.group;
+                    int head = static_cast<int>(it.first + lane / kChunks - token * p.group);
+                    for (int r = lane / kChunks; r < tiles * 128; r += kStep) {
+                        const bool row = it.first + r < it.rows;
+                        if (mine)
+                            cp_async_16(smem_base + ((r >> 7) * S::kBoxes + chunk / 8) * S::kQueryBox + (r & 127) * 128 + (((chunk ^ r) & 7) << 4),
+                                        row ? q + (it.tokens.first + token) * p.q_st + head * p.q_sh : q, row && there ? 16 : 0);
+                        for (head += kStep; head >= p.group; head -= p.group) ++token;
+                    }
+                    cp_async_arrive(bar);
+                    if (lane == 0) mbar_arrive(bar);
+                }
+            }
+            ok = mbar_wait(smem_u32(&tail->next_full), asked & 1, abort_flag, 0x8f);
+            if (!ok) break;
+            ++asked;
+            have = next_block(smem_u32(tail->next), &id);
+            fence_proxy_async_smem();  // read before the next answer is written
+            __syncwarp();
+        }
+        cp_async_wait_all();
     } else if (warp >= kSoftmax + 2) {
         // ---------------- keys and values ----------------
         const int loader = warp - kSoftmax - 2;
@@ -446,107 +571,113 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const bool my_part = my_chunk < 2 * ksteps;
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
-        uint32_t stage = 0, phase = 0;
-        bool ok = true;
-        // Boxes: a warp fetches every third.  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
+        // Boxes: a warp fetches every second.  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
         constexpr int kMost = (BN / 16 + kLoaders - 1) / kLoaders;
         int mine = 0;
         for (int n = loader; n < boxes; n += kLoaders) ++mine;
         const uint32_t my_bytes = mine * S::kBoxes * box_rows * 128;
-        int next_id = -1, next_at = 0;
-        auto look_up = [&](int i) {
-            if (lane >= boxes) return;
-            const int j = block_start<BN>(it, i) + lane * box_rows;
-            next_id = -1;
-            if (j < p.capacity) {
-                const int page = page_of(p, j);
-                next_at = j - page * p.page;
-                next_id = __ldg(p.table + it.b * p.table_st + page);
-            }
-        };
-        if (begin < end) look_up(begin);
-        for (int i = begin; i < end && ok; ++i) {
-            const int first = block_start<BN>(it, i);
-            const bool whole = boxes > 0 && (first + BN <= it.sink_end || (first >= it.lo && first + BN <= it.hi)) &&
-                               __all_sync(0xffffffffu, lane >= boxes || (next_id >= 0 && next_id < p.pages));
-            uint32_t mask[kLooks];
-            int id[kLooks], at[kLooks], box_page[kMost], box_place[kMost];
-            if (whole) {
-#pragma unroll
-                for (int n = 0; n < kMost; ++n) {
-                    const int box = loader + n * kLoaders;
-                    box_page[n] = __shfl_sync(0xffffffffu, next_id, box);
-                    box_place[n] = __shfl_sync(0xffffffffu, next_at, box);
+        uint32_t stage = 0, phase = 0, count = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            ok = take(n);
+            if (!ok || tail->item[n & 1].none) break;
+            const Item it = tail->item[n & 1];
+            release(n);
+            int next_id = -1, next_at = 0;
+            auto look_up = [&](int i) {
+                if (lane >= boxes) return;
+                const int j = block_start<BN>(it, i) + lane * box_rows;
+                next_id = -1;
+                if (j < p.capacity) {
+                    const int page = page_of(p, j);
+                    next_at = j - page * p.page;
+                    next_id = __ldg(p.table + it.b * p.table_st + page);
                 }
-            } else {
-#pragma unroll
-                for (int l = 0; l < kLooks; ++l) {
-                    const int j = first + 32 * l + lane;
-                    int64_t block = 0;
-                    at[l] = 0;
-                    const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at[l]);
-                    id[l] = static_cast<int>(block);
-                    mask[l] = __ballot_sync(0xffffffffu, seen);
-                }
-            }
-            if (i + 1 < end) look_up(i + 1);
-            for (int part = 0; part < 2; ++part) {
-                ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
-                if (!ok) break;
-                const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
+            };
+            if (it.begin < it.end) look_up(it.begin);
+            for (int i = it.begin; i < it.end && ok; ++i, ++count) {
+                const int first = block_start<BN>(it, i);
+                const bool whole = boxes > 0 && (first + BN <= it.sink_end || (first >= it.lo && first + BN <= it.hi)) &&
+                                   __all_sync(0xffffffffu, lane >= boxes || (next_id >= 0 && next_id < p.pages));
+                uint32_t mask[kLooks];
+                int id[kLooks], at[kLooks], box_page[kMost], box_place[kMost];
                 if (whole) {
-                    if (lane == 0) {
-                        if (loader == 0) {
-                            if (part == 0) *reinterpret_cast<uint4 *>(tail->valid[i % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
-                            tail->copied[stage] = 0;
-                        }
-                        mbar_expect_tx(bar, my_bytes);
-                        mbar_arrive_n(bar, 32);
-                    }
-                    __syncwarp();
-                    const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
 #pragma unroll
-                    for (int n = 0; n < kMost; ++n) {
-                        const int box = loader + n * kLoaders;
-                        if (box >= boxes) break;
-#pragma unroll
-                        for (int column = 0; column < S::kBoxes; ++column)
-                            tma_load_4d_warp(dst + column * S::kBox + box * box_rows * 128, map, column * 64, box_place[n], it.kvh, box_page[n], bar);
+                    for (int k = 0; k < kMost; ++k) {
+                        const int box = loader + k * kLoaders;
+                        box_page[k] = __shfl_sync(0xffffffffu, next_id, box);
+                        box_place[k] = __shfl_sync(0xffffffffu, next_at, box);
                     }
                 } else {
-                    if (loader == 0 && lane == 0) {
-                        tail->copied[stage] = 1;
 #pragma unroll
-                        for (int l = 0; part == 0 && l < kLooks; ++l) tail->valid[i % kValid][l] = mask[l];
+                    for (int l = 0; l < kLooks; ++l) {
+                        const int j = first + 32 * l + lane;
+                        int64_t block = 0;
+                        at[l] = 0;
+                        const bool seen = j < it.hi && (j < it.sink_end || j >= it.lo) && find_place(p, it.b, j, &block, &at[l]);
+                        id[l] = static_cast<int>(block);
+                        mask[l] = __ballot_sync(0xffffffffu, seen);
                     }
-                    const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
-                    const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
-#pragma unroll
-                    for (int group = 0; group < BN / 16; ++group) {
-                        if (group % kLoaders != loader) continue;
-                        const int l = group / 2;
-                        const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
-#pragma unroll
-                        for (int r = 0; r < 16; r += kStep) {
-                            const int key = group * 16 % 32 + r + my_key;
-                            const T *row = base + __shfl_sync(0xffffffffu, offset, key);
-                            if (my_part)
-                                cp_async_16(dst + my_box + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
-                                            my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
-                        }
-                    }
-                    cp_async_arrive(bar);
-                    if (lane == 0) mbar_arrive(bar);
                 }
-                if (++stage == S::kStages) {
-                    stage = 0;
-                    phase ^= 1;
+                if (i + 1 < it.end) look_up(i + 1);
+                for (int part = 0; part < 2; ++part) {
+                    ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
+                    if (!ok) break;
+                    const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
+                    if (whole) {
+                        if (lane == 0) {
+                            if (loader == 0) {
+                                if (part == 0) *reinterpret_cast<uint4 *>(tail->valid[count % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
+                                tail->copied[stage] = 0;
+                            }
+                            mbar_expect_tx(bar, my_bytes);
+                            mbar_arrive_n(bar, 32);
+                        }
+                        __syncwarp();
+                        const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
+#pragma unroll
+                        for (int k = 0; k < kMost; ++k) {
+                            const int box = loader + k * kLoaders;
+                            if (box >= boxes) break;
+#pragma unroll
+                            for (int column = 0; column < S::kBoxes; ++column)
+                                tma_load_4d_warp(dst + column * S::kBox + box * box_rows * 128, map, column * 64, box_place[k], it.kvh, box_page[k], bar);
+                        }
+                    } else {
+                        if (loader == 0 && lane == 0) {
+                            tail->copied[stage] = 1;
+#pragma unroll
+                            for (int l = 0; part == 0 && l < kLooks; ++l) tail->valid[count % kValid][l] = mask[l];
+                        }
+                        const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
+                        const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
+#pragma unroll
+                        for (int group = 0; group < BN / 16; ++group) {
+                            if (group % kLoaders != loader) continue;
+                            const int l = group / 2;
+                            const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
+#pragma unroll
+                            for (int r = 0; r < 16; r += kStep) {
+                                const int key = group * 16 % 32 + r + my_key;
+                                const T *row = base + __shfl_sync(0xffffffffu, offset, key);
+                                if (my_part)
+                                    cp_async_16(dst + my_box + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
+                                                my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
+                            }
+                        }
+                        cp_async_arrive(bar);
+                        if (lane == 0) mbar_arrive(bar);
+                    }
+                    if (++stage == S::kStages) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
             }
         }
         cp_async_wait_all();
-    } else if (warp == kSoftmax || (S::kTiles == 2 && warp == kSoftmax + 1 && two)) {
+    } else if (warp >= kSoftmax && warp < kSoftmax + S::kTiles) {
         // ---------------- MMA ----------------
         const uint32_t tile = warp_uniform(warp - kSoftmax);
         constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -554,11 +685,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         constexpr uint32_t s_desc = make_idesc(1, kFmt, kFmt, 0, 0, 128, 64);
         const uint32_t o_desc = make_idesc(1, kFmt, kFmt, 0, 1, 128, ksteps * 16);
         constexpr uint32_t kSubStep = 64 * 128 >> 4;  // 64 rows of a box
-        // Counters and descriptors in a form that the compiler knows to be the same in all lanes; with others an MMA takes 60 clocks
-        // to issue, as long as it runs.
-        const int all = static_cast<int>(warp_uniform(steps));
-        const bool alone = warp_uniform(S::kTiles == 2 && !two) != 0;  // frees stages for the row tile that is not there, too
-        const uint32_t q_lo = warp_uniform(smem_desc_lo(smem_base, 16));
+        // Counters and descriptors in a form that the compiler knows to be the same in all lanes
+        const uint32_t q_lo = warp_uniform(smem_desc_lo(smem_base, 16)) + tile * (S::kBoxes * S::kQueryBox >> 4);
         const uint32_t k_lo = warp_uniform(smem_desc_lo(ring, 16)), v_lo = warp_uniform(smem_desc_lo(ring, S::kBox));
         const uint32_t bars = warp_uniform(smem_u32(tail));
         auto bar_of = [&](const uint64_t *bar) { return bars + static_cast<uint32_t>(reinterpret_cast<const uint8_t *>(bar) - reinterpret_cast<const uint8_t *>(tail)); };
@@ -571,17 +699,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             return there;
         };
         auto product_s = [&](uint32_t odd, uint32_t b) {
-            const uint32_t a = q_lo + tile * (S::kBoxes * S::kQueryBox >> 4);
             const uint32_t d = tmem_base + tile * 128 + odd * 64;
             if (S::kBoxes == 2 && ksteps == 8) {
-                mma_ss_x8(d, a, a + (S::kQueryBox >> 4), b, b + (S::kBox >> 4), kHi, s_desc);
+                mma_ss_x8(d, q_lo, q_lo + (S::kQueryBox >> 4), b, b + (S::kBox >> 4), kHi, s_desc);
             } else {
 #pragma unroll
                 for (int box = 0; box < S::kBoxes; ++box)
                     if (box * 4 + 4 <= ksteps)
-                        mma_ss_x4(d, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
+                        mma_ss_x4(d, q_lo + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
                 for (int k = ksteps & ~3; k < ksteps; ++k)
-                    mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
+                    mma_f16_ss_warp(d, desc64(q_lo + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
                                     desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
             }
             tc_commit_warp(bar_of(tail->s_full[0]) + (tile * 2 + odd) * 8);
@@ -591,12 +718,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + tile * 128 + odd * 64, b, kHi, o_desc, accumulate);
             tc_commit_warp(bar_of(tail->o_done[0]) + (tile * 2 + odd) * 8);
         };
-        // the tiles of keys and values that the next product takes, and its half of them: keys in the even stages' order
+        // The tiles of keys and values that the next product takes, and its half of them: keys in the even stages, values in the
+        // odd ones.  A stage is free when the products so far of both row tiles are done; of one that is not there, too.
         uint32_t k_stage = 0, k_phase = 0, k_half = 0, v_stage = 1, v_phase = 0, v_half = 0;
-        auto advance = [&](uint32_t &stage, uint32_t &phase, uint32_t &half) {
-            if (++half < S::kSub) return;
-            half = 0;
-            // its last step: the stage is free when the MMAs so far are done
+        bool alone = false;
+        auto leave = [&](uint32_t &stage, uint32_t &phase) {
             tc_commit_warp(bar_of(tail->empty) + stage * 8);
             if (alone) tc_commit_warp(bar_of(tail->empty) + stage * 8);
             stage += 2;
@@ -605,171 +731,195 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 phase ^= 1;
             }
         };
-        bool ok = all > 0 && mbar_wait(bar_of(&tail->q_full), 0, abort_flag, 0x91);
-        for (int step = 0; step < 2 && step < all && ok; ++step) {
-            if (k_half == 0) ok = landed(k_stage, k_phase, 0x92);
-            if (!ok) break;
-            tc_fence_after();
-            product_s(step, k_lo + k_stage * kStageStep + k_half * kSubStep);
-            advance(k_stage, k_phase, k_half);
-        }
-        for (int step = 0; step < all && ok; ++step) {
-            const uint32_t odd = step & 1;
-            const bool ahead = step + 2 < all;
-            if (v_half == 0) ok = landed(v_stage, v_phase, 0x93);
-            if (ok && ahead && k_half == 0) ok = landed(k_stage, k_phase, 0x94);
-            ok = ok && mbar_wait(bar_of(tail->p_full[0]) + (tile * 2 + odd) * 8, (step >> 1) & 1, abort_flag, 0x95);
-            if (!ok) break;
-            tc_fence_after();
-            product_o(odd, v_lo + v_stage * kStageStep + v_half * kSubStep, step > 0);
-            if (ahead) product_s(odd, k_lo + k_stage * kStageStep + k_half * kSubStep);
-            advance(v_stage, v_phase, v_half);
-            if (ahead) advance(k_stage, k_phase, k_half);
+        auto advance = [&](uint32_t &stage, uint32_t &phase, uint32_t &half) {
+            if (++half < S::kSub) return;
+            half = 0;
+            leave(stage, phase);
+        };
+        uint32_t done = 0;               // steps of this row tile
+        uint32_t queries = 0, outs = 0;  // items with a query; items of this row tile
+        uint32_t taken = 0;              // tiles of keys
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            ok = take(n);
+            if (!ok || tail->item[n & 1].none) break;
+            const int all = static_cast<int>(warp_uniform(tail->item[n & 1].steps));
+            const bool two = warp_uniform(tail->item[n & 1].two) != 0;
+            const int tiles = static_cast<int>(warp_uniform(tail->item[n & 1].end - tail->item[n & 1].begin));
+            release(n);
+            if (all == 0) continue;
+            if (tile == 1 && !two) {  // the other row tile frees what this one does not take
+                ++queries;
+                taken += tiles;
+                k_stage = warp_uniform(taken % (S::kStages / 2) * 2);
+                v_stage = k_stage + 1;
+                k_phase = v_phase = warp_uniform(taken / (S::kStages / 2) & 1);
+                continue;
+            }
+            taken += tiles;
+            alone = S::kTiles == 2 && !two;
+            ok = mbar_wait(bar_of(&tail->q_full), queries & 1, abort_flag, 0x91);
+            if (!box_query) fence_proxy_async_smem();
+            ++queries;
+            auto query_taken = [&] {
+                tc_commit_warp(bar_of(&tail->q_empty));
+                if (alone) tc_commit_warp(bar_of(&tail->q_empty));
+            };
+            for (int step = 0; step < 2 && step < all && ok; ++step) {
+                if (k_half == 0) ok = landed(k_stage, k_phase, 0x92);
+                if (!ok) break;
+                tc_fence_after();
+                product_s((done + step) & 1, k_lo + k_stage * kStageStep + k_half * kSubStep);
+                if (step + 1 == all) query_taken();
+                advance(k_stage, k_phase, k_half);
+            }
+            // the softmax has read the O of the item before
+            if (ok && outs > 0) ok = mbar_wait(bar_of(tail->o_free) + tile * 8, (outs - 1) & 1, abort_flag, 0x93);
+            ++outs;
+            for (int step = 0; step < all && ok; ++step, ++done) {
+                const uint32_t odd = done & 1;
+                const bool ahead = step + 2 < all;
+                if (v_half == 0) ok = landed(v_stage, v_phase, 0x94);
+                if (ok && ahead && k_half == 0) ok = landed(k_stage, k_phase, 0x95);
+                ok = ok && mbar_wait(bar_of(tail->p_full[0]) + (tile * 2 + odd) * 8, (done >> 1) & 1, abort_flag, 0x96);
+                if (!ok) break;
+                tc_fence_after();
+                product_o(odd, v_lo + v_stage * kStageStep + v_half * kSubStep, step > 0);
+                if (ahead) {
+                    product_s(odd, k_lo + k_stage * kStageStep + k_half * kSubStep);
+                    if (step + 3 == all) query_taken();
+                }
+                advance(v_stage, v_phase, v_half);
+                if (ahead) advance(k_stage, k_phase, k_half);
+            }
+            // tiles whose second half was not taken
+            if (ok && k_half != 0) {
+                k_half = v_half = 0;
+                leave(k_stage, k_phase);
+                leave(v_stage, v_phase);
+            }
         }
     } else if (warp < 8 * S::kTiles) {
         // ---------------- softmax and epilogue: half a row a thread ----------------
-        const int tile = warp >> 3, half = (warp >> 2) & 1;
-        const int64_t row0 = it.first + tile * 128 + (warp & 3) * 32;  // this warp's first row
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        if (end > begin) {
-            // the warp's rows of the query: 16-byte chunks into 128-byte rows, swizzled; the scale's sign and zero go with them
-            const uint32_t with = factor == 0.0f ? 0u : 0xffffffffu, flip = factor < 0.0f ? 0x80008000u : 0u;
-            constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
-            const int chunk = lane % kChunks;
-            uint8_t *dst = smem + (tile * S::kBoxes + chunk / 8) * S::kQueryBox;
-#pragma unroll 4
-            for (int r = half; r < 32 / kStep; r += 2) {
-                const int local = r * kStep + lane / kChunks, row = (warp & 3) * 32 + local;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row0 + local < it.rows && chunk * 8 < p.dim) {
-                    const int64_t token = (row0 + local) / p.group;
-                    const int head = it.kvh * p.group + static_cast<int>(row0 + local - token * p.group);
-                    v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (it.tokens.first + token) * p.q_st + head * p.q_sh + chunk * 8));
-                }
-                if (chunk < 2 * ksteps)
-                    *reinterpret_cast<uint4 *>(dst + row * 128 + (((chunk ^ row) & 7) << 4)) =
-                        make_uint4((v.x & with) ^ flip, (v.y & with) ^ flip, (v.z & with) ^ flip, (v.w & with) ^ flip);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&tail->q_full));
-        }
-        const int64_t my_row = row0 + lane;
-        const bool mine = my_row < it.rows;
-        const int place = mine ? place_of(p, it.tokens, my_row) : -1;
-        const Range range = visible_range(p, place);
-        const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
-        const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
-        const float scale = factor == 0.0f ? 1.0f : fabsf(factor);
-        float base = -INFINITY;  // unscaled
-        float2 sum2 = make_float2(0.0f, 0.0f);
-        bool ok = true;
-        const bool works = end > begin && (tile == 0 || two);
-        const int my_lane = (warp & 3) * 32 + lane;
+        const int tile = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const int my_lane = quarter * 32 + lane;
+        // The running maximum is one of unscaled scores, which takes a positive scale: with a negative one, or 0, the scores take its
+        // sign.
+        const float scale = factor == 0.0f ? 1.0f : fabsf(factor), sign = factor < 0.0f ? -1.0f : 0.0f;
         // the two warps that share rows
-        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + (warp & 3)) : "memory"); };
+        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quarter) : "memory"); };
         const int o_from = half == 0 ? 0 : (ksteps + 1) / 2, o_to = half == 0 ? (ksteps + 1) / 2 : ksteps;  // 16 columns of O each
-        for (int n = 0; n < steps && works; ++n) {
-            const int i = begin + n / S::kSub;
-            // a wait that gave up ends the waits, not the steps: the warps of a row meet in every one
-            ok = ok && mbar_wait(smem_u32(&tail->s_full[tile][n & 1]), (n >> 1) & 1, abort_flag, 0x98);
-            // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
-            if (n > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][n & 1]), ((n - 2) >> 1) & 1, abort_flag, 0x9b);
-            tc_fence_after();
-            const uint32_t s_addr = tmem_base + lanes + tile * 128 + (n & 1) * 64;
-            uint32_t s[32];
-            tmem_ld_32x32(s_addr + half * 32, s);
-            const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[i % kValid][n % S::kSub * 2]);
-            const int start = block_start<BN>(it, i) + n % S::kSub * 64;
-            const bool whole = (start + 64 <= first_range.sink_end || (start >= last_range.lo && start + 64 <= first_range.hi)) &&
-                               (valid.x & valid.y) == 0xffffffffu;
-            tmem_ld_wait();
-            if (!whole) {
-                const int at = start + half * 32;
-                const uint32_t see = (half == 0 ? valid.x : valid.y) & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (!(see >> j & 1)) s[j] = 0xff800000u;  // -inf
-            }
-            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) m[c] = max3(m[c], __uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1]));
-            }
-            float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
-            tail->half[tile][n & 1][half][my_lane] = most;
-            tc_fence_before();  // the other half's P comes where this one's S was
+        uint32_t done = 0, count = 0;  // steps of this row tile; tiles of keys
+        for (int item = 0;; ++item) {
+            // A wait that gave up ends the warps of a row together; inside an item it ends the waits, not the steps, for the warps meet
+            // in every one.
+            bool ok = take(item);
+            if (lane == 0) tail->going[tile][quarter][half] = ok && !tail->item[item & 1].none;
             meet();
-            tc_fence_after();
-            most = fmaxf(most, tail->half[tile][n & 1][half ^ 1][my_lane]);
-            const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
-            if (__any_sync(0xffffffffu, move)) {
-                const float now = move ? most : base;
-                const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
-                sum2 = mul2(sum2, make_float2(keep, keep));
-                if (n > 0) {
-                    ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][(n - 1) & 1]), ((n - 1) >> 1) & 1, abort_flag, 0x99);
-                    tc_fence_after();
-                    for (int c = o_from; c < o_to; ++c) {
-                        uint32_t o[16];
-                        const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
-                        tmem_ld_32x16(addr, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                        tmem_st_32x16(addr, o);
-                    }
-                }
-                base = now;
-            }
-            const float offset = base == -INFINITY ? 0.0f : -base * scale;
-            const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
-            // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another; the sum
-            // takes the weights unrounded
-            uint32_t w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float2 x = fma2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, offset2);
-                const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                sum2 = add2(sum2, e);
-                w[j] = pack2<T>(e.x, e.y);
-            }
-            tmem_st_32x16(s_addr + half * 16, w);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile][n & 1]));
-        }
-        // the places of the step before the last, which both warps have read
-        tail->half[tile][steps & 1][half][my_lane] = sum2.x + sum2.y;
-        meet();
-        const float sum = tail->half[tile][steps & 1][0][my_lane] + tail->half[tile][steps & 1][1][my_lane];
-        const float top = base * scale;
-        const int64_t token = my_row / p.group;
-        const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
-        const int64_t out_row = (it.tokens.first + token) * p.heads + head;
-        if (works) {
-            const int last = steps - 1;
-            ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][last & 1]), (last >> 1) & 1, abort_flag, 0x9a);
-            tc_fence_after();
-        }
-        if (scratch.splits > 1) {
-            const int64_t at = (static_cast<int64_t>(split) * p.tokens * p.heads) + out_row;
-            if (mine && half == 0) scratch.stat[at] = make_float2(top, sum);
-            for (int c = o_from; c < o_to && works; ++c) {
-                uint32_t o[16];
-                tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
+            const bool go = tail->going[tile][quarter][0] != 0 && tail->going[tile][quarter][1] != 0;
+            meet();
+            if (!go) break;
+            const Item &it = tail->item[item & 1];
+            const int64_t row0 = it.first + tile * 128 + quarter * 32;  // this warp's first row
+            const int64_t my_row = row0 + lane;
+            const bool mine = my_row < it.rows;
+            const Range range = visible_range(p, mine ? place_of(p, it.tokens, my_row) : -1);
+            const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
+            const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
+            float base = -INFINITY;  // unscaled
+            float2 sum2 = make_float2(0.0f, 0.0f);
+            const int steps = it.steps;
+            const bool works = steps > 0 && (tile == 0 || it.two);
+            for (int n = 0; n < steps && works; ++n, ++done) {
+                const int i = it.begin + n / S::kSub;
+                const uint32_t odd = done & 1;
+                ok = ok && mbar_wait(smem_u32(&tail->s_full[tile][odd]), (done >> 1) & 1, abort_flag, 0x98);
+                // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
+                if (done > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][odd]), ((done - 2) >> 1) & 1, abort_flag, 0x9b);
+                tc_fence_after();
+                const uint32_t s_addr = tmem_base + lanes + tile * 128 + odd * 64;
+                uint32_t s[32];
+                tmem_ld_32x32(s_addr + half * 32, s);
+                const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[(count + n / S::kSub) % kValid][n % S::kSub * 2]);
+                const int start = block_start<BN>(it, i) + n % S::kSub * 64;
+                const bool whole = (start + 64 <= first_range.sink_end || (start >= last_range.lo && start + 64 <= first_range.hi)) &&
+                                   (valid.x & valid.y) == 0xffffffffu;
                 tmem_ld_wait();
-                if (mine) {
-                    float *dst = scratch.part + at * p.dim + c * 16;
+                if (factor <= 0.0f) {
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4)
-                        if (c * 16 + j < p.dim) *reinterpret_cast<uint4 *>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    for (int j = 0; j < 32; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) * sign);
                 }
+                if (!whole) {
+                    const int at = start + half * 32;
+                    const uint32_t see = (half == 0 ? valid.x : valid.y) & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (!(see >> j & 1)) s[j] = 0xff800000u;  // -inf
+                }
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) m[c] = max3(m[c], __uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1]));
+                }
+                float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+                tail->half[tile][odd][half][my_lane] = most;
+                tc_fence_before();  // the other half's P comes where this one's S was
+                meet();
+                tc_fence_after();
+                most = fmaxf(most, tail->half[tile][odd][half ^ 1][my_lane]);
+                const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+                if (__any_sync(0xffffffffu, move)) {
+                    const float now = move ? most : base;
+                    const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                    sum2 = mul2(sum2, make_float2(keep, keep));
+                    if (n > 0) {
+                        ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
+                        tc_fence_after();
+                        for (int c = o_from; c < o_to; ++c) {
+                            uint32_t o[16];
+                            const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
+                            tmem_ld_32x16(addr, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_st_32x16(addr, o);
+                        }
+                    }
+                    base = now;
+                }
+                const float offset = base == -INFINITY ? 0.0f : -base * scale;
+                const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+                // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another; the
+                // sum takes the weights unrounded
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float2 x = fma2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, offset2);
+                    const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                    sum2 = add2(sum2, e);
+                    w[j] = pack2<T>(e.x, e.y);
+                }
+                tmem_st_32x16(s_addr + half * 16, w);
+                tmem_st_wait();
+                tc_fence_before();
                 __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile][odd]));
             }
-        } else {
+            count += it.end - it.begin;
+            // the places of the step before the last, which both warps have read
+            tail->half[tile][done & 1][half][my_lane] = sum2.x + sum2.y;
+            meet();
+            const float sum = tail->half[tile][done & 1][0][my_lane] + tail->half[tile][done & 1][1][my_lane];
+            const float top = base * scale;
+            const int64_t token = my_row / p.group;
+            const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
+            const int64_t out_row = (it.tokens.first + token) * p.heads + head;
+            if (works) {
+                ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag, 0x9a);
+                tc_fence_after();
+            }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             bool bad = false;
             for (int c = o_from; c < o_to; ++c) {
@@ -780,25 +930,48 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
                     tmem_ld_wait();
                 }
-                uint32_t w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float a = __uint_as_float(o[2 * j]), b = __uint_as_float(o[2 * j + 1]);
-                    bad |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
-                    w[j] = pack2<T>(a * inv, b * inv);
+                if (works && c + 1 == o_to) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&tail->o_free[tile]));
                 }
-                if (mine) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + out_row * p.dim + c * 16);
-                    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (c * 16 + 8 < p.dim) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                if (scratch.splits > 1) {
+                    if (mine && works) {
+                        float *dst = scratch.part + (static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row) * p.dim + c * 16;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            if (c * 16 + j < p.dim) *reinterpret_cast<uint4 *>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    }
+                } else {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float a = __uint_as_float(o[2 * j]), b = __uint_as_float(o[2 * j + 1]);
+                        bad |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
+                        w[j] = pack2<T>(a * inv, b * inv);
+                    }
+                    if (mine) {
+                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + out_row * p.dim + c * 16);
+                        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (c * 16 + 8 < p.dim) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
                 }
                 __syncwarp();
             }
-            if (mine && half == 0) p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+            if (works && o_from == o_to) {  // (one step of 16 columns: the second half has none)
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&tail->o_free[tile]));
+            }
+            if (mine && half == 0) {
+                if (scratch.splits > 1)
+                    scratch.stat[static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row] = make_float2(top, sum);
+                else
+                    p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
+            }
             // rows that are not finite although their weights are, when both halves are written
-            tail->half[tile][(steps + 1) & 1][half][my_lane] = bad ? 1.0f : 0.0f;
+            tail->half[tile][(done + 1) & 1][half][my_lane] = bad ? 1.0f : 0.0f;
             meet();
-            bad = bad || tail->half[tile][(steps + 1) & 1][half ^ 1][my_lane] != 0.0f;
+            bad = bad || tail->half[tile][(done + 1) & 1][half ^ 1][my_lane] != 0.0f;
             uint32_t again = __ballot_sync(0xffffffffu, half == 0 && mine && bad && sum == sum);
             if (again != 0 && met_not_finite<T>(p, it, low, high)) {
                 __syncwarp();
@@ -808,6 +981,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                  place_of(p, it.tokens, row));
                 }
             }
+            release(item);
         }
     }
 
@@ -906,7 +1080,20 @@ bool cache_map(CUtensorMap *map, const Problem &p, const void *base, int64_t sb,
         if (sizes[i + 1] == 1) strides[i] = p.dim;  // takes no step
         if (strides[i] <= 0 || strides[i] >= 1ll << 38) return false;
     }
-    return make_tmap_4d(map, base, sizes, strides, 64, rows);
+    const int box[4] = {64, rows, 1, 1};
+    return make_tmap_4d(map, base, sizes, strides, box);
+}
+
+// The query: columns, heads of a group, groups, tokens.
+bool query_map(CUtensorMap *map, const Problem &p) {
+    const int64_t sizes[4] = {p.dim, p.group, p.kv_heads, p.tokens};
+    int64_t strides[3] = {p.q_sh, p.q_sh * p.group, p.q_st};
+    for (int i = 0; i < 3; ++i) {
+        if (sizes[i + 1] == 1) strides[i] = p.dim;  // takes no step
+        if (strides[i] <= 0 || strides[i] >= 1ll << 38) return false;
+    }
+    const int box[4] = {64, p.group, 1, 128 / p.group};
+    return make_tmap_4d(map, p.q, sizes, strides, box);
 }
 
 template <typename T, int DP>
@@ -921,8 +1108,11 @@ int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStrea
     if (p.page % 16 != 0 || p.pages == 0 || !cache_map(&tmap_k, p, p.k, p.k_sb, p.k_st, p.k_sh, box_rows) ||
         !cache_map(&tmap_v, p, p.v, p.v_sb, p.v_st, p.v_sh, box_rows))
         box_rows = 0;
+    // the query's rows of a tile in one box, where the group's heads divide a tile
+    CUtensorMap tmap_q = {};
+    const bool box_query = 128 % p.group == 0 && query_map(&tmap_q, p);
     QMM_CUDA_OK(launch_pdl(prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch,
-                           tmap_k, tmap_v, box_rows));
+                           tmap_k, tmap_v, tmap_q, box_rows, box_query));
     if (plan.splits > 1) {
         const int64_t joins = (p.tokens * p.heads + 7) / 8;
         QMM_CUDA_OK(launch_pdl(prompt_join_kernel<T, Shape<DP>::kBN, Shape<DP>::kRows>, dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, p, scratch));

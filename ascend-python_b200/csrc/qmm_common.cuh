@@ -52,9 +52,9 @@ int sm_count();
 int make_tmap_2d(CUtensorMap *map, const void *base, int elem_bytes, uint64_t inner, uint64_t outer,
                  uint64_t ld, uint32_t box_inner, uint32_t box_outer, bool swizzle128);
 
-// Tensor map of 16-bit elements with four dimensions, the first dense: boxes of box0 x box1 (x 1 x 1) elements, 128-byte swizzle,
+// Tensor map of 16-bit elements with four dimensions, the first dense: boxes of `box` elements, 128-byte swizzle,
 // zeros out of range.  `strides`: of dimensions 1 to 3, in elements.  False (and no error text): it cannot be made.
-bool make_tmap_4d(CUtensorMap *map, const void *base, const int64_t sizes[4], const int64_t strides[3], uint32_t box0, uint32_t box1);
+bool make_tmap_4d(CUtensorMap *map, const void *base, const int64_t sizes[4], const int64_t strides[3], const int box[4]);
 
 // ---------------------------------------------------------------------------
 // Device side
