@@ -14,6 +14,8 @@
 //
 // Two threads have a row, half of the 64 keys each, and tell each other their maxima through shared memory: four softmax warps a
 // scheduler keep its units busier than two with a whole row a thread (8192 tokens, 32/8 heads of 128: TIMES).
+// An item of one row tile, as a few drafted tokens are, gives both halves of the CTA its rows, every second 64 keys each; their O
+// and sums are added at the end.
 // S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
 // one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
@@ -82,7 +84,9 @@ struct Tail {
     Item item[2];
     uint32_t copied[6];            // stage: by cp.async
     float half[2][2][2][128];      // [row tile][step % 2][half]: maxima; then sums
+    float base[2][128];            // [row tile]
     uint32_t going[2][4][2];       // [row tile][quarter][half]: the warp has an item
+    uint32_t parity[2][4];         // [row tile][quarter]: of the steps so far
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -475,47 +479,55 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 
     if (warp == kSoftmax + 4) {
         // ---------------- items, and the query ----------------
-        uint32_t id = blockIdx.x;
+        uint32_t id = blockIdx.x, asked = 0, queries = 0;
         bool have = true, ok = true;
-        uint32_t asked = 0, queries = 0;
         int n = 0;
-        while (ok) {
-            if (have && lane == 0) {
-                mbar_expect_tx(smem_u32(&tail->next_full), 16);
-                ask_next_block(smem_u32(tail->next), smem_u32(&tail->next_full));
-            }
-            __syncwarp();
+        while (ok && have) {
+            // a block is asked for when the item before the present one is done, not earlier: what is taken cannot go to another CTA
+            ok = mbar_wait(smem_u32(&tail->item_empty[n & 1]), (n >> 1 & 1) ^ 1, abort_flag, 0x9e);
+            if (!ok) break;
             Item it;
             bool found = false;
-            if (have) {
+            while (true) {
+                if (n > 0 || asked > 0) {
+                    if (lane == 0) {
+                        mbar_expect_tx(smem_u32(&tail->next_full), 16);
+                        ask_next_block(smem_u32(tail->next), smem_u32(&tail->next_full));
+                    }
+                    __syncwarp();
+                    ok = mbar_wait(smem_u32(&tail->next_full), (asked - 1) & 1, abort_flag, 0x8f);
+                    if (!ok) break;
+                    have = next_block(smem_u32(tail->next), &id);
+                    fence_proxy_async_smem();  // read before the next answer is written
+                    __syncwarp();
+                    if (!have) break;
+                }
+                ++asked;
                 clear_rest<T>(p, scratch, id, gridDim.x);
                 it.split = id % scratch.splits;
                 it.kvh = id / scratch.splits % p.kv_heads;
                 found = find_item<BN, S::kRows>(p, id / scratch.splits / p.kv_heads, it);
+                if (found) break;
             }
-            if (found || !have) {
-                ok = mbar_wait(smem_u32(&tail->item_empty[n & 1]), (n >> 1 & 1) ^ 1, abort_flag, 0x9e);
-                if (!ok) break;
-                if (found) {
-                    it.begin = static_cast<int>(static_cast<int64_t>(it.blocks) * it.split / scratch.splits);
-                    it.end = static_cast<int>(static_cast<int64_t>(it.blocks) * (it.split + 1) / scratch.splits);
-                    it.two = S::kTiles == 2 && it.first + 128 < it.rows;
-                    // the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
-                    it.steps = (it.end - it.begin) * S::kSub;
-                    if (S::kSub == 2 && it.end > it.begin) {
-                        const int last = block_start<BN>(it, it.end - 1);
-                        if (last + 64 >= (it.end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --it.steps;
-                    }
+            if (!ok) break;
+            if (found) {
+                it.begin = static_cast<int>(static_cast<int64_t>(it.blocks) * it.split / scratch.splits);
+                it.end = static_cast<int>(static_cast<int64_t>(it.blocks) * (it.split + 1) / scratch.splits);
+                it.two = S::kTiles == 2 && it.first + 128 < it.rows;
+                // the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
+                it.steps = (it.end - it.begin) * S::kSub;
+                if (S::kSub == 2 && it.end > it.begin) {
+                    const int last = block_start<BN>(it, it.end - 1);
+                    if (last + 64 >= (it.end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --it.steps;
                 }
-                it.none = !found;
-                if (lane == 0) {
-                    tail->item[n & 1] = it;
-                    mbar_arrive(smem_u32(&tail->item_full[n & 1]));
-                }
-                __syncwarp();
-                ++n;
             }
-            if (!have) break;
+            it.none = !found;
+            if (lane == 0) {
+                tail->item[n & 1] = it;
+                mbar_arrive(smem_u32(&tail->item_full[n & 1]));
+            }
+            __syncwarp();
+            ++n;
             if (found && it.steps > 0) {
                 ok = mbar_wait(smem_u32(&tail->q_empty), (queries & 1) ^ 1, abort_flag, 0x9f);
                 if (!ok) break;
@@ -553,12 +565,6 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     if (lane == 0) mbar_arrive(bar);
                 }
             }
-            ok = mbar_wait(smem_u32(&tail->next_full), asked & 1, abort_flag, 0x8f);
-            if (!ok) break;
-            ++asked;
-            have = next_block(smem_u32(tail->next), &id);
-            fence_proxy_async_smem();  // read before the next answer is written
-            __syncwarp();
         }
         cp_async_wait_all();
     } else if (warp >= kSoftmax + 2) {
@@ -686,7 +692,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const uint32_t o_desc = make_idesc(1, kFmt, kFmt, 0, 1, 128, ksteps * 16);
         constexpr uint32_t kSubStep = 64 * 128 >> 4;  // 64 rows of a box
         // Counters and descriptors in a form that the compiler knows to be the same in all lanes
-        const uint32_t q_lo = warp_uniform(smem_desc_lo(smem_base, 16)) + tile * (S::kBoxes * S::kQueryBox >> 4);
+        const uint32_t q_lo = warp_uniform(smem_desc_lo(smem_base, 16));
         const uint32_t k_lo = warp_uniform(smem_desc_lo(ring, 16)), v_lo = warp_uniform(smem_desc_lo(ring, S::kBox));
         const uint32_t bars = warp_uniform(smem_u32(tail));
         auto bar_of = [&](const uint64_t *bar) { return bars + static_cast<uint32_t>(reinterpret_cast<const uint8_t *>(bar) - reinterpret_cast<const uint8_t *>(tail)); };
@@ -698,17 +704,17 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             if (tail->copied[stage] != 0) fence_proxy_async_smem();
             return there;
         };
-        auto product_s = [&](uint32_t odd, uint32_t b) {
+        auto product_s = [&](uint32_t odd, uint32_t a, uint32_t b) {
             const uint32_t d = tmem_base + tile * 128 + odd * 64;
             if (S::kBoxes == 2 && ksteps == 8) {
-                mma_ss_x8(d, q_lo, q_lo + (S::kQueryBox >> 4), b, b + (S::kBox >> 4), kHi, s_desc);
+                mma_ss_x8(d, a, a + (S::kQueryBox >> 4), b, b + (S::kBox >> 4), kHi, s_desc);
             } else {
 #pragma unroll
                 for (int box = 0; box < S::kBoxes; ++box)
                     if (box * 4 + 4 <= ksteps)
-                        mma_ss_x4(d, q_lo + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
+                        mma_ss_x4(d, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
                 for (int k = ksteps & ~3; k < ksteps; ++k)
-                    mma_f16_ss_warp(d, desc64(q_lo + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
+                    mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
                                     desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
             }
             tc_commit_warp(bar_of(tail->s_full[0]) + (tile * 2 + odd) * 8);
@@ -719,12 +725,11 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             tc_commit_warp(bar_of(tail->o_done[0]) + (tile * 2 + odd) * 8);
         };
         // The tiles of keys and values that the next product takes, and its half of them: keys in the even stages, values in the
-        // odd ones.  A stage is free when the products so far of both row tiles are done; of one that is not there, too.
+        // odd ones.  A stage is free when the products so far of both MMA warps are done.
         uint32_t k_stage = 0, k_phase = 0, k_half = 0, v_stage = 1, v_phase = 0, v_half = 0;
-        bool alone = false;
+        bool shared = false;
         auto leave = [&](uint32_t &stage, uint32_t &phase) {
             tc_commit_warp(bar_of(tail->empty) + stage * 8);
-            if (alone) tc_commit_warp(bar_of(tail->empty) + stage * 8);
             stage += 2;
             if (stage >= S::kStages) {
                 stage -= S::kStages;
@@ -732,69 +737,61 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             }
         };
         auto advance = [&](uint32_t &stage, uint32_t &phase, uint32_t &half) {
-            if (++half < S::kSub) return;
-            half = 0;
+            if (!shared) {
+                if (++half < S::kSub) return;
+                half = 0;
+            }
             leave(stage, phase);
         };
-        uint32_t done = 0;               // steps of this row tile
-        uint32_t queries = 0, outs = 0;  // items with a query; items of this row tile
-        uint32_t taken = 0;              // tiles of keys
+        uint32_t done = 0;               // steps of this warp
+        uint32_t queries = 0, outs = 0;  // items with a query; items that this warp had steps of
         bool ok = true;
         for (int n = 0; ok; ++n) {
             ok = take(n);
             if (!ok || tail->item[n & 1].none) break;
-            const int all = static_cast<int>(warp_uniform(tail->item[n & 1].steps));
-            const bool two = warp_uniform(tail->item[n & 1].two) != 0;
-            const int tiles = static_cast<int>(warp_uniform(tail->item[n & 1].end - tail->item[n & 1].begin));
+            const int steps = static_cast<int>(warp_uniform(tail->item[n & 1].steps));
+            shared = warp_uniform(S::kTiles == 2 && !tail->item[n & 1].two) != 0;
             release(n);
-            if (all == 0) continue;
-            if (tile == 1 && !two) {  // the other row tile frees what this one does not take
-                ++queries;
-                taken += tiles;
-                k_stage = warp_uniform(taken % (S::kStages / 2) * 2);
-                v_stage = k_stage + 1;
-                k_phase = v_phase = warp_uniform(taken / (S::kStages / 2) & 1);
-                continue;
-            }
-            taken += tiles;
-            alone = S::kTiles == 2 && !two;
+            if (steps == 0) continue;
+            const int all = !shared ? steps : tile == 0 ? (steps + 1) / 2 : steps / 2;
+            const uint32_t a = q_lo + (shared ? 0 : tile * (S::kBoxes * S::kQueryBox >> 4));
+            k_half = v_half = shared ? tile : 0;
             ok = mbar_wait(bar_of(&tail->q_full), queries & 1, abort_flag, 0x91);
             if (!box_query) fence_proxy_async_smem();
             ++queries;
-            auto query_taken = [&] {
-                tc_commit_warp(bar_of(&tail->q_empty));
-                if (alone) tc_commit_warp(bar_of(&tail->q_empty));
-            };
+            if (all == 0) tc_commit_warp(bar_of(&tail->q_empty));
             for (int step = 0; step < 2 && step < all && ok; ++step) {
-                if (k_half == 0) ok = landed(k_stage, k_phase, 0x92);
+                if (shared || k_half == 0) ok = landed(k_stage, k_phase, 0x92);
                 if (!ok) break;
                 tc_fence_after();
-                product_s((done + step) & 1, k_lo + k_stage * kStageStep + k_half * kSubStep);
-                if (step + 1 == all) query_taken();
+                product_s((done + step) & 1, a, k_lo + k_stage * kStageStep + k_half * kSubStep);
+                if (step + 1 == all) tc_commit_warp(bar_of(&tail->q_empty));
                 advance(k_stage, k_phase, k_half);
             }
             // the softmax has read the O of the item before
-            if (ok && outs > 0) ok = mbar_wait(bar_of(tail->o_free) + tile * 8, (outs - 1) & 1, abort_flag, 0x93);
-            ++outs;
+            if (ok && all > 0) {
+                if (outs > 0) ok = mbar_wait(bar_of(tail->o_free) + tile * 8, (outs - 1) & 1, abort_flag, 0x93);
+                ++outs;
+            }
             for (int step = 0; step < all && ok; ++step, ++done) {
                 const uint32_t odd = done & 1;
                 const bool ahead = step + 2 < all;
-                if (v_half == 0) ok = landed(v_stage, v_phase, 0x94);
-                if (ok && ahead && k_half == 0) ok = landed(k_stage, k_phase, 0x95);
+                if (shared || v_half == 0) ok = landed(v_stage, v_phase, 0x94);
+                if (ok && ahead && (shared || k_half == 0)) ok = landed(k_stage, k_phase, 0x95);
                 ok = ok && mbar_wait(bar_of(tail->p_full[0]) + (tile * 2 + odd) * 8, (done >> 1) & 1, abort_flag, 0x96);
                 if (!ok) break;
                 tc_fence_after();
                 product_o(odd, v_lo + v_stage * kStageStep + v_half * kSubStep, step > 0);
                 if (ahead) {
-                    product_s(odd, k_lo + k_stage * kStageStep + k_half * kSubStep);
-                    if (step + 3 == all) query_taken();
+                    product_s(odd, a, k_lo + k_stage * kStageStep + k_half * kSubStep);
+                    if (step + 3 == all) tc_commit_warp(bar_of(&tail->q_empty));
                 }
                 advance(v_stage, v_phase, v_half);
                 if (ahead) advance(k_stage, k_phase, k_half);
             }
-            // tiles whose second half was not taken
-            if (ok && k_half != 0) {
-                k_half = v_half = 0;
+            // tiles whose second half was not taken; not before they have come, lest a stage be freed twice by one warp
+            if (ok && S::kSub == 2 && (steps & 1) && (!shared || tile == 1)) {
+                ok = landed(k_stage, k_phase, 0x8d) && landed(v_stage, v_phase, 0x8c);
                 leave(k_stage, k_phase);
                 leave(v_stage, v_phase);
             }
@@ -809,19 +806,24 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const float scale = factor == 0.0f ? 1.0f : fabsf(factor), sign = factor < 0.0f ? -1.0f : 0.0f;
         // the two warps that share rows
         auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quarter) : "memory"); };
+        // all four warps of a quarter
+        auto meet_quarter = [&] { asm volatile("bar.sync %0, 128;" ::"r"(9 + quarter) : "memory"); };
         const int o_from = half == 0 ? 0 : (ksteps + 1) / 2, o_to = half == 0 ? (ksteps + 1) / 2 : ksteps;  // 16 columns of O each
-        uint32_t done = 0, count = 0;  // steps of this row tile; tiles of keys
+        uint32_t done = 0, count = 0;  // steps of this warp; tiles of keys
         for (int item = 0;; ++item) {
             // A wait that gave up ends the warps of a row together; inside an item it ends the waits, not the steps, for the warps meet
             // in every one.
             bool ok = take(item);
             if (lane == 0) tail->going[tile][quarter][half] = ok && !tail->item[item & 1].none;
-            meet();
-            const bool go = tail->going[tile][quarter][0] != 0 && tail->going[tile][quarter][1] != 0;
-            meet();
+            S::kTiles == 2 ? meet_quarter() : meet();
+            bool go = tail->going[0][quarter][0] != 0 && tail->going[0][quarter][1] != 0;
+            if (S::kTiles == 2) go = go && tail->going[1][quarter][0] != 0 && tail->going[1][quarter][1] != 0;
+            S::kTiles == 2 ? meet_quarter() : meet();
             if (!go) break;
             const Item &it = tail->item[item & 1];
-            const int64_t row0 = it.first + tile * 128 + quarter * 32;  // this warp's first row
+            // One row tile: both groups of warps have its rows, the second one the second 64 of every 128 keys.
+            const bool shared = S::kTiles == 2 && !it.two;
+            const int64_t row0 = it.first + (shared ? 0 : tile * 128) + quarter * 32;  // this warp's first row
             const int64_t my_row = row0 + lane;
             const bool mine = my_row < it.rows;
             const Range range = visible_range(p, mine ? place_of(p, it.tokens, my_row) : -1);
@@ -829,10 +831,11 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
             float base = -INFINITY;  // unscaled
             float2 sum2 = make_float2(0.0f, 0.0f);
-            const int steps = it.steps;
-            const bool works = steps > 0 && (tile == 0 || it.two);
-            for (int n = 0; n < steps && works; ++n, ++done) {
-                const int i = it.begin + n / S::kSub;
+            const int steps = !shared ? it.steps : tile == 0 ? (it.steps + 1) / 2 : it.steps / 2;
+            const bool works = steps > 0;
+            for (int n = 0; n < steps; ++n, ++done) {
+                const int tile_of = shared ? n : n / S::kSub, part = shared ? tile : n % S::kSub;
+                const int i = it.begin + tile_of;
                 const uint32_t odd = done & 1;
                 ok = ok && mbar_wait(smem_u32(&tail->s_full[tile][odd]), (done >> 1) & 1, abort_flag, 0x98);
                 // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
@@ -841,8 +844,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 const uint32_t s_addr = tmem_base + lanes + tile * 128 + odd * 64;
                 uint32_t s[32];
                 tmem_ld_32x32(s_addr + half * 32, s);
-                const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[(count + n / S::kSub) % kValid][n % S::kSub * 2]);
-                const int start = block_start<BN>(it, i) + n % S::kSub * 64;
+                const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[(count + tile_of) % kValid][part * 2]);
+                const int start = block_start<BN>(it, i) + part * 64;
                 const bool whole = (start + 64 <= first_range.sink_end || (start >= last_range.lo && start + 64 <= first_range.hi)) &&
                                    (valid.x & valid.y) == 0xffffffffu;
                 tmem_ld_wait();
@@ -907,36 +910,63 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile][odd]));
             }
-            count += it.end - it.begin;
             // the places of the step before the last, which both warps have read
             tail->half[tile][done & 1][half][my_lane] = sum2.x + sum2.y;
-            meet();
-            const float sum = tail->half[tile][done & 1][0][my_lane] + tail->half[tile][done & 1][1][my_lane];
-            const float top = base * scale;
-            const int64_t token = my_row / p.group;
-            const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
-            const int64_t out_row = (it.tokens.first + token) * p.heads + head;
+            if (half == 0) tail->base[tile][my_lane] = base;
             if (works) {
                 ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag, 0x9a);
                 tc_fence_after();
             }
+            if (lane == 0) tail->parity[tile][quarter] = done & 1;
+            if (shared)
+                meet_quarter();  // both groups' products are done, too
+            else
+                meet();
+            tc_fence_after();
+            // the row's weights of the two groups' sums: one group has them all, or both a part
+            float keep[2] = {1.0f, 0.0f}, sum = 0.0f;
+            const int first = shared ? 0 : tile;
+            {
+                const uint32_t odd = tail->parity[first][quarter];
+                sum = tail->half[first][odd][0][my_lane] + tail->half[first][odd][1][my_lane];
+            }
+            bool other = false;
+            if (shared) {
+                const float base0 = tail->base[0][my_lane], base1 = tail->base[1][my_lane];
+                base = fmaxf(base0, base1);
+                other = it.steps > 1;
+                keep[0] = exp2_fast(base == -INFINITY ? 0.0f : (base0 - base) * scale);
+                keep[1] = other ? exp2_fast(base == -INFINITY ? 0.0f : (base1 - base) * scale) : 0.0f;
+                const uint32_t odd = tail->parity[1][quarter];
+                sum *= keep[0];
+                if (other) sum = fmaf(tail->half[1][odd][0][my_lane] + tail->half[1][odd][1][my_lane], keep[1], sum);
+            }
+            const float top = base * scale;
+            const int64_t token = my_row / p.group;
+            const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
+            const int64_t out_row = (it.tokens.first + token) * p.heads + head;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             bool bad = false;
-            for (int c = o_from; c < o_to; ++c) {
+            // 16 columns of O at a time: of a row's two warps, or four, each has its share
+            const int turns = shared ? 4 : 2, turn = shared ? tile * 2 + half : half;
+            for (int c = turn; c < ksteps; c += turns) {
                 uint32_t o[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = 0;
-                if (works) {
-                    tmem_ld_32x16(tmem_base + lanes + S::kO + tile * 128 + c * 16, o);
+                if (it.steps > 0) {
+                    tmem_ld_32x16(tmem_base + lanes + S::kO + first * 128 + c * 16, o);
                     tmem_ld_wait();
-                }
-                if (works && c + 1 == o_to) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&tail->o_free[tile]));
+                    if (other) {
+                        uint32_t o1[16];
+                        tmem_ld_32x16(tmem_base + lanes + S::kO + 128 + c * 16, o1);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), keep[1], __uint_as_float(o[j]) * keep[0]));
+                    }
                 }
                 if (scratch.splits > 1) {
-                    if (mine && works) {
+                    if (mine && it.steps > 0) {
                         float *dst = scratch.part + (static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row) * p.dim + c * 16;
 #pragma unroll
                         for (int j = 0; j < 16; j += 4)
@@ -958,21 +988,25 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 }
                 __syncwarp();
             }
-            if (works && o_from == o_to) {  // (one step of 16 columns: the second half has none)
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&tail->o_free[tile]));
-            }
-            if (mine && half == 0) {
+            if (mine && turn == 0) {
                 if (scratch.splits > 1)
                     scratch.stat[static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row] = make_float2(top, sum);
                 else
                     p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
             }
-            // rows that are not finite although their weights are, when both halves are written
+            // O may be written again, and rows that are not finite although their weights are can be, when all warps of a row are here
             tail->half[tile][(done + 1) & 1][half][my_lane] = bad ? 1.0f : 0.0f;
-            meet();
-            bad = bad || tail->half[tile][(done + 1) & 1][half ^ 1][my_lane] != 0.0f;
-            uint32_t again = __ballot_sync(0xffffffffu, half == 0 && mine && bad && sum == sum);
+            tc_fence_before();
+            if (shared)
+                meet_quarter();
+            else
+                meet();
+            if (works && lane == 0) mbar_arrive(smem_u32(&tail->o_free[tile]));
+            for (int k = 0; k < turns; ++k) {
+                const int from = shared ? k >> 1 : tile;
+                bad = bad || tail->half[from][tail->parity[from][quarter] ^ 1][k & 1][my_lane] != 0.0f;
+            }
+            uint32_t again = __ballot_sync(0xffffffffu, turn == 0 && mine && bad && sum == sum);
             if (again != 0 && met_not_finite<T>(p, it, low, high)) {
                 __syncwarp();
                 for (; again != 0; again &= again - 1) {
@@ -981,6 +1015,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                                  place_of(p, it.tokens, row));
                 }
             }
+            count += it.end - it.begin;
             release(item);
         }
     }
