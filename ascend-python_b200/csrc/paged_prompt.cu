@@ -12,15 +12,14 @@
 // hardware's order of the blocks balances the work as it does without; the next item's keys, values and query are fetched, and
 // its first S made, while the softmax ends the present one.  (A CTA an item cost 7 us for each.)
 //
-// Two threads have a row, half of the 64 keys each, and tell each other their maxima through shared memory: four softmax warps a
-// scheduler keep its units busier than two with a whole row a thread (8192 tokens, 32/8 heads of 128: TIMES).
 // An item of one row tile, as a few drafted tokens are, gives both halves of the CTA its rows, every second 64 keys each; their O
 // and sums are added at the end.
 // S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
 // one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
-// Warps 0..7 and 8..15: softmax and epilogue of the two row tiles.  Warps 16 and 17: MMA, one for each row tile, so
-// that the tensor pipe has the one's products while the other waits at its barriers.  Warps 18 and 19: keys and values.  Warp 20: items, and the query.  Where a page
+// Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warps 8 and 9: MMA, one for each row tile, so that the tensor
+// pipe has the one's products while the other waits at its barriers.  Warps 10 to 13: keys and values.  Warp 14: items, and the
+// query.  Where a page
 // holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
 // and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
@@ -34,9 +33,9 @@ namespace paged {
 
 namespace {
 
-constexpr int kSoftmax = 16;   // warps
-constexpr int kThreads = 672;
-constexpr int kLoaders = 2;  // warps
+constexpr int kSoftmax = 8;    // warps
+constexpr int kLoaders = 4;    // warps
+constexpr int kThreads = 32 * (kSoftmax + 2 + kLoaders + 1);
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
@@ -83,10 +82,8 @@ struct Tail {
     alignas(16) uint32_t next[4];  // the answer to the request for a further block
     Item item[2];
     uint32_t copied[6];            // stage: by cp.async
-    float half[2][2][2][128];      // [row tile][step % 2][half]: maxima; then sums
-    float base[2][128];            // [row tile]
-    uint32_t going[2][4][2];       // [row tile][quarter][half]: the warp has an item
-    uint32_t parity[2][4];         // [row tile][quarter]: of the steps so far
+    float sum[2][128], base[2][128];  // [group of softmax warps][row]
+    uint32_t bad[2][4], going[2][4];  // [group][quarter]: rows that are not finite; the warp has an item
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -438,13 +435,13 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(smem_u32(&tail->s_full[i >> 1][i & 1]), 1);
-            mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 8);
+            mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 4);
             mbar_init(smem_u32(&tail->o_done[i >> 1][i & 1]), 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&tail->o_free[i]), 8);
+            mbar_init(smem_u32(&tail->o_free[i]), 4);
             mbar_init(smem_u32(&tail->item_full[i]), 1);
-            mbar_init(smem_u32(&tail->item_empty[i]), 9 * S::kTiles + kLoaders);  // the warps that take items
+            mbar_init(smem_u32(&tail->item_empty[i]), 5 * S::kTiles + kLoaders);  // the warps that take items
         }
         mbar_init(smem_u32(&tail->q_full), 33);
         mbar_init(smem_u32(&tail->q_empty), S::kTiles);
@@ -477,7 +474,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         if (lane == 0) mbar_arrive(smem_u32(&tail->item_empty[n & 1]));
     };
 
-    if (warp == kSoftmax + 4) {
+    if (warp == kSoftmax + 2 + kLoaders) {
         // ---------------- items, and the query ----------------
         uint32_t id = blockIdx.x, asked = 0, queries = 0;
         bool have = true, ok = true;
@@ -577,7 +574,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const bool my_part = my_chunk < 2 * ksteps;
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
-        // Boxes: a warp fetches every second.  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
+        // Boxes: a warp fetches every fourth (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
         constexpr int kMost = (BN / 16 + kLoaders - 1) / kLoaders;
         int mine = 0;
@@ -796,160 +793,147 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 leave(v_stage, v_phase);
             }
         }
-    } else if (warp < 8 * S::kTiles) {
-        // ---------------- softmax and epilogue: half a row a thread ----------------
-        const int tile = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+    } else if (warp < 4 * S::kTiles) {
+        // ---------------- softmax and epilogue: a row a thread ----------------
+        const int group = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const int my_lane = quarter * 32 + lane;
         // The running maximum is one of unscaled scores, which takes a positive scale: with a negative one, or 0, the scores take its
         // sign.
         const float scale = factor == 0.0f ? 1.0f : fabsf(factor), sign = factor < 0.0f ? -1.0f : 0.0f;
-        // the two warps that share rows
-        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + quarter) : "memory"); };
-        // all four warps of a quarter
-        auto meet_quarter = [&] { asm volatile("bar.sync %0, 128;" ::"r"(9 + quarter) : "memory"); };
-        const int o_from = half == 0 ? 0 : (ksteps + 1) / 2, o_to = half == 0 ? (ksteps + 1) / 2 : ksteps;  // 16 columns of O each
+        // the warps of both groups that have a quarter of the rows, or two such quarters
+        auto meet = [&] {
+            if (S::kTiles == 2) asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+        };
         uint32_t done = 0, count = 0;  // steps of this warp; tiles of keys
         for (int item = 0;; ++item) {
-            // A wait that gave up ends the warps of a row together; inside an item it ends the waits, not the steps, for the warps meet
-            // in every one.
+            // A wait that gave up ends the warps that meet together; inside an item it ends the waits, not the steps.
             bool ok = take(item);
-            if (lane == 0) tail->going[tile][quarter][half] = ok && !tail->item[item & 1].none;
-            S::kTiles == 2 ? meet_quarter() : meet();
-            bool go = tail->going[0][quarter][0] != 0 && tail->going[0][quarter][1] != 0;
-            if (S::kTiles == 2) go = go && tail->going[1][quarter][0] != 0 && tail->going[1][quarter][1] != 0;
-            S::kTiles == 2 ? meet_quarter() : meet();
+            if (lane == 0) tail->going[group][quarter] = ok && !tail->item[item & 1].none;
+            __syncwarp();
+            meet();
+            const bool go = tail->going[0][quarter] != 0 && tail->going[S::kTiles - 1][quarter] != 0;
+            meet();
             if (!go) break;
             const Item &it = tail->item[item & 1];
             // One row tile: both groups of warps have its rows, the second one the second 64 of every 128 keys.
             const bool shared = S::kTiles == 2 && !it.two;
-            const int64_t row0 = it.first + (shared ? 0 : tile * 128) + quarter * 32;  // this warp's first row
-            const int64_t my_row = row0 + lane;
-            const bool mine = my_row < it.rows;
-            const Range range = visible_range(p, mine ? place_of(p, it.tokens, my_row) : -1);
-            const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
-            const Range first_range = visible_range(p, low), last_range = visible_range(p, high);
+            const int steps = !shared ? it.steps : group == 0 ? (it.steps + 1) / 2 : it.steps / 2;
             float base = -INFINITY;  // unscaled
             float2 sum2 = make_float2(0.0f, 0.0f);
-            const int steps = !shared ? it.steps : tile == 0 ? (it.steps + 1) / 2 : it.steps / 2;
-            const bool works = steps > 0;
-            for (int n = 0; n < steps; ++n, ++done) {
-                const int tile_of = shared ? n : n / S::kSub, part = shared ? tile : n % S::kSub;
-                const int i = it.begin + tile_of;
-                const uint32_t odd = done & 1;
-                ok = ok && mbar_wait(smem_u32(&tail->s_full[tile][odd]), (done >> 1) & 1, abort_flag, 0x98);
-                // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
-                if (done > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][odd]), ((done - 2) >> 1) & 1, abort_flag, 0x9b);
-                tc_fence_after();
-                const uint32_t s_addr = tmem_base + lanes + tile * 128 + odd * 64;
-                uint32_t s[32];
-                tmem_ld_32x32(s_addr + half * 32, s);
-                const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[(count + tile_of) % kValid][part * 2]);
-                const int start = block_start<BN>(it, i) + part * 64;
-                const bool whole = (start + 64 <= first_range.sink_end || (start >= last_range.lo && start + 64 <= first_range.hi)) &&
-                                   (valid.x & valid.y) == 0xffffffffu;
-                tmem_ld_wait();
-                if (factor <= 0.0f) {
+            if (steps > 0) {
+                const int64_t row0 = it.first + (shared ? 0 : group * 128) + quarter * 32;
+                const Range range = visible_range(p, row0 + lane < it.rows ? place_of(p, it.tokens, row0 + lane) : -1);
+                // what all rows of the warp see
+                const Range low = visible_range(p, place_of(p, it.tokens, min(row0, it.rows - 1)));
+                const int all_lo = visible_range(p, place_of(p, it.tokens, min(row0 + 31, it.rows - 1))).lo;
+                const int begin = it.begin, sink_blocks = it.sink_blocks, after_sinks = it.first_block - it.sink_blocks;
+                for (int n = 0; n < steps; ++n, ++done) {
+                    const int at_tile = shared ? n : n / S::kSub, part = shared ? group : n % S::kSub;
+                    const uint32_t odd = done & 1;
+                    ok = ok && mbar_wait(smem_u32(&tail->s_full[group][odd]), (done >> 1) & 1, abort_flag, 0x98);
+                    // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
+                    if (done > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd]), ((done - 2) >> 1) & 1, abort_flag, 0x9b);
+                    tc_fence_after();
+                    const uint32_t s_addr = tmem_base + lanes + group * 128 + odd * 64;
+                    uint32_t s[2][32];
+                    tmem_ld_32x32(s_addr, s[0]);
+                    tmem_ld_32x32(s_addr + 32, s[1]);
+                    const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[(count + at_tile) % kValid][part * 2]);
+                    const int i = begin + at_tile, start = (i < sink_blocks ? i : i + after_sinks) * BN + part * 64;
+                    const bool whole = (start + 64 <= low.sink_end || (start >= all_lo && start + 64 <= low.hi)) && (valid.x & valid.y) == 0xffffffffu;
+                    tmem_ld_wait();
+                    if (factor <= 0.0f) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) * sign);
-                }
-                if (!whole) {
-                    const int at = start + half * 32;
-                    const uint32_t see = (half == 0 ? valid.x : valid.y) & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
+                        for (int j = 0; j < 64; ++j) s[j / 32][j % 32] = __float_as_uint(__uint_as_float(s[j / 32][j % 32]) * sign);
+                    }
+                    if (!whole) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (!(see >> j & 1)) s[j] = 0xff800000u;  // -inf
-                }
-                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int c = 0; c < 2; ++c) {
+                            const int at = start + c * 32;
+                            const uint32_t see = (c == 0 ? valid.x : valid.y) & bits(0, range.hi - at) & (bits(0, range.sink_end - at) | bits(range.lo - at, 32));
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) m[c] = max3(m[c], __uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1]));
-                }
-                float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
-                tail->half[tile][odd][half][my_lane] = most;
-                tc_fence_before();  // the other half's P comes where this one's S was
-                meet();
-                tc_fence_after();
-                most = fmaxf(most, tail->half[tile][odd][half ^ 1][my_lane]);
-                const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
-                if (__any_sync(0xffffffffu, move)) {
-                    const float now = move ? most : base;
-                    const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
-                    sum2 = mul2(sum2, make_float2(keep, keep));
-                    if (n > 0) {
-                        ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
-                        tc_fence_after();
-                        for (int c = o_from; c < o_to; ++c) {
-                            uint32_t o[16];
-                            const uint32_t addr = tmem_base + lanes + S::kO + tile * 128 + c * 16;
-                            tmem_ld_32x16(addr, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                            tmem_st_32x16(addr, o);
+                            for (int j = 0; j < 32; ++j)
+                                if (!(see >> j & 1)) s[c][j] = 0xff800000u;  // -inf
                         }
                     }
-                    base = now;
-                }
-                const float offset = base == -INFINITY ? 0.0f : -base * scale;
-                const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
-                // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another; the
-                // sum takes the weights unrounded
-                uint32_t w[16];
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float2 x = fma2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), scale2, offset2);
-                    const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                    sum2 = add2(sum2, e);
-                    w[j] = pack2<T>(e.x, e.y);
+                    for (int j = 0; j < 64; j += 8) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            m[c] = max3(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
+                    }
+                    const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+                    const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float now = move ? most : base;
+                        const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                        sum2 = mul2(sum2, make_float2(keep, keep));
+                        if (n > 0) {
+                            ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
+                            tc_fence_after();
+                            for (int c = 0; c < ksteps; ++c) {
+                                uint32_t o[16];
+                                const uint32_t addr = tmem_base + lanes + S::kO + group * 128 + c * 16;
+                                tmem_ld_32x16(addr, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                                tmem_st_32x16(addr, o);
+                            }
+                        }
+                        base = now;
+                    }
+                    const float offset = base == -INFINITY ? 0.0f : -base * scale;
+                    const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+                    // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another;
+                    // the sum takes the weights unrounded
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
+                            const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            sum2 = add2(sum2, e);
+                            w[j] = pack2<T>(e.x, e.y);
+                        }
+                        tmem_st_32x16(s_addr + c * 16, w);
+                    }
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[group][odd]));
                 }
-                tmem_st_32x16(s_addr + half * 16, w);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[tile][odd]));
+                ok = ok && mbar_wait(smem_u32(&tail->o_done[group][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag, 0x9a);
             }
-            // the places of the step before the last, which both warps have read
-            tail->half[tile][done & 1][half][my_lane] = sum2.x + sum2.y;
-            if (half == 0) tail->base[tile][my_lane] = base;
-            if (works) {
-                ok = ok && mbar_wait(smem_u32(&tail->o_done[tile][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag, 0x9a);
-                tc_fence_after();
-            }
-            if (lane == 0) tail->parity[tile][quarter] = done & 1;
-            if (shared)
-                meet_quarter();  // both groups' products are done, too
-            else
-                meet();
-            tc_fence_after();
-            // the row's weights of the two groups' sums: one group has them all, or both a part
-            float keep[2] = {1.0f, 0.0f}, sum = 0.0f;
-            const int first = shared ? 0 : tile;
-            {
-                const uint32_t odd = tail->parity[first][quarter];
-                sum = tail->half[first][odd][0][my_lane] + tail->half[first][odd][1][my_lane];
-            }
-            bool other = false;
+            float sum = sum2.x + sum2.y, keep[2] = {1.0f, 0.0f};
+            const int first = shared ? 0 : group;
+            const bool other = shared && it.steps > 1;  // the second group has sums, too
             if (shared) {
+                tail->sum[group][my_lane] = sum;
+                tail->base[group][my_lane] = base;
+                tc_fence_before();
+                meet();  // both groups' products are done, too
                 const float base0 = tail->base[0][my_lane], base1 = tail->base[1][my_lane];
                 base = fmaxf(base0, base1);
-                other = it.steps > 1;
                 keep[0] = exp2_fast(base == -INFINITY ? 0.0f : (base0 - base) * scale);
-                keep[1] = other ? exp2_fast(base == -INFINITY ? 0.0f : (base1 - base) * scale) : 0.0f;
-                const uint32_t odd = tail->parity[1][quarter];
-                sum *= keep[0];
-                if (other) sum = fmaf(tail->half[1][odd][0][my_lane] + tail->half[1][odd][1][my_lane], keep[1], sum);
+                if (other) keep[1] = exp2_fast(base == -INFINITY ? 0.0f : (base1 - base) * scale);
+                sum = tail->sum[0][my_lane] * keep[0];
+                if (other) sum = fmaf(tail->sum[1][my_lane], keep[1], sum);
             }
+            tc_fence_after();
+            const int64_t row0 = it.first + (shared ? 0 : group * 128) + quarter * 32, my_row = row0 + lane;
+            const bool mine = my_row < it.rows;
             const float top = base * scale;
             const int64_t token = my_row / p.group;
             const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
             const int64_t out_row = (it.tokens.first + token) * p.heads + head;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             bool bad = false;
-            // 16 columns of O at a time: of a row's two warps, or four, each has its share
-            const int turns = shared ? 4 : 2, turn = shared ? tile * 2 + half : half;
-            for (int c = turn; c < ksteps; c += turns) {
+            // 16 columns of O at a time; two groups that share the rows take turns
+            for (int c = shared ? group : 0; c < ksteps; c += shared ? 2 : 1) {
                 uint32_t o[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[j] = 0;
@@ -988,31 +972,31 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 }
                 __syncwarp();
             }
-            if (mine && turn == 0) {
+            if (mine && group == first) {
                 if (scratch.splits > 1)
                     scratch.stat[static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row] = make_float2(top, sum);
                 else
                     p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
             }
-            // O may be written again, and rows that are not finite although their weights are can be, when all warps of a row are here
-            tail->half[tile][(done + 1) & 1][half][my_lane] = bad ? 1.0f : 0.0f;
+            // rows that are not finite although their weights are; O may be written again when all that share it have read it
+            uint32_t again = __ballot_sync(0xffffffffu, mine && bad && sum == sum);
             tc_fence_before();
-            if (shared)
-                meet_quarter();
-            else
-                meet();
-            if (works && lane == 0) mbar_arrive(smem_u32(&tail->o_free[tile]));
-            for (int k = 0; k < turns; ++k) {
-                const int from = shared ? k >> 1 : tile;
-                bad = bad || tail->half[from][tail->parity[from][quarter] ^ 1][k & 1][my_lane] != 0.0f;
-            }
-            uint32_t again = __ballot_sync(0xffffffffu, turn == 0 && mine && bad && sum == sum);
-            if (again != 0 && met_not_finite<T>(p, it, low, high)) {
+            if (shared) {
+                if (lane == 0) tail->bad[group][quarter] = again;
                 __syncwarp();
-                for (; again != 0; again &= again - 1) {
-                    const int64_t row = row0 + __ffs(again) - 1, t = row / p.group;
-                    plain_row<T>(p, it.b, it.tokens.first + t, it.kvh * p.group + static_cast<int>(row - t * p.group),
-                                 place_of(p, it.tokens, row));
+                meet();
+                again = group == 0 ? tail->bad[0][quarter] | tail->bad[1][quarter] : 0;
+            }
+            if (steps > 0 && lane == 0) mbar_arrive(smem_u32(&tail->o_free[group]));
+            if (again != 0) {
+                const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
+                if (met_not_finite<T>(p, it, low, high)) {
+                    __syncwarp();
+                    for (; again != 0; again &= again - 1) {
+                        const int64_t row = row0 + __ffs(again) - 1, t = row / p.group;
+                        plain_row<T>(p, it.b, it.tokens.first + t, it.kvh * p.group + static_cast<int>(row - t * p.group),
+                                     place_of(p, it.tokens, row));
+                    }
                 }
             }
             count += it.end - it.begin;
