@@ -18,7 +18,8 @@
 // one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
 //
 // Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warps 8 and 9: MMA, one for each row tile, so that the tensor
-// pipe has the one's products while the other waits at its barriers.  Warps 10 to 13: keys and values.  Warp 14: items, and the
+// pipe has the one's products while the other waits at its barriers.  Warps 10 and 11: keys; 12 and 13: values.  (In
+// one order, keys would wait for the values before them, which are free two steps later.)  Warp 14: items, and the
 // query.  Where a page
 // holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
@@ -34,9 +35,10 @@ namespace paged {
 namespace {
 
 constexpr int kSoftmax = 8;    // warps
-constexpr int kLoaders = 4;    // warps
-constexpr int kThreads = 32 * (kSoftmax + 2 + kLoaders + 1);
+constexpr int kLoaders = 2;    // warps, of keys and as many of values
+constexpr int kThreads = 32 * (kSoftmax + 2 + 2 * kLoaders + 1);
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMix = 4;          // every fourth pair of weights comes from the FMA pipe
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
 // DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: two S of 64 for each row tile, then O; 256
@@ -230,10 +232,27 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+// 2^x of two numbers, not infinite and not NaN, on the FMA pipe: x = n + f with n whole and f in [-1/2, 1/2], a polynomial of degree 5
+// for 2^f (the coefficients are a least-maximum fit of the relative error; in fp32 it is off by 2^-22 at most), and n added to its
+// exponent.  Below -125 the result is 2^-125.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which is then in the low bits
+    x.x = fmaxf(x.x, -125.0f);
+    x.y = fmaxf(x.y, -125.0f);
+    const float2 n = add2(x, make_float2(kRound, kRound));
+    const float2 f = fma2(add2(n, make_float2(-kRound, -kRound)), make_float2(-1.0f, -1.0f), x);
+    float2 y = fma2(f, make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f), make_float2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
+    y = fma2(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+    y = fma2(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+    y = fma2(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
+    y = fma2(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -441,7 +460,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&tail->o_free[i]), 4);
             mbar_init(smem_u32(&tail->item_full[i]), 1);
-            mbar_init(smem_u32(&tail->item_empty[i]), 5 * S::kTiles + kLoaders);  // the warps that take items
+            mbar_init(smem_u32(&tail->item_empty[i]), 5 * S::kTiles + 2 * kLoaders);  // the warps that take items
         }
         mbar_init(smem_u32(&tail->q_full), 33);
         mbar_init(smem_u32(&tail->q_empty), S::kTiles);
@@ -474,7 +493,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         if (lane == 0) mbar_arrive(smem_u32(&tail->item_empty[n & 1]));
     };
 
-    if (warp == kSoftmax + 2 + kLoaders) {
+    if (warp == kSoftmax + 2 + 2 * kLoaders) {
         // ---------------- items, and the query ----------------
         uint32_t id = blockIdx.x, asked = 0, queries = 0;
         bool have = true, ok = true;
@@ -566,7 +585,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         cp_async_wait_all();
     } else if (warp >= kSoftmax + 2) {
         // ---------------- keys and values ----------------
-        const int loader = warp - kSoftmax - 2;
+        const int part = (warp - kSoftmax - 2) / kLoaders, loader = (warp - kSoftmax - 2) % kLoaders;  // keys 0, values 1
         constexpr int kChunks = DP / 8, kStep = 32 / kChunks;
         constexpr int kLooks = BN / 32;  // places that a lane looks up; every loader all of them
         const int my_key = lane / kChunks, my_chunk = lane % kChunks;
@@ -574,13 +593,14 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const bool my_part = my_chunk < 2 * ksteps;
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
-        // Boxes: a warp fetches every fourth (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
+        // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
         constexpr int kMost = (BN / 16 + kLoaders - 1) / kLoaders;
         int mine = 0;
         for (int n = loader; n < boxes; n += kLoaders) ++mine;
         const uint32_t my_bytes = mine * S::kBoxes * box_rows * 128;
-        uint32_t stage = 0, phase = 0, count = 0;
+        const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
+        uint32_t stage = part, phase = 0, count = 0;  // even stages: keys
         bool ok = true;
         for (int n = 0; ok; ++n) {
             ok = take(n);
@@ -624,58 +644,56 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     }
                 }
                 if (i + 1 < it.end) look_up(i + 1);
-                for (int part = 0; part < 2; ++part) {
-                    ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
-                    if (!ok) break;
-                    const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
-                    if (whole) {
-                        if (lane == 0) {
-                            if (loader == 0) {
-                                if (part == 0) *reinterpret_cast<uint4 *>(tail->valid[count % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
-                                tail->copied[stage] = 0;
-                            }
-                            mbar_expect_tx(bar, my_bytes);
-                            mbar_arrive_n(bar, 32);
+                ok = mbar_wait(smem_u32(&tail->empty[stage]), phase ^ 1, abort_flag, 0x90);
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&tail->full[stage]), dst = ring + stage * S::kStage;
+                if (whole) {
+                    if (lane == 0) {
+                        if (loader == 0) {
+                            if (part == 0) *reinterpret_cast<uint4 *>(tail->valid[count % kValid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
+                            tail->copied[stage] = 0;
                         }
-                        __syncwarp();
-                        const CUtensorMap *map = part == 0 ? &tmap_k : &tmap_v;
-#pragma unroll
-                        for (int k = 0; k < kMost; ++k) {
-                            const int box = loader + k * kLoaders;
-                            if (box >= boxes) break;
-#pragma unroll
-                            for (int column = 0; column < S::kBoxes; ++column)
-                                tma_load_4d_warp(dst + column * S::kBox + box * box_rows * 128, map, column * 64, box_place[k], it.kvh, box_page[k], bar);
-                        }
-                    } else {
-                        if (loader == 0 && lane == 0) {
-                            tail->copied[stage] = 1;
-#pragma unroll
-                            for (int l = 0; part == 0 && l < kLooks; ++l) tail->valid[count % kValid][l] = mask[l];
-                        }
-                        const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
-                        const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
-#pragma unroll
-                        for (int group = 0; group < BN / 16; ++group) {
-                            if (group % kLoaders != loader) continue;
-                            const int l = group / 2;
-                            const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
-#pragma unroll
-                            for (int r = 0; r < 16; r += kStep) {
-                                const int key = group * 16 % 32 + r + my_key;
-                                const T *row = base + __shfl_sync(0xffffffffu, offset, key);
-                                if (my_part)
-                                    cp_async_16(dst + my_box + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
-                                                my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
-                            }
-                        }
-                        cp_async_arrive(bar);
-                        if (lane == 0) mbar_arrive(bar);
+                        mbar_expect_tx(bar, my_bytes);
+                        mbar_arrive_n(bar, 32);
                     }
-                    if (++stage == S::kStages) {
-                        stage = 0;
-                        phase ^= 1;
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < kMost; ++k) {
+                        const int box = loader + k * kLoaders;
+                        if (box >= boxes) break;
+#pragma unroll
+                        for (int column = 0; column < S::kBoxes; ++column)
+                            tma_load_4d_warp(dst + column * S::kBox + box * box_rows * 128, map, column * 64, box_place[k], it.kvh, box_page[k], bar);
                     }
+                } else {
+                    if (loader == 0 && lane == 0) {
+                        tail->copied[stage] = 1;
+#pragma unroll
+                        for (int l = 0; part == 0 && l < kLooks; ++l) tail->valid[count % kValid][l] = mask[l];
+                    }
+                    const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
+                    const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
+#pragma unroll
+                    for (int group = 0; group < BN / 16; ++group) {
+                        if (group % kLoaders != loader) continue;
+                        const int l = group / 2;
+                        const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
+#pragma unroll
+                        for (int r = 0; r < 16; r += kStep) {
+                            const int key = group * 16 % 32 + r + my_key;
+                            const T *row = base + __shfl_sync(0xffffffffu, offset, key);
+                            if (my_part)
+                                cp_async_16(dst + my_box + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
+                                            my_chunk < row_chunks && (mask[l] >> key & 1) ? 16 : 0);
+                        }
+                    }
+                    cp_async_arrive(bar);
+                    if (lane == 0) mbar_arrive(bar);
+                }
+                stage += 2;
+                if (stage >= S::kStages) {
+                    stage -= S::kStages;
+                    phase ^= 1;
                 }
             }
         }
@@ -862,44 +880,57 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     for (int j = 0; j < 64; j += 8) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            m[c] = max3(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
+                            m[c] = max3_nan(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
                     }
-                    const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
-                    const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float now = move ? most : base;
-                        const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
-                        sum2 = mul2(sum2, make_float2(keep, keep));
-                        if (n > 0) {
-                            ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
-                            tc_fence_after();
-                            for (int c = 0; c < ksteps; ++c) {
-                                uint32_t o[16];
-                                const uint32_t addr = tmem_base + lanes + S::kO + group * 128 + c * 16;
-                                tmem_ld_32x16(addr, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                                tmem_st_32x16(addr, o);
-                            }
-                        }
-                        base = now;
-                    }
-                    const float offset = base == -INFINITY ? 0.0f : -base * scale;
-                    const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+                    const float most = max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
                     // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another;
                     // the sum takes the weights unrounded
+                    auto weights = [&](auto mixed, float offset) {
+                        const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w[16];
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t w[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
-                            const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                            sum2 = add2(sum2, e);
-                            w[j] = pack2<T>(e.x, e.y);
+                            for (int j = 0; j < 16; ++j) {
+                                const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
+                                float2 e;
+                                if (decltype(mixed)::value && j % kMix == kMix - 1)
+                                    e = exp2_poly(x);
+                                else
+                                    e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                                sum2 = add2(sum2, e);
+                                w[j] = pack2<T>(e.x, e.y);
+                            }
+                            tmem_st_32x16(s_addr + c * 16, w);
                         }
-                        tmem_st_32x16(s_addr + c * 16, w);
+                    };
+                    // Most steps are seen whole and move no base.  (A maximum that is not finite counts as one that moves: exp2_poly
+                    // takes finite numbers alone.)
+                    const bool settled = (most - base) * scale <= kGrowth && most < INFINITY;
+                    if (__all_sync(0xffffffffu, settled && whole)) {
+                        weights(std::true_type{}, -base * scale);
+                    } else {
+                        const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+                        if (__any_sync(0xffffffffu, move)) {
+                            const float now = move ? most : base;
+                            const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                            sum2 = mul2(sum2, make_float2(keep, keep));
+                            if (n > 0) {
+                                ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
+                                tc_fence_after();
+                                for (int c = 0; c < ksteps; ++c) {
+                                    uint32_t o[16];
+                                    const uint32_t addr = tmem_base + lanes + S::kO + group * 128 + c * 16;
+                                    tmem_ld_32x16(addr, o);
+                                    tmem_ld_wait();
+#pragma unroll
+                                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                                    tmem_st_32x16(addr, o);
+                                }
+                            }
+                            base = now;
+                        }
+                        weights(std::false_type{}, base == -INFINITY ? 0.0f : -base * scale);
                     }
                     tmem_st_wait();
                     tc_fence_before();
