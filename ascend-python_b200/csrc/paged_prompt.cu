@@ -3,9 +3,8 @@
 // Rows: the tokens of one sequence times the query heads of one key-value head, token by token, in tiles of 128; so a few tokens
 // of a wide group fill a tile as well as many of a narrow one, and every key that is read serves the whole group.
 //
-// For 64 keys at a time, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory.  P, rounded to the
-// values' type, lies in the first half of the columns of its S, as the second product's operand in tensor memory.  The softmax
-// is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
+// For 64 keys at a time, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory, and P, rounded to the
+// values' type, is the second product's operand in tensor memory.  The softmax is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
 // maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.
 //
 // A CTA goes on to a further block of the grid, as long as there are blocks that have not begun (cluster launch control), so the
@@ -14,8 +13,9 @@
 //
 // An item of one row tile, as a few drafted tokens are, gives both halves of the CTA its rows, every second 64 keys each; their O
 // and sums are added at the end.
-// S is double-buffered, so the softmax of 64 keys runs beside the products of the 64 before and after (128 keys at a time, with
-// one S, it waited 1350 of 3900 clocks for P V and the next Q K^T), and two row tiles share the keys (dimensions up to 128).
+// The softmax has its scores in registers and gives S back at once: the next Q K^T runs beside it, and so does P V of the step
+// before, for P has two places of its own (with P in S's place and S twice, it waited 450 of 2400 clocks a step).  Two row tiles
+// share the keys (dimensions up to 128).
 //
 // Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warps 8 and 9: MMA, one for each row tile, so that the tensor
 // pipe has the one's products while the other waits at its barriers.  Warps 10 and 11: keys; 12 and 13: values.  (In
@@ -41,8 +41,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMix = 4;          // every fourth pair of weights comes from the FMA pipe
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
-// DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: two S of 64 for each row tile, then O; 256
-// columns of O leave room for one row tile.
+// DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: for each row tile S, 64, and two P, 32 each; then
+// O.  256 columns of O leave room for one row tile.
 template <int DP>
 struct Shape {
     static constexpr int kTiles = DP == 256 ? 1 : 2;
@@ -78,7 +78,7 @@ struct Item {
 constexpr int kValid = 8;  // tiles of keys whose masks are kept: more than may be under way
 struct Tail {
     uint64_t full[6], empty[6];
-    uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][step % 2]
+    uint64_t s_full[2], s_free[2], p_full[2][2], o_done[2][2];  // [row tile], [row tile][step % 2]
     uint64_t o_free[2], q_full, q_empty, item_full[2], item_empty[2], next_full;
     alignas(16) uint32_t valid[kValid][4];
     alignas(16) uint32_t next[4];  // the answer to the request for a further block
@@ -453,11 +453,12 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             mbar_init(smem_u32(&tail->empty[s]), S::kTiles);     // every row tile's products
         }
         for (int i = 0; i < 4; ++i) {
-            mbar_init(smem_u32(&tail->s_full[i >> 1][i & 1]), 1);
             mbar_init(smem_u32(&tail->p_full[i >> 1][i & 1]), 4);
             mbar_init(smem_u32(&tail->o_done[i >> 1][i & 1]), 1);
         }
         for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&tail->s_full[i]), 1);
+            mbar_init(smem_u32(&tail->s_free[i]), 4);
             mbar_init(smem_u32(&tail->o_free[i]), 4);
             mbar_init(smem_u32(&tail->item_full[i]), 1);
             mbar_init(smem_u32(&tail->item_empty[i]), 5 * S::kTiles + 2 * kLoaders);  // the warps that take items
@@ -719,8 +720,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             if (tail->copied[stage] != 0) fence_proxy_async_smem();
             return there;
         };
-        auto product_s = [&](uint32_t odd, uint32_t a, uint32_t b) {
-            const uint32_t d = tmem_base + tile * 128 + odd * 64;
+        auto product_s = [&](uint32_t a, uint32_t b) {
+            const uint32_t d = tmem_base + tile * 128;
             if (S::kBoxes == 2 && ksteps == 8) {
                 mma_ss_x8(d, a, a + (S::kQueryBox >> 4), b, b + (S::kBox >> 4), kHi, s_desc);
             } else {
@@ -732,11 +733,11 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
                                     desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
             }
-            tc_commit_warp(bar_of(tail->s_full[0]) + (tile * 2 + odd) * 8);
+            tc_commit_warp(bar_of(tail->s_full) + tile * 8);
         };
         // 16 keys a MMA: eight columns of P; 16 rows of 128 bytes of V, its next 64 columns a box further
         auto product_o = [&](uint32_t odd, uint32_t b, uint32_t accumulate) {
-            mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + tile * 128 + odd * 64, b, kHi, o_desc, accumulate);
+            mma_ts_x4(tmem_base + S::kO + tile * 128, tmem_base + tile * 128 + 64 + odd * 32, b, kHi, o_desc, accumulate);
             tc_commit_warp(bar_of(tail->o_done[0]) + (tile * 2 + odd) * 8);
         };
         // The tiles of keys and values that the next product takes, and its half of them: keys in the even stages, values in the
@@ -758,7 +759,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             }
             leave(stage, phase);
         };
-        uint32_t done = 0;               // steps of this warp
+        uint32_t done = 0, made = 0;     // steps of this warp; S made
         uint32_t queries = 0, outs = 0;  // items with a query; items that this warp had steps of
         bool ok = true;
         for (int n = 0; ok; ++n) {
@@ -775,34 +776,32 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             if (!box_query) fence_proxy_async_smem();
             ++queries;
             if (all == 0) tc_commit_warp(bar_of(&tail->q_empty));
-            for (int step = 0; step < 2 && step < all && ok; ++step) {
-                if (shared || k_half == 0) ok = landed(k_stage, k_phase, 0x92);
-                if (!ok) break;
+            auto make_s = [&](int step) {
+                // the softmax has taken the S before
+                if (made > 0) ok = ok && mbar_wait(bar_of(tail->s_free) + tile * 8, (made - 1) & 1, abort_flag, 0x92);
+                if (shared || k_half == 0) ok = ok && landed(k_stage, k_phase, 0x93);
+                if (!ok) return;
                 tc_fence_after();
-                product_s((done + step) & 1, a, k_lo + k_stage * kStageStep + k_half * kSubStep);
+                product_s(a, k_lo + k_stage * kStageStep + k_half * kSubStep);
+                ++made;
                 if (step + 1 == all) tc_commit_warp(bar_of(&tail->q_empty));
                 advance(k_stage, k_phase, k_half);
-            }
-            // the softmax has read the O of the item before
-            if (ok && all > 0) {
-                if (outs > 0) ok = mbar_wait(bar_of(tail->o_free) + tile * 8, (outs - 1) & 1, abort_flag, 0x93);
-                ++outs;
-            }
+            };
+            if (all > 0) make_s(0);
             for (int step = 0; step < all && ok; ++step, ++done) {
                 const uint32_t odd = done & 1;
-                const bool ahead = step + 2 < all;
-                if (shared || v_half == 0) ok = landed(v_stage, v_phase, 0x94);
-                if (ok && ahead && (shared || k_half == 0)) ok = landed(k_stage, k_phase, 0x95);
+                if (step + 1 < all) make_s(step + 1);
+                if (shared || v_half == 0) ok = ok && landed(v_stage, v_phase, 0x94);
+                if (step == 0) {
+                    // the softmax has read the O of the item before
+                    if (outs > 0) ok = ok && mbar_wait(bar_of(tail->o_free) + tile * 8, (outs - 1) & 1, abort_flag, 0x95);
+                    ++outs;
+                }
                 ok = ok && mbar_wait(bar_of(tail->p_full[0]) + (tile * 2 + odd) * 8, (done >> 1) & 1, abort_flag, 0x96);
                 if (!ok) break;
                 tc_fence_after();
                 product_o(odd, v_lo + v_stage * kStageStep + v_half * kSubStep, step > 0);
-                if (ahead) {
-                    product_s(odd, a, k_lo + k_stage * kStageStep + k_half * kSubStep);
-                    if (step + 3 == all) tc_commit_warp(bar_of(&tail->q_empty));
-                }
                 advance(v_stage, v_phase, v_half);
-                if (ahead) advance(k_stage, k_phase, k_half);
             }
             // tiles whose second half was not taken; not before they have come, lest a stage be freed twice by one warp
             if (ok && S::kSub == 2 && (steps & 1) && (!shared || tile == 1)) {
@@ -849,11 +848,12 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 for (int n = 0; n < steps; ++n, ++done) {
                     const int at_tile = shared ? n : n / S::kSub, part = shared ? group : n % S::kSub;
                     const uint32_t odd = done & 1;
-                    ok = ok && mbar_wait(smem_u32(&tail->s_full[group][odd]), (done >> 1) & 1, abort_flag, 0x98);
-                    // a barrier for even and one for odd steps, each waited for in every phase, so that a phase's parity is its own
+                    ok = ok && mbar_wait(smem_u32(&tail->s_full[group]), done & 1, abort_flag, 0x98);
+                    // this step's place of P is free.  (A barrier for even and one for odd steps, each waited for in every phase, so
+                    // that a phase's parity is its own.)
                     if (done > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd]), ((done - 2) >> 1) & 1, abort_flag, 0x9b);
                     tc_fence_after();
-                    const uint32_t s_addr = tmem_base + lanes + group * 128 + odd * 64;
+                    const uint32_t s_addr = tmem_base + lanes + group * 128, p_addr = s_addr + 64 + odd * 32;
                     uint32_t s[2][32];
                     tmem_ld_32x32(s_addr, s[0]);
                     tmem_ld_32x32(s_addr + 32, s[1]);
@@ -861,6 +861,9 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     const int i = begin + at_tile, start = (i < sink_blocks ? i : i + after_sinks) * BN + part * 64;
                     const bool whole = (start + 64 <= low.sink_end || (start >= all_lo && start + 64 <= low.hi)) && (valid.x & valid.y) == 0xffffffffu;
                     tmem_ld_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&tail->s_free[group]));
                     if (factor <= 0.0f) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) s[j / 32][j % 32] = __float_as_uint(__uint_as_float(s[j / 32][j % 32]) * sign);
@@ -901,7 +904,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                                 sum2 = add2(sum2, e);
                                 w[j] = pack2<T>(e.x, e.y);
                             }
-                            tmem_st_32x16(s_addr + c * 16, w);
+                            tmem_st_32x16(p_addr + c * 16, w);
                         }
                     };
                     // Most steps are seen whole and move no base.  (A maximum that is not finite counts as one that moves: exp2_poly
