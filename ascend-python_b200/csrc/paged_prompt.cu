@@ -15,7 +15,10 @@
 // and sums are added at the end.
 // The softmax has its scores in registers and gives S back at once: the next Q K^T runs beside it, and so does P V of the step
 // before, for P has two places of its own (with P in S's place and S twice, it waited 450 of 2400 clocks a step).  Two row tiles
-// share the keys (dimensions up to 128).
+// share the keys (dimensions up to 128).  What bounds a step (8192 tokens, 32/8 heads of 128: 2250 clocks for 64 keys, the products
+// take 1240): the softmax warps' chain, wait, load, maximum, and 64 exponentials a thread, which the special-function unit, shared by the
+// two row tiles, takes 1024 clocks for.  A quarter to a half of them as a polynomial on the FMA pipe, two threads a row, and row
+// tiles half a step apart were all slower or the same.
 //
 // Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warps 8 and 9: MMA, one for each row tile, so that the tensor
 // pipe has the one's products while the other waits at its barriers.  Warps 10 and 11: keys; 12 and 13: values.  (In
@@ -38,7 +41,6 @@ constexpr int kSoftmax = 8;    // warps
 constexpr int kLoaders = 2;    // warps, of keys and as many of values
 constexpr int kThreads = 32 * (kSoftmax + 2 + 2 * kLoaders + 1);
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMix = 4;          // every fourth pair of weights comes from the FMA pipe
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
 // DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: for each row tile S, 64, and two P, 32 each; then
@@ -232,27 +234,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
-}
-// 2^x of two numbers, not infinite and not NaN, on the FMA pipe: x = n + f with n whole and f in [-1/2, 1/2], a polynomial of degree 5
-// for 2^f (the coefficients are a least-maximum fit of the relative error; in fp32 it is off by 2^-22 at most), and n added to its
-// exponent.  Below -125 the result is 2^-125.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which is then in the low bits
-    x.x = fmaxf(x.x, -125.0f);
-    x.y = fmaxf(x.y, -125.0f);
-    const float2 n = add2(x, make_float2(kRound, kRound));
-    const float2 f = fma2(add2(n, make_float2(-kRound, -kRound)), make_float2(-1.0f, -1.0f), x);
-    float2 y = fma2(f, make_float2(0x1.5c08e6p-10f, 0x1.5c08e6p-10f), make_float2(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
-    y = fma2(y, f, make_float2(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
-    y = fma2(y, f, make_float2(0x1.ebf918p-3f, 0x1.ebf918p-3f));
-    y = fma2(y, f, make_float2(0x1.62e428p-1f, 0x1.62e428p-1f));
-    y = fma2(y, f, make_float2(0x1.000002p+0f, 0x1.000002p+0f));
-    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -883,57 +868,51 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     for (int j = 0; j < 64; j += 8) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            m[c] = max3_nan(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
+                            m[c] = max3(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
                     }
-                    const float most = max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+                    const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+                    const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float now = move ? most : base;
+                        const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
+                        sum2 = mul2(sum2, make_float2(keep, keep));
+                        if (n > 0) {
+                            ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
+                            tc_fence_after();
+                            for (int c = 0; c < ksteps; ++c) {
+                                uint32_t o[16];
+                                const uint32_t addr = tmem_base + lanes + S::kO + group * 128 + c * 16;
+                                tmem_ld_32x16(addr, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                                tmem_st_32x16(addr, o);
+                            }
+                        }
+                        base = now;
+                    }
                     // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another;
                     // the sum takes the weights unrounded
-                    auto weights = [&](auto mixed, float offset) {
-                        const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+                    const float offset = base == -INFINITY ? 0.0f : -base * scale;
+                    const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t w[16];
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[16];
+                        float2 e[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
-                                float2 e;
-                                if (decltype(mixed)::value && j % kMix == kMix - 1)
-                                    e = exp2_poly(x);
-                                else
-                                    e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                                sum2 = add2(sum2, e);
-                                w[j] = pack2<T>(e.x, e.y);
-                            }
-                            tmem_st_32x16(p_addr + c * 16, w);
+                        for (int j = 0; j < 16; ++j)
+                            e[j] = fma2(make_float2(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, offset2);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) e[j] = make_float2(exp2_fast(e[j].x), exp2_fast(e[j].y));
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = pack2<T>(e[j].x, e[j].y);
+                        tmem_st_32x16(p_addr + c * 16, w);
+#pragma unroll
+                        for (int k = 8; k > 0; k >>= 1) {
+#pragma unroll
+                            for (int j = 0; j < k; ++j) e[j] = add2(e[j], e[j + k]);
                         }
-                    };
-                    // Most steps are seen whole and move no base.  (A maximum that is not finite counts as one that moves: exp2_poly
-                    // takes finite numbers alone.)
-                    const bool settled = (most - base) * scale <= kGrowth && most < INFINITY;
-                    if (__all_sync(0xffffffffu, settled && whole)) {
-                        weights(std::true_type{}, -base * scale);
-                    } else {
-                        const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
-                        if (__any_sync(0xffffffffu, move)) {
-                            const float now = move ? most : base;
-                            const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
-                            sum2 = mul2(sum2, make_float2(keep, keep));
-                            if (n > 0) {
-                                ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
-                                tc_fence_after();
-                                for (int c = 0; c < ksteps; ++c) {
-                                    uint32_t o[16];
-                                    const uint32_t addr = tmem_base + lanes + S::kO + group * 128 + c * 16;
-                                    tmem_ld_32x16(addr, o);
-                                    tmem_ld_wait();
-#pragma unroll
-                                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                                    tmem_st_32x16(addr, o);
-                                }
-                            }
-                            base = now;
-                        }
-                        weights(std::false_type{}, base == -INFINITY ? 0.0f : -base * scale);
+                        sum2 = add2(sum2, e[0]);
                     }
                     tmem_st_wait();
                     tc_fence_before();
