@@ -55,13 +55,11 @@ __device__ __forceinline__ int64_t load_index(const void *base, int64_t at, int 
     return wide ? __ldg(static_cast<const long long *>(base) + at) : __ldg(static_cast<const int *>(base) + at);
 }
 
-// The token's sines and cosines, made by the CTA's first threads.
-__device__ __forceinline__ void make_turns(const RotaryParams &p, int64_t token, float *s_cos, float *s_sin) {
-    for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
-        const int64_t place = load_index(p.positions, axis_of(p, i) * p.pos_sa + token * p.pos_st, p.wide_positions);
-        const double half_turns = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + i)) * 0.31830988618379067154;
-        sincospif(static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns)), s_sin + i, s_cos + i);
-    }
+// The cosine and sine of a token's pair.
+__device__ __forceinline__ void make_turn(const RotaryParams &p, int64_t token, int pair, float *c, float *s) {
+    const int64_t place = load_index(p.positions, axis_of(p, pair) * p.pos_sa + token * p.pos_st, p.wide_positions);
+    const double half_turns = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + pair)) * 0.31830988618379067154;
+    sincospif(static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns)), s, c);
 }
 
 // Where the token goes in the cache; false: nowhere.
@@ -101,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     pdl_launch_dependents();
     pdl_wait();
     const int64_t token = blockIdx.x;
-    make_turns(p, token, s_cos, s_sin);
+    for (int i = threadIdx.x; i < p.pairs; i += kThreads) make_turn(p, token, i, s_cos + i, s_sin + i);
     __syncthreads();
     int64_t block = 0, at = 0;
     const bool write = !p.cached || find_slot(p, token, &block, &at);
@@ -142,14 +140,19 @@ struct Vec {
 // 16-byte vectors.  A thread has the same part of every row it comes to: with halves, the vector of the first elements of its
 // pairs and that of the second ones, or one vector behind the pairs; interleaved, one vector.  The first kAhead rows are under
 // way while the sines and cosines are made.
-constexpr int kAhead = 3;
-template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p, int shift) {
+//
+// TOKENS a CTA: four where there are enough, for then every thread makes a sine and cosine (of 64 pairs) and has five rows under
+// way (8192 tokens, 32 + 8 heads of 128, bf16: one 38.1 us, TIMES of the 26.0 that the copy bandwidth allows).
+constexpr int kAhead = 5;
+template <typename T, bool INTERLEAVED, int TOKENS>
+__global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p, int64_t tokens, int shift) {
     constexpr int E = Vec<T>::kElems;
-    __shared__ __align__(16) float s_cos[kMostPairs], s_sin[kMostPairs];
+    __shared__ __align__(16) float s_cos[TOKENS][kMostPairs], s_sin[TOKENS][kMostPairs];
+    __shared__ int64_t s_block[TOKENS], s_at[TOKENS];  // where a token goes in the cache; block < 0: nowhere
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t token = blockIdx.x;
+    const int64_t token0 = static_cast<int64_t>(blockIdx.x) * TOKENS;
+    const int here = static_cast<int>(min(static_cast<int64_t>(TOKENS), tokens - token0));
     const int part = threadIdx.x & ((1 << shift) - 1);  // 1 << shift: a row's parts, rounded up
     const int turning = INTERLEAVED ? 2 * p.pairs / E : p.pairs / E;
     const int parts = INTERLEAVED ? p.dim / E : turning + (p.dim - 2 * p.pairs) / E;
@@ -157,42 +160,61 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
     const int e0 = (INTERLEAVED || turns ? part : part + turning) * E;  // first vector
     const int e1 = e0 + p.pairs;                                        // second one
     const bool two = !INTERLEAVED && turns;
-    int64_t block = 0, at = 0;
-    const bool write = !p.cached || find_slot(p, token, &block, &at);
-    const int rows = part < parts ? p.heads + (write ? p.kv_heads * (p.cached ? 2 : 1) : 0) : 0;
+    const int rows = p.heads + p.kv_heads * (p.cached ? 2 : 1);  // of a token
+    const int all = part < parts ? rows * here : 0;
     const int stride = kThreads >> shift;
+    auto token_of = [&](int row) {
+        int token = 0;
+#pragma unroll
+        for (int i = 1; i < TOKENS; ++i) token += row >= i * rows;
+        return token;
+    };
     bool made = false;
-    for (int row0 = threadIdx.x >> shift; !made || row0 < rows; row0 += kAhead * stride) {
+    for (int row0 = threadIdx.x >> shift; !made || row0 < all; row0 += kAhead * stride) {
         uint4 x[kAhead], y[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int row = row0 + i * stride;
-            if (row >= rows) break;
+            if (row >= all) break;
+            const int token = token_of(row);
             const T *src;
             T *dst;
-            find_row(p, token, row, block, at, &src, &dst);
+            find_row(p, token0 + token, row - token * rows, 0, 0, &src, &dst);
             x[i] = __ldg(reinterpret_cast<const uint4 *>(src + e0));
             if (two) y[i] = __ldg(reinterpret_cast<const uint4 *>(src + e1));
         }
         if (!made) {
-            make_turns(p, token, s_cos, s_sin);
+            if (p.cached && threadIdx.x < here) {
+                int64_t block = -1, at = 0;
+                if (!find_slot(p, token0 + threadIdx.x, &block, &at)) block = -1;
+                s_block[threadIdx.x] = block;
+                s_at[threadIdx.x] = at;
+            }
+            for (int i = threadIdx.x; i < p.pairs * here; i += kThreads) {
+                const int token = i / p.pairs, pair = i - token * p.pairs;
+                make_turn(p, token0 + token, pair, &s_cos[token][pair], &s_sin[token][pair]);
+            }
             __syncthreads();
             made = true;
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int row = row0 + i * stride;
-            if (row >= rows) break;
+            if (row >= all) break;
+            const int token = token_of(row), of = row - token * rows;
+            const int64_t block = p.cached ? s_block[token] : 0, at = p.cached ? s_at[token] : 0;
+            if (of >= p.heads && block < 0) continue;
             const T *src;
             T *dst;
-            find_row(p, token, row, block, at, &src, &dst);
-            if (turns && row < p.heads + p.kv_heads) {
+            find_row(p, token0 + token, of, block, at, &src, &dst);
+            if (turns && of < p.heads + p.kv_heads) {
+                const float *cosine = s_cos[token], *sine = s_sin[token];
                 float a[E], b[E];
                 Vec<T>::unpack(x[i], a);
                 if (INTERLEAVED) {
 #pragma unroll
                     for (int j = 0; j < E; j += 2) {
-                        const float c = s_cos[(e0 + j) >> 1], s = s_sin[(e0 + j) >> 1];
+                        const float c = cosine[(e0 + j) >> 1], s = sine[(e0 + j) >> 1];
                         b[j] = turned_first(a[j], a[j + 1], c, s);
                         b[j + 1] = turned_second(a[j], a[j + 1], c, s);
                     }
@@ -201,7 +223,7 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
                     Vec<T>::unpack(y[i], b);
 #pragma unroll
                     for (int j = 0; j < E; ++j) {
-                        const float c = s_cos[e0 + j], s = s_sin[e0 + j], first = a[j];
+                        const float c = cosine[e0 + j], s = sine[e0 + j], first = a[j];
                         a[j] = turned_first(first, b[j], c, s);
                         b[j] = turned_second(first, b[j], c, s);
                     }
@@ -236,8 +258,12 @@ int launch_rotary(const RotaryParams &p, int64_t tokens, cudaStream_t stream) {
     const int parts = p.interleaved ? p.dim / E : (p.dim - p.pairs) / E;
     int shift = 0;
     while (1 << shift < parts) ++shift;
-    QMM_CUDA_OK(launch_pdl(p.interleaved ? rotary_vec_kernel<T, true> : rotary_vec_kernel<T, false>, grid, dim3(kThreads), 0, stream,
-                           p, shift));
+    // four tokens a CTA where that leaves two CTAs for every SM
+    constexpr int kTokens = 4;
+    const bool many = tokens >= 2ll * kTokens * sm_count();
+    auto kern = p.interleaved ? (many ? rotary_vec_kernel<T, true, kTokens> : rotary_vec_kernel<T, true, 1>)
+                              : (many ? rotary_vec_kernel<T, false, kTokens> : rotary_vec_kernel<T, false, 1>);
+    QMM_CUDA_OK(launch_pdl(kern, many ? dim3(static_cast<unsigned>((tokens + kTokens - 1) / kTokens)) : grid, dim3(kThreads), 0, stream, p, tokens, shift));
     return QMM_OK;
 }
 
