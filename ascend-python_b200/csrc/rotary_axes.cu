@@ -137,15 +137,16 @@ struct Vec {
     }
 };
 
-// 16-byte vectors.  A thread has the same part of every row it comes to: with halves, the vector of the first elements of its
-// pairs and that of the second ones, or one vector behind the pairs; interleaved, one vector.  The first kAhead rows are under
+// 16-byte vectors.  A part of a row is, with halves, the vector of the first elements of its pairs and that of the second ones, or
+// one vector behind the pairs; interleaved, one vector.  The first kAhead rows are under
 // way while the sines and cosines are made.
 //
-// TOKENS a CTA: four where there are enough, for then every thread makes a sine and cosine (of 64 pairs) and has five rows under
-// way (8192 tokens, 32 + 8 heads of 128, bf16: one 38.1 us, TIMES of the 26.0 that the copy bandwidth allows).
-constexpr int kAhead = 5;
+// TOKENS a CTA: two where there are enough, so that 64 pairs' sines and cosines keep half the threads busy and three parts a thread
+// are under way (8192 tokens, 32 + 8 heads of 128, bf16: one token 40.6 us, two 28.9, four 30.0 to 32.7, of the 26.0 that the copy
+// bandwidth allows).
+constexpr int kAhead = 3;
 template <typename T, bool INTERLEAVED, int TOKENS>
-__global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p, int64_t tokens, int shift) {
+__global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p, int64_t tokens, unsigned magic) {
     constexpr int E = Vec<T>::kElems;
     __shared__ __align__(16) float s_cos[TOKENS][kMostPairs], s_sin[TOKENS][kMostPairs];
     __shared__ int64_t s_block[TOKENS], s_at[TOKENS];  // where a token goes in the cache; block < 0: nowhere
@@ -153,35 +154,40 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
     pdl_wait();
     const int64_t token0 = static_cast<int64_t>(blockIdx.x) * TOKENS;
     const int here = static_cast<int>(min(static_cast<int64_t>(TOKENS), tokens - token0));
-    const int part = threadIdx.x & ((1 << shift) - 1);  // 1 << shift: a row's parts, rounded up
-    const int turning = INTERLEAVED ? 2 * p.pairs / E : p.pairs / E;
+    const int turning = INTERLEAVED ? 2 * p.pairs / E : p.pairs / E;  // parts of a row that turn
     const int parts = INTERLEAVED ? p.dim / E : turning + (p.dim - 2 * p.pairs) / E;
-    const bool turns = part < turning;
-    const int e0 = (INTERLEAVED || turns ? part : part + turning) * E;  // first vector
-    const int e1 = e0 + p.pairs;                                        // second one
-    const bool two = !INTERLEAVED && turns;
     const int rows = p.heads + p.kv_heads * (p.cached ? 2 : 1);  // of a token
-    const int all = part < parts ? rows * here : 0;
-    const int stride = kThreads >> shift;
-    auto token_of = [&](int row) {
-        int token = 0;
+    const int all = rows * here * parts;
+    // a part of a row: its token, row and vectors
+    struct Spot {
+        int token, row, e0, e1;
+        bool turns, two;
+    };
+    auto spot_of = [&](int item) {
+        Spot s;
+        const int row = magic != 0 ? static_cast<int>(__umulhi(item, magic)) : item, part = item - row * parts;  // item / parts
+        s.token = 0;
 #pragma unroll
-        for (int i = 1; i < TOKENS; ++i) token += row >= i * rows;
-        return token;
+        for (int i = 1; i < TOKENS; ++i) s.token += row >= i * rows;
+        s.row = row - s.token * rows;
+        s.turns = part < turning;
+        s.e0 = (INTERLEAVED || s.turns ? part : part + turning) * E;  // first vector
+        s.e1 = s.e0 + p.pairs;                                        // second one
+        s.two = !INTERLEAVED && s.turns;
+        return s;
     };
     bool made = false;
-    for (int row0 = threadIdx.x >> shift; !made || row0 < all; row0 += kAhead * stride) {
+    for (int item0 = threadIdx.x; !made || item0 < all; item0 += kAhead * kThreads) {
         uint4 x[kAhead], y[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int row = row0 + i * stride;
-            if (row >= all) break;
-            const int token = token_of(row);
+            if (item0 + i * kThreads >= all) break;
+            const Spot at = spot_of(item0 + i * kThreads);
             const T *src;
             T *dst;
-            find_row(p, token0 + token, row - token * rows, 0, 0, &src, &dst);
-            x[i] = __ldg(reinterpret_cast<const uint4 *>(src + e0));
-            if (two) y[i] = __ldg(reinterpret_cast<const uint4 *>(src + e1));
+            find_row(p, token0 + at.token, at.row, 0, 0, &src, &dst);
+            x[i] = __ldg(reinterpret_cast<const uint4 *>(src + at.e0));
+            if (at.two) y[i] = __ldg(reinterpret_cast<const uint4 *>(src + at.e1));
         }
         if (!made) {
             if (p.cached && threadIdx.x < here) {
@@ -199,22 +205,21 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int row = row0 + i * stride;
-            if (row >= all) break;
-            const int token = token_of(row), of = row - token * rows;
-            const int64_t block = p.cached ? s_block[token] : 0, at = p.cached ? s_at[token] : 0;
-            if (of >= p.heads && block < 0) continue;
+            if (item0 + i * kThreads >= all) break;
+            const Spot at = spot_of(item0 + i * kThreads);
+            const int64_t block = p.cached ? s_block[at.token] : 0, place = p.cached ? s_at[at.token] : 0;
+            if (at.row >= p.heads && block < 0) continue;
             const T *src;
             T *dst;
-            find_row(p, token0 + token, of, block, at, &src, &dst);
-            if (turns && of < p.heads + p.kv_heads) {
-                const float *cosine = s_cos[token], *sine = s_sin[token];
+            find_row(p, token0 + at.token, at.row, block, place, &src, &dst);
+            if (at.turns && at.row < p.heads + p.kv_heads) {
+                const float *cosine = s_cos[at.token], *sine = s_sin[at.token];
                 float a[E], b[E];
                 Vec<T>::unpack(x[i], a);
                 if (INTERLEAVED) {
 #pragma unroll
                     for (int j = 0; j < E; j += 2) {
-                        const float c = cosine[(e0 + j) >> 1], s = sine[(e0 + j) >> 1];
+                        const float c = cosine[(at.e0 + j) >> 1], s = sine[(at.e0 + j) >> 1];
                         b[j] = turned_first(a[j], a[j + 1], c, s);
                         b[j + 1] = turned_second(a[j], a[j + 1], c, s);
                     }
@@ -223,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
                     Vec<T>::unpack(y[i], b);
 #pragma unroll
                     for (int j = 0; j < E; ++j) {
-                        const float c = cosine[e0 + j], s = sine[e0 + j], first = a[j];
+                        const float c = cosine[at.e0 + j], s = sine[at.e0 + j], first = a[j];
                         a[j] = turned_first(first, b[j], c, s);
                         b[j] = turned_second(first, b[j], c, s);
                     }
@@ -231,8 +236,8 @@ __global__ void __launch_bounds__(kThreads) rotary_vec_kernel(const __grid_const
                     y[i] = Vec<T>::pack(b);
                 }
             }
-            *reinterpret_cast<uint4 *>(dst + e0) = x[i];
-            if (two) *reinterpret_cast<uint4 *>(dst + e1) = y[i];
+            *reinterpret_cast<uint4 *>(dst + at.e0) = x[i];
+            if (at.two) *reinterpret_cast<uint4 *>(dst + at.e1) = y[i];
         }
     }
 }
@@ -256,14 +261,14 @@ int launch_rotary(const RotaryParams &p, int64_t tokens, cudaStream_t stream) {
         return QMM_OK;
     }
     const int parts = p.interleaved ? p.dim / E : (p.dim - p.pairs) / E;
-    int shift = 0;
-    while (1 << shift < parts) ++shift;
-    // four tokens a CTA where that leaves two CTAs for every SM
-    constexpr int kTokens = 4;
+    // item * magic >> 32 = item / parts, as long as item * parts is below 2^32; 0: parts is 1
+    const unsigned magic = parts > 1 ? 0xffffffffu / parts + 1 : 0;
+    // two tokens a CTA where that leaves two CTAs for every SM
+    constexpr int kTokens = 2;
     const bool many = tokens >= 2ll * kTokens * sm_count();
     auto kern = p.interleaved ? (many ? rotary_vec_kernel<T, true, kTokens> : rotary_vec_kernel<T, true, 1>)
                               : (many ? rotary_vec_kernel<T, false, kTokens> : rotary_vec_kernel<T, false, 1>);
-    QMM_CUDA_OK(launch_pdl(kern, many ? dim3(static_cast<unsigned>((tokens + kTokens - 1) / kTokens)) : grid, dim3(kThreads), 0, stream, p, tokens, shift));
+    QMM_CUDA_OK(launch_pdl(kern, many ? dim3(static_cast<unsigned>((tokens + kTokens - 1) / kTokens)) : grid, dim3(kThreads), 0, stream, p, tokens, magic));
     return QMM_OK;
 }
 

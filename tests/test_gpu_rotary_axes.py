@@ -50,9 +50,9 @@ def within(got, ref, x):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("mode", ["half", "interleave"])
 @pytest.mark.parametrize("dim,pairs", [(64, 32), (128, 64), (128, 32), (80, 40), (80, 16), (256, 128), (6, 3), (7, 2), (64, 31), (10, 0),
-                                       (1, 0), (24, 6)])
+                                       (1, 0), (24, 6), (8, 4), (16, 8), (200, 96)])
 def test_head_dimensions(npu, paged, dev, dim, pairs, mode, dtype):
-    for T in (1, 37):
+    for T in (1, 37, 701):
         q, k, _, positions, inv_freq = make(dev, T, dim=dim, pairs=pairs, dtype=dtype, seed=dim)
         got = npu.npu_rotary_axes(q, k, positions, inv_freq, sections=[pairs], rotary_mode=mode)
         for x, y in zip((q, k), got):
