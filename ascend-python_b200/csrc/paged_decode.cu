@@ -188,11 +188,12 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 
     // the list's length, and whether all sequences are short
     int64_t total = 0;
-    int longest = 0;
+    int longest = 0, last_n = 0;  // last_n: tiles of sequence `lane`, of up to 32
     for (int b = lane; b < p.batch; b += 32) {
         const int n = sequence_of<KEYS>(p, b).tiles;
         total += n;
         longest = max(longest, n);
+        last_n = n;
     }
     for (int o = 16; o > 0; o >>= 1) {
         total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -201,7 +202,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
     total *= items;
     const int64_t all_items = static_cast<int64_t>(p.batch) * items;
     const bool whole = longest <= kShort / KEYS && all_items <= 2 * scratch.workers;
-    const int64_t range = (total + scratch.workers - 1) / scratch.workers;  // of a CTA
+    const int64_t range = total < 0x7fffffff ? (static_cast<unsigned>(total) + scratch.workers - 1) / static_cast<unsigned>(scratch.workers)
+                                             : (total + scratch.workers - 1) / scratch.workers;  // of a CTA
     if (!scratch.by_item && threadIdx.x == 0) scratch.cut[worker] = make_int4(-1, 0, 0, 0);
 
     // one round for the CTA's range; where head tiles are whole, one for each that the CTA has
@@ -212,7 +214,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         load.at = 0;
         load.b = load.item = load.from = load.to = 0;
         if (whole) {
-            load.b = static_cast<int>(round / items);
+            load.b = static_cast<int>(static_cast<unsigned>(round) / static_cast<unsigned>(items));  // few
             load.item = static_cast<int>(round - static_cast<int64_t>(load.b) * items);
             load.s = sequence_of<KEYS>(p, load.b);
             load.from = load.s.tiles * warp / S::kWarps;
@@ -232,7 +234,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             // sequences that see nothing, and where this warp's range begins
             for (int b0 = 0; b0 < p.batch; b0 += 32) {
                 const int b = b0 + lane;
-                const int n = b < p.batch ? sequence_of<KEYS>(p, b).tiles : 1;
+                const int n = b < p.batch ? (p.batch <= 32 ? last_n : sequence_of<KEYS>(p, b).tiles) : 1;
                 if (warp == 0) {
                     for (uint32_t none = __ballot_sync(0xffffffffu, n == 0); none != 0; none &= none - 1) {
                         const int e = b0 + __ffs(none) - 1;
@@ -541,64 +543,72 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         __syncthreads();
 
         // ---- the warps' parts: neighbours of one head tile are added in their order (a warp's second part is its last) ----
-        for (int i = 0; i < 2 * S::kWarps;) {
-            if (!s_parts[i].valid) {
-                ++i;
-                continue;
-            }
-            const Part head = s_parts[i];
-            int n = i;
-            bool ends = head.ends;
-            while (!ends && ++n < 2 * S::kWarps)
-                if (s_parts[n].valid) ends = s_parts[n].ends;
-            n = min(n + 1, 2 * S::kWarps);
-            const int kvh = head.item / tiles, tile = head.item - kvh * tiles;
-            const int rows = min(kRows, p.group - tile * kRows);
-            const int64_t first = static_cast<int64_t>(worker) * S::kWarps * 2;
-            const int64_t to_part = (scratch.cta_parts + 2 * worker + head.begins) * scratch.rows;
-            for (int idx = threadIdx.x; idx < rows * (p.dim / 4); idx += kThreads) {
-                const int row = idx / (p.dim / 4), d = (idx - row * (p.dim / 4)) * 4;
-                float2 stat[2 * S::kWarps];
-                float4 x[2 * S::kWarps];
-                float now = -INFINITY;
+        // Every thread has four columns of a row of all of them, loaded together: one after the other, a part's latency each, took 10
+        // of 133 us (64 sequences of 500 to 8000 places, 64/8 heads of 128).
+        const int64_t first_part = static_cast<int64_t>(worker) * S::kWarps * 2;
+        for (int idx = threadIdx.x; idx < scratch.rows * (p.dim / 4); idx += kThreads) {
+            const int row = idx / (p.dim / 4), d = (idx - row * (p.dim / 4)) * 4;
+            float2 stat[2 * S::kWarps];
+            float4 x[2 * S::kWarps];
 #pragma unroll
-                for (int w = 0; w < 2 * S::kWarps; ++w) {
-                    stat[w] = make_float2(-INFINITY, 0.0f);
-                    x[w] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (w >= i && w < n && s_parts[w].valid) {
-                        stat[w] = __ldcg(scratch.stat + (first + w) * scratch.rows + row);
-                        x[w] = __ldcg(reinterpret_cast<const float4 *>(scratch.part + ((first + w) * scratch.rows + row) * p.dim + d));
+            for (int i = 0; i < 2 * S::kWarps; ++i) {
+                if (s_parts[i].valid) {  // (rows behind the last of a head tile are never written and never used)
+                    stat[i] = __ldcg(scratch.stat + (first_part + i) * scratch.rows + row);
+                    x[i] = __ldcg(reinterpret_cast<const float4 *>(scratch.part + ((first_part + i) * scratch.rows + row) * p.dim + d));
+                }
+            }
+            float now = -INFINITY, all = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            bool open = false, begins = false;
+            int last_part = 0;
+            auto close = [&](bool ends) {
+                const Part &part = s_parts[last_part];
+                const int kvh = part.item / tiles, tile = part.item - kvh * tiles;
+                if (row < min(kRows, p.group - tile * kRows)) {
+                    if (begins && ends) {
+                        const int64_t to = static_cast<int64_t>(part.b) * p.heads + kvh * p.group + tile * kRows + row;
+                        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+                        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to * p.dim + d) =
+                            make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+                        if (d == 0) p.lse[to] = all == 0.0f ? -INFINITY : now * kLn2 + logf(all);
+                    } else {
+                        const int64_t to = (scratch.cta_parts + 2 * worker + begins) * scratch.rows + row;
+                        *reinterpret_cast<float4 *>(scratch.part + to * p.dim + d) = v;
+                        if (d == 0) scratch.stat[to] = make_float2(now, all);
                     }
-                    now = fmaxf(now, stat[w].x);
                 }
-                const float base = now == -INFINITY ? 0.0f : now;
-                float all = 0.0f;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (idx == 0 && begins && !whole) {
+                    const int64_t index = static_cast<int64_t>(part.b) * items + part.item;
+                    if (!ends)
+                        scratch.cut[scratch.by_item ? index : worker] = make_int4(worker, part.last, part.b, part.item);
+                    else if (scratch.by_item)
+                        scratch.cut[index] = make_int4(-1, 0, 0, 0);
+                }
+                open = false;
+            };
 #pragma unroll
-                for (int w = 0; w < 2 * S::kWarps; ++w) {
-                    const float weight = exp2_fast(stat[w].x - base);
-                    all = fmaf(stat[w].y, weight, all);
-                    v.x = fmaf(x[w].x, weight, v.x);
-                    v.y = fmaf(x[w].y, weight, v.y);
-                    v.z = fmaf(x[w].z, weight, v.z);
-                    v.w = fmaf(x[w].w, weight, v.w);
-                }
-                if (head.begins && ends) {
-                    const int64_t to = static_cast<int64_t>(head.b) * p.heads + kvh * p.group + tile * kRows + row;
-                    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-                    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + to * p.dim + d) =
-                        make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-                    if (d == 0) p.lse[to] = all == 0.0f ? -INFINITY : now * kLn2 + logf(all);
+            for (int i = 0; i < 2 * S::kWarps; ++i) {
+                if (!s_parts[i].valid) continue;
+                if (!open) {
+                    open = true;
+                    begins = s_parts[i].begins != 0;
+                    now = stat[i].x;
+                    all = stat[i].y;
+                    v = x[i];
                 } else {
-                    *reinterpret_cast<float4 *>(scratch.part + (to_part + row) * p.dim + d) = v;
-                    if (d == 0) scratch.stat[to_part + row] = make_float2(now, all);
+                    const float most = fmaxf(now, stat[i].x), base = most == -INFINITY ? 0.0f : most;
+                    const float keep = exp2_fast(now - base), add = exp2_fast(stat[i].x - base);
+                    all = fmaf(stat[i].y, add, all * keep);
+                    v.x = fmaf(x[i].x, add, v.x * keep);
+                    v.y = fmaf(x[i].y, add, v.y * keep);
+                    v.z = fmaf(x[i].z, add, v.z * keep);
+                    v.w = fmaf(x[i].w, add, v.w * keep);
+                    now = most;
                 }
+                last_part = i;
+                if (s_parts[i].ends) close(true);
             }
-            if (threadIdx.x == 0 && head.begins && !whole && (scratch.by_item || !ends)) {
-                scratch.cut[scratch.by_item ? static_cast<int64_t>(head.b) * items + head.item : worker] =
-                    make_int4(ends ? -1 : worker, head.last, head.b, head.item);
-            }
-            i = n;
+            if (open) close(false);
         }
         __syncthreads();
     }
@@ -625,37 +635,41 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch s
         const int from = share_parts ? static_cast<int>(static_cast<int64_t>(parts) * warp / kJoinWarps) : 0;
         const int to = share_parts ? static_cast<int>(static_cast<int64_t>(parts) * (warp + 1) / kJoinWarps) : parts;
         auto place = [&](int i) { return (scratch.cta_parts + static_cast<int64_t>(cut.x + i) * 2 + (i == 0)) * scratch.rows + row; };
-        float top = -INFINITY;
-        for (int i = from + lane; i < to; i += 32) top = fmaxf(top, scratch.stat[place(i)].x);
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f, acc[8] = {};
-        for (int i0 = from; i0 < to; i0 += 32) {
-            float weight = 0.0f;
-            if (i0 + lane < to) {
-                const float2 st = scratch.stat[place(i0 + lane)];
-                weight = exp2_fast(st.x - base);
-                sum += st.y * weight;
-            }
-            const int n = min(32, to - i0);
-#pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const float w = __shfl_sync(0xffffffffu, weight, i);
+        // Four parts at a time, their statistics and sums loaded together, onto a running maximum.
+        float top = -INFINITY, sum = 0.0f, acc[8] = {};
+        for (int i0 = from; i0 < to; i0 += 4) {
+            float2 stat[4];
+            float4 v[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                stat[i] = make_float2(-INFINITY, 0.0f);
+                v[i][0] = v[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i0 + i >= to) continue;
+                stat[i] = scratch.stat[place(i0 + i)];
                 const float *src = scratch.part + place(i0 + i) * p.dim;
 #pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (c * 128 + lane * 4 < p.dim) v[i][c] = *reinterpret_cast<const float4 *>(src + c * 128 + lane * 4);
+            }
+            const float now = fmaxf(fmaxf(fmaxf(top, stat[0].x), fmaxf(stat[1].x, stat[2].x)), stat[3].x);
+            const float base = now == -INFINITY ? 0.0f : now, keep = exp2_fast(top - base);
+            sum *= keep;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] *= keep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float w = exp2_fast(stat[i].x - base);
+                sum = fmaf(stat[i].y, w, sum);
+#pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const int d = c * 128 + lane * 4;
-                    if (d < p.dim) {
-                        const float4 v = *reinterpret_cast<const float4 *>(src + d);
-                        acc[4 * c] = fmaf(v.x, w, acc[4 * c]);
-                        acc[4 * c + 1] = fmaf(v.y, w, acc[4 * c + 1]);
-                        acc[4 * c + 2] = fmaf(v.z, w, acc[4 * c + 2]);
-                        acc[4 * c + 3] = fmaf(v.w, w, acc[4 * c + 3]);
-                    }
+                    acc[4 * c] = fmaf(v[i][c].x, w, acc[4 * c]);
+                    acc[4 * c + 1] = fmaf(v[i][c].y, w, acc[4 * c + 1]);
+                    acc[4 * c + 2] = fmaf(v[i][c].z, w, acc[4 * c + 2]);
+                    acc[4 * c + 3] = fmaf(v[i][c].w, w, acc[4 * c + 3]);
                 }
             }
+            top = now;
         }
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (share_parts) {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
