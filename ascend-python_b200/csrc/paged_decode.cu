@@ -294,8 +294,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         int slot = 0, value_place[kLooks], value_entry[kLooks], value_head = -1;
         uint32_t value_seen[kLooks], seen[kLooks];
         // A lane always has the same chunk, of rows kStep apart.  Rows of 16 places lie evenly apart where a page holds a
-        // multiple of 16 (tiles begin at multiples of 16), so a tile that is seen whole takes one address for 16 places; else
-        // each row its own.
+        // multiple of 16 (tiles begin at multiples of 16), and take one address; else each row its own.
         constexpr int kStep = 32 / kChunks;
         const int my_key = lane / kChunks, my_chunk = lane % kChunks;
         const bool my_part = my_chunk < 2 * ksteps;
@@ -306,23 +305,38 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         auto copy_tile = [&](const void *cache, int64_t sb, int64_t st, int64_t sh) {
             const uint32_t dst = ring + slot * kTileBytes + my_dst;
             int64_t offset[kLooks];
-            bool full = even;
+            bool full = true;
 #pragma unroll
             for (int l = 0; l < kLooks; ++l) {
                 offset[l] = value_seen[l] >> lane & 1 ? value_entry[l] * sb + value_place[l] * st + value_head * sh : 0;
                 full = full && value_seen[l] == 0xffffffffu;
             }
             const T *base = static_cast<const T *>(cache) + my_offset;
-            if (full) {
+            if (even) {
                 const T *row[KEYS / 16];
 #pragma unroll
-                for (int h = 0; h < KEYS / 16; ++h) row[h] = base + __shfl_sync(0xffffffffu, offset[h / 2], 16 * (h % 2)) + my_key * st;
+                for (int h = 0; h < KEYS / 16; ++h) {
+                    // from the first of them that is seen
+                    const uint32_t of = value_seen[h / 2] >> 16 * (h % 2) & 0xffffu;
+                    const int from = of != 0 ? __ffs(of) - 1 : 0;
+                    row[h] = base + __shfl_sync(0xffffffffu, offset[h / 2], 16 * (h % 2) + from) + (my_key - from) * st;
+                }
                 if (my_part) {
+                    if (full) {
 #pragma unroll
-                    for (int i = 0; i < KEYS / kStep; ++i) {
-                        const int first = kStep * i;
-                        cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row[first / 16], 16);
-                        row[first / 16] += kStep * st;
+                        for (int i = 0; i < KEYS / kStep; ++i) {
+                            const int first = kStep * i;
+                            cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), row[first / 16], 16);
+                            row[first / 16] += kStep * st;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < KEYS / kStep; ++i) {
+                            const int first = kStep * i;
+                            const bool ok = value_seen[first / 32] >> ((first & 31) + my_key) & 1;
+                            cp_async_16((dst ^ ((first & 7) << 4)) + first * (DP * 2), ok ? row[first / 16] : base, ok ? 16 : 0);
+                            row[first / 16] += kStep * st;
+                        }
                     }
                 }
                 return;
