@@ -48,9 +48,9 @@ def seen(place, capacity, window, sinks):
     return [j for j in range(min(place + 1, capacity)) if window == 0 or place - j < window or j < sinks]
 
 
-def attention(q, k_cache, v_cache, table, lens, query_start=None, scale=None, window=0, sinks=0):
-    """(out, lse, weight, error): the operator in float64 and, for bounds, sum_j p_j |v_j| and the largest sum_d |q_d k_jd| * scale
-    of each row; places are gathered one row at a time."""
+def attention(q, k_cache, v_cache, table, lens, query_start=None, scale=None, window=0, sinks=0, only=None):
+    """(out, lse, weight, spread, reach): the operator in float64 and, for bounds, sum_j p_j |v_j|, sum_j |v_j| and the largest sum_d |q_d k_jd| * scale
+    of each row; places are gathered one row at a time.  only: the tokens that are computed."""
     T, H, D = q.shape
     pages, page, KV, _ = k_cache.shape
     scale = D ** -0.5 if scale is None else scale
@@ -62,7 +62,7 @@ def attention(q, k_cache, v_cache, table, lens, query_start=None, scale=None, wi
     rows = rows_of(lens.tolist(), None if query_start is None else query_start.tolist(), T)
     tables = table.tolist()
     for t, (b, place) in enumerate(rows):
-        if b < 0:
+        if b < 0 or (only is not None and t not in only):
             continue
         js = [j for j in seen(place, table.shape[1] * page, window, sinks) if 0 <= tables[b][j // page] < pages]
         if not js:

@@ -153,6 +153,65 @@ def test_prompt_few_tokens_long_cache(npu, paged, dev):
     check(npu, paged, *make(dev, [20011], [7], heads=8, kv=2, dim=256, seed=3), window=9000, sinks=70)
 
 
+def check_rows(npu, paged, q, k, v, table, lens, starts, count, **kw):
+    """check() for some of many rows."""
+    out, lse = call(npu, q, k, v, table, lens, starts, **kw)
+    only = set(random.Random(1).sample(range(q.shape[0]), count)) | {0, q.shape[0] - 1}
+    ref = paged.attention(q, k, v, table, lens, starts, only=only, **kw)
+    bound, lse_bound = paged.attention_bounds(q.dtype, q.shape[2], *ref)
+    rows = torch.tensor(sorted(only), device=q.device)
+    assert bool(((out.double() - ref[0]).abs() <= bound)[rows].all())
+    none = ref[1] == -math.inf
+    assert torch.equal((lse == -math.inf)[rows], none[rows])
+    assert bool(((lse.double() - ref[1]).abs() <= lse_bound)[rows][~none[rows]].all())
+    assert bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("heads,kv,dim,page", [(32, 8, 128, 16), (20, 4, 128, 64), (28, 4, 64, 128), (16, 16, 96, 24), (16, 2, 256, 32),
+                                               (64, 1, 128, 16), (12, 4, 256, 7)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 3)])
+def test_prompt_more_items_than_the_gpu_takes_at_once(npu, paged, dev, heads, kv, dim, page, window, sinks):
+    """CTAs that go on from item to item: one row tile and two, odd and even numbers of steps, items without any."""
+    rng = random.Random(dim + heads)
+    new = [rng.choice([0, 1, 3, rng.randrange(30), rng.randrange(300)]) for _ in range(90)] + [1000]
+    lens = [max(0, n + rng.choice([0, 0, -2, rng.randrange(40), rng.randrange(700)])) for n in new]
+    check_rows(npu, paged, *make(dev, lens, new, heads=heads, kv=kv, dim=dim, page=page, seed=heads, tail=2), 150, window=window, sinks=sinks)
+
+
+def test_decode_large_batch(npu, paged, dev):
+    rng = random.Random(9)
+    lens = [rng.choice([rng.randrange(700), rng.randrange(3000)]) for _ in range(300)]
+    check_rows(npu, paged, *make(dev, lens, heads=32, kv=8, dim=128, seed=1), 60)
+    check_rows(npu, paged, *make(dev, lens, heads=40, kv=2, dim=64, seed=2), 60, window=500, sinks=5)
+
+
+def test_tokens_before_the_first_and_behind_the_last(npu, paged, dev):
+    """Rows of no sequence in front and behind, and a sequence that has pages of another one, whose prefix it shares."""
+    q, k, v, table, lens, starts = make(dev, [200, 200, 90], [40, 40, 0], dim=128, seed=21, tail=60)
+    table[1, :10] = table[0, :10]
+    check(npu, paged, q, k, v, table, lens, starts + 7)
+    check(npu, paged, q[:3], k, v, table, lens, None)
+    q, k, v, table, lens, starts = make(dev, [20011, 100], [4, 2], heads=8, kv=2, dim=128, seed=22, tail=3)  # split
+    check(npu, paged, q, k, v, table, lens, starts + 2)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_values_not_finite_where_a_row_is_split(npu, paged, dev, dim):
+    """As above for a few tokens over a long cache, whose parts are added by another kernel."""
+    for window, sinks in ((0, 0), (3000, 3)):
+        q, k, v, table, lens, starts = make(dev, [9000, 5000], [6, 5], heads=8, kv=2, dim=dim, seed=23)
+        ref = paged.attention(q, k, v, table, lens, starts, window=window, sinks=sinks)
+        bound = paged.attention_bounds(q.dtype, dim, *ref)[0]
+        for b, j in ((0, 8997), (0, 5997), (1, 4998), (1, 1)):
+            v2 = v.clone()
+            v2[table[b, j // 16], j % 16, 0, 3] = math.nan
+            out, _ = call(npu, q, k, v2, table, lens, starts, window=window, sinks=sinks)
+            rows = paged.rows_of(lens.tolist(), starts.tolist(), q.shape[0])
+            hit = torch.zeros_like(out, dtype=torch.bool)
+            hit[:, :4, 3] = torch.tensor([s == b and j <= p and (window == 0 or p - j < window or j < sinks) for s, p in rows], device=dev)[:, None]
+            assert bool(out[hit].isnan().all()) and bool(((out.double() - ref[0]).abs() <= bound)[~hit].all()), (window, b, j)
+
+
 def test_prompt_many_sequences(npu, paged, dev):
     rng = random.Random(6)
     new = [rng.choice([0, 1, rng.randrange(9)]) for _ in range(700)]

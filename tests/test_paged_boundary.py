@@ -147,3 +147,84 @@ def test_oracle_against_loops():
                     z = complex(x[t, 1, m], x[t, 1, n]) * complex(math.cos(angle), math.sin(angle))
                     assert abs(float(y[t, 1, m]) - z.real) < 1e-12 and abs(float(y[t, 1, n]) - z.imag) < 1e-12
             assert torch.equal(y[..., 8:], x[..., 8:])
+
+
+def test_short_cut_calls_are_the_operators(pkg):
+    """What the shim's positional calls leave to torch.ops, and that what they take reaches the operator."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    sys.path.insert(0, str(PKG_DIR))
+    try:
+        import torch_npu
+    finally:
+        sys.path.pop(0)
+
+    class Record(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if func.namespace != "npu":
+                return func(*args, **(kwargs or {}))
+            seen.append((func.name().split("::")[1], len(args) + len(kwargs or {})))
+            return tuple(torch.zeros(1) for _ in func._schema.returns) if len(func._schema.returns) > 1 else torch.zeros(1)
+
+    x, c, i, f = torch.zeros((2, 2, 8)), torch.zeros((1, 4, 2, 8)), torch.zeros(2, dtype=torch.int32), torch.ones(4)
+    calls = {"npu_rotary_axes": [lambda **k: torch_npu.npu_rotary_axes(x, x, i, f, **k), {}, {"sections": [4]}, {"sections": (4,)},
+                                 {"rotary_mode": "interleave", "axis_order": "cyclic"}],
+             "npu_rotary_axes_cache": [lambda **k: torch_npu.npu_rotary_axes_cache(x, x, x, i, f, c, c, i, **k), {}, {"sections": [4]}],
+             "npu_paged_attention": [lambda **k: torch_npu.npu_paged_attention(x, c, c, i[:, None], i, **k), {}, {"scale_value": 0.5},
+                                     {"scale_value": 1, "window": 3, "sinks": 2}],
+             "npu_paged_prompt_attention": [lambda **k: torch_npu.npu_paged_prompt_attention(x, c, c, i[:, None], i, i, **k), {}, {"window": 3}]}
+    for name, (call, *options) in calls.items():
+        for option in options:
+            seen = []
+            with Record():
+                call(**option)
+            assert [n for n, _ in seen] == [name]
+    for bad in ({"sections": [1.5]}, {"sections": 4.0}, {"rotary_mode": 3}):
+        with pytest.raises((RuntimeError, TypeError)):
+            torch_npu.npu_rotary_axes(x, x, i, f, **bad)
+    with pytest.raises((RuntimeError, TypeError)):
+        torch_npu.npu_paged_attention(x, c, c, i[:, None], i, window="x")
+
+
+def test_workspace_sizes(capi):
+    """The scratch is bounded by the GPU, not by the batch or the cache, where sums of tokens are not kept; and grows with what is."""
+    lib, n = capi.lib(), ctypes.c_size_t(0)
+
+    def decode(*a):
+        assert lib.qmm_paged_attention_workspace_size(*a, ctypes.byref(n)) == 0
+        return n.value
+
+    def prompt(*a):
+        assert lib.qmm_paged_prompt_attention_workspace_size(*a, ctypes.byref(n)) == 0
+        return n.value
+
+    assert decode(0, 8, 2, 64, 100) == 0 and decode(4, 0, 2, 64, 100) == 0
+    assert decode(1, 64, 8, 128, 1 << 20) == decode(4096, 64, 8, 128, 1 << 20) <= 40 << 20
+    assert prompt(0, 0, 8, 2, 64, 100) == 0
+    assert prompt(100000, 10, 32, 8, 128, 1 << 17) == 0          # enough tiles for every SM: nothing is split
+    assert prompt(4, 1, 32, 8, 128, 400) == 0                     # short: nothing to split
+    few = prompt(4, 1, 32, 8, 128, 1 << 17)
+    assert 0 < few <= 64 * 4 * 32 * (128 + 2) * 4
+    assert lib.qmm_paged_attention_workspace_size(-1, 8, 2, 64, 100, ctypes.byref(n)) == 1
+    assert lib.qmm_paged_prompt_attention_workspace_size(4, 1, 8, 0, 64, 100, ctypes.byref(n)) == 1
+
+
+@pytest.mark.gpu
+def test_workspaces_that_are_too_small(capi, dev):
+    """A scratch that is missing, too small or off its alignment is refused before any launch."""
+    lib = capi.lib()
+    cache = torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16, device=dev)
+    q, out, lse = torch.zeros((2, 4, 64), dtype=torch.bfloat16, device=dev), torch.empty((2, 4, 64), dtype=torch.bfloat16, device=dev), torch.empty((2, 4), device=dev)
+    table, lens, start = torch.zeros((2, 100), dtype=torch.int32, device=dev), torch.ones(2, dtype=torch.int32, device=dev), torch.arange(3, dtype=torch.int32, device=dev)
+    n = ctypes.c_size_t(0)
+    lib.qmm_paged_attention_workspace_size(2, 4, 2, 64, 1600, ctypes.byref(n))
+    scratch = torch.empty(n.value + 16, dtype=torch.uint8, device=dev)
+    for pointer, size in ((None, n.value), (scratch.data_ptr(), n.value - 1), (scratch.data_ptr() + 8, n.value)):
+        rc = lib.qmm_paged_attention(q.data_ptr(), 0, 2, 4, 256, 64, capi.kv_cache(cache, cache), table.data_ptr(), 100, 100, lens.data_ptr(), 1.0,
+                                     0, 0, out.data_ptr(), lse.data_ptr(), pointer, size, None)
+        assert rc == 6 and b"workspace" in lib.qmm_last_error()
+    lib.qmm_paged_prompt_attention_workspace_size(2, 2, 4, 2, 64, 1600, ctypes.byref(n))
+    assert n.value > 0
+    rc = lib.qmm_paged_prompt_attention(q.data_ptr(), 0, 2, 4, 256, 64, capi.kv_cache(cache, cache), table.data_ptr(), 100, 100, lens.data_ptr(),
+                                        start.data_ptr(), 2, 1.0, 0, 0, out.data_ptr(), lse.data_ptr(), scratch.data_ptr(), n.value - 1, None)
+    assert rc == 6 and b"workspace" in lib.qmm_last_error()
