@@ -28,6 +28,7 @@
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
 // and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
 // come out not finite are looked at again (see mended).
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -68,6 +69,7 @@ struct Tokens {
 struct Item {
     Tokens tokens;
     int64_t first, rows;  // this item's first row, and all of the sequence's
+    int token, head;      // of the first row, from the sequence's first and the group's
     int b, kvh;
     int sink_end, lo, hi;
     int sink_blocks, first_block, blocks;  // tiles of keys that hold places that are seen
@@ -109,19 +111,32 @@ struct Plan {
     size_t part_bytes, bytes;
 };
 
-// The tiles of a call are known on the device alone; what the host knows bounds them.  Few tiles are split over the cache.
-Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places) {
+// The items of a call are known on the device alone; what the host knows bounds them.  Where they are few, each is split over the
+// cache.  An estimate in microseconds decides (measured: 1.2 for a tile of 128 keys and one row tile, 2.4 for two, 1.5 for 64 keys
+// of more than 128 dimensions, 3 for an item; the parts of rows, written and read, at 5 TB/s, and 4 for the second kernel): the
+// CTAs' mean load, lengths being 0.6 of the longest, and half an item, or one item alone.  (Before, 4 CTAs an SM were aimed at: 1184
+// tokens through a window of 1024, 32/8 heads of 128, took 111 us, twice as many tokens, whose items were not split, 77.)
+// seen: the places that an item sees at most.
+Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seen) {
     Plan plan;
     const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
-    const int rows = dim > 128 ? Shape<256>::kRows : Shape<128>::kRows;
-    plan.pairs = tokens * group / rows + (batch < tokens ? batch : tokens);
+    const int rows = dim > 128 ? Shape<256>::kRows : Shape<128>::kRows, keys = dim > 128 ? Shape<256>::kBN : Shape<128>::kBN;
+    const int64_t sequences = batch < tokens ? batch : tokens;
+    plan.pairs = tokens * group / rows + sequences;
     plan.splits = 1;
     const int64_t ctas = plan.pairs * kv_heads, sms = sm_count();
     if (ctas > 0 && ctas < 2 * sms) {
-        const int64_t most = places / 512;
-        int64_t s = (4 * sms + ctas - 1) / ctas;
-        s = s < most ? s : most;
-        plan.splits = static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
+        const int64_t tiles = (seen + keys - 1) / keys;
+        const double tile = dim > 128 ? 1.5 : tokens * group > 128 * sequences ? 2.4 : 1.2;
+        double best = 0.0;
+        for (int s = 1; s <= 64 && (s == 1 || s <= tiles); ++s) {
+            const double item = tile * tiles / s + 3.0, load = ctas * s * (0.6 * tile * tiles / s + 3.0) / sms + 0.5 * item;
+            const double us = (load > item ? load : item) + (s > 1 ? 4.0 + tokens * heads * dim * 8.0 * s / 5e6 : 0.0);
+            if (s == 1 || us < best) {
+                best = us;
+                plan.splits = s;
+            }
+        }
     }
     const size_t all = plan.splits > 1 ? static_cast<size_t>(plan.splits) * tokens * heads : 0;
     plan.part_bytes = all * dim * sizeof(float);
@@ -141,15 +156,23 @@ __device__ __forceinline__ Tokens tokens_of(const Problem &p, int b) {
     return t;
 }
 
-__device__ __forceinline__ int place_of(const Problem &p, const Tokens &t, int64_t row) {
-    const int64_t at = t.place + row / p.group;
-    return at < 0 ? -1 : static_cast<int>(at);
+// The token, from the sequence's first, and the group's head of an item's row; and its place.
+__device__ __forceinline__ int token_of(const Problem &p, const Item &it, int row, int *head) {
+    const uint32_t at = static_cast<uint32_t>(it.head + row), group = static_cast<uint32_t>(p.group), token = at / group;
+    *head = static_cast<int>(at - token * group);
+    return it.token + static_cast<int>(token);
+}
+__device__ __forceinline__ int place_of(const Problem &p, const Item &it, int row) {
+    int head;
+    return max(-1, it.tokens.place + token_of(p, it, row, &head));
 }
 
 template <int BN, int ROWS>
 __device__ __forceinline__ void cover(const Problem &p, Item &it) {
-    const int64_t last = min(it.rows, it.first + ROWS) - 1;
-    const Range a = visible_range(p, place_of(p, it.tokens, it.first)), z = visible_range(p, place_of(p, it.tokens, last));
+    it.token = static_cast<int>(it.first / p.group);
+    it.head = static_cast<int>(it.first - static_cast<int64_t>(it.token) * p.group);
+    const int last = static_cast<int>(min(it.rows - it.first, static_cast<int64_t>(ROWS))) - 1;
+    const Range a = visible_range(p, place_of(p, it, 0)), z = visible_range(p, place_of(p, it, last));
     it.sink_end = z.sink_end;
     it.lo = a.lo;
     it.hi = z.hi;
@@ -227,6 +250,18 @@ __device__ __forceinline__ bool met_not_finite(const Problem &p, const Item &it,
     if (holds_not_finite<T>(p, it.b, it.kvh, a.hi, it.hi)) return true;
     if (holds_not_finite<T>(p, it.b, it.kvh, a.sink_end, min(it.sink_end, it.hi))) return true;
     return holds_not_finite<T>(p, it.b, it.kvh, max(it.lo, a.sink_end), min(z.lo, it.hi));
+}
+
+// Those of the rows `low` to `high` again, one by one, that their bits say are not finite, if that may come from places that they do not see.
+template <typename T>
+__device__ __noinline__ void mend(const Problem &p, const Item &it, int low, int high, uint32_t again) {
+    if (!met_not_finite<T>(p, it, place_of(p, it, low), place_of(p, it, high))) return;
+    __syncwarp();
+    for (; again != 0; again &= again - 1) {
+        int head;
+        const int row = low + __ffs(again) - 1, token = token_of(p, it, row, &head);
+        plain_row<T>(p, it.b, it.tokens.first + token, it.kvh * p.group + head, place_of(p, it, row));
+    }
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -396,6 +431,17 @@ __device__ __forceinline__ bool next_block(uint32_t answer, uint32_t *block) {
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
+// 32 bytes to global memory, a whole sector where it begins at one.
+__device__ __forceinline__ void store_32(void *dst, const uint32_t *x) {
+    if ((reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]),
+                     "r"(x[5]), "r"(x[6]), "r"(x[7])
+                     : "memory");
+    } else {
+        static_cast<uint4 *>(dst)[0] = make_uint4(x[0], x[1], x[2], x[3]);
+        static_cast<uint4 *>(dst)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+    }
+}
 // Bits [from, to) of a word, the bounds being any numbers.
 __device__ __forceinline__ uint32_t bits(int from, int to) {
     const uint32_t low = to <= 0 ? 0u : to >= 32 ? 0xffffffffu : (1u << to) - 1;
@@ -491,7 +537,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             Item it;
             bool found = false;
             while (true) {
-                if (n > 0 || asked > 0) {
+                if (asked > 0) {
+                    clear_rest<T>(p, scratch, id, gridDim.x);
                     if (lane == 0) {
                         mbar_expect_tx(smem_u32(&tail->next_full), 16);
                         ask_next_block(smem_u32(tail->next), smem_u32(&tail->next_full));
@@ -505,7 +552,6 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     if (!have) break;
                 }
                 ++asked;
-                clear_rest<T>(p, scratch, id, gridDim.x);
                 it.split = id % scratch.splits;
                 it.kvh = id / scratch.splits % p.kv_heads;
                 found = find_item<BN, S::kRows>(p, id / scratch.splits / p.kv_heads, it);
@@ -513,8 +559,9 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             }
             if (!ok) break;
             if (found) {
-                it.begin = static_cast<int>(static_cast<int64_t>(it.blocks) * it.split / scratch.splits);
-                it.end = static_cast<int>(static_cast<int64_t>(it.blocks) * (it.split + 1) / scratch.splits);
+                const uint32_t blocks = it.blocks, splits = scratch.splits;  // at most 2^25 and 64
+                it.begin = static_cast<int>(blocks * it.split / splits);
+                it.end = static_cast<int>(blocks * (it.split + 1) / splits);
                 it.two = S::kTiles == 2 && it.first + 128 < it.rows;
                 // the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
                 it.steps = (it.end - it.begin) * S::kSub;
@@ -543,7 +590,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     }
                     __syncwarp();
                     for (int tile = 0; tile < tiles; ++tile) {
-                        const int token = static_cast<int>(it.tokens.first + (it.first + tile * 128) / p.group);
+                        int head;
+                        const int token = static_cast<int>(it.tokens.first) + token_of(p, it, tile * 128, &head);
 #pragma unroll
                         for (int column = 0; column < S::kBoxes; ++column)
                             tma_load_4d_warp(smem_base + (tile * S::kBoxes + column) * S::kQueryBox, &tmap_q, column * 64, 0, it.kvh, token, bar);
@@ -554,8 +602,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     const int chunk = lane % kChunks;
                     const bool mine = chunk < 2 * ksteps, there = chunk * 8 < p.dim;
                     const T *q = static_cast<const T *>(p.q) + it.kvh * p.group * p.q_sh + (there ? chunk * 8 : 0);
-                    int64_t token = (it.first + lane / kChunks) / p.group;
-                    int head = static_cast<int>(it.first + lane / kChunks - token * p.group);
+                    int head;
+                    int64_t token = token_of(p, it, lane / kChunks, &head);
                     for (int r = lane / kChunks; r < tiles * 128; r += kStep) {
                         const bool row = it.first + r < it.rows;
                         if (mine)
@@ -660,13 +708,12 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     const T *base = static_cast<const T *>(part == 0 ? p.k : p.v) + my_offset;
                     const int64_t sb = part == 0 ? p.k_sb : p.v_sb, st = part == 0 ? p.k_st : p.v_st, head = it.kvh * (part == 0 ? p.k_sh : p.v_sh);
 #pragma unroll
-                    for (int group = 0; group < BN / 16; ++group) {
-                        if (group % kLoaders != loader) continue;
-                        const int l = group / 2;
+                    for (int l = 0; l < kLooks; ++l) {
+                        static_assert(kLoaders == 2, "each takes 16 of 32 keys");
                         const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
-#pragma unroll
-                        for (int r = 0; r < 16; r += kStep) {
-                            const int key = group * 16 % 32 + r + my_key;
+                        // a short loop: unrolled, these copies were 42 KB of code, and what the other warps ran was fetched again and again
+#pragma unroll 1
+                        for (int key = loader * 16 + my_key; key < loader * 16 + 16; key += kStep) {
                             const T *row = base + __shfl_sync(0xffffffffu, offset, key);
                             if (my_part)
                                 cp_async_16(dst + my_box + (l * 32 + key) * 128 + (((my_chunk ^ key) & 7) << 4), row,
@@ -714,6 +761,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 for (int box = 0; box < S::kBoxes; ++box)
                     if (box * 4 + 4 <= ksteps)
                         mma_ss_x4(d, a + box * (S::kQueryBox >> 4), b + box * (S::kBox >> 4), kHi, s_desc, box > 0);
+#pragma unroll 1
                 for (int k = ksteps & ~3; k < ksteps; ++k)
                     mma_f16_ss_warp(d, desc64(a + (k >> 2) * (S::kQueryBox >> 4) + (k & 3) * 2, kHi),
                                     desc64(b + (k >> 2) * (S::kBox >> 4) + (k & 3) * 2, kHi), s_desc, k > 0);
@@ -772,10 +820,10 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 if (step + 1 == all) tc_commit_warp(bar_of(&tail->q_empty));
                 advance(k_stage, k_phase, k_half);
             };
-            if (all > 0) make_s(0);
-            for (int step = 0; step < all && ok; ++step, ++done) {
-                const uint32_t odd = done & 1;
+            for (int step = -1; step < all && ok; ++step) {
                 if (step + 1 < all) make_s(step + 1);
+                if (step < 0) continue;
+                const uint32_t odd = done & 1;
                 if (shared || v_half == 0) ok = ok && landed(v_stage, v_phase, 0x94);
                 if (step == 0) {
                     // the softmax has read the O of the item before
@@ -787,6 +835,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 tc_fence_after();
                 product_o(odd, v_lo + v_stage * kStageStep + v_half * kSubStep, step > 0);
                 advance(v_stage, v_phase, v_half);
+                ++done;
             }
             // tiles whose second half was not taken; not before they have come, lest a stage be freed twice by one warp
             if (ok && S::kSub == 2 && (steps & 1) && (!shared || tile == 1)) {
@@ -821,14 +870,15 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             // One row tile: both groups of warps have its rows, the second one the second 64 of every 128 keys.
             const bool shared = S::kTiles == 2 && !it.two;
             const int steps = !shared ? it.steps : group == 0 ? (it.steps + 1) / 2 : it.steps / 2;
+            const int row0 = (shared ? 0 : group * 128) + quarter * 32;  // this warp's first one
+            const int rows = static_cast<int>(min(it.rows - it.first, static_cast<int64_t>(S::kRows)));
             float base = -INFINITY;  // unscaled
             float2 sum2 = make_float2(0.0f, 0.0f);
             if (steps > 0) {
-                const int64_t row0 = it.first + (shared ? 0 : group * 128) + quarter * 32;
-                const Range range = visible_range(p, row0 + lane < it.rows ? place_of(p, it.tokens, row0 + lane) : -1);
+                const Range range = visible_range(p, row0 + lane < rows ? place_of(p, it, row0 + lane) : -1);
                 // what all rows of the warp see
-                const Range low = visible_range(p, place_of(p, it.tokens, min(row0, it.rows - 1)));
-                const int all_lo = visible_range(p, place_of(p, it.tokens, min(row0 + 31, it.rows - 1))).lo;
+                const Range low = visible_range(p, place_of(p, it, min(row0, rows - 1)));
+                const int all_lo = visible_range(p, place_of(p, it, min(row0 + 31, rows - 1))).lo;
                 const int begin = it.begin, sink_blocks = it.sink_blocks, after_sinks = it.first_block - it.sink_blocks;
                 for (int n = 0; n < steps; ++n, ++done) {
                     const int at_tile = shared ? n : n / S::kSub, part = shared ? group : n % S::kSub;
@@ -937,50 +987,59 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 if (other) sum = fmaf(tail->sum[1][my_lane], keep[1], sum);
             }
             tc_fence_after();
-            const int64_t row0 = it.first + (shared ? 0 : group * 128) + quarter * 32, my_row = row0 + lane;
-            const bool mine = my_row < it.rows;
+            const bool mine = row0 + lane < rows;
             const float top = base * scale;
-            const int64_t token = my_row / p.group;
-            const int head = it.kvh * p.group + static_cast<int>(my_row - token * p.group);
-            const int64_t out_row = (it.tokens.first + token) * p.heads + head;
+            int head;
+            const int64_t token = token_of(p, it, row0 + lane, &head);
+            const int64_t out_row = (it.tokens.first + token) * p.heads + it.kvh * p.group + head;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            bool bad = false;
-            // 16 columns of O at a time; two groups that share the rows take turns
-            for (int c = shared ? group : 0; c < ksteps; c += shared ? 2 : 1) {
-                uint32_t o[16];
+            float2 zeros = make_float2(0.0f, 0.0f);  // or NaN, if any of O is not finite
+            // 32 columns of O at a time; two groups that share the rows take turns
+            for (int c = shared ? 2 * group : 0; c < ksteps; c += shared ? 4 : 2) {
+                uint32_t o[32];
+                const uint32_t addr = tmem_base + lanes + S::kO + first * 128 + c * 16;
+                const int halves = c + 1 < ksteps ? 2 : 1;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = 0;
+                for (int j = 0; j < 32; ++j) o[j] = 0;
                 if (it.steps > 0) {
-                    tmem_ld_32x16(tmem_base + lanes + S::kO + first * 128 + c * 16, o);
+                    tmem_ld_32x32(addr, o);
                     tmem_ld_wait();
                     if (other) {
-                        uint32_t o1[16];
-                        tmem_ld_32x16(tmem_base + lanes + S::kO + 128 + c * 16, o1);
+                        uint32_t o1[32];
+                        tmem_ld_32x32(addr + 128, o1);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
+                        for (int j = 0; j < 32; ++j)
                             o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), keep[1], __uint_as_float(o[j]) * keep[0]));
                     }
                 }
-                if (scratch.splits > 1) {
-                    if (mine && it.steps > 0) {
-                        float *dst = scratch.part + (static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row) * p.dim + c * 16;
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            if (c * 16 + j < p.dim) *reinterpret_cast<uint4 *>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                    }
-                } else {
-                    uint32_t w[8];
+                for (int half = 0; half < 2; ++half) {
+                    if (half == halves) break;
+                    const uint32_t *x = o + 16 * half;
+                    const int column = c * 16 + 16 * half;
+                    if (scratch.splits > 1) {
+                        if (mine && it.steps > 0) {
+                            float *dst = scratch.part + (static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row) * p.dim + column;
+                            store_32(dst, x);
+                            if (column + 8 < p.dim) store_32(dst + 8, x + 8);
+                        }
+                    } else {
+                        uint32_t w[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float a = __uint_as_float(o[2 * j]), b = __uint_as_float(o[2 * j + 1]);
-                        bad |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
-                        w[j] = pack2<T>(a * inv, b * inv);
-                    }
-                    if (mine) {
-                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + out_row * p.dim + c * 16);
-                        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                        if (c * 16 + 8 < p.dim) dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 a = make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                            zeros = fma2(a, make_float2(0.0f, 0.0f), zeros);
+                            const float2 y = mul2(a, make_float2(inv, inv));
+                            w[j] = pack2<T>(y.x, y.y);
+                        }
+                        if (mine) {
+                            T *dst = static_cast<T *>(p.out) + out_row * p.dim + column;
+                            if (column + 8 < p.dim)
+                                store_32(dst, w);
+                            else
+                                *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                 }
                 __syncwarp();
@@ -992,7 +1051,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
             }
             // rows that are not finite although their weights are; O may be written again when all that share it have read it
-            uint32_t again = __ballot_sync(0xffffffffu, mine && bad && sum == sum);
+            uint32_t again = __ballot_sync(0xffffffffu, mine && zeros.x + zeros.y != 0.0f && sum == sum);
             tc_fence_before();
             if (shared) {
                 if (lane == 0) tail->bad[group][quarter] = again;
@@ -1001,17 +1060,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 again = group == 0 ? tail->bad[0][quarter] | tail->bad[1][quarter] : 0;
             }
             if (steps > 0 && lane == 0) mbar_arrive(smem_u32(&tail->o_free[group]));
-            if (again != 0) {
-                const int low = place_of(p, it.tokens, min(row0, it.rows - 1)), high = place_of(p, it.tokens, min(row0 + 31, it.rows - 1));
-                if (met_not_finite<T>(p, it, low, high)) {
-                    __syncwarp();
-                    for (; again != 0; again &= again - 1) {
-                        const int64_t row = row0 + __ffs(again) - 1, t = row / p.group;
-                        plain_row<T>(p, it.b, it.tokens.first + t, it.kvh * p.group + static_cast<int>(row - t * p.group),
-                                     place_of(p, it.tokens, row));
-                    }
-                }
-            }
+            if (again != 0) mend<T>(p, it, row0, min(row0 + 31, rows - 1), again);
             count += it.end - it.begin;
             release(item);
         }
@@ -1095,7 +1144,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
         const int64_t at = (token - it.tokens.first) * p.group + head - it.kvh * p.group;
         it.first = at / ROWS * ROWS;
         cover<BN, ROWS>(p, it);
-        const int place = place_of(p, it.tokens, at);
+        const int place = place_of(p, it, static_cast<int>(at - it.first));
         if (met_not_finite<T>(p, it, place, place)) {
             __syncwarp();
             plain_row<T>(p, it.b, token, head, place);
@@ -1166,7 +1215,14 @@ size_t prompt_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv
 }
 
 int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
-    const Plan plan = make_plan(p.tokens, p.batch, p.heads, p.kv_heads, p.dim, static_cast<int64_t>(p.max_pages) * p.page);
+    const int64_t places = static_cast<int64_t>(p.max_pages) * p.page;
+    Plan plan = make_plan(p.tokens, p.batch, p.heads, p.kv_heads, p.dim, places);
+    if (p.window > 0) {
+        // an item's rows see the window of the first and a place for each further token; the workspace is for no window
+        const Plan narrow = make_plan(p.tokens, p.batch, p.heads, p.kv_heads, p.dim,
+                                      std::min(places, static_cast<int64_t>(p.window) + p.sinks + 256 / std::min(p.group, 256)));
+        if (narrow.splits < plan.splits) plan = narrow;
+    }
     if (plan.bytes > 0 && (workspace_bytes < plan.bytes || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
         return fail(QMM_ERR_WORKSPACE, "qmm_paged_prompt_attention: needs a workspace of " + std::to_string(plan.bytes) + " bytes, 16-byte aligned");
     Scratch scratch;
