@@ -64,7 +64,7 @@ static int describe(Problem *p, const char *op, const void *query, int dtype, in
     p->tokens = tokens;
     p->pages = cache->pages;
     const int64_t capacity = cache->pages == 0 ? 0 : max_pages * cache->page_size;
-    p->capacity = static_cast<int>(capacity < 0x7fffffff ? capacity : 0x7fffffff);
+    p->capacity = static_cast<int>(capacity < 0x7fffff00 ? capacity : 0x7fffff00);  // indices run up to a tile further
     p->scale = static_cast<float>(scale);
     return QMM_OK;
 }

@@ -243,13 +243,15 @@ __device__ __noinline__ bool holds_not_finite(const Problem &p, int b, int kvh, 
 }
 
 // Whether rows whose places are `low` to `high` may have met a value that is not finite at a place that they do not see but that
-// the CTA's other rows do.
+// is in the CTA's tiles, of the other rows or beside what they see.
 template <typename T>
 __device__ __forceinline__ bool met_not_finite(const Problem &p, const Item &it, int low, int high) {
+    constexpr int kMost = 128;  // places of a tile
     const Range a = visible_range(p, low), z = visible_range(p, high);
-    if (holds_not_finite<T>(p, it.b, it.kvh, a.hi, it.hi)) return true;
-    if (holds_not_finite<T>(p, it.b, it.kvh, a.sink_end, min(it.sink_end, it.hi))) return true;
-    return holds_not_finite<T>(p, it.b, it.kvh, max(it.lo, a.sink_end), min(z.lo, it.hi));
+    const int limit = min(p.capacity, it.tokens.place + it.tokens.count), hi = min(it.hi, limit - kMost) + kMost;
+    if (holds_not_finite<T>(p, it.b, it.kvh, a.hi, hi)) return true;
+    if (it.sink_end > 0 && holds_not_finite<T>(p, it.b, it.kvh, a.sink_end, min(it.sink_end, hi - kMost) + kMost)) return true;
+    return holds_not_finite<T>(p, it.b, it.kvh, max(it.lo - kMost, a.sink_end), min(z.lo, hi));
 }
 
 // Those of the rows `low` to `high` again, one by one, that their bits say are not finite, if that may come from places that they do not see.
@@ -628,6 +630,9 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
         // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
+        // A tile that is seen in part comes in boxes, too, where its boxes that are seen lie before the sequence's end: what else they
+        // hold was written by earlier tokens, and is masked; a box that is not seen is one that is, once more.  The rest of a page
+        // behind the end may be anything, NaN as well, and comes as zeros.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
         constexpr int kMost = (BN / 16 + kLoaders - 1) / kLoaders;
         int mine = 0;
@@ -641,12 +646,15 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             if (!ok || tail->item[n & 1].none) break;
             const Item it = tail->item[n & 1];
             release(n);
+            const int limit = min(p.capacity, it.tokens.place + it.tokens.count);  // the sequence's end
             int next_id = -1, next_at = 0;
+            bool next_seen = false;
             auto look_up = [&](int i) {
                 if (lane >= boxes) return;
                 const int j = block_start<BN>(it, i) + lane * box_rows;
                 next_id = -1;
-                if (j < p.capacity) {
+                next_seen = j < it.hi && (j < it.sink_end || j > it.lo - box_rows);
+                if (next_seen && j <= limit - box_rows) {
                     const int page = page_of(p, j);
                     next_at = j - page * p.page;
                     next_id = __ldg(p.table + it.b * p.table_st + page);
@@ -655,16 +663,16 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             if (it.begin < it.end) look_up(it.begin);
             for (int i = it.begin; i < it.end && ok; ++i, ++count) {
                 const int first = block_start<BN>(it, i);
-                const bool whole = boxes > 0 && (first + BN <= it.sink_end || (first >= it.lo && first + BN <= it.hi)) &&
-                                   __all_sync(0xffffffffu, lane >= boxes || (next_id >= 0 && next_id < p.pages));
+                const uint32_t seen_boxes = __ballot_sync(0xffffffffu, next_seen);
+                const bool whole = seen_boxes != 0 && __all_sync(0xffffffffu, !next_seen || (next_id >= 0 && next_id < p.pages));
                 uint32_t mask[kLooks];
                 int id[kLooks], at[kLooks], box_page[kMost], box_place[kMost];
                 if (whole) {
 #pragma unroll
                     for (int k = 0; k < kMost; ++k) {
-                        const int box = loader + k * kLoaders;
-                        box_page[k] = __shfl_sync(0xffffffffu, next_id, box);
-                        box_place[k] = __shfl_sync(0xffffffffu, next_at, box);
+                        const int box = loader + k * kLoaders, from = seen_boxes >> box & 1 ? box : __ffs(seen_boxes) - 1;
+                        box_page[k] = __shfl_sync(0xffffffffu, next_id, from);
+                        box_place[k] = __shfl_sync(0xffffffffu, next_at, from);
                     }
                 } else {
 #pragma unroll
