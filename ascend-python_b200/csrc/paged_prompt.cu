@@ -271,6 +271,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two warps' turns: a barrier for each, at which the one waits and the other does not.
+__device__ __forceinline__ void turn_take(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void turn_over(int bar) { asm volatile("bar.arrive %0, 64;" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -429,6 +432,20 @@ __device__ __forceinline__ bool next_block(uint32_t answer, uint32_t *block) {
         : "memory");
     *block = x;
     return got != 0;
+}
+// Whether a barrier's phase is done, without waiting: asked some time before the answer is used, for it takes 100 clocks.
+__device__ __forceinline__ uint32_t mbar_done(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done;
 }
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -880,33 +897,42 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             const int steps = !shared ? it.steps : group == 0 ? (it.steps + 1) / 2 : it.steps / 2;
             const int row0 = (shared ? 0 : group * 128) + quarter * 32;  // this warp's first one
             const int rows = static_cast<int>(min(it.rows - it.first, static_cast<int64_t>(S::kRows)));
+            // Two row tiles take turns at the exponentials of a step, quarter by quarter: both at once, they would wait for the special-function
+            // unit together, and leave it together.
+            const bool turns = S::kTiles == 2 && !shared;
             float base = -INFINITY;  // unscaled
             float2 sum2 = make_float2(0.0f, 0.0f);
             if (steps > 0) {
                 const Range range = visible_range(p, row0 + lane < rows ? place_of(p, it, row0 + lane) : -1);
-                // what all rows of the warp see
+                // what all rows of the warp see: places up to sink_last + 63, and from all_lo to hi_last + 63
                 const Range low = visible_range(p, place_of(p, it, min(row0, rows - 1)));
                 const int all_lo = visible_range(p, place_of(p, it, min(row0 + 31, rows - 1))).lo;
-                const int begin = it.begin, sink_blocks = it.sink_blocks, after_sinks = it.first_block - it.sink_blocks;
+                const int sink_last = low.sink_end - 64, hi_last = low.hi - 64;
+                // a step's first place and the masks of its places: from one tile to the next, but for the gap behind the sinks
+                int start = block_start<BN>(it, it.begin) + (shared ? group * 64 : 0);
+                const int stride = shared ? BN : 64, gap = (it.first_block - it.sink_blocks) * BN;
+                int sink_steps = (it.sink_blocks - it.begin) * (shared ? 1 : S::kSub);  // until the gap
+                const uint32_t valid_stride = shared || S::kSub == 1 ? 16 : 8;
+                uint32_t valid_at = (count * 16 + (shared ? group * 8 : 0)) % (kValid * 16);
+                if (turns && group == 1) turn_over(5 + quarter);
                 for (int n = 0; n < steps; ++n, ++done) {
-                    const int at_tile = shared ? n : n / S::kSub, part = shared ? group : n % S::kSub;
                     const uint32_t odd = done & 1;
                     ok = ok && mbar_wait(smem_u32(&tail->s_full[group]), done & 1, abort_flag, 0x98);
-                    // this step's place of P is free.  (A barrier for even and one for odd steps, each waited for in every phase, so
-                    // that a phase's parity is its own.)
-                    if (done > 1) ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd]), ((done - 2) >> 1) & 1, abort_flag, 0x9b);
                     tc_fence_after();
                     const uint32_t s_addr = tmem_base + lanes + group * 128, p_addr = s_addr + 64 + odd * 32;
                     uint32_t s[2][32];
                     tmem_ld_32x32(s_addr, s[0]);
                     tmem_ld_32x32(s_addr + 32, s[1]);
-                    const uint2 valid = *reinterpret_cast<const uint2 *>(&tail->valid[(count + at_tile) % kValid][part * 2]);
-                    const int i = begin + at_tile, start = (i < sink_blocks ? i : i + after_sinks) * BN + part * 64;
-                    const bool whole = (start + 64 <= low.sink_end || (start >= all_lo && start + 64 <= low.hi)) && (valid.x & valid.y) == 0xffffffffu;
+                    const uint2 valid = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint8_t *>(tail->valid) + valid_at);
+                    // whether this step's place of P is free.  (A barrier for even and one for odd steps, each waited for in every
+                    // phase, so that a phase's parity is its own.)
+                    const uint32_t p_bar = smem_u32(&tail->o_done[group][odd]), p_phase = ((done - 2) >> 1) & 1;
+                    const bool free = done < 2 || mbar_done(p_bar, p_phase) != 0;
                     tmem_ld_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&tail->s_free[group]));
+                    const bool whole = (start <= sink_last || (start >= all_lo && start <= hi_last)) && (valid.x & valid.y) == 0xffffffffu;
                     if (factor <= 0.0f) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) s[j / 32][j % 32] = __float_as_uint(__uint_as_float(s[j / 32][j % 32]) * sign);
@@ -951,8 +977,12 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     }
                     // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another;
                     // the sum takes the weights unrounded
-                    const float offset = base == -INFINITY ? 0.0f : -base * scale;
+                    float offset = base == -INFINITY ? 0.0f : -base * scale;
+                    if (turns) turn_take(5 + 4 * group + quarter);
+                    asm volatile("" : "+f"(offset));  // no exponential before the turn
                     const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
+                    if (!free) ok = ok && mbar_wait(p_bar, p_phase, abort_flag, 0x9b);
+                    tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t w[16];
@@ -972,6 +1002,10 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                         }
                         sum2 = add2(sum2, e[0]);
                     }
+                    start += stride;
+                    if (--sink_steps == 0) start += gap;
+                    valid_at = (valid_at + valid_stride) % (kValid * 16);
+                    if (turns && (group == 0 || n + 1 < steps)) turn_over(9 - 4 * group + quarter);
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
