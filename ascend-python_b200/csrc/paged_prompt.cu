@@ -737,7 +737,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                         static_assert(kLoaders == 2, "each takes 16 of 32 keys");
                         const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
                         // a short loop: unrolled, these copies were 42 KB of code, and what the other warps ran was fetched again and again
-#pragma unroll 1
+#pragma unroll 2
                         for (int key = loader * 16 + my_key; key < loader * 16 + 16; key += kStep) {
                             const T *row = base + __shfl_sync(0xffffffffu, offset, key);
                             if (my_part)
@@ -835,9 +835,9 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             ++queries;
             if (all == 0) tc_commit_warp(bar_of(&tail->q_empty));
             auto make_s = [&](int step) {
+                if (shared || k_half == 0) ok = ok && landed(k_stage, k_phase, 0x93);
                 // the softmax has taken the S before
                 if (made > 0) ok = ok && mbar_wait(bar_of(tail->s_free) + tile * 8, (made - 1) & 1, abort_flag, 0x92);
-                if (shared || k_half == 0) ok = ok && landed(k_stage, k_phase, 0x93);
                 if (!ok) return;
                 tc_fence_after();
                 product_s(a, k_lo + k_stage * kStageStep + k_half * kSubStep);
