@@ -4,8 +4,9 @@
 // of a wide group fill a tile as well as many of a narrow one, and every key that is read serves the whole group.
 //
 // For 64 keys at a time, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory, and P, rounded to the
-// values' type, is the second product's operand in tensor memory.  The softmax is one pass: a thread has a row, its running base (a maximum) and sum.  The base moves, and O is rescaled, only when a row's
-// maximum has grown by more than 2^8 since; until then the weights are up to 2^8 and as exact.
+// values' type, is the second product's operand in tensor memory.  The softmax is one pass: a thread has a row, its running base
+// (a maximum) and sum.  The base moves, and O is rescaled, only when a row's maximum has grown by more than 2^8 since; until then
+// the weights are up to 2^8 and as exact.
 //
 // A CTA goes on to a further block of the grid, as long as there are blocks that have not begun (cluster launch control), so the
 // hardware's order of the blocks balances the work as it does without; the next item's keys, values and query are fetched, and
@@ -13,21 +14,26 @@
 //
 // An item of one row tile, as a few drafted tokens are, gives both halves of the CTA its rows, every second 64 keys each; their O
 // and sums are added at the end.
+//
 // The softmax has its scores in registers and gives S back at once: the next Q K^T runs beside it, and so does P V of the step
-// before, for P has two places of its own (with P in S's place and S twice, it waited 450 of 2400 clocks a step).  Two row tiles
-// share the keys (dimensions up to 128).  What bounds a step (8192 tokens, 32/8 heads of 128: 2250 clocks for 64 keys, the products
-// take 1240): the softmax warps' chain, wait, load, maximum, and 64 exponentials a thread, which the special-function unit, shared by the
-// two row tiles, takes 1024 clocks for.  A quarter to a half of them as a polynomial on the FMA pipe, two threads a row, and row
-// tiles half a step apart were all slower or the same.
+// before, for P has two places of its own.  Two row tiles share the keys (dimensions up to 128), and take turns at the
+// exponentials.  What bounds a step (8192 tokens, 32/8 heads of 128: 1830 clocks for 64 keys, 480 to 555 us in all as the clock goes; the
+// products alone take 1280): the chain of a softmax warp, its wait (200), load and maximum (450), exponentials (700 at least, of
+// which the special-function unit has 512 to itself) and hand-over.  Slower or the same were: part of the exponentials as a
+// polynomial on the FMA pipe, two threads a row, the row tiles half a step apart without turns, S twice with P in its place.
+//
+// The warps run different code, and evict one another's from the instruction cache where it is long (at 160 KB the same loops took
+// 2250 clocks a step, and an item's end 8000): what is rare is called or looped, and each part is in the code once.
 //
 // Warps 0..3 and 4..7: softmax and epilogue of the two row tiles.  Warps 8 and 9: MMA, one for each row tile, so that the tensor
-// pipe has the one's products while the other waits at its barriers.  Warps 10 and 11: keys; 12 and 13: values.  (In
-// one order, keys would wait for the values before them, which are free two steps later.)  Warp 14: items, and the
-// query.  Where a page
-// holds a multiple of 16 places, a tile that is seen whole comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
-// warps took 1.7 us for the 64 KiB of a block, more than its products take); other tiles by cp.async, any page size
-// and strides, and rows that no row of the CTA sees are zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is not finite; rows that
-// come out not finite are looked at again (see mended).
+// pipe has the one's products while the other waits at its barriers.  Warps 10 and 11: keys; 12 and 13: values.  (In one order,
+// keys would wait for the values before them, which are free two steps later.)  Warp 14: items, and the query.
+//
+// Where a page holds a multiple of 16 places, a tile comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
+// warps took 1.7 us for the 64 KiB of a block, more than its products take); the tile with the sequence's end and tiles with pages
+// that are none come by cp.async, as all do with other page sizes and strides, and rows that no row of the CTA sees are
+// zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is
+// not finite; rows that come out not finite are looked at again (mend).
 #include <algorithm>
 #include <type_traits>
 
@@ -129,7 +135,8 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
         const int64_t tiles = (seen + keys - 1) / keys;
         const double tile = dim > 128 ? 1.5 : tokens * group > 128 * sequences ? 2.4 : 1.2;
         double best = 0.0;
-        for (int s = 1; s <= 64 && (s == 1 || s <= tiles); ++s) {
+        const int64_t most = std::min<int64_t>(tiles, (256ll << 20) / (tokens * heads * std::max<int64_t>(dim, 1) * 4));  // 256 MiB of parts
+        for (int s = 1; s <= 64 && (s == 1 || s <= most); ++s) {
             const double item = tile * tiles / s + 3.0, load = ctas * s * (0.6 * tile * tiles / s + 3.0) / sms + 0.5 * item;
             const double us = (load > item ? load : item) + (s > 1 ? 4.0 + tokens * heads * dim * 8.0 * s / 5e6 : 0.0);
             if (s == 1 || us < best) {
@@ -646,7 +653,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const bool my_part = my_chunk < 2 * ksteps;
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
-        // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a tile's g-th box a tile ahead.
+        // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a
+        // tile's g-th box a tile ahead.
         // A tile that is seen in part comes in boxes, too, where its boxes that are seen lie before the sequence's end: what else they
         // hold was written by earlier tokens, and is masked; a box that is not seen is one that is, once more.  The rest of a page
         // behind the end may be anything, NaN as well, and comes as zeros.

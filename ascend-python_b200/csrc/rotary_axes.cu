@@ -11,8 +11,9 @@
 // made in 64 bits, in half turns, reduced to [-1, 1] there, and only then rounded for sincospif (off by 2^-25 half turns).
 // The rotation is fp32 with one rounding to the tensors' type at the end.
 //
-// Bound by HBM: every element is read and written once.  One CTA a token: its threads have their first loads under way while n
-// of them make the token's sines and cosines, which all heads share, in shared memory.
+// Bound by HBM: every element is read and written once.  One CTA for two tokens: its threads have their first loads under way
+// while n of them make a token's sines and cosines, which all heads share, in shared memory.  8192 tokens, 32/8 heads of 128 on
+// three axes: 29 us, 5.8 TB/s, 0.89 of a copy (one token a CTA 38 us, four 32).
 #include "qmm_common.cuh"
 
 namespace qmm {

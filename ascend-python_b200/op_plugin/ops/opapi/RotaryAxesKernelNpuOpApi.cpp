@@ -99,6 +99,12 @@ at::Tensor npu_rotary_axes_cache(const at::Tensor &query, const at::Tensor &key,
     const qmm_kv_cache cache = op_plugin_utils::describe_cache(op, key_cache, value_cache, query);
     TORCH_CHECK(cache.kv_heads == key.size(1) && cache.dim == key.size(2), op, ": the cache should hold ", key.size(1), " heads of ",
                 key.size(2), ", but it is ", key_cache.sizes());
+    for (const auto &c : {key_cache, value_cache}) {
+        for (int64_t d = 0; d < 3; ++d) {
+            TORCH_CHECK(c.size(d) == 1 || c.stride(d) != 0, op, ": the places of a cache that is written should not overlap, but its strides are ",
+                        c.strides());
+        }
+    }
     const int slot_dtype = index_dtype(op, "slots", slots);
     TORCH_CHECK(slots.dim() == 1 && slots.size(0) == r.tokens, op, ": slots should hold ", r.tokens, " tokens, but they are ",
                 slots.sizes());

@@ -205,3 +205,5 @@ def test_refusals(npu, dev):
     refused("int32 or int64", q, k, v, positions, inv_freq, kc, vc, slots.float(), sections=s)
     refused("should hold 4 tokens", q, k, v, positions, inv_freq, kc, vc, slots[:3], sections=s)
     refused("should be on", q, k, v, positions, inv_freq, kc, vc, slots.cpu(), sections=s)
+    one = [c[:1].expand(4, -1, -1, -1) for c in (kc, vc)]
+    refused("should not overlap", q, k, v, positions, inv_freq, *one, slots, sections=s)
