@@ -415,7 +415,7 @@ QMM_API int qmm_rotary_axes_cache(const void *query, int64_t query_stride_token,
  * seen are not followed, and the places not read.  Scores, softmax and sums are fp32.
  * query: bf16 or f16 like the cache, [batch, heads, dim]; out: dense; lse: [batch, heads]; block_table: int32 [batch, max_pages],
  * rows table_stride apart; dim: a multiple of 8 up to 256; query and caches begin at 16-byte boundaries, their strides are
- * multiples of 8 elements.  The workspace (16-byte aligned, of the size that the first function gives for max_places =
+ * multiples of 8 elements; a sequence has up to 2^31 - 256 places.  The workspace (16-byte aligned, of the size that the first function gives for max_places =
  * max_pages * page_size) holds nothing between calls; calls that may run at the same time need one each.
  */
 QMM_API int qmm_paged_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_places,
@@ -431,7 +431,8 @@ QMM_API int qmm_paged_attention(const void *query, int dtype, int64_t batch, int
  * form, test/test_custom_ops/test_prompt_flash_attention.py): whole prompts, later chunks of them, a few
  * drafted tokens.  Sequence b has the tokens query_start[b] ... query_start[b + 1] - 1 of `query` ([tokens, heads, dim]), n of
  * them; its i-th is at place p = seq_lens[b] - n + i and sees what qmm_paged_attention says.  query_start: int32 [batch + 1], not
- * decreasing.  Tokens of no sequence have out 0 and lse -inf.
+ * decreasing.  Tokens of no sequence have out 0 and lse -inf.  Of a page that holds a place that is seen, places beside it may be
+ * read as well, in front of the sequence's end; whatever they hold, the results are those of the places that are seen.
  */
 QMM_API int qmm_paged_prompt_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
                                                       int64_t max_places, size_t *bytes);
