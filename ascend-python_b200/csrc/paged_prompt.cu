@@ -82,6 +82,7 @@ struct Item {
     int split, begin, end;                 // the tiles of this item
     int steps;                             // of 64 keys
     int two;                               // the second row tile has rows
+    int cut;                               // its rows have parts in the workspace
     int none;                              // there is no further item
 };
 
@@ -89,7 +90,7 @@ constexpr int kValid = 8;  // tiles of keys whose masks are kept: more than may 
 struct Tail {
     uint64_t full[6], empty[6];
     uint64_t s_full[2], s_free[2], p_full[2][2], o_done[2][2];  // [row tile], [row tile][step % 2]
-    uint64_t o_free[2], q_full, q_empty, item_full[2], item_empty[2], next_full;
+    uint64_t o_free[2], q_full, q_empty, item_full[2], item_empty[2], item_loaded, next_full;
     alignas(16) uint32_t valid[kValid][4];
     alignas(16) uint32_t next[4];  // the answer to the request for a further block
     Item item[2];
@@ -103,25 +104,29 @@ constexpr size_t smem_bytes() {
     return 1024 + Shape<DP>::kQuery + Shape<DP>::kStages * Shape<DP>::kStage + sizeof(Tail);
 }
 
-// Workspace (splits > 1): part[split][token * heads + head][dim], stat[split][..] (base, sum).
+// Workspace (splits > 1): part[split][token * heads + head][dim], stat[split][..] (base, sum), pieces.
 struct Scratch {
     float *part;
     float2 *stat;
-    int splits;
+    int *pieces;  // of them that a call uses; 1: none
+    int splits, sms;
+    float tile;  // microseconds
     uint32_t *status;
 };
 
 struct Plan {
     int64_t pairs;  // at most
     int splits;
-    size_t part_bytes, bytes;
+    double tile;
+    size_t part_bytes, stat_bytes, bytes;
 };
 
-// The items of a call are known on the device alone; what the host knows bounds them.  Where they are few, each is split over the
-// cache.  An estimate in microseconds decides (measured: 1.2 for a tile of 128 keys and one row tile, 2.4 for two, 1.5 for 64 keys
-// of more than 128 dimensions, 3 for an item; the parts of rows, written and read, at 5 TB/s, and 4 for the second kernel): the
-// CTAs' mean load, lengths being 0.6 of the longest, and half an item, or one item alone.  (Before, 4 CTAs an SM were aimed at: 1184
-// tokens through a window of 1024, 32/8 heads of 128, took 111 us, twice as many tokens, whose items were not split, 77.)
+// The items of a call are known on the device alone; what the host knows bounds them.  Where they are few, each may be cut into
+// pieces (choose_pieces), of which the host says how many at most: as many as give every SM one, or by an estimate in
+// microseconds for lengths that are 0.6 of the longest in the mean (measured: 1.2 for a tile of 128 keys and one row tile, 2.4 for two, 1.5 for
+// 64 keys of more than 128 dimensions, 3 for an item; the parts of rows, written and read, at 5 TB/s, and 4 for the second kernel): the
+// CTAs' mean load and half an item, or one item alone.  (Before, 4 CTAs an SM were aimed at: 1184 tokens through a window of
+// 1024, 32/8 heads of 128, took 111 us, twice as many tokens, whose items were not cut, 77.)
 // seen: the places that an item sees at most.
 Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seen) {
     Plan plan;
@@ -130,24 +135,28 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
     const int64_t sequences = batch < tokens ? batch : tokens;
     plan.pairs = tokens * group / rows + sequences;
     plan.splits = 1;
+    plan.tile = dim > 128 ? 1.5 : tokens * group > 128 * sequences ? 2.4 : 1.2;
     const int64_t ctas = plan.pairs * kv_heads, sms = sm_count();
     if (ctas > 0 && ctas < 2 * sms) {
         const int64_t tiles = (seen + keys - 1) / keys;
-        const double tile = dim > 128 ? 1.5 : tokens * group > 128 * sequences ? 2.4 : 1.2;
+        const double tile = plan.tile;
         double best = 0.0;
         const int64_t most = std::min<int64_t>(tiles, (256ll << 20) / (tokens * heads * std::max<int64_t>(dim, 1) * 4));  // 256 MiB of parts
         for (int s = 1; s <= 64 && (s == 1 || s <= most); ++s) {
-            const double item = tile * tiles / s + 3.0, load = ctas * s * (0.6 * tile * tiles / s + 3.0) / sms + 0.5 * item;
+            const double item = tile * tiles / s + 3.0;
+            const double load = ctas * (0.6 * tile * tiles + 3.0 * (s == 1 ? 1.0 : 0.6 * s + 0.5)) / sms + 0.5 * item;
             const double us = (load > item ? load : item) + (s > 1 ? 4.0 + tokens * heads * dim * 8.0 * s / 5e6 : 0.0);
             if (s == 1 || us < best) {
                 best = us;
                 plan.splits = s;
             }
         }
+        if (plan.splits > 1) plan.splits = static_cast<int>(std::max<int64_t>(plan.splits, std::min({most, sms / ctas, static_cast<int64_t>(64)})));
     }
     const size_t all = plan.splits > 1 ? static_cast<size_t>(plan.splits) * tokens * heads : 0;
     plan.part_bytes = all * dim * sizeof(float);
-    plan.bytes = plan.part_bytes + all * sizeof(float2);
+    plan.stat_bytes = (all * sizeof(float2) + 15) / 16 * 16;
+    plan.bytes = all > 0 ? plan.part_bytes + plan.stat_bytes + 16 : 0;
     return plan;
 }
 
@@ -217,6 +226,65 @@ __device__ __forceinline__ bool find_item(const Problem &p, int64_t pair, Item &
         return true;
     }
     return false;
+}
+
+// The tiles of keys of a sequence's item that has most, or somewhat more, and its items of one key-value head.
+template <int BN, int ROWS>
+__device__ __forceinline__ int most_blocks(const Problem &p, int b, int64_t *items) {
+    const Tokens t = tokens_of(p, b);
+    *items = (static_cast<int64_t>(t.count) * p.group + ROWS - 1) / ROWS;
+    if (t.count == 0) return 0;
+    const Range z = visible_range(p, max(-1, t.place + t.count - 1));
+    int blocks = z.hi / BN + 1;
+    if (p.window > 0) blocks = static_cast<int>(min(static_cast<int64_t>(blocks), (static_cast<int64_t>(p.window) + ROWS / p.group) / BN + 2));
+    return blocks + (z.sink_end + BN - 1) / BN;
+}
+
+// How many pieces the longest sequence is cut into, and their length in tiles, which is that of all sequences' pieces, so that an
+// item is as long as another; by one warp, alike in all CTAs.  The times are those of make_plan, in tiles.  (Cut into as many
+// pieces whatever their length, drafts over 2000 to 16000 places took 110 us, not 100; cut at all, equal lengths of 8000 took 107,
+// not 95.)
+template <int BN, int ROWS>
+__device__ __noinline__ int2 choose_pieces(const Problem &p, const Scratch &scratch) {
+    const int lane = threadIdx.x & 31;
+    int longest = 1;
+    float items = 0.0f, total = 0.0f;
+    for (int b = lane; b < p.batch; b += 32) {
+        int64_t n;
+        const int blocks = most_blocks<BN, ROWS>(p, b, &n);
+        longest = max(longest, blocks);
+        items += static_cast<float>(n * p.kv_heads);
+        total += static_cast<float>(n * p.kv_heads) * blocks;
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+        items += __shfl_xor_sync(0xffffffffu, items, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    const float sms = static_cast<float>(scratch.sms), start = 3.0f / scratch.tile, join = 4.0f / scratch.tile;
+    const float part = static_cast<float>(p.tokens * p.heads) * p.dim * (8.0f / 5e6f / scratch.tile);
+    // as many as give every SM one, and powers of two
+    int2 best = make_int2(1, longest);
+    float least = INFINITY;
+    for (int i = 0; i < 8; ++i) {
+        const int n = i < 7 ? 1 << i : static_cast<int>(sms / fmaxf(items, 1.0f));
+        if (n < 1 || n > scratch.splits || n > longest) continue;
+        const int piece = (longest + n - 1) / n;
+        float count = 0.0f;
+        for (int b = lane; b < p.batch; b += 32) {
+            int64_t m;
+            const int blocks = most_blocks<BN, ROWS>(p, b, &m);
+            count += static_cast<float>(m * p.kv_heads) * static_cast<float>((blocks + piece - 1) / piece);
+        }
+        for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+        const float item = piece + start;
+        const float time = (count <= sms ? item : fmaxf(item, (total + count * start) / sms + 0.5f * item)) + (n > 1 ? join + part * n : 0.0f);
+        if (time < least) {
+            least = time;
+            best = make_int2(n, piece);
+        }
+    }
+    return best;
 }
 
 template <int BN>
@@ -522,6 +590,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         }
         mbar_init(smem_u32(&tail->q_full), 33);
         mbar_init(smem_u32(&tail->q_empty), S::kTiles);
+        mbar_init(smem_u32(&tail->item_loaded), 1);
         mbar_init(smem_u32(&tail->next_full), 1);
         tail->abort_flag = 0;
         mbar_fence_init();
@@ -554,11 +623,15 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
     if (warp == kSoftmax + 2 + 2 * kLoaders) {
         // ---------------- items, and the query ----------------
         uint32_t id = blockIdx.x, asked = 0, queries = 0;
+        const int2 pieces = scratch.splits > 1 ? choose_pieces<BN, S::kRows>(p, scratch) : make_int2(1, 0);
+        if (scratch.splits > 1 && lane == 0) *scratch.pieces = pieces.x;  // the same from all CTAs
+        const uint32_t units = gridDim.x / scratch.splits;
         bool have = true, ok = true;
         int n = 0;
         while (ok && have) {
-            // a block is asked for when the item before the present one is done, not earlier: what is taken cannot go to another CTA
-            ok = mbar_wait(smem_u32(&tail->item_empty[n & 1]), (n >> 1 & 1) ^ 1, abort_flag, 0x9e);
+            // a block is asked for when the present item's last keys are, not earlier: what is taken cannot go to another CTA
+            if (n > 0) ok = mbar_wait(smem_u32(&tail->item_loaded), (n - 1) & 1, abort_flag, 0x9c);
+            ok = ok && mbar_wait(smem_u32(&tail->item_empty[n & 1]), (n >> 1 & 1) ^ 1, abort_flag, 0x9e);
             if (!ok) break;
             Item it;
             bool found = false;
@@ -578,16 +651,28 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     if (!have) break;
                 }
                 ++asked;
-                it.split = id % scratch.splits;
-                it.kvh = id / scratch.splits % p.kv_heads;
-                found = find_item<BN, S::kRows>(p, id / scratch.splits / p.kv_heads, it);
-                if (found) break;
+                it.split = id / units;
+                if (it.split >= pieces.x) continue;
+                it.kvh = id % units % p.kv_heads;
+                found = find_item<BN, S::kRows>(p, id % units / p.kv_heads, it);
+                if (!found) continue;
+                it.begin = 0;
+                it.end = it.blocks;
+                it.cut = pieces.x > 1;
+                if (!it.cut) break;
+                it.begin = min(it.split * pieces.y, it.blocks);
+                it.end = it.split + 1 < pieces.x ? min(it.begin + pieces.y, it.blocks) : it.blocks;
+                if (it.begin < it.end) break;
+                const int rows = static_cast<int>(min(it.rows - it.first, static_cast<int64_t>(S::kRows)));
+                for (int r = lane; r < rows; r += 32) {
+                    int head;
+                    const int64_t token = it.tokens.first + token_of(p, it, r, &head);
+                    scratch.stat[(it.split * p.tokens + token) * p.heads + it.kvh * p.group + head] = make_float2(-INFINITY, 0.0f);
+                }
+                found = false;
             }
             if (!ok) break;
             if (found) {
-                const uint32_t blocks = it.blocks, splits = scratch.splits;  // at most 2^25 and 64
-                it.begin = static_cast<int>(blocks * it.split / splits);
-                it.end = static_cast<int>(blocks * (it.split + 1) / splits);
                 it.two = S::kTiles == 2 && it.first + 128 < it.rows;
                 // the last tile's second half may lie behind all that is seen (a tile of sinks may have some of the window)
                 it.steps = (it.end - it.begin) * S::kSub;
@@ -762,6 +847,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     phase ^= 1;
                 }
             }
+            if (part == 0 && loader == 0 && lane == 0) mbar_arrive(smem_u32(&tail->item_loaded));
         }
         cp_async_wait_all();
     } else if (warp >= kSoftmax && warp < kSoftmax + S::kTiles) {
@@ -1068,7 +1154,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     if (half == halves) break;
                     const uint32_t *x = o + 16 * half;
                     const int column = c * 16 + 16 * half;
-                    if (scratch.splits > 1) {
+                    if (it.cut) {
                         if (mine && it.steps > 0) {
                             float *dst = scratch.part + (static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row) * p.dim + column;
                             store_32(dst, x);
@@ -1095,7 +1181,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 __syncwarp();
             }
             if (mine && group == first) {
-                if (scratch.splits > 1)
+                if (it.cut)
                     scratch.stat[static_cast<int64_t>(it.split) * p.tokens * p.heads + out_row] = make_float2(top, sum);
                 else
                     p.lse[out_row] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
@@ -1132,24 +1218,25 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), rows = p.tokens * p.heads;
-    if (row >= rows) return;
+    const int splits = *scratch.pieces;
+    if (row >= rows || splits == 1) return;
     float top = -INFINITY;
-    for (int i = lane; i < scratch.splits; i += 32) top = fmaxf(top, scratch.stat[i * rows + row].x);
+    for (int i = lane; i < splits; i += 32) top = fmaxf(top, scratch.stat[i * rows + row].x);
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, acc[8] = {};
-    for (int i0 = 0; i0 < scratch.splits; i0 += 32) {
+    for (int i0 = 0; i0 < splits; i0 += 32) {
         float weight = 0.0f;
         bool any = false;
-        if (i0 + lane < scratch.splits) {
+        if (i0 + lane < splits) {
             const float2 st = scratch.stat[(i0 + lane) * rows + row];
             weight = exp2_fast(st.x - base);
             sum = fmaf(st.y, weight, sum);
-            any = st.y != 0.0f;  // a split without blocks has written no part
+            any = st.y != 0.0f;  // a split without tiles has written no part
         }
         const uint32_t has = __ballot_sync(0xffffffffu, any);
 #pragma unroll 4
-        for (int i = 0; i < min(32, scratch.splits - i0); ++i) {
+        for (int i = 0; i < min(32, splits - i0); ++i) {
             const float w = __shfl_sync(0xffffffffu, weight, i);
             if (!(has >> i & 1)) continue;
             const float *src = scratch.part + ((i0 + i) * rows + row) * p.dim;
@@ -1278,7 +1365,10 @@ int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace
     Scratch scratch;
     scratch.part = static_cast<float *>(workspace);
     scratch.stat = reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + plan.part_bytes);
+    scratch.pieces = reinterpret_cast<int *>(static_cast<uint8_t *>(workspace) + plan.part_bytes + plan.stat_bytes);
     scratch.splits = plan.splits;
+    scratch.sms = sm_count();
+    scratch.tile = static_cast<float>(plan.tile);
     scratch.status = device_status_word();
     return dtype == QMM_DTYPE_BF16 ? launch_t<__nv_bfloat16>(p, plan, scratch, stream) : launch_t<__half>(p, plan, scratch, stream);
 }

@@ -195,6 +195,37 @@ def test_tokens_before_the_first_and_behind_the_last(npu, paged, dev):
     check(npu, paged, q, k, v, table, lens, starts + 2)
 
 
+@pytest.mark.parametrize("dim,heads,kv", [(128, 8, 2), (64, 16, 2), (256, 4, 2), (80, 12, 4)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2500, 4)])
+def test_pieces_of_ragged_sequences(npu, paged, dev, dim, heads, kv, window, sinks):
+    """Few tokens: long sequences are cut, short ones are not, some see nothing; short ones alone in a table that could hold
+    much; what a captured graph does when the lengths change."""
+    rng = random.Random(dim)
+    lens, new = [20011, 100, 0, 5000, 17, -3, 9000, 2], [3, 2, 2, 40, 1, 1, 0, 4]
+    check(npu, paged, *make(dev, lens, new, heads=heads, kv=kv, dim=dim, seed=25, tail=3), window=window, sinks=sinks)
+    state = make(dev, [90, 33, 1, 128], [4, 3, 1, 2], heads=heads, kv=kv, dim=dim, seed=26, columns=3000)
+    check(npu, paged, *state, window=window, sinks=sinks)
+    lens = [rng.randrange(20, 6000) for _ in range(12)]
+    q, k, v, table, lens, starts = make(dev, lens, [rng.randrange(1, 7) for _ in lens], heads=heads, kv=kv, dim=dim, seed=27)
+    graph = torch.cuda.CUDAGraph()
+    call(npu, q, k, v, table, lens, starts, window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = call(npu, q, k, v, table, lens, starts, window=window, sinks=sinks)
+    for change in (lambda n: n, lambda n: (n // 50).clamp(min=1), lambda n: n * 0, lambda n: n.roll(3).minimum(n)):
+        kept = lens.clone()
+        lens.copy_(change(lens))
+        graph.replay()
+        want = call(npu, q, k, v, table, lens, starts, window=window, sinks=sinks)
+        assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+        ref = paged.attention(q, k, v, table, lens, starts, window=window, sinks=sinks)
+        bound, lse_bound = paged.attention_bounds(q.dtype, dim, *ref)
+        assert bool(((got[0].double() - ref[0]).abs() <= bound).all())
+        none = ref[1] == -math.inf
+        assert torch.equal(got[1] == -math.inf, none) and bool(((got[1].double() - ref[1]).abs() <= lse_bound)[~none].all())
+        lens.copy_(kept)
+
+
 @pytest.mark.parametrize("dim", [128, 256])
 def test_values_not_finite_where_a_row_is_split(npu, paged, dev, dim):
     """As above for a few tokens over a long cache, whose parts are added by another kernel."""
