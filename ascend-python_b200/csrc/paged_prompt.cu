@@ -29,7 +29,7 @@
 // pipe has the one's products while the other waits at its barriers.  Warps 10 and 11: keys; 12 and 13: values.  (In one order,
 // keys would wait for the values before them, which are free two steps later.)  Warp 14: items, and the query.
 //
-// Where a page holds a multiple of 16 places, a tile comes by TMA, in boxes of 16 to 128 places and 64 columns (by cp.async two
+// Where a page holds a multiple of 8 places, a tile comes by TMA, in boxes of 8 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); the tile with the sequence's end and tiles with pages
 // that are none come by cp.async, as all do with other page sizes and strides, and rows that no row of the CTA sees are
 // zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is
@@ -744,7 +744,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         // hold was written by earlier tokens, and is masked; a box that is not seen is one that is, once more.  The rest of a page
         // behind the end may be anything, NaN as well, and comes as zeros.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
-        constexpr int kMost = (BN / 16 + kLoaders - 1) / kLoaders;
+        constexpr int kMost = (BN / 8 + kLoaders - 1) / kLoaders;
         int mine = 0;
         for (int n = loader; n < boxes; n += kLoaders) ++mine;
         const uint32_t my_bytes = mine * S::kBoxes * box_rows * 128;
@@ -1321,9 +1321,9 @@ int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStrea
     QMM_CUDA_OK(cudaFuncSetAttribute(prompt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<DP>())));
     CUtensorMap tmap_k = {}, tmap_v = {};
     // as many places a box as begin together in any page and any tile
-    int box_rows = 16;
+    int box_rows = 8;
     while (2 * box_rows <= Shape<DP>::kBN && p.page % (2 * box_rows) == 0) box_rows *= 2;
-    if (p.page % 16 != 0 || p.pages == 0 || !cache_map(&tmap_k, p, p.k, p.k_sb, p.k_st, p.k_sh, box_rows) ||
+    if (p.page % 8 != 0 || p.pages == 0 || !cache_map(&tmap_k, p, p.k, p.k_sb, p.k_st, p.k_sh, box_rows) ||
         !cache_map(&tmap_v, p, p.v, p.v_sb, p.v_st, p.v_sh, box_rows))
         box_rows = 0;
     // the query's rows of a tile in one box, where the group's heads divide a tile
