@@ -828,6 +828,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 #pragma unroll
                     for (int l = 0; l < kLooks; ++l) {
                         static_assert(kLoaders == 2, "each takes 16 of 32 keys");
+                        // keys that are not seen may be anything, for their scores are masked; values are multiplied by 0
+                        if (part == 0 && (mask[l] >> loader * 16 & 0xffff) == 0) continue;
                         const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
                         // a short loop: unrolled, these copies were 42 KB of code, and what the other warps ran was fetched again and again
 #pragma unroll 2
