@@ -312,8 +312,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 full = full && value_seen[l] == 0xffffffffu;
             }
             const T *base = static_cast<const T *>(cache) + my_offset;
-            // (which way is the usual one is said throughout, so that the loop lies close together: its warps wait for instructions a
-            // quarter of the time)
+            // (which way is the usual one is said throughout, so that the loop lies close together: its warps wait for
+            // instructions a quarter of the time)
             if (__builtin_expect(even, 1)) {
                 const T *row[KEYS / 16];
 #pragma unroll
@@ -559,8 +559,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         __syncthreads();
 
         // ---- the warps' parts: neighbours of one head tile are added in their order (a warp's second part is its last) ----
-        // Every thread has four columns of a row of all of them, loaded together: one after the other, a part's latency each, took 10
-        // of 133 us (64 sequences of 500 to 8000 places, 64/8 heads of 128).
+        // Every thread has four columns of a row of all of them, loaded together: one after the other, a part's latency each,
+        // took 10 of 133 us (64 sequences of 500 to 8000 places, 64/8 heads of 128).
         const int64_t first_part = static_cast<int64_t>(worker) * S::kWarps * 2;
         for (int idx = threadIdx.x; idx < scratch.rows * (p.dim / 4); idx += kThreads) {
             const int row = idx / (p.dim / 4), d = (idx - row * (p.dim / 4)) * 4;

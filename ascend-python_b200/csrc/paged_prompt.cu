@@ -17,10 +17,11 @@
 //
 // The softmax has its scores in registers and gives S back at once: the next Q K^T runs beside it, and so does P V of the step
 // before, for P has two places of its own.  Two row tiles share the keys (dimensions up to 128), and take turns at the
-// exponentials.  What bounds a step (8192 tokens, 32/8 heads of 128: 1830 clocks for 64 keys, 480 to 555 us in all as the clock goes; the
-// products alone take 1280): the chain of a softmax warp, its wait (200), load and maximum (450), exponentials (700 at least, of
-// which the special-function unit has 512 to itself) and hand-over.  Slower or the same were: part of the exponentials as a
-// polynomial on the FMA pipe, two threads a row, the row tiles half a step apart without turns, S twice with P in its place.
+// exponentials.  What bounds a step (8192 tokens, 32/8 heads of 128: 1830 clocks for 64 keys, 470 to 555 us in all as the clock
+// goes; the products alone take 1280): the chain of a softmax warp, its wait (200), load and maximum (450), exponentials (700
+// at least, of which the special-function unit has 512 to itself) and hand-over.  Slower or the same were: part of the
+// exponentials as a polynomial on the FMA pipe, two threads a row, the row tiles half a step apart without turns, S twice with
+// P in its place.
 //
 // The warps run different code, and evict one another's from the instruction cache where it is long (at 160 KB the same loops took
 // 2250 clocks a step, and an item's end 8000): what is rare is called or looped, and each part is in the code once.
@@ -50,8 +51,8 @@ constexpr int kThreads = 32 * (kSoftmax + 2 + 2 * kLoaders + 1);
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
 
-// DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: for each row tile S, 64, and two P, 32 each; then
-// O.  256 columns of O leave room for one row tile.
+// DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: for each row tile S, 64, and two P, 32
+// each; then O.  256 columns of O leave room for one row tile.
 template <int DP>
 struct Shape {
     static constexpr int kTiles = DP == 256 ? 1 : 2;
@@ -123,10 +124,10 @@ struct Plan {
 
 // The items of a call are known on the device alone; what the host knows bounds them.  Where they are few, each may be cut into
 // pieces (choose_pieces), of which the host says how many at most: as many as give every SM one, or by an estimate in
-// microseconds for lengths that are 0.6 of the longest in the mean (measured: 1.2 for a tile of 128 keys and one row tile, 2.4 for two, 1.5 for
-// 64 keys of more than 128 dimensions, 3 for an item; the parts of rows, written and read, at 5 TB/s, and 4 for the second kernel): the
-// CTAs' mean load and half an item, or one item alone.  (Before, 4 CTAs an SM were aimed at: 1184 tokens through a window of
-// 1024, 32/8 heads of 128, took 111 us, twice as many tokens, whose items were not cut, 77.)
+// microseconds for lengths that are 0.6 of the longest in the mean (measured: 1.2 for a tile of 128 keys and one row tile, 2.4
+// for two, 1.5 for 64 keys of more than 128 dimensions, 3 for an item; the parts of rows, written and read, at 5 TB/s, and 4
+// for the second kernel): the CTAs' mean load and half an item, or one item alone.  (Before, 4 CTAs an SM were aimed at: 1184
+// tokens through a window of 1024, 32/8 heads of 128, took 111 us, twice as many tokens, whose items were not cut, 77.)
 // seen: the places that an item sees at most.
 Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seen) {
     Plan plan;
@@ -242,7 +243,7 @@ __device__ __forceinline__ int most_blocks(const Problem &p, int b, int64_t *ite
 
 // How many pieces the longest sequence is cut into, and their length in tiles, which is that of all sequences' pieces, so that an
 // item is as long as another; by one warp, alike in all CTAs.  The times are those of make_plan, in tiles.  (Cut into as many
-// pieces whatever their length, drafts over 2000 to 16000 places took 110 us, not 100; cut at all, equal lengths of 8000 took 107,
+// pieces whatever their length, drafts over 2000 to 16000 places took 110 us, not 104; cut at all, equal lengths of 8000 took 107,
 // not 95.)
 template <int BN, int ROWS>
 __device__ __noinline__ int2 choose_pieces(const Problem &p, const Scratch &scratch) {
@@ -329,7 +330,8 @@ __device__ __forceinline__ bool met_not_finite(const Problem &p, const Item &it,
     return holds_not_finite<T>(p, it.b, it.kvh, max(it.lo - kMost, a.sink_end), min(z.lo, hi));
 }
 
-// Those of the rows `low` to `high` again, one by one, that their bits say are not finite, if that may come from places that they do not see.
+// Those of the rows `low` to `high` again, one by one, that their bits say are not finite, if that may come from places that
+// they do not see.
 template <typename T>
 __device__ __noinline__ void mend(const Problem &p, const Item &it, int low, int high, uint32_t again) {
     if (!met_not_finite<T>(p, it, place_of(p, it, low), place_of(p, it, high))) return;
@@ -738,11 +740,11 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const bool my_part = my_chunk < 2 * ksteps;
         const uint32_t my_box = (my_chunk / 8) * S::kBox;
         const int my_offset = my_chunk < row_chunks ? my_chunk * 8 : 0;
-        // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the page of a
-        // tile's g-th box a tile ahead.
-        // A tile that is seen in part comes in boxes, too, where its boxes that are seen lie before the sequence's end: what else they
-        // hold was written by earlier tokens, and is masked; a box that is not seen is one that is, once more.  The rest of a page
-        // behind the end may be anything, NaN as well, and comes as zeros.
+        // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the
+        // page of a tile's g-th box a tile ahead.  A tile that is seen in part comes in boxes, too, where its boxes that are
+        // seen lie before the sequence's end: what else they hold was written by earlier tokens, and is masked; a box that is
+        // not seen is one that is, once more.  The rest of a page behind the end may be anything, NaN as well, and comes as
+        // zeros.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
         constexpr int kMost = (BN / 8 + kLoaders - 1) / kLoaders;
         int mine = 0;
@@ -831,7 +833,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                         // keys that are not seen may be anything, for their scores are masked; values are multiplied by 0
                         if (part == 0 && (mask[l] >> loader * 16 & 0xffff) == 0) continue;
                         const int64_t offset = mask[l] >> lane & 1 ? id[l] * sb + at[l] * st + head : 0;
-                        // a short loop: unrolled, these copies were 42 KB of code, and what the other warps ran was fetched again and again
+                        // a short loop: unrolled, these copies were 42 KB of code, and what the other warps ran was fetched
+                        // again and again
 #pragma unroll 2
                         for (int key = loader * 16 + my_key; key < loader * 16 + 16; key += kStep) {
                             const T *row = base + __shfl_sync(0xffffffffu, offset, key);
@@ -970,8 +973,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         const int group = warp >> 2, quarter = warp & 3;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const int my_lane = quarter * 32 + lane;
-        // The running maximum is one of unscaled scores, which takes a positive scale: with a negative one, or 0, the scores take its
-        // sign.
+        // The running maximum is one of unscaled scores, which takes a positive scale: with a negative one, or 0, the scores
+        // take its sign.
         const float scale = factor == 0.0f ? 1.0f : fabsf(factor), sign = factor < 0.0f ? -1.0f : 0.0f;
         // the warps of both groups that have a quarter of the rows, or two such quarters
         auto meet = [&] {
@@ -993,8 +996,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             const int steps = !shared ? it.steps : group == 0 ? (it.steps + 1) / 2 : it.steps / 2;
             const int row0 = (shared ? 0 : group * 128) + quarter * 32;  // this warp's first one
             const int rows = static_cast<int>(min(it.rows - it.first, static_cast<int64_t>(S::kRows)));
-            // Two row tiles take turns at the exponentials of a step, quarter by quarter: both at once, they would wait for the special-function
-            // unit together, and leave it together.
+            // Two row tiles take turns at the exponentials of a step, quarter by quarter: both at once, they would wait for the
+            // special-function unit together, and leave it together.
             const bool turns = S::kTiles == 2 && !shared;
             float base = -INFINITY;  // unscaled
             float2 sum2 = make_float2(0.0f, 0.0f);
