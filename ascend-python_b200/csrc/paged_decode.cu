@@ -16,6 +16,8 @@
 // their order.  (The warps of a CTA taking the tiles of one sequence in turn, with a join at its end, cost about 3 us a sequence:
 // 64 sequences of 500 to 8000 places, 64/8 heads of 128, 131 us.)  Where every sequence is short and head tiles are few, CTAs
 // have whole ones in turn, cut for their warps alone.  Nothing depends on timing, and nothing has to be zero before a call.
+#include <type_traits>
+
 #include "paged_common.cuh"
 
 namespace qmm {
@@ -153,6 +155,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Powers of two by which weights are larger than exp(score - maximum) until the log-sum: f16 has no full step below 2^-14 and
+// nothing below 2^-25, so a weight of 1 for the largest score would lose the many keys of a long cache that lie 2^-25 and more
+// below one that stands out; with 2^15 what is lost lies 2^-40 below it.  bf16 has the exponents of fp32.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 
 // What a warp left of a head tile, for the CTA to add up.
 struct Part {
@@ -487,9 +495,14 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     sum[0] *= keep[0];
                     sum[1] *= keep[1];
                 }
-                // the weights, rounded to the type of the values (the sum takes them unrounded: 2^-9 or 2^-12 of each weight,
-                // independent of one another), as they lie are the second product's first operand
+                // the weights, rounded to the type of the values, as they lie are the second product's first operand.  That is half a
+                // step, 2^-8 or 2^-11, of each weight (of f16 weights below 2^-29 of the largest: 2^-40 of that one).  The sum
+                // takes them unrounded, so equal weights are all off alike.
                 uint32_t a[KEYS / 16][4];
+                if (kLift<T> != 0.0f) {
+                    base[0] -= kLift<T>;
+                    base[1] -= kLift<T>;
+                }
 #pragma unroll
                 for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
@@ -528,7 +541,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             for (int r = 0; r < 2; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                top[r] *= scale;
+                top[r] = fmaf(top[r], scale, -kLift<T>);  // the sums are 2^kLift times those of exp(score - maximum)
                 const int row = r0 + r * 8;
                 if (row >= rows) continue;
                 if (begins && ends) {

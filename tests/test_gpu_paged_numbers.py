@@ -1,0 +1,50 @@
+"""Attention over the paged cache where its numbers can go wrong: one key that has nearly all the weight."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged_attention import call, npu  # noqa: F401  (fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def steps(dev, scores, dtype, heads=4, dim=64, page=64, new=None, batch=1):
+    """Keys whose scores (scale 1) are `scores`, the same for every head; all sequences have the same pages."""
+    n = scores.numel()
+    pages = -(-n // page)
+    k, v = torch.zeros((2, pages * page, 1, dim), dtype=dtype, device=dev)
+    k[:n, 0, 0] = scores.to(dtype)
+    table = torch.arange(pages, dtype=torch.int32, device=dev).repeat(batch, 1)
+    q = torch.zeros((batch * (new or 1), heads, dim), dtype=dtype, device=dev)
+    q[..., 0] = 1.0
+    lens = torch.full((batch,), n, dtype=torch.int32, device=dev)
+    starts = None if new is None else torch.arange(batch + 1, dtype=torch.int32, device=dev) * new
+    return q, k.view(pages, page, 1, dim), v.view(pages, page, 1, dim), table, lens, starts
+
+
+# (new tokens, sequences): one token, whose places all warps share; as many sequences as give a warp a long stretch
+FORMS = [(None, 1), (None, 300)]
+
+
+@pytest.mark.parametrize("new,batch", FORMS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("below", [13.0, 15.9, 16.3])
+def test_one_key_with_nearly_all_the_weight(npu, dev, below, dtype, new, batch):
+    """131071 keys far below the first, which has the value 0 where theirs is 1: their small weights are the whole output.
+
+    A weight is rounded once (u relative, all alike), the output too; the sums are fp32, of at most 131072 terms in some 8192 steps of
+    16 of one sign: 2^-24 each if every step rounds the same way, which is 2^-11.
+    """
+    n = 131072
+    scores = torch.full((n,), -below, device=dev)
+    scores[0] = 0.0
+    q, k, v, table, lens, starts = steps(dev, scores, dtype, new=new, batch=batch)
+    v[:] = 1.0
+    v[0, 0] = 0.0
+    out, lse = call(npu, q, k, v, table, lens, starts, scale_value=1.0)
+    mass = (n - 1) * math.exp(float(k[0, 1, 0, 0]))
+    want = mass / (1 + mass)
+    u = torch.finfo(dtype).eps / 2
+    assert (out.double() / want - 1).abs().max().item() <= 2 * u + 2.0 ** -11
+    assert (lse.double() - math.log1p(mass)).abs().max().item() <= 2.0 ** -11
