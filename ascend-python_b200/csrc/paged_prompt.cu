@@ -5,8 +5,8 @@
 //
 // For 64 keys at a time, S = Q K^T and O += P V are tcgen05 products with accumulators in tensor memory, and P, rounded to the
 // values' type, is the second product's operand in tensor memory.  The softmax is one pass: a thread has a row, its running base
-// (a maximum) and sum.  The base moves, and O is rescaled, only when a row's maximum has grown by more than 2^8 since; until then
-// the weights are up to 2^8 and as exact.
+// (a maximum) and sum.  The base moves, and O is rescaled, only when a row's maximum has grown by more than 2^8 (f16: 2^4) since;
+// until then the weights are that much larger and as exact.
 //
 // A CTA goes on to a further block of the grid, as long as there are blocks that have not begun (cluster launch control), so the
 // hardware's order of the blocks balances the work as it does without; the next item's keys, values and query are fetched, and
@@ -49,7 +49,15 @@ constexpr int kSoftmax = 8;    // warps
 constexpr int kLoaders = 2;    // warps, of keys and as many of values
 constexpr int kThreads = 32 * (kSoftmax + 2 + 2 * kLoaders + 1);
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kGrowth = 8.0f;  // of a row's maximum, in powers of two, before its base moves
+// Growth of a row's maximum, in powers of two, before its base moves; and powers of two by which weights are larger than
+// exp(score - base) until the log-sum.  f16 has no full step below 2^-14 and nothing below 2^-25, so with a weight of 1 at the base
+// the many keys of a long cache that lie 2^-25 and more below one that stands out would be lost: the two together take its range up
+// to 2^15, and what is lost lies 2^-36 below the largest.  (Scores that are normal with a deviation of 1 grow by less than 2^4
+// behind the first 64.)  bf16 has the exponents of fp32.
+template <typename T>
+constexpr float kGrowth = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.0f - kGrowth<T> : 0.0f;
 
 // DP: the head dimension rounded up to 64, 128 or 256.  Tensor memory, 512 columns: for each row tile S, 64, and two P, 32
 // each; then O.  256 columns of O leave room for one row tile.
@@ -1054,7 +1062,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                             m[c] = max3(m[c], __uint_as_float(s[j / 32][j % 32 + 2 * c]), __uint_as_float(s[j / 32][j % 32 + 2 * c + 1]));
                     }
                     const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
-                    const bool move = most > base && (most - base) * scale > kGrowth;  // from -inf always
+                    const bool move = most > base && (most - base) * scale > kGrowth<T>;  // from -inf always
                     if (__any_sync(0xffffffffu, move)) {
                         const float now = move ? most : base;
                         const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
@@ -1074,9 +1082,10 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                         }
                         base = now;
                     }
-                    // P in the type of the values, half a step of it off each weight (2^-9 or 2^-12), one independent of another;
-                    // the sum takes the weights unrounded
-                    float offset = base == -INFINITY ? 0.0f : -base * scale;
+                    // P in the type of the values: off by half a step, 2^-8 or 2^-11, of each weight (of f16 weights below 2^-25
+                    // of the largest: 2^-36 of that one).  The sum takes the weights unrounded, so equal weights are all off
+                    // alike.
+                    float offset = base == -INFINITY ? 0.0f : fmaf(-base, scale, kLift<T>);
                     if (turns) turn_take(5 + 4 * group + quarter);
                     asm volatile("" : "+f"(offset));  // no exponential before the turn
                     const float2 scale2 = make_float2(scale, scale), offset2 = make_float2(offset, offset);
@@ -1129,7 +1138,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             }
             tc_fence_after();
             const bool mine = row0 + lane < rows;
-            const float top = base * scale;
+            const float top = fmaf(base, scale, -kLift<T>);  // the sums are 2^kLift times those of exp(score - base)
             int head;
             const int64_t token = token_of(p, it, row0 + lane, &head);
             const int64_t out_row = (it.tokens.first + token) * p.heads + it.kvh * p.group + head;

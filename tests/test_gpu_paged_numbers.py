@@ -1,10 +1,11 @@
-"""Attention over the paged cache where its numbers can go wrong: one key that has nearly all the weight."""
+"""Attention over the paged cache where its numbers can go wrong: one key that has nearly all the weight, and runs of
+equal scores."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_paged_attention import call, npu  # noqa: F401  (fixture)
+from test_gpu_paged_attention import call, npu, paged  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -23,8 +24,9 @@ def steps(dev, scores, dtype, heads=4, dim=64, page=64, new=None, batch=1):
     return q, k.view(pages, page, 1, dim), v.view(pages, page, 1, dim), table, lens, starts
 
 
-# (new tokens, sequences): one token, whose places all warps share; as many sequences as give a warp a long stretch
-FORMS = [(None, 1), (None, 300)]
+# (new tokens, sequences): one token, whose places all warps share; as many sequences as give a warp a long stretch; a prompt's
+# token, whose places are split; as many as leave nothing to split
+FORMS = [(None, 1), (None, 300), (1, 1), (1, 300)]
 
 
 @pytest.mark.parametrize("new,batch", FORMS)
@@ -48,3 +50,20 @@ def test_one_key_with_nearly_all_the_weight(npu, dev, below, dtype, new, batch):
     u = torch.finfo(dtype).eps / 2
     assert (out.double() / want - 1).abs().max().item() <= 2 * u + 2.0 ** -11
     assert (lse.double() - math.log1p(mass)).abs().max().item() <= 2.0 ** -11
+
+
+@pytest.mark.parametrize("new,batch", FORMS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rise", [0.3, 1.0, 2.7, 5.5])
+def test_equal_scores_behind_lower_ones(npu, paged, dev, rise, dtype, new, batch):
+    """Keys of one score behind a stretch of lower ones: where the base of the weights stays behind, all have the same weight,
+    rounded the same way, while their sum is not rounded.  The bound has that rounding (u) beside the output's."""
+    scores = torch.full((3000,), rise, device=dev)
+    scores[:130] = 0.0
+    q, k, v, table, lens, starts = steps(dev, scores, dtype, new=new, batch=batch)
+    v.uniform_(0.9, 1.1, generator=torch.Generator(device=dev).manual_seed(3))
+    out, lse = call(npu, q, k, v, table, lens, starts, scale_value=1.0)
+    one = None if starts is None else starts[:2]
+    ref = paged.attention(q[:1], k, v, table[:1], lens[:1], one, scale=1.0)
+    bound, lse_bound = paged.attention_bounds(dtype, q.shape[2], *ref)
+    assert bool(((out.double() - ref[0]).abs() <= bound).all()) and bool(((lse.double() - ref[1]).abs() <= lse_bound).all())
