@@ -52,10 +52,14 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Growth of a row's maximum, in powers of two, before its base moves; and powers of two by which weights are larger than
 // exp(score - base) until the log-sum.  f16 has no full step below 2^-14 and nothing below 2^-25, so with a weight of 1 at the base
 // the many keys of a long cache that lie 2^-25 and more below one that stands out would be lost: the two together take its range up
-// to 2^15, and what is lost lies 2^-36 below the largest.  (Scores that are normal with a deviation of 1 grow by less than 2^4
-// behind the first 64.)  bf16 has the exponents of fp32.
+// to 2^15, and what is lost lies 2^-36 below the largest.  Scores that are normal with a deviation of 1 grow by less than 2^4
+// behind the first 64, but by more behind a few, as sinks are: where a row's first keys are not 64, the base begins 2^3 above them,
+// and what is lost may lie 2^-33 below the largest (6 chunks of 100 to 2000 tokens, window 1024, 4 sinks: 87 to 91 us, without
+// that 92 to 95).  bf16 has the exponents of fp32.
 template <typename T>
 constexpr float kGrowth = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+template <typename T>
+constexpr float kSpare = std::is_same<T, __half>::value ? 3.0f : 0.0f;
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 15.0f - kGrowth<T> : 0.0f;
 
@@ -1064,7 +1068,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
                     const bool move = most > base && (most - base) * scale > kGrowth<T>;  // from -inf always
                     if (__any_sync(0xffffffffu, move)) {
-                        const float now = move ? most : base;
+                        float now = move ? most : base;
+                        if (kSpare<T> > 0.0f && move && base == -INFINITY && !whole) now += fminf(kSpare<T> / scale, 1e30f);
                         const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
                         sum2 = mul2(sum2, make_float2(keep, keep));
                         if (n > 0) {
@@ -1083,7 +1088,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                         base = now;
                     }
                     // P in the type of the values: off by half a step, 2^-8 or 2^-11, of each weight (of f16 weights below 2^-25
-                    // of the largest: 2^-36 of that one).  The sum takes the weights unrounded, so equal weights are all off
+                    // of the largest: up to 2^-33 of that one).  The sum takes the weights unrounded, so equal weights are all off
                     // alike.
                     float offset = base == -INFINITY ? 0.0f : fmaf(-base, scale, kLift<T>);
                     if (turns) turn_take(5 + 4 * group + quarter);

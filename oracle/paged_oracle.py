@@ -88,12 +88,13 @@ def attention_bounds(dtype, dim, out, lse, weight, spread, reach):
     d = (dim + 3) * 2^-24 * reach (reach: its terms' absolute sum).  A weight is exp of it (2^-21 covers exp2's own error, the
     rounding of the largest score and of the sums' rescaling), rounded to the type for the product with the values (u), so
         |out - ref| <= u |ref| + (u + 2 d + 2^-20) sum p |v|   and   |lse - ref| <= d + 2^-20 + 2^-22 |lse|.
-    f16 has no full step below 2^-14: what lies there is off by up to 2^-25.  An output is as it is; weights are multiplied by 2^11 at
-    least, so that the largest is 2^11 or more and the others are off by up to 2^-36 of it.
+    f16 has no full step below 2^-14: what lies there is off by up to 2^-25.  An output is as it is; weights are multiplied by
+    2^11 at least, relative to a score that is 2^3 above the largest at most, so that the largest is 2^8 or more and the others
+    are off by up to 2^-33 of it.
     """
     u = torch.finfo(dtype).eps / 2
     d = (dim + 3) * 2.0 ** -24 * reach
     bound = u * out.abs() + (u + 2 * d[..., None] + 2.0 ** -20) * weight
     if dtype == torch.float16:
-        bound = bound + 2.0 ** -36 * spread + 2.0 ** -25
+        bound = bound + 2.0 ** -33 * spread + 2.0 ** -25
     return bound, d + 2.0 ** -20 + 2.0 ** -22 * lse.abs().nan_to_num(posinf=0.0)
