@@ -755,8 +755,9 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         // Boxes: a warp fetches every second (a box takes it some 100 clocks to issue).  Lane g of a warp has looked up the
         // page of a tile's g-th box a tile ahead.  A tile that is seen in part comes in boxes, too, where its boxes that are
         // seen lie before the sequence's end: what else they hold was written by earlier tokens, and is masked; a box that is
-        // not seen is one that is, once more.  The rest of a page behind the end may be anything, NaN as well, and comes as
-        // zeros.
+        // not seen is one behind the cache's last page, which is zeros.  (A box that is seen, once more, would give the rows that
+        // see an infinite value in it 0 times that value as well.)  The rest of a page behind the end may be anything, NaN
+        // as well, and comes as zeros.
         const int boxes = box_rows > 0 ? BN / box_rows : 0;
         constexpr int kMost = (BN / 8 + kLoaders - 1) / kLoaders;
         int mine = 0;
@@ -794,9 +795,9 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 if (whole) {
 #pragma unroll
                     for (int k = 0; k < kMost; ++k) {
-                        const int box = loader + k * kLoaders, from = seen_boxes >> box & 1 ? box : __ffs(seen_boxes) - 1;
-                        box_page[k] = __shfl_sync(0xffffffffu, next_id, from);
-                        box_place[k] = __shfl_sync(0xffffffffu, next_at, from);
+                        const int box = loader + k * kLoaders;
+                        box_page[k] = __shfl_sync(0xffffffffu, next_seen ? next_id : static_cast<int>(p.pages), box);
+                        box_place[k] = __shfl_sync(0xffffffffu, next_at, box);
                     }
                 } else {
 #pragma unroll

@@ -1,11 +1,11 @@
-"""Attention over the paged cache where its numbers can go wrong: one key that has nearly all the weight, and runs of
-equal scores."""
+"""Attention over the paged cache where its numbers can go wrong: one key that has nearly all the weight, runs of equal scores, values
+that are not finite."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_paged_attention import call, npu, paged  # noqa: F401  (fixtures)
+from test_gpu_paged_attention import call, make, npu, paged  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +67,35 @@ def test_equal_scores_behind_lower_ones(npu, paged, dev, rise, dtype, new, batch
     ref = paged.attention(q[:1], k, v, table[:1], lens[:1], one, scale=1.0)
     bound, lse_bound = paged.attention_bounds(dtype, q.shape[2], *ref)
     assert bool(((out.double() - ref[0]).abs() <= bound).all()) and bool(((lse.double() - ref[1]).abs() <= lse_bound).all())
+
+
+def same_as_definition(npu, paged, q, k, v, table, lens, starts, **kw):
+    """Infinities and NaN as the definition has them, the rest within its bounds."""
+    out, lse = call(npu, q, k, v, table, lens, starts, **kw)
+    ref = paged.attention(q, k, v, table, lens, starts, **kw)
+    bound, lse_bound = paged.attention_bounds(q.dtype, q.shape[2], *ref)
+    odd = ~ref[0].isfinite()
+    got = out.double()
+    assert torch.equal(got[odd].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), ref[0][odd].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
+    assert bool(((got - ref[0]).abs() <= bound)[~odd].all())
+    none = ref[1] == -math.inf
+    assert torch.equal(lse == -math.inf, none) and bool(((lse.double() - ref[1]).abs() <= lse_bound)[~none].all())
+    return odd
+
+
+@pytest.mark.parametrize("window,sinks,page,dim", [(40, 4, 16, 128), (200, 4, 16, 128), (300, 20, 32, 256), (100, 3, 8, 64), (100, 4, 20, 128),
+                                                   (0, 0, 16, 128), (1, 140, 64, 64)])
+@pytest.mark.parametrize("split", [False, True])
+def test_infinite_values(npu, paged, dev, window, sinks, page, dim, split):
+    """A value that is infinite makes the rows that see it infinite, not NaN, whatever comes beside it in a tile; two of both signs NaN."""
+    lens, new = ([3000, 1500], [6, 5]) if split else ([900, 700], [300, 260])
+    for tokens in (None, new):
+        q, k, v, table, length, starts = make(dev, lens, tokens, heads=4, kv=2, dim=dim, page=page, seed=dim + page)
+        hit = 0
+        for places in ((1,), (130,), (lens[0] - 3,), (2, lens[0] - 2)):
+            for sign in (1.0, -1.0):
+                v2 = v.clone()
+                for i, j in enumerate(places):
+                    v2[table[0, j // page], j % page, 1, 3] = math.inf * sign * (-1) ** i
+                hit += int(same_as_definition(npu, paged, q, k, v2, table, length, starts, window=window, sinks=sinks).sum())
+        assert hit > 0
