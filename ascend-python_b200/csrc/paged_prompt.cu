@@ -34,7 +34,7 @@
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); the tile with the sequence's end and tiles with pages
 // that are none come by cp.async, as all do with other page sizes and strides, and rows that no row of the CTA sees are
 // zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is
-// not finite; rows that come out not finite are looked at again (mend).
+// not finite; rows that come out not finite beside such a value are made again, by plain sums, at the CTA's end (remake_rows).
 #include <algorithm>
 #include <type_traits>
 
@@ -110,6 +110,8 @@ struct Tail {
     uint32_t copied[6];            // stage: by cp.async
     float sum[2][128], base[2][128];  // [group of softmax warps][row]
     uint32_t bad[2][4], going[2][4];  // [group][quarter]: rows that are not finite; the warp has an item
+    uint32_t again[2][2][4];  // [item % 2][row tile][quarter]: rows to be made again when the CTA's last item is done
+    uint32_t remake;          // there are such rows
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -342,16 +344,61 @@ __device__ __forceinline__ bool met_not_finite(const Problem &p, const Item &it,
     return holds_not_finite<T>(p, it.b, it.kvh, max(it.lo - kMost, a.sink_end), min(z.lo, hi));
 }
 
-// Those of the rows `low` to `high` again, one by one, that their bits say are not finite, if that may come from places that
-// they do not see.
+// Rows of an item again, those that their bits say, `row0` the first, by all warps of the CTA, which share the keys.  kRemade at a
+// time; `room`: shared memory for their queries and a part of each a warp.  (264 such rows of each of 8 CTAs, heads of 128: 7 ms over
+// 4000 places, 266 over 131072.  One row at a time took 3.5 times as long.)
+constexpr int kRemade = 4;
 template <typename T>
-__device__ __noinline__ void mend(const Problem &p, const Item &it, int low, int high, uint32_t again) {
-    if (!met_not_finite<T>(p, it, place_of(p, it, low), place_of(p, it, high))) return;
-    __syncwarp();
-    for (; again != 0; again &= again - 1) {
-        int head;
-        const int row = low + __ffs(again) - 1, token = token_of(p, it, row, &head);
-        plain_row<T>(p, it.b, it.tokens.first + token, it.kvh * p.group + head, place_of(p, it, row));
+__device__ __noinline__ void remake_rows(const Problem &p, const Item &it, int row0, uint32_t again, float *room) {
+    constexpr int kWarps = kThreads / 32, kPart = 256 + 2;
+    static_assert((kRemade * (kPlainDim + kWarps * kPart)) * sizeof(float) <= Shape<64>::kQuery + Shape<64>::kStages * Shape<64>::kStage, "room");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    while (again != 0) {
+        int place[kRemade], head[kRemade];
+        int64_t token[kRemade];
+        RowPart r[kRemade];
+#pragma unroll
+        for (int i = 0; i < kRemade; ++i) {
+            place[i] = -1;
+            token[i] = head[i] = 0;
+            if (again == 0) continue;
+            const int row = row0 + __ffs(again) - 1;
+            again &= again - 1;
+            place[i] = place_of(p, it, row);
+            token[i] = it.tokens.first + token_of(p, it, row, &head[i]);
+            head[i] += it.kvh * p.group;
+            if (warp == i) stage_query<T>(p, token[i], head[i], room + i * kPlainDim);
+        }
+        __syncthreads();
+        rows_part<T, kRemade>(p, it.b, it.kvh, place, room, warp, kWarps, r);
+        float *parts = room + kRemade * kPlainDim;
+#pragma unroll
+        for (int i = 0; i < kRemade; ++i) {
+            float *mine = parts + (i * kWarps + warp) * kPart;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) mine[c * 32 + lane] = r[i].acc[c];
+            if (lane == 0) {
+                mine[256] = r[i].top;
+                mine[257] = r[i].total;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRemade; ++i) {
+            if (warp != i || place[i] < 0) continue;
+            RowPart all = {{}, -INFINITY, 0.0f};
+            for (int w = 0; w < kWarps; ++w) {
+                const float *one = parts + (i * kWarps + w) * kPart;
+                const float top = fmaxf(all.top, one[256]), base = top == -INFINITY ? 0.0f : top;
+                const float keep = expf(all.top - base), add = expf(one[256] - base);
+                all.top = top;
+                all.total = fmaf(one[257], add, all.total * keep);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) all.acc[c] = fmaf(one[c * 32 + lane], add, all.acc[c] * keep);
+            }
+            write_row<T>(p, token[i], head[i], all);
+        }
+        __syncthreads();
     }
 }
 
@@ -607,6 +654,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         mbar_init(smem_u32(&tail->item_loaded), 1);
         mbar_init(smem_u32(&tail->next_full), 1);
         tail->abort_flag = 0;
+        tail->remake = 0;
+        for (int i = 0; i < 16; ++i) tail->again[i >> 3][i >> 2 & 1][i & 3] = 0;
         mbar_fence_init();
         if (box_rows > 0) {
             tma_prefetch_desc(&tmap_k);
@@ -652,6 +701,11 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             while (true) {
                 if (asked > 0) {
                     clear_rest<T>(p, scratch, id, gridDim.x);
+                    // Rows are to be made again: no further item.  (What is left begins as blocks of its own.)  An item before the
+                    // last two has said so by now, so that these are still in their places.
+                    have = *reinterpret_cast<volatile uint32_t *>(&tail->remake) == 0;
+                    have = __all_sync(0xffffffffu, have);
+                    if (!have) break;
                     if (lane == 0) {
                         mbar_expect_tx(smem_u32(&tail->next_full), 16);
                         ask_next_block(smem_u32(tail->next), smem_u32(&tail->next_full));
@@ -695,9 +749,12 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     if (last + 64 >= (it.end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --it.steps;
                 }
             }
-            it.none = !found;
             if (lane == 0) {
-                tail->item[n & 1] = it;
+                it.none = 0;
+                if (found)
+                    tail->item[n & 1] = it;
+                else
+                    tail->item[n & 1].none = 1;  // the rest is that of an item whose rows may have to be made again
                 mbar_arrive(smem_u32(&tail->item_full[n & 1]));
             }
             __syncwarp();
@@ -1216,7 +1273,13 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 again = group == 0 ? tail->bad[0][quarter] | tail->bad[1][quarter] : 0;
             }
             if (steps > 0 && lane == 0) mbar_arrive(smem_u32(&tail->o_free[group]));
-            if (again != 0) mend<T>(p, it, row0, min(row0 + 31, rows - 1), again);
+            // Are they so by values that they do not see, they are made again, but not here: the other warps' waits are limited, and a
+            // row takes as long as its places ask for.  (This looks at some 1200 places at most.)
+            if (again != 0 && !met_not_finite<T>(p, it, place_of(p, it, row0), place_of(p, it, min(row0 + 31, rows - 1)))) again = 0;
+            if (lane == 0) {
+                tail->again[item & 1][group][quarter] = again;
+                if (again != 0) tail->remake = 1;
+            }
             count += it.end - it.begin;
             release(item);
         }
@@ -1229,11 +1292,19 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
+    if (tail->remake == 0 || *abort_flag != 0) return;
+    // ---------------- rows that came beside values that are not finite, again, when no warp waits for another ----------------
+    // The CTA's last two items (no further one is taken once one has such rows).
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t again = tail->again[i >> 3][i >> 2 & 1][i & 3];
+        if (again != 0) remake_rows<T>(p, tail->item[i >> 3], (i >> 2 & 1) * 128 + (i & 3) * 32, again, reinterpret_cast<float *>(smem));
+    }
 }
 
 // Joins the splits of a row, in their order: a warp a row.
 template <typename T, int BN, int ROWS>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
+    __shared__ __align__(16) float s_query[8][kPlainDim];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -1303,8 +1374,11 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
         cover<BN, ROWS>(p, it);
         const int place = place_of(p, it, static_cast<int>(at - it.first));
         if (met_not_finite<T>(p, it, place, place)) {
+            RowPart r;
+            stage_query<T>(p, token, head, s_query[threadIdx.x >> 5]);
             __syncwarp();
-            plain_row<T>(p, it.b, token, head, place);
+            rows_part<T, 1>(p, it.b, it.kvh, &place, s_query[threadIdx.x >> 5], 0, 1, &r);
+            write_row<T>(p, token, head, r);
         }
     }
 }
