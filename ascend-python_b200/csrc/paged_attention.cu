@@ -27,7 +27,8 @@ static int describe(Problem *p, const char *op, const void *query, int dtype, in
                 name + ": the query's heads must be a multiple of the cache's");
     QMM_REQUIRE(tokens < 0x7fffffff && batch < 0x7fffffff && heads <= 65535 && max_pages <= 0x7fffffff && cache->pages <= 0x7fffffff,
                 name + ": sizes out of range");
-    QMM_REQUIRE(scale == scale && scale - scale == 0.0, name + ": scale_value must be finite");
+    const float factor = static_cast<float>(scale) * 1.4426950408889634f;  // as the kernels take it
+    QMM_REQUIRE(factor - factor == 0.0f, name + ": scale_value must be finite, and so must it times log2(e) in fp32");
     QMM_REQUIRE(vectors(query, stride_token, stride_head, 0) &&
                     vectors(cache->key, cache->key_stride_page, cache->key_stride_place, cache->key_stride_head) &&
                     vectors(cache->value, cache->value_stride_page, cache->value_stride_place, cache->value_stride_head),
