@@ -8,6 +8,8 @@ static bool vectors(const void *base, int64_t a, int64_t b, int64_t c) {
     return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ((a | b | c) & 7) == 0;
 }
 
+static bool words(const void *base) { return (reinterpret_cast<uintptr_t>(base) & 3) == 0; }
+
 // The arguments of both entries as a Problem.
 static int describe(Problem *p, const char *op, const void *query, int dtype, int64_t tokens, int64_t heads, int64_t stride_token,
                     int64_t stride_head, const qmm_kv_cache *cache, const int32_t *block_table, int64_t table_stride,
@@ -33,6 +35,8 @@ static int describe(Problem *p, const char *op, const void *query, int dtype, in
                     vectors(cache->key, cache->key_stride_page, cache->key_stride_place, cache->key_stride_head) &&
                     vectors(cache->value, cache->value_stride_page, cache->value_stride_place, cache->value_stride_head),
                 name + ": query and caches must begin at 16-byte boundaries, with strides of multiples of 8 elements");
+    QMM_REQUIRE(vectors(out, 0, 0, 0) && words(lse) && words(block_table) && words(seq_lens),
+                name + ": out must begin at a 16-byte boundary, lse, block_table and seq_lens at 4-byte boundaries");
     p->q = query;
     p->q_st = stride_token;
     p->q_sh = stride_head;
@@ -118,6 +122,7 @@ int qmm_paged_prompt_attention(const void *query, int dtype, int64_t tokens, int
                                         query_stride_head, cache, block_table, table_stride, max_pages, seq_lens, batch,
                                         scale_value, window, sinks, out, lse);
     if (rc != QMM_OK) return rc;
+    QMM_REQUIRE(qmm::paged::words(query_start), "qmm_paged_prompt_attention: query_start must begin at 4-byte boundaries");
     p.start = query_start;
     if (tokens == 0 || heads == 0) return QMM_OK;
     return qmm::paged::launch_prompt(p, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));

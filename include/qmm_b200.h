@@ -414,8 +414,8 @@ QMM_API int qmm_rotary_axes_cache(const void *query, int64_t query_stride_token,
  * A row that sees nothing (seq_lens[b] <= 0: padding) has out 0 and lse -inf.  Entries of the table for places that are not
  * seen are not followed, and the places not read.  Scores, softmax and sums are fp32.
  * query: bf16 or f16 like the cache, [batch, heads, dim]; out: dense; lse: [batch, heads]; block_table: int32 [batch, max_pages],
- * rows table_stride apart; scale_value: finite, as is scale_value * log2(e) in fp32; dim: a multiple of 8 up to 256; query and
- * caches begin at 16-byte boundaries, their strides are multiples of 8 elements; a sequence has up to 2^31 - 256 places.  The
+ * rows table_stride apart; scale_value: finite, as is scale_value * log2(e) in fp32; dim: a multiple of 8 up to 256; query,
+ * caches and out begin at 16-byte boundaries, the strides of the former are multiples of 8 elements; a sequence has up to 2^31 - 256 places.  The
  * workspace (16-byte aligned, of the size that the first function gives for max_places = max_pages * page_size) holds nothing
  * between calls; calls that may run at the same time need one each.
  */

@@ -1,7 +1,7 @@
 """Calls of the attention over a paged cache that its C entries refuse, without a GPU."""
 import pytest
 
-from test_paged_boundary import _attention
+from test_paged_boundary import _attention, _cache
 
 
 @pytest.mark.parametrize("scale", [1e39, -1e39, 3e38, -3e38, 2.4e38, 1.7e308])
@@ -15,3 +15,18 @@ def test_scales_beyond_fp32(capi, scale):
 def test_scales_within_fp32(capi, scale):
     for rc, message in _attention(capi, scale=scale, heads=0):
         assert rc == 0, message
+
+
+def test_operands_off_their_alignment(capi):
+    """Outputs are written in 16-byte vectors (log-sums: 4), tables and lengths are read as 32-bit words."""
+    lib, n = capi.lib(), 1 << 20
+    place = dict(out=n, lse=n, table=n, lens=n, start=n)
+    for name, off in (("out", 2), ("out", 8), ("lse", 2), ("table", 2), ("lens", 1), ("start", 2)):
+        a = {**place, name: n + off}
+        calls = {"qmm_paged_prompt_attention": lambda: lib.qmm_paged_prompt_attention(
+            n, 0, 2, 4, 256, 64, _cache(capi), a["table"], 4, 4, a["lens"], a["start"], 2, 1.0, 0, 0, a["out"], a["lse"], None, 0, None)}
+        if name != "start":
+            calls["qmm_paged_attention"] = lambda: lib.qmm_paged_attention(
+                n, 0, 2, 4, 256, 64, _cache(capi), a["table"], 4, 4, a["lens"], 1.0, 0, 0, a["out"], a["lse"], None, 0, None)
+        for op, call in calls.items():
+            assert call() == 1 and "boundaries" in lib.qmm_last_error().decode(), (op, name, lib.qmm_last_error())
