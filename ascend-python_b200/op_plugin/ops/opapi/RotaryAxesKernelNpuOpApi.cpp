@@ -96,7 +96,7 @@ at::Tensor npu_rotary_axes_cache(const at::Tensor &query, const at::Tensor &key,
     TORCH_CHECK(value.scalar_type() == query.scalar_type() && value.sizes() == key.sizes(), op,
                 ": value should have dtype and shape of key (", key.scalar_type(), " ", key.sizes(), "), but it is ",
                 value.scalar_type(), " ", value.sizes());
-    const qmm_kv_cache cache = op_plugin_utils::describe_cache(op, key_cache, value_cache, query);
+    qmm_kv_cache cache = op_plugin_utils::describe_cache(op, key_cache, value_cache, query);
     TORCH_CHECK(cache.kv_heads == key.size(1) && cache.dim == key.size(2), op, ": the cache should hold ", key.size(1), " heads of ",
                 key.size(2), ", but it is ", key_cache.sizes());
     for (const auto &c : {key_cache, value_cache}) {
@@ -109,6 +109,9 @@ at::Tensor npu_rotary_axes_cache(const at::Tensor &query, const at::Tensor &key,
     TORCH_CHECK(slots.dim() == 1 && slots.size(0) == r.tokens, op, ": slots should hold ", r.tokens, " tokens, but they are ",
                 slots.sizes());
     const at::Tensor v = op_plugin_utils::dense_rows(value);
+    // a cache that shares its storage with a lazy clone gets its own, now that it is written
+    cache.key = key_cache.mutable_data_ptr();
+    cache.value = value_cache.mutable_data_ptr();
     at::Tensor q = op_plugin_utils::empty_output(query.sizes(), query, query.scalar_type());
     EXEC_QMM_CMD(qmm_rotary_axes_cache, r.q.const_data_ptr(), r.q.stride(0), r.q.stride(1), r.k.const_data_ptr(), r.k.stride(0),
                  r.k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1), op_plugin_utils::qmm_dtype(query.scalar_type()),
