@@ -97,6 +97,7 @@ struct Item {
     int two;                               // the second row tile has rows
     int cut;                               // its rows have parts in the workspace
     int none;                              // there is no further item
+    int far;                               // where its rows' sums are put by (far_sums); -1: nowhere
 };
 
 constexpr int kValid = 8;  // tiles of keys whose masks are kept: more than may be under way
@@ -112,6 +113,7 @@ struct Tail {
     uint32_t bad[2][4], going[2][4];  // [group][quarter]: rows that are not finite; the warp has an item
     uint32_t again[2][2][4];  // [item % 2][row tile][quarter]: rows to be made again when the CTA's last item is done
     uint32_t remake;          // there are such rows
+    int far;                  // this CTA's place for sums that are put by; -1: none
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -119,11 +121,22 @@ constexpr size_t smem_bytes() {
     return 1024 + Shape<DP>::kQuery + Shape<DP>::kStages * Shape<DP>::kStage + sizeof(Tail);
 }
 
-// Workspace (splits > 1): part[split][token * heads + head][dim], stat[split][..] (base, sum), pieces.
+// O in tensor memory loses what its products are cut to as they are added, all towards 0: of n values of one sign some n * 2^-28 (so
+// measured: 2^20 places, f16, 0.0029 of the sum).  Items of more than kRun steps put O by in memory every kRun steps and begin
+// again from 0 (far_sums), so that this stays within 2^-11; tables of up to kNear places hold few such steps more than that, and go
+// without.
+constexpr int kRun = 1024;
+constexpr int64_t kNear = 1 << 17;
+
+// Workspace (splits > 1): part[split][token * heads + head][dim], stat[split][..] (base, sum), pieces; with tables of more than
+// kNear places far[place][row tile][128][far_stride], a place for every SM, and which of them are taken.
 struct Scratch {
     float *part;
     float2 *stat;
     int *pieces;  // of them that a call uses; 1: none
+    float *far;
+    int *far_taken;
+    int far_places, far_stride;
     int splits, sms;
     float tile;  // microseconds
     uint32_t *status;
@@ -133,8 +146,10 @@ struct Plan {
     int64_t pairs;  // at most
     int splits;
     double tile;
-    size_t part_bytes, stat_bytes, bytes;
+    bool far;
+    size_t part_bytes, stat_bytes, far_bytes, taken_bytes, bytes;
 };
+int far_stride(int64_t dim) { return static_cast<int>((dim + 15) / 16 * 16 + 4); }  // a row of O, its base, and 16-byte vectors
 
 // The items of a call are known on the device alone; what the host knows bounds them.  Where they are few, each may be cut into
 // pieces (choose_pieces), of which the host says how many at most: as many as give every SM one, or by an estimate in
@@ -152,11 +167,14 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
     plan.splits = 1;
     plan.tile = dim > 128 ? 1.5 : tokens * group > 128 * sequences ? 2.4 : 1.2;
     const int64_t ctas = plan.pairs * kv_heads, sms = sm_count();
+    plan.far = seen > kNear && ctas > 0;
+    plan.far_bytes = plan.far ? static_cast<size_t>(sms) * rows * far_stride(dim) * sizeof(float) : 0;
+    plan.taken_bytes = plan.far ? (static_cast<size_t>(sms) * sizeof(int) + 15) / 16 * 16 : 0;
     if (ctas > 0 && ctas < 2 * sms) {
         const int64_t tiles = (seen + keys - 1) / keys;
         const double tile = plan.tile;
         double best = 0.0;
-        const int64_t most = std::min<int64_t>(tiles, (256ll << 20) / (tokens * heads * std::max<int64_t>(dim, 1) * 4));  // 256 MiB of parts
+        const int64_t most = std::min<int64_t>(tiles, ((256ll << 20) - static_cast<int64_t>(plan.far_bytes)) / (tokens * heads * std::max<int64_t>(dim, 1) * 4));  // 256 MiB
         for (int s = 1; s <= 64 && (s == 1 || s <= most); ++s) {
             const double item = tile * tiles / s + 3.0;
             const double load = ctas * (0.6 * tile * tiles + 3.0 * (s == 1 ? 1.0 : 0.6 * s + 0.5)) / sms + 0.5 * item;
@@ -171,7 +189,7 @@ Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, i
     const size_t all = plan.splits > 1 ? static_cast<size_t>(plan.splits) * tokens * heads : 0;
     plan.part_bytes = all * dim * sizeof(float);
     plan.stat_bytes = (all * sizeof(float2) + 15) / 16 * 16;
-    plan.bytes = all > 0 ? plan.part_bytes + plan.stat_bytes + 16 : 0;
+    plan.bytes = (all > 0 ? plan.part_bytes + plan.stat_bytes + 16 : 0) + plan.far_bytes + plan.taken_bytes;
     return plan;
 }
 
@@ -406,6 +424,47 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// A place for sums that are put by, for as long as the CTA lives; by one thread.  There are as many as SMs, which have a CTA each.
+__device__ __noinline__ int take_far(const Scratch &scratch) {
+    const int first = static_cast<int>(blockIdx.x % static_cast<unsigned>(scratch.far_places));
+    for (int i = 0; i < scratch.far_places; ++i) {
+        const int at = (first + i) % scratch.far_places;
+        if (atomicCAS(scratch.far_taken + at, 0, 1) == 0) {
+            __threadfence();
+            return at;
+        }
+    }
+    return -1;
+}
+// O of a warp's 32 rows (a row a lane), relative to `base`, is added to what was put by, and begins again from 0 (back: the other way
+// round).  begins: nothing has been put by.
+__device__ __noinline__ void far_sums(const Scratch &scratch, int row, uint32_t o_addr, int ksteps, float base, float scale, bool begins, bool back) {
+    float *far = scratch.far + static_cast<int64_t>(row) * scratch.far_stride;
+    float4 *sums = reinterpret_cast<float4 *>(far);
+    float &far_base = far[scratch.far_stride - 4];
+    const float keep = begins || base == -INFINITY ? 1.0f : exp2_fast((far_base - base) * scale);
+    for (int c = 0; c < ksteps; ++c) {
+        uint32_t o[16];
+        tmem_ld_32x16(o_addr + c * 16, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float4 x = begins ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : sums[c * 4 + j];
+            x.x = fmaf(x.x, keep, __uint_as_float(o[4 * j]));
+            x.y = fmaf(x.y, keep, __uint_as_float(o[4 * j + 1]));
+            x.z = fmaf(x.z, keep, __uint_as_float(o[4 * j + 2]));
+            x.w = fmaf(x.w, keep, __uint_as_float(o[4 * j + 3]));
+            if (!back) sums[c * 4 + j] = x;
+            o[4 * j] = back ? __float_as_uint(x.x) : 0u;
+            o[4 * j + 1] = back ? __float_as_uint(x.y) : 0u;
+            o[4 * j + 2] = back ? __float_as_uint(x.z) : 0u;
+            o[4 * j + 3] = back ? __float_as_uint(x.w) : 0u;
+        }
+        tmem_st_32x16(o_addr + c * 16, o);
+    }
+    far_base = base;
+    tmem_st_wait();
 }
 // Two warps' turns: a barrier for each, at which the one waits and the other does not.
 __device__ __forceinline__ void turn_take(int bar) { asm volatile("bar.sync %0, 64;" ::"r"(bar) : "memory"); }
@@ -655,6 +714,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         mbar_init(smem_u32(&tail->next_full), 1);
         tail->abort_flag = 0;
         tail->remake = 0;
+        tail->far = -1;
         for (int i = 0; i < 16; ++i) tail->again[i >> 3][i >> 2 & 1][i & 3] = 0;
         mbar_fence_init();
         if (box_rows > 0) {
@@ -747,6 +807,12 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 if (S::kSub == 2 && it.end > it.begin) {
                     const int last = block_start<BN>(it, it.end - 1);
                     if (last + 64 >= (it.end - 1 < it.sink_blocks && it.lo >= last + BN ? it.sink_end : it.hi)) --it.steps;
+                }
+                it.far = -1;
+                if (scratch.far_places > 0 && it.steps > kRun) {
+                    if (lane == 0 && tail->far < 0) tail->far = take_far(scratch);
+                    __syncwarp();
+                    it.far = tail->far;
                 }
             }
             if (lane == 0) {
@@ -1083,6 +1149,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                 int sink_steps = (it.sink_blocks - it.begin) * (shared ? 1 : S::kSub);  // until the gap
                 const uint32_t valid_stride = shared || S::kSub == 1 ? 16 : 8;
                 uint32_t valid_at = (count * 16 + (shared ? group * 8 : 0)) % (kValid * 16);
+                const int far_from = it.far >= 0 ? kRun : 0x7fffffff, far_row = (it.far * S::kTiles + group) * 128 + my_lane;
                 if (turns && group == 1) turn_over(5 + quarter);
                 for (int n = 0; n < steps; ++n, ++done) {
                     const uint32_t odd = done & 1;
@@ -1125,7 +1192,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     }
                     const float most = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
                     const bool move = most > base && (most - base) * scale > kGrowth<T>;  // from -inf always
-                    if (__any_sync(0xffffffffu, move)) {
+                    const bool put_by = n >= far_from && (n & (kRun - 1)) == 0;
+                    if (__any_sync(0xffffffffu, move || put_by)) {
                         float now = move ? most : base;
                         if (kSpare<T> > 0.0f && move && base == -INFINITY && !whole) now += fminf(kSpare<T> / scale, 1e30f);
                         const float keep = exp2_fast(now == -INFINITY ? 0.0f : (base - now) * scale);
@@ -1133,7 +1201,8 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                         if (n > 0) {
                             ok = ok && mbar_wait(smem_u32(&tail->o_done[group][odd ^ 1]), ((done - 1) >> 1) & 1, abort_flag, 0x99);
                             tc_fence_after();
-                            for (int c = 0; c < ksteps; ++c) {
+                            if (put_by) far_sums(scratch, far_row, tmem_base + lanes + S::kO + group * 128, ksteps, base, scale, n == kRun, false);
+                            for (int c = 0; c < ksteps && !put_by; ++c) {
                                 uint32_t o[16];
                                 const uint32_t addr = tmem_base + lanes + S::kO + group * 128 + c * 16;
                                 tmem_ld_32x16(addr, o);
@@ -1183,6 +1252,10 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     if (lane == 0) mbar_arrive(smem_u32(&tail->p_full[group][odd]));
                 }
                 ok = ok && mbar_wait(smem_u32(&tail->o_done[group][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag, 0x9a);
+                if (steps > far_from) {
+                    tc_fence_after();
+                    far_sums(scratch, far_row, tmem_base + lanes + S::kO + group * 128, ksteps, base, scale, false, true);
+                }
             }
             float sum = sum2.x + sum2.y, keep[2] = {1.0f, 0.0f};
             const int first = shared ? 0 : group;
@@ -1288,6 +1361,10 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && tail->abort_flag != 0 && scratch.status != nullptr) atomicMax(scratch.status, tail->abort_flag);
+    if (threadIdx.x == 0 && tail->far >= 0) {
+        __threadfence();
+        atomicExch(scratch.far_taken + tail->far, 0);
+    }
     if (warp == kSoftmax) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
@@ -1423,7 +1500,8 @@ int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStrea
     // the query's rows of a tile in one box, where the group's heads divide a tile
     CUtensorMap tmap_q = {};
     const bool box_query = 128 % p.group == 0 && query_map(&tmap_q, p);
-    QMM_CUDA_OK(launch_pdl(prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch,
+    if (plan.far) QMM_CUDA_OK(cudaMemsetAsync(scratch.far_taken, 0, plan.taken_bytes, stream));
+    QMM_CUDA_OK(launch_pdl_if(!plan.far, prompt_kernel<T, DP>, dim3(static_cast<unsigned>(ctas > 0 ? ctas : 1)), dim3(kThreads), smem_bytes<DP>(), stream, p, scratch,
                            tmap_k, tmap_v, tmap_q, box_rows, box_query));
     if (plan.splits > 1) {
         const int64_t joins = (p.tokens * p.heads + 7) / 8;
@@ -1452,14 +1530,20 @@ int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace
         // an item's rows see the window of the first and a place for each further token; the workspace is for no window
         const Plan narrow = make_plan(p.tokens, p.batch, p.heads, p.kv_heads, p.dim,
                                       std::min(places, static_cast<int64_t>(p.window) + p.sinks + 256 / std::min(p.group, 256)));
-        if (narrow.splits < plan.splits) plan = narrow;
+        if (narrow.splits < plan.splits || (narrow.splits == plan.splits && !narrow.far)) plan = narrow;
     }
     if (plan.bytes > 0 && (workspace_bytes < plan.bytes || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
         return fail(QMM_ERR_WORKSPACE, "qmm_paged_prompt_attention: needs a workspace of " + std::to_string(plan.bytes) + " bytes, 16-byte aligned");
     Scratch scratch;
-    scratch.part = static_cast<float *>(workspace);
-    scratch.stat = reinterpret_cast<float2 *>(static_cast<uint8_t *>(workspace) + plan.part_bytes);
-    scratch.pieces = reinterpret_cast<int *>(static_cast<uint8_t *>(workspace) + plan.part_bytes + plan.stat_bytes);
+    uint8_t *base = static_cast<uint8_t *>(workspace);
+    scratch.far = reinterpret_cast<float *>(base);
+    scratch.far_taken = reinterpret_cast<int *>(base + plan.far_bytes);
+    scratch.far_places = plan.far ? sm_count() : 0;
+    scratch.far_stride = far_stride(p.dim);
+    base += plan.far_bytes + plan.taken_bytes;
+    scratch.part = reinterpret_cast<float *>(base);
+    scratch.stat = reinterpret_cast<float2 *>(base + plan.part_bytes);
+    scratch.pieces = reinterpret_cast<int *>(base + plan.part_bytes + plan.stat_bytes);
     scratch.splits = plan.splits;
     scratch.sms = sm_count();
     scratch.tile = static_cast<float>(plan.tile);
