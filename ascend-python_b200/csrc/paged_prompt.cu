@@ -114,6 +114,7 @@ struct Tail {
     uint32_t again[2][2][4];  // [item % 2][row tile][quarter]: rows to be made again when the CTA's last item is done
     uint32_t remake;          // there are such rows
     int far;                  // this CTA's place for sums that are put by; -1: none
+    uint32_t loaded;          // tiles of keys that have been asked for
     uint32_t tmem_base, abort_flag;
 };
 template <int DP>
@@ -642,6 +643,25 @@ __device__ __forceinline__ uint32_t mbar_done(uint32_t bar, uint32_t parity) {
         : "memory");
     return done;
 }
+// mbar_wait for what takes as long as an item has keys: its limit begins anew when the tiles that have been asked for are more.
+__device__ __noinline__ bool wait_while_moving(uint32_t bar, uint32_t parity, volatile uint32_t *moving, volatile uint32_t *abort_flag, uint32_t where) {
+    uint64_t since = globaltimer_ns();
+    uint32_t last = *moving, spins = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++spins & 0xffu) != 0) continue;
+        if (*abort_flag != 0) return false;
+        const uint32_t now = *moving;
+        const uint64_t time = globaltimer_ns();
+        if (now != last) {
+            last = now;
+            since = time;
+        } else if (time - since > kWaitLimitNs) {
+            *abort_flag = DEV_STATUS_WAIT_TIMEOUT | where;
+            return false;
+        }
+    }
+    return true;
+}
 __device__ __forceinline__ void mbar_arrive_n(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -715,6 +735,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         tail->abort_flag = 0;
         tail->remake = 0;
         tail->far = -1;
+        tail->loaded = 0;
         for (int i = 0; i < 16; ++i) tail->again[i >> 3][i >> 2 & 1][i & 3] = 0;
         mbar_fence_init();
         if (box_rows > 0) {
@@ -753,7 +774,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
         int n = 0;
         while (ok && have) {
             // a block is asked for when the present item's last keys are, not earlier: what is taken cannot go to another CTA
-            if (n > 0) ok = mbar_wait(smem_u32(&tail->item_loaded), (n - 1) & 1, abort_flag, 0x9c);
+            if (n > 0) ok = wait_while_moving(smem_u32(&tail->item_loaded), (n - 1) & 1, &tail->loaded, abort_flag, 0x9c);
             ok = ok && mbar_wait(smem_u32(&tail->item_empty[n & 1]), (n >> 1 & 1) ^ 1, abort_flag, 0x9e);
             if (!ok) break;
             Item it;
@@ -982,6 +1003,7 @@ prompt_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     cp_async_arrive(bar);
                     if (lane == 0) mbar_arrive(bar);
                 }
+                if (part == 0 && loader == 0 && lane == 0) *reinterpret_cast<volatile uint32_t *>(&tail->loaded) = count + 1;
                 stage += 2;
                 if (stage >= S::kStages) {
                     stage -= S::kStages;
