@@ -16,6 +16,7 @@
 // their order.  (The warps of a CTA taking the tiles of one sequence in turn, with a join at its end, cost about 3 us a sequence:
 // 64 sequences of 500 to 8000 places, 64/8 heads of 128, 131 us.)  Where every sequence is short and head tiles are few, CTAs
 // have whole ones in turn, cut for their warps alone.  Nothing depends on timing, and nothing has to be zero before a call.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_common.cuh"
@@ -27,6 +28,11 @@ namespace {
 
 constexpr int kRows = 16;     // query heads of a tile
 constexpr int kShort = 512;   // places that a CTA's warps share rather than several CTAs
+// The tensor cores cut sums as they add, towards 0: n values of one sign lose some n * 2^-28 (f16, 2^18 places a warp: two half steps).
+// So the kernel for calls that may give a warp more than kNear places puts a warp's sums by after every kRun of them.  (For all
+// calls, that code cost 32 sequences through a window of 4096 places 1 of 31 us.)
+constexpr int kRun = 65536;
+constexpr int64_t kNear = 2 * kRun;
 constexpr int kSlots = 3;     // of a warp's ring: keys, values, the next keys
 constexpr int kTileBytes = 8192;
 
@@ -167,7 +173,8 @@ struct Part {
     int valid, b, item, begins, ends, last;  // last: the CTA that has the head tile's last place
 };
 
-template <typename T, int DP>
+// FAR: a warp may have more than kNear places.
+template <typename T, int DP, bool FAR>
 __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 2)
 decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch) {
     using S = Shape<DP>;
@@ -418,7 +425,34 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
             float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+            // A long piece adds what it has to fp32 sums in its part of the workspace and begins again from 0 (back: the other way round).
+            auto put_by = [&](bool first, bool back) {
+                const int rows = min(kRows, p.group - piece.item % tiles * kRows);
+                const int64_t part0 = ((static_cast<int64_t>(worker) * S::kWarps + warp) * 2 + (piece.from == 0)) * scratch.rows;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = r0 + r * 8;
+                    float *sums = scratch.part + (part0 + row) * p.dim + c0;
+                    float keep = 1.0f;
+                    if (row < rows && !first && top[r] != -INFINITY) keep = exp2_fast((scratch.stat[part0 + row].x - top[r]) * scale);
+                    __syncwarp();
+                    if (row < rows && (lane & 3) == 0) scratch.stat[part0 + row].x = top[r];
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n) {
+                        float2 x = make_float2(0.0f, 0.0f);
+                        if (row < rows && n * 8 < p.dim) {
+                            if (!first) x = *reinterpret_cast<const float2 *>(sums + n * 8);
+                            x.x = fmaf(x.x, keep, o[n][2 * r]);
+                            x.y = fmaf(x.y, keep, o[n][2 * r + 1]);
+                            if (!back) *reinterpret_cast<float2 *>(sums + n * 8) = x;
+                        }
+                        o[n][2 * r] = back ? x.x : 0.0f;
+                        o[n][2 * r + 1] = back ? x.y : 0.0f;
+                    }
+                }
+            };
             for (int g = piece.from; g < piece.to; ++g) {
+                if (FAR && g != piece.from && (g - piece.from) % (kRun / KEYS) == 0) put_by(g - piece.from == kRun / KEYS, false);
                 // scores of 16 rows x KEYS keys: accumulators of 8 keys
                 float s[KEYS / 8][4];
 #pragma unroll
@@ -530,6 +564,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     }
                 }
             }
+
+            if (FAR && piece.to - piece.from > kRun / KEYS) put_by(false, true);
 
             // ---- the piece's end: rows to the outputs, or sums to the workspace ----
             const int kvh = piece.item / tiles, tile = piece.item - kvh * tiles;
@@ -736,10 +772,20 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch s
     }
 }
 
+template <typename T, int DP, bool FAR>
+int launch_decode_kernel(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStream_t stream) {
+    QMM_CUDA_OK(cudaFuncSetAttribute(decode_kernel<T, DP, FAR>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<DP>::kSmem)));
+    QMM_CUDA_OK(launch_pdl(decode_kernel<T, DP, FAR>, dim3(plan.workers), dim3(Shape<DP>::kWarps * 32), Shape<DP>::kSmem, stream, p, scratch));
+    return QMM_OK;
+}
+
 template <typename T, int DP>
-int launch(const Problem &p, const Plan &plan, Scratch scratch, cudaStream_t stream) {
-    QMM_CUDA_OK(cudaFuncSetAttribute(decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Shape<DP>::kSmem)));
-    QMM_CUDA_OK(launch_pdl(decode_kernel<T, DP>, dim3(plan.workers), dim3(Shape<DP>::kWarps * 32), Shape<DP>::kSmem, stream, p, scratch));
+int launch(const Problem &p, const Plan &plan, const Scratch &scratch, cudaStream_t stream) {
+    // what a warp may have: of one head tile what a token sees, of all of them an equal share
+    const int64_t seen = p.window > 0 ? std::min<int64_t>(p.capacity, static_cast<int64_t>(p.window) + p.sinks) : p.capacity;
+    const bool far = seen > kNear && seen > kNear * plan.workers * Shape<DP>::kWarps / plan.items;
+    const int rc = far ? launch_decode_kernel<T, DP, true>(p, plan, scratch, stream) : launch_decode_kernel<T, DP, false>(p, plan, scratch, stream);
+    if (rc != QMM_OK) return rc;
     // all sequences are short whatever their lengths are, and no head tile is cut
     if (p.capacity <= kShort && plan.items <= 2 * plan.workers) return QMM_OK;
     const int64_t indices = scratch.by_item ? plan.items : plan.workers;

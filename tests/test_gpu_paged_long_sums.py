@@ -1,4 +1,4 @@
-"""Prompts over a million places and more, which no second kernel joins: sums that stay exact over long items."""
+"""Attention over a million places and more where one CTA, or one warp, has all of them: sums that stay exact over long stretches."""
 import math
 
 import pytest
@@ -28,10 +28,10 @@ def make_long(dev, places, heads, dim, dtype, batch, seed=0, distinct=16, rise=0
     return q, k, v, table, lens, torch.arange(batch + 1, dtype=torch.int32, device=dev)
 
 
-def definition(q, k, v, table):
-    """(out, lse) of the first row in 64 bits: every page's keys as often as the table names it."""
+def definition(q, k, v, table, row=0):
+    """(out, lse) of a row in 64 bits, of a sequence that sees all that the table names: every page's keys as often as it does."""
     times = torch.bincount(table[0].long(), minlength=k.shape[0]).double().repeat_interleave(PAGE)
-    x = q[0].double() @ k.view(-1, k.shape[-1]).double().t() * q.shape[2] ** -0.5
+    x = q[row].double() @ k.view(-1, k.shape[-1]).double().t() * q.shape[2] ** -0.5
     lse = torch.logsumexp(x + times.log(), 1)
     p = torch.exp(x - lse[:, None]) * times
     return p @ v.view(-1, v.shape[-1]).double(), lse
@@ -52,6 +52,33 @@ def test_long_sums(npu, dev, heads, dim, places, batch, dtype, rise):
     assert (lse[0].double() - want_lse).abs().max().item() <= 2.0 ** -12
     if batch > 1:
         assert torch.equal(out[1:], v[table[1, 0].long(), 0].expand(batch - 1, heads, dim))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,dim", [(4, 64), (20, 128), (1, 256), (3, 72)])
+@pytest.mark.parametrize("rise", [0.0, 9.0])
+def test_long_sums_of_single_tokens(npu, dev, heads, dim, dtype, rise):
+    """As above; 301 sequences of 2^21 places, some shorter, give a warp half a million places of one or of neighbours."""
+    q, k, v, table, lens, _ = make_long(dev, 1 << 21, heads, dim, dtype, 301, seed=dim, rise=rise)
+    lens[:] = 1 << 21
+    lens[5:9] = torch.tensor([1, 3, 0, 1], device=dev)
+    out, lse = call(npu, q, k, v, table, lens, None)
+    u = torch.finfo(dtype).eps / 2
+    for row in (0, 1, 4, 9, 77, 150, 300):
+        want, want_lse = definition(q, k, v, table, row)
+        assert ((out[row].double() / want - 1).abs().max().item()) <= 2 * u + 2.0 ** -11 + 2.0 ** -12
+        assert (lse[row].double() - want_lse).abs().max().item() <= 2.0 ** -12
+    assert torch.equal(out[5], v[table[5, 0].long(), 0].expand(heads, dim)) and not out[7].any() and bool((lse[7] == -math.inf).all())
+    assert bool(out.isfinite().all())
+
+
+def test_values_of_one_over_long_stretches_of_single_tokens(npu, dev):
+    for heads, dim in ((4, 64), (20, 128), (1, 256)):
+        q, k, v, table, lens, _ = make_long(dev, 1 << 21, heads, dim, torch.float16, 301, seed=9)
+        v.fill_(1.0)
+        lens[:] = 1 << 21
+        out, _ = call(npu, q, k, v, table, lens, None)
+        assert (out.double() - 1).abs().max().item() <= 2.0 ** -11 + 2.0 ** -11
 
 
 def test_values_of_one_over_long_items(npu, dev):
