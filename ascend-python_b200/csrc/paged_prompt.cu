@@ -17,8 +17,8 @@
 //
 // The softmax has its scores in registers and gives S back at once: the next Q K^T runs beside it, and so does P V of the step
 // before, for P has two places of its own.  Two row tiles share the keys (dimensions up to 128), and take turns at the
-// exponentials.  What bounds a step (8192 tokens, 32/8 heads of 128: 1830 clocks for 64 keys, 470 to 555 us in all as the clock
-// goes; the products alone take 1280): the chain of a softmax warp, its wait (200), load and maximum (450), exponentials (700
+// exponentials.  What bounds a step (8192 tokens, 32/8 heads of 128: 1830 clocks for 64 keys, in all 488 us in a graph and 540 to
+// 550 by calls one after the other, when the clock goes down; the products alone take 1280): the chain of a softmax warp, its wait (200), load and maximum (450), exponentials (700
 // at least, of which the special-function unit has 512 to itself) and hand-over.  Slower or the same were: part of the
 // exponentials as a polynomial on the FMA pipe, two threads a row, the row tiles half a step apart without turns, S twice with
 // P in its place.
@@ -32,9 +32,10 @@
 //
 // Where a page holds a multiple of 8 places, a tile comes by TMA, in boxes of 8 to 128 places and 64 columns (by cp.async two
 // warps took 1.7 us for the 64 KiB of a block, more than its products take); the tile with the sequence's end and tiles with pages
-// that are none come by cp.async, as all do with other page sizes and strides, and rows that no row of the CTA sees are
-// zero-filled.  A key that some rows see and others do not is a product with 0 for those, which is only wrong where its value is
-// not finite; rows that come out not finite beside such a value are made again, by plain sums, at the CTA's end (remake_rows).
+// that are none come by cp.async, as all do with other page sizes and strides.  What no row of the CTA sees: a box is zeros; in a
+// box that is seen in part it is what the page holds; by cp.async a value is zeros, and a key what shared memory held, for its
+// scores are masked.  A value that some rows see and others do not is a product with 0 for those, which is only wrong where it
+// is not finite; rows that come out not finite beside such a value are made again, by plain sums, at the CTA's end (remake_rows).
 #include <algorithm>
 #include <type_traits>
 
@@ -154,9 +155,11 @@ int far_stride(int64_t dim) { return static_cast<int>((dim + 15) / 16 * 16 + 4);
 
 // The items of a call are known on the device alone; what the host knows bounds them.  Where they are few, each may be cut into
 // pieces (choose_pieces), of which the host says how many at most: as many as give every SM one, or by an estimate in
-// microseconds for lengths that are 0.6 of the longest in the mean (measured: 1.2 for a tile of 128 keys and one row tile, 2.4
-// for two, 1.5 for 64 keys of more than 128 dimensions, 3 for an item; the parts of rows, written and read, at 5 TB/s, and 4
-// for the second kernel): the CTAs' mean load and half an item, or one item alone.  (Before, 4 CTAs an SM were aimed at: 1184
+// microseconds: the CTAs' mean load and half an item, or one item alone.  It takes 1.2 for a tile of 128 keys and one row tile, 2.4
+// for two, 1.5 for 64 keys of more than 128 dimensions (measured, an item on every SM over 16384 and 65536 places, the difference:
+// 1.08 for heads of 64 and 128, 1.75 to 1.82, 1.09; in short items, with masks and cold code, up to the figures taken), 3 for an
+// item, 5 TB/s for the parts of rows, written and read, 4 for the second kernel; and, as lengths are not known, 0.6 of the longest in
+// the mean, which is a guess: choose_pieces, which knows them, takes no more pieces than are good.  (Before, 4 CTAs an SM were aimed at: 1184
 // tokens through a window of 1024, 32/8 heads of 128, took 111 us, twice as many tokens, whose items were not cut, 77.)
 // seen: the places that an item sees at most.
 Plan make_plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t seen) {
