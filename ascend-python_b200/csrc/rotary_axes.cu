@@ -349,6 +349,8 @@ int qmm_rotary_axes_cache(const void *query, int64_t query_stride_token, int64_t
     QMM_REQUIRE(cache != nullptr, "qmm_rotary_axes_cache: no cache given");
     QMM_REQUIRE(cache->pages >= 0 && cache->page_size >= 1 && cache->pages <= 0x7fffffff && cache->page_size <= 0x7fffffff,
                 "qmm_rotary_axes_cache: pages must be non-negative, their size positive");
+    QMM_REQUIRE(cache->pages == 0 || cache->key != cache->value,
+                "qmm_rotary_axes_cache: keys and values must have places of their own, but they begin at the same address");
     QMM_REQUIRE(slot_dtype == QMM_DTYPE_I32 || slot_dtype == QMM_DTYPE_I64, "qmm_rotary_axes_cache: slots must be int32 or int64");
     p.q = query;
     p.q_st = query_stride_token;

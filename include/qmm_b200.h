@@ -394,7 +394,8 @@ QMM_API int qmm_rotary_axes(const void *query, int64_t query_stride_token, int64
  * qmm_rotary_axes whose keys go to the cache instead of an output, together with the values (torch op `npu_rotary_axes_cache`).
  * Token t is written to place slots[t] % page_size of page slots[t] / page_size; a slot outside [0, pages * page_size) writes
  * nothing (padding; its query row is turned all the same).  Slots inside are to differ: of two tokens with the same slot either
- * may remain, in part.  All other places of the cache keep what they held.
+ * may remain, in part.  Places of the cache are not to overlap; keys and values at one address are refused.  All other places of the
+ * cache keep what they held.
  */
 QMM_API int qmm_rotary_axes_cache(const void *query, int64_t query_stride_token, int64_t query_stride_head, const void *key,
                                   int64_t key_stride_token, int64_t key_stride_head, const void *value,

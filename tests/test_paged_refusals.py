@@ -1,4 +1,6 @@
 """Calls of the attention over a paged cache that its C entries refuse, without a GPU."""
+import ctypes
+
 import pytest
 
 from test_paged_boundary import _attention, _cache
@@ -30,3 +32,15 @@ def test_operands_off_their_alignment(capi):
                 n, 0, 2, 4, 256, 64, _cache(capi), a["table"], 4, 4, a["lens"], 1.0, 0, 0, a["out"], a["lse"], None, 0, None)
         for op, call in calls.items():
             assert call() == 1 and "boundaries" in lib.qmm_last_error().decode(), (op, name, lib.qmm_last_error())
+
+
+def test_keys_and_values_at_one_address(capi):
+    """A cache that is written: which of the two would remain is left to chance."""
+    lib, one = capi.lib(), (ctypes.c_int64 * 1)(4)
+
+    def call(cache):
+        return lib.qmm_rotary_axes_cache(None, 0, 0, None, 0, 0, None, 0, 0, 0, 0, 4, None, 3, 0, 1, None, 4, one, 1, 0, 0, cache, None, 3, 1, None, None)
+
+    assert call(_cache(capi, dim=8)) == 0
+    assert call(_cache(capi, dim=8, value=1 << 20)) == 1 and "same address" in lib.qmm_last_error().decode()
+    assert call(_cache(capi, dim=8, key=None, value=None, pages=0)) == 0
