@@ -37,6 +37,8 @@ EXPORTED_SYMBOLS = (
     "qmm_all_gather_mm", "qmm_quant_matmul_int8_workspace_size", "qmm_quant_matmul_int8",
     "qmm_rotary_axes", "qmm_rotary_axes_cache", "qmm_paged_attention_workspace_size", "qmm_paged_attention",
     "qmm_paged_prompt_attention_workspace_size", "qmm_paged_prompt_attention",
+    "qmm_rotary_axes_quant_cache", "qmm_paged_quant_attention_workspace_size", "qmm_paged_quant_attention",
+    "qmm_paged_cache_dequant",
 )
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
@@ -55,6 +57,13 @@ class KvCache(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("key", "value")] + \
         [(n, ctypes.c_int64) for n in ("pages", "page_size", "kv_heads", "dim", "key_stride_page", "key_stride_place",
                                        "key_stride_head", "value_stride_page", "value_stride_place", "value_stride_head")]
+
+
+class KvScales(ctypes.Structure):
+    """``qmm_kv_scales``: the scales of an int8 cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("key", "value")] + \
+        [(n, ctypes.c_int64) for n in ("key_stride_page", "key_stride_place", "key_stride_head", "value_stride_page",
+                                       "value_stride_place", "value_stride_head")]
 
 
 def _export_nccl_path() -> None:
@@ -176,6 +185,16 @@ def lib() -> ctypes.CDLL:
         L.qmm_paged_prompt_attention_workspace_size.argtypes = [i64] * 6 + [c.POINTER(c.c_size_t)]
         L.qmm_paged_prompt_attention.argtypes = [p, i, i64, i64, i64, i64, cache, p, i64, i64, p, p, i64, c.c_double, i64, i64, p,
                                                  p, p, c.c_size_t, p]
+        scales = c.POINTER(KvScales)
+        L.qmm_rotary_axes_quant_cache.argtypes = [p, i64, i64, p, i64, i64, p, i64, i64, i, i64, i64, p, i, i64, i64, p, i64,
+                                                  c.POINTER(i64), i64, i, i, cache, scales, p, i, i64, p, p]
+        L.qmm_paged_quant_attention_workspace_size.argtypes = [i64] * 5 + [c.POINTER(c.c_size_t)]
+        L.qmm_paged_quant_attention.argtypes = [p, i, i64, i64, i64, i64, cache, scales, p, i64, i64, p, c.c_double, i64, i64, p, p,
+                                                p, c.c_size_t, p]
+        L.qmm_paged_cache_dequant.argtypes = [cache, scales, p, i64, i64, p, p, i64, cache, i, p, i64, i64, p]
+        for name in ("qmm_rotary_axes_quant_cache", "qmm_paged_quant_attention_workspace_size", "qmm_paged_quant_attention",
+                     "qmm_paged_cache_dequant"):
+            getattr(L, name).restype = c.c_int
         for name in ("qmm_rotary_axes", "qmm_rotary_axes_cache", "qmm_paged_attention_workspace_size", "qmm_paged_attention",
                      "qmm_paged_prompt_attention_workspace_size", "qmm_paged_prompt_attention"):
             getattr(L, name).restype = c.c_int
@@ -439,6 +458,12 @@ def kv_cache(key_cache, value_cache) -> KvCache:
     return KvCache(key_cache.data_ptr(), value_cache.data_ptr(), *key_cache.shape, *key_cache.stride()[:3], *value_cache.stride()[:3])
 
 
+def kv_scales(key_scale, value_scale) -> KvScales:
+    """fp32 [pages, heads, page size] scales of an int8 cache, any strides."""
+    (kb, kh, kt), (vb, vh, vt) = key_scale.stride(), value_scale.stride()
+    return KvScales(key_scale.data_ptr(), value_scale.data_ptr(), kb, kt, kh, vb, vt, vh)
+
+
 def _rotary_arguments(positions, inv_freq, sections, interleaved, cyclic):
     positions = positions.reshape(-1, positions.shape[-1])
     sections = list(sections) if sections else [inv_freq.numel()]
@@ -489,3 +514,46 @@ def paged_attention(query, key_cache, value_cache, block_table, seq_lens, query_
                                    D ** -0.5 if scale_value is None else scale_value, window, sinks, _ptr(out), _ptr(lse),
                                    _ptr(scratch), int(n.value), _stream()), name)
     return out, lse
+
+
+def rotary_axes_quant_cache(query, key, value, positions, inv_freq, key_cache, value_cache, key_scale, value_scale, slots, sections=(),
+                            interleaved=False, cyclic=False):
+    """rotary_axes_cache with an int8 cache (see qmm_rotary_axes_quant_cache); returns the query turned."""
+    T, H, D = query.shape
+    q = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    with torch.cuda.device(query.device):
+        check(lib().qmm_rotary_axes_quant_cache(
+            _ptr(query), *query.stride()[:2], _ptr(key), *key.stride()[:2], _ptr(value), *value.stride()[:2], dtype_code(query.dtype),
+            T, H, *_rotary_arguments(positions, inv_freq, sections, interleaved, cyclic), kv_cache(key_cache, value_cache),
+            kv_scales(key_scale, value_scale), _ptr(slots), DTYPE_I64 if slots.dtype == torch.int64 else DTYPE_I32, slots.stride(0), _ptr(q),
+            _stream()), "qmm_rotary_axes_quant_cache")
+    return q
+
+
+def paged_quant_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, scale_value=None, window=0,
+                          sinks=0):
+    """(out, lse) of one new token a sequence over an int8 cache (see qmm_paged_quant_attention)."""
+    B, H, D = query.shape
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=query.device)
+    n = ctypes.c_size_t(0)
+    check(lib().qmm_paged_quant_attention_workspace_size(B, H, key_cache.shape[2], D, block_table.shape[1] * key_cache.shape[1],
+                                                         ctypes.byref(n)), "qmm_paged_quant_attention_workspace_size")
+    scratch = torch.empty(int(n.value), dtype=torch.uint8, device=query.device)
+    with torch.cuda.device(query.device):
+        check(lib().qmm_paged_quant_attention(
+            _ptr(query), dtype_code(query.dtype), B, H, *query.stride()[:2], kv_cache(key_cache, value_cache),
+            kv_scales(key_scale, value_scale), _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(seq_lens),
+            D ** -0.5 if scale_value is None else scale_value, window, sinks, _ptr(out), _ptr(lse), _ptr(scratch), int(n.value),
+            _stream()), "qmm_paged_quant_attention")
+    return out, lse
+
+
+def paged_cache_dequant(key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, key_out, value_out, out_table,
+                        first_places=None):
+    """Reads an int8 cache back into pages of another type (see qmm_paged_cache_dequant)."""
+    with torch.cuda.device(key_cache.device):
+        check(lib().qmm_paged_cache_dequant(
+            kv_cache(key_cache, value_cache), kv_scales(key_scale, value_scale), _ptr(block_table), block_table.stride(0),
+            block_table.shape[1], _ptr(seq_lens), _ptr(first_places), seq_lens.numel(), kv_cache(key_out, value_out),
+            dtype_code(key_out.dtype), _ptr(out_table), out_table.stride(0), out_table.shape[1], _stream()), "qmm_paged_cache_dequant")

@@ -17,7 +17,7 @@ in ``TorchLibrary.cpp`` so that ``torch.ops.npu.<name>`` resolves.
 The schema grammar handled is the subset these operators use:
 ``Tensor``, ``Tensor(a!)`` (written in place), ``Tensor?``, ``str``, ``int``, ``int[]``,
 ``float``, ``float?``, ``bool``, ``ScalarType?``, keyword-only marker ``*``, defaults, and
-``Tensor`` / tuple-of-``Tensor`` returns.
+``Tensor``, tuple-of-``Tensor`` and ``()`` returns.
 
 Usage: ``python -m codegen.gen_backend_stubs --source_yaml <yaml> [<yaml> ...] --output_dir <dir>``
 """
@@ -85,6 +85,8 @@ class OpSchema:
     schema: str
 
     def cpp_return(self) -> str:
+        if not self.returns:
+            return "void"
         if len(self.returns) == 1:
             return "at::Tensor"
         return "::std::tuple<" + ",".join("at::Tensor" for _ in self.returns) + ">"

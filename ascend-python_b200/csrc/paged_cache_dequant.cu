@@ -1,0 +1,226 @@
+// Reading an int8 paged key-value cache back into pages of another type (npu_paged_cache_dequant): place j of sequence b, code times
+// scale, goes to place j of the sequence in a second block table.
+//
+// Bound by HBM: a code is read once, its value written once; the scales are a thirty-second of that or less.  The places of all
+// sequences are one list, cut into equal ranges for the warps, wherever sequences begin and end, so ragged lengths load the GPU
+// alike.  A lane has the same vectors of eight codes in all places of its range: their head, and where they lie in a place's rows, are
+// found once.
+#include "paged_common.cuh"
+
+namespace qmm {
+namespace paged {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kCtas = 4;  // an SM
+
+struct Side {
+    void *k, *v;
+    int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+    const int32_t *table;
+    int64_t table_st, pages;
+    int page, page_shift, capacity;
+};
+
+struct Copy {
+    Side from, to;
+    QuantScales scales;
+    const int32_t *lens, *first;
+    int batch, kv_heads, dim;
+};
+
+// Places [lo, hi) of sequence b are copied.
+__device__ __forceinline__ void places_of(const Copy &c, int b, int *lo, int *hi) {
+    *lo = c.first != nullptr ? max(0, __ldg(c.first + b)) : 0;
+    *hi = max(*lo, min(__ldg(c.lens + b), min(c.from.capacity, c.to.capacity)));
+}
+
+__device__ __forceinline__ bool find_page(const Side &s, int b, int j, int64_t *block, int *at) {
+    const int i = s.page_shift >= 0 ? j >> s.page_shift : j / s.page;
+    const int32_t id = __ldg(s.table + b * s.table_st + i);
+    *block = id;
+    *at = j - i * s.page;
+    return id >= 0 && id < s.pages;
+}
+
+// V: codes of a vector, 8 or 1.
+template <typename T, int V>
+__device__ __forceinline__ void write_values(T *dst, const int8_t *src, float scale);
+template <>
+__device__ __forceinline__ void write_values<float, 1>(float *dst, const int8_t *src, float scale) { *dst = static_cast<float>(*src) * scale; }
+template <>
+__device__ __forceinline__ void write_values<__half, 1>(__half *dst, const int8_t *src, float scale) { *dst = from_float<__half>(static_cast<float>(*src) * scale); }
+template <>
+__device__ __forceinline__ void write_values<__nv_bfloat16, 1>(__nv_bfloat16 *dst, const int8_t *src, float scale) {
+    *dst = from_float<__nv_bfloat16>(static_cast<float>(*src) * scale);
+}
+
+// Four codes as floats.
+__device__ __forceinline__ void unpack4(uint32_t w, float *f) {
+    w ^= 0x80808080u;  // u = code + 128; 0x4b0000uu is 2^23 + u
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+}
+
+// A vector of eight values.
+template <typename T>
+__device__ __forceinline__ void store8(T *dst, const float (&f)[8]) {
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+}
+template <>
+__device__ __forceinline__ void store8<float>(float *dst, const float (&f)[8]) {
+    reinterpret_cast<float4 *>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4 *>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+constexpr int kVectors = 4;  // of a lane, at once
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kWarps * 32) dequant_kernel(const __grid_constant__ Copy c) {
+    const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps, worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    int64_t total = 0;
+    for (int b = lane; b < c.batch; b += 32) {
+        int lo, hi;
+        places_of(c, b, &lo, &hi);
+        total += hi - lo;
+    }
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int64_t range = (total + workers - 1) / workers;
+    const int64_t begin = min(total, worker * range), end = min(total, begin + range);
+    if (begin >= end) return;
+    // the sequence and place where the range begins
+    int b = 0, lo = 0, hi = 0;
+    int64_t before = 0;
+    for (;; ++b) {
+        places_of(c, b, &lo, &hi);
+        if (before + (hi - lo) > begin) break;
+        before += hi - lo;
+    }
+    const int row = c.dim / V, vectors = 2 * c.kv_heads * row;  // of a head's row, of a place's keys and values
+    for (int base = 0; base < vectors; base += 32 * kVectors) {
+        const int8_t *src[kVectors];
+        const float *scale[kVectors];
+        T *dst[kVectors];
+        bool value[kVectors];
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const int n = base + 32 * i + lane;
+            const int head_of = min(n, vectors - 1) / row, e = (min(n, vectors - 1) - head_of * row) * V;
+            value[i] = head_of >= c.kv_heads;
+            const int head = value[i] ? head_of - c.kv_heads : head_of;
+            src[i] = n >= vectors ? nullptr : static_cast<const int8_t *>(value[i] ? c.from.v : c.from.k) + head * (value[i] ? c.from.v_sh : c.from.k_sh) + e;
+            scale[i] = (value[i] ? c.scales.v : c.scales.k) + head * (value[i] ? c.scales.v_sh : c.scales.k_sh);
+            dst[i] = static_cast<T *>(value[i] ? c.to.v : c.to.k) + head * (value[i] ? c.to.v_sh : c.to.k_sh) + e;
+        }
+        int s = b, s_hi = hi;
+        int j = lo + static_cast<int>(begin - before);
+        for (int64_t n = begin; n < end; ++n, ++j) {
+            while (j >= s_hi) places_of(c, ++s, &j, &s_hi);
+            int64_t from, to;
+            int from_at, to_at;
+            if (!find_page(c.from, s, j, &from, &from_at) | !find_page(c.to, s, j, &to, &to_at)) continue;
+#pragma unroll
+            for (int i = 0; i < kVectors; ++i) {
+                if (src[i] == nullptr) continue;
+                const int8_t *x = src[i] + from * (value[i] ? c.from.v_sb : c.from.k_sb) + from_at * (value[i] ? c.from.v_st : c.from.k_st);
+                const float by = __ldg(scale[i] + from * (value[i] ? c.scales.v_sb : c.scales.k_sb) + from_at * (value[i] ? c.scales.v_st : c.scales.k_st));
+                T *y = dst[i] + to * (value[i] ? c.to.v_sb : c.to.k_sb) + to_at * (value[i] ? c.to.v_st : c.to.k_st);
+                if constexpr (V == 8) {
+                    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(x));
+                    float f[8];
+                    unpack4(w.x, f);
+                    unpack4(w.y, f + 4);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) f[k] *= by;
+                    store8<T>(y, f);
+                } else {
+                    write_values<T, 1>(y, x, by);
+                }
+            }
+        }
+    }
+}
+
+template <typename T>
+int launch_t(const Copy &c, bool vectors, cudaStream_t stream) {
+    auto kern = vectors ? dequant_kernel<T, 8> : dequant_kernel<T, 1>;
+    QMM_CUDA_OK(launch_pdl(kern, dim3(kCtas * sm_count()), dim3(kWarps * 32), 0, stream, c));
+    return QMM_OK;
+}
+
+void take_table(Side *s, const qmm_kv_cache *cache, const int32_t *table, int64_t table_stride, int64_t max_pages) {
+    s->k = const_cast<void *>(cache->key);
+    s->v = const_cast<void *>(cache->value);
+    s->k_sb = cache->key_stride_page;
+    s->k_st = cache->key_stride_place;
+    s->k_sh = cache->key_stride_head;
+    s->v_sb = cache->value_stride_page;
+    s->v_st = cache->value_stride_place;
+    s->v_sh = cache->value_stride_head;
+    s->table = table;
+    s->table_st = table_stride;
+    s->pages = cache->pages;
+    s->page = static_cast<int>(cache->page_size);
+    s->page_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (s->page == 1 << i) s->page_shift = i;
+    const int64_t capacity = cache->pages == 0 ? 0 : max_pages * cache->page_size;
+    s->capacity = static_cast<int>(capacity < 0x7fffff00 ? capacity : 0x7fffff00);
+}
+
+bool begins_at(int bytes, int size, const void *base, int64_t a, int64_t b, int64_t c) {
+    return (reinterpret_cast<uintptr_t>(base) & (bytes - 1)) == 0 && ((a | b | c) & (bytes / size - 1)) == 0;
+}
+
+}  // namespace
+
+}  // namespace paged
+}  // namespace qmm
+
+using qmm::fail;
+
+extern "C" int qmm_paged_cache_dequant(const qmm_kv_cache *cache, const qmm_kv_scales *scales, const int32_t *block_table,
+                                       int64_t table_stride, int64_t max_pages, const int32_t *seq_lens, const int32_t *first_places,
+                                       int64_t batch, const qmm_kv_cache *out, int out_dtype, const int32_t *out_table,
+                                       int64_t out_table_stride, int64_t out_max_pages, void *stream) {
+    using namespace qmm::paged;
+    const std::string name("qmm_paged_cache_dequant");
+    QMM_REQUIRE(cache != nullptr && scales != nullptr && out != nullptr, name + ": no cache, no scales or no output given");
+    QMM_REQUIRE(batch >= 0 && max_pages >= 0 && out_max_pages >= 0 && cache->pages >= 0 && out->pages >= 0, name + ": sizes must be non-negative");
+    QMM_REQUIRE(cache->page_size >= 1 && cache->page_size <= 0x7fffffff && out->page_size >= 1 && out->page_size <= 0x7fffffff,
+                name + ": the page sizes must be positive");
+    QMM_REQUIRE(batch < 0x7fffffff && max_pages <= 0x7fffffff && out_max_pages <= 0x7fffffff && cache->pages <= 0x7fffffff && out->pages <= 0x7fffffff,
+                name + ": sizes out of range");
+    QMM_REQUIRE(cache->kv_heads >= 1 && cache->kv_heads <= 65535 && cache->dim >= 1 && cache->dim <= 256,
+                name + ": between 1 and 65535 heads, of a dimension up to 256");
+    QMM_REQUIRE(cache->kv_heads == out->kv_heads && cache->dim == out->dim, name + ": cache and output must have the same heads and dimension");
+    QMM_REQUIRE(out_dtype == QMM_DTYPE_BF16 || out_dtype == QMM_DTYPE_F16 || out_dtype == QMM_DTYPE_F32, name + ": the output must be bf16, f16 or f32");
+    QMM_REQUIRE(out->pages == 0 || out->key != out->value, name + ": keys and values must have places of their own, but they begin at the same address");
+    const int size = out_dtype == QMM_DTYPE_F32 ? 4 : 2;
+    for (const void *x : {static_cast<const void *>(scales->key), static_cast<const void *>(scales->value), static_cast<const void *>(block_table),
+                          static_cast<const void *>(seq_lens), static_cast<const void *>(first_places), static_cast<const void *>(out_table)})
+        QMM_REQUIRE((reinterpret_cast<uintptr_t>(x) & 3) == 0, name + ": scales, tables and lengths must begin at 4-byte boundaries");
+    QMM_REQUIRE(begins_at(size, size, out->key, 0, 0, 0) && begins_at(size, size, out->value, 0, 0, 0), name + ": the output must begin at a boundary of its type");
+    if (batch == 0) return QMM_OK;
+    Copy c;
+    take_table(&c.from, cache, block_table, table_stride, max_pages);
+    take_table(&c.to, out, out_table, out_table_stride, out_max_pages);
+    c.scales = {scales->key, scales->value, scales->key_stride_page, scales->key_stride_place, scales->key_stride_head,
+                scales->value_stride_page, scales->value_stride_place, scales->value_stride_head};
+    c.lens = seq_lens;
+    c.first = first_places;
+    c.batch = static_cast<int>(batch);
+    c.kv_heads = static_cast<int>(cache->kv_heads);
+    c.dim = static_cast<int>(cache->dim);
+    const bool vectors = c.dim % 8 == 0 && begins_at(8, 1, c.from.k, c.from.k_sb, c.from.k_st, c.from.k_sh) &&
+                         begins_at(8, 1, c.from.v, c.from.v_sb, c.from.v_st, c.from.v_sh) &&
+                         begins_at(16, size, c.to.k, c.to.k_sb, c.to.k_st, c.to.k_sh) && begins_at(16, size, c.to.v, c.to.v_sb, c.to.v_st, c.to.v_sh);
+    const cudaStream_t on = static_cast<cudaStream_t>(stream);
+    if (out_dtype == QMM_DTYPE_BF16) return launch_t<__nv_bfloat16>(c, vectors, on);
+    if (out_dtype == QMM_DTYPE_F16) return launch_t<__half>(c, vectors, on);
+    return launch_t<float>(c, vectors, on);
+}

@@ -32,6 +32,13 @@ struct Problem {
     float scale;
 };
 
+// The scales of an 8-bit cache's rows: that of (page, place, head) of the keys is k[page * k_sb + place * k_st + head * k_sh].
+struct QuantScales {
+    const float *k, *v;
+    int64_t k_sb, k_st, k_sh;
+    int64_t v_sb, v_st, v_sh;
+};
+
 struct Range {
     int sink_end, lo, hi;
 };
@@ -206,6 +213,8 @@ __device__ __forceinline__ void empty_row(const Problem &p, int64_t token, int h
 
 size_t decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
 int launch_decode(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+size_t quant_decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
+int launch_quant_decode(const Problem &p, const QuantScales &scales, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 size_t prompt_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places);
 int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 

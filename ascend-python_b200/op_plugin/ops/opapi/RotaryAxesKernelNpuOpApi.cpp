@@ -1,5 +1,5 @@
-// npu_rotary_axes and npu_rotary_axes_cache: rotary positions on one or several axes, and the same with the write of keys and
-// values into a paged cache.  They have no counterpart in the reference; host conventions are those of npu_rms_norm and its
+// npu_rotary_axes, npu_rotary_axes_cache and npu_rotary_axes_quant_cache: rotary positions on one or several axes, and the same with
+// the write of keys and values into a paged cache of their type or of int8.  They have no counterpart in the reference; host conventions are those of npu_rms_norm and its
 // fusion (RmsNormKernelNpuOpApi.cpp): dense outputs with the input's options, strided inputs taken as they are.
 #include "op_plugin/OpApiInterface.h"
 #include "op_plugin/utils/paged_cache.h"
@@ -99,12 +99,7 @@ at::Tensor npu_rotary_axes_cache(const at::Tensor &query, const at::Tensor &key,
     qmm_kv_cache cache = op_plugin_utils::describe_cache(op, key_cache, value_cache, query);
     TORCH_CHECK(cache.kv_heads == key.size(1) && cache.dim == key.size(2), op, ": the cache should hold ", key.size(1), " heads of ",
                 key.size(2), ", but it is ", key_cache.sizes());
-    for (const auto &c : {key_cache, value_cache}) {
-        for (int64_t d = 0; d < 3; ++d) {
-            TORCH_CHECK(c.size(d) == 1 || c.stride(d) != 0, op, ": the places of a cache that is written should not overlap, but its strides are ",
-                        c.strides());
-        }
-    }
+    op_plugin_utils::check_written(op, {key_cache, value_cache});
     const int slot_dtype = index_dtype(op, "slots", slots);
     TORCH_CHECK(slots.dim() == 1 && slots.size(0) == r.tokens, op, ": slots should hold ", r.tokens, " tokens, but they are ",
                 slots.sizes());
@@ -119,6 +114,43 @@ at::Tensor npu_rotary_axes_cache(const at::Tensor &query, const at::Tensor &key,
                  r.position_stride_token, static_cast<const float *>(r.inv_freq.const_data_ptr()), r.inv_freq.numel(),
                  r.sections.data(), r.axes, r.interleaved, r.cyclic, &cache, slots.const_data_ptr(), slot_dtype, slots.stride(0),
                  q.data_ptr(), op_plugin_utils::current_stream(query));
+    return q;
+}
+
+at::Tensor npu_rotary_axes_quant_cache(const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
+                                       const at::Tensor &positions, const at::Tensor &inv_freq, const at::Tensor &key_cache,
+                                       const at::Tensor &value_cache, const at::Tensor &key_scale, const at::Tensor &value_scale,
+                                       const at::Tensor &slots, at::IntArrayRef sections, c10::string_view rotary_mode,
+                                       c10::string_view axis_order)
+{
+    const char *op = "npu_rotary_axes_quant_cache";
+    c10::OptionalDeviceGuard guard;
+    if (query.is_cuda()) guard.reset_device(query.device());
+    const Rotary r = check_rotary(op, query, key, positions, inv_freq, sections, rotary_mode, axis_order);
+    TORCH_CHECK(value.device() == query.device() && slots.device() == query.device(), op, ": all tensors should be on ", query.device());
+    TORCH_CHECK(value.scalar_type() == query.scalar_type() && value.sizes() == key.sizes(), op,
+                ": value should have dtype and shape of key (", key.scalar_type(), " ", key.sizes(), "), but it is ",
+                value.scalar_type(), " ", value.sizes());
+    op_plugin_utils::QuantCache cache = op_plugin_utils::describe_quant_cache(op, key_cache, value_cache, key_scale, value_scale, query);
+    TORCH_CHECK(cache.codes.kv_heads == key.size(1) && cache.codes.dim == key.size(2), op, ": the cache should hold ", key.size(1),
+                " heads of ", key.size(2), ", but it is ", key_cache.sizes());
+    op_plugin_utils::check_written(op, {key_cache, value_cache, key_scale, value_scale});
+    const int slot_dtype = index_dtype(op, "slots", slots);
+    TORCH_CHECK(slots.dim() == 1 && slots.size(0) == r.tokens, op, ": slots should hold ", r.tokens, " tokens, but they are ",
+                slots.sizes());
+    const at::Tensor v = op_plugin_utils::dense_rows(value);
+    // a cache that shares its storage with a lazy clone gets its own, now that it is written
+    cache.codes.key = key_cache.mutable_data_ptr();
+    cache.codes.value = value_cache.mutable_data_ptr();
+    cache.scales.key = static_cast<const float *>(key_scale.mutable_data_ptr());
+    cache.scales.value = static_cast<const float *>(value_scale.mutable_data_ptr());
+    at::Tensor q = op_plugin_utils::empty_output(query.sizes(), query, query.scalar_type());
+    EXEC_QMM_CMD(qmm_rotary_axes_quant_cache, r.q.const_data_ptr(), r.q.stride(0), r.q.stride(1), r.k.const_data_ptr(), r.k.stride(0),
+                 r.k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1), op_plugin_utils::qmm_dtype(query.scalar_type()),
+                 r.tokens, query.size(1), r.positions.const_data_ptr(), r.position_dtype, r.position_stride_axis,
+                 r.position_stride_token, static_cast<const float *>(r.inv_freq.const_data_ptr()), r.inv_freq.numel(),
+                 r.sections.data(), r.axes, r.interleaved, r.cyclic, &cache.codes, &cache.scales, slots.const_data_ptr(), slot_dtype,
+                 slots.stride(0), q.data_ptr(), op_plugin_utils::current_stream(query));
     return q;
 }
 

@@ -116,6 +116,17 @@ PyObject *call(const Op &op, const A &...a)
     }());
 }
 
+// The same of an operator that returns nothing.
+template <typename Op, typename... A>
+PyObject *call_void(const Op &op, const A &...a)
+{
+    {
+        pybind11::gil_scoped_release release;
+        op.call(a...);
+    }
+    Py_RETURN_NONE;
+}
+
 template <typename Signature>
 c10::TypedOperatorHandle<Signature> find(const char *name)
 {
@@ -218,6 +229,24 @@ PyObject *rotary_axes_cache(PyObject *, PyObject *const *args, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *rotary_axes_quant_cache(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<at::Tensor(const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                           const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                           const at::Tensor &, const at::Tensor &, at::IntArrayRef, c10::string_view,
+                                           c10::string_view)>("npu::npu_rotary_axes_quant_cache");
+    Arguments a(args, n, 13);
+    if (!a.ok) return not_here();
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &positions = a.tensor(3), &inv_freq = a.tensor(4);
+    const at::Tensor &k_cache = a.tensor(5), &v_cache = a.tensor(6), &k_scale = a.tensor(7), &v_scale = a.tensor(8), &slots = a.tensor(9);
+    const std::vector<int64_t> sections = a.integers(10);
+    const c10::string_view mode = a.text(11), order = a.text(12);
+    return a.ok ? call(op, q, k, v, positions, inv_freq, k_cache, v_cache, k_scale, v_scale, slots, at::IntArrayRef(sections), mode, order)
+                : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
@@ -230,6 +259,38 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
     const c10::optional<double> scale = a.optional_number(5);
     const int64_t window = a.integer(6), sinks = a.integer(7);
     return a.ok ? call(op, q, k, v, table, lens, scale, window, sinks) : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *paged_quant_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<std::tuple<at::Tensor, at::Tensor>(const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                                   const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                                   const at::Tensor &, c10::optional<double>, int64_t,
+                                                                   int64_t)>("npu::npu_paged_quant_attention");
+    Arguments a(args, n, 10);
+    if (!a.ok) return not_here();
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &k_scale = a.tensor(3), &v_scale = a.tensor(4);
+    const at::Tensor &table = a.tensor(5), &lens = a.tensor(6);
+    const c10::optional<double> scale = a.optional_number(7);
+    const int64_t window = a.integer(8), sinks = a.integer(9);
+    return a.ok ? call(op, q, k, v, k_scale, v_scale, table, lens, scale, window, sinks) : not_here();
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *paged_cache_dequant(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    static const auto op = find<void(const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                     const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                     const Optional &)>("npu::npu_paged_cache_dequant");
+    Arguments a(args, n, 10);
+    if (!a.ok) return not_here();
+    const at::Tensor &k = a.tensor(0), &v = a.tensor(1), &k_scale = a.tensor(2), &v_scale = a.tensor(3), &table = a.tensor(4);
+    const at::Tensor &lens = a.tensor(5), &k_out = a.tensor(6), &v_out = a.tensor(7), &out_table = a.tensor(8);
+    const Optional first = a.optional(9);
+    return a.ok ? call_void(op, k, v, k_scale, v_scale, table, lens, k_out, v_out, out_table, first) : not_here();
     END_HANDLE_TH_ERRORS
 }
 
@@ -261,7 +322,10 @@ PyMethodDef methods[] = {method<dynamic_quant>("dynamic_quant"),
                          method<weight_quant_batchmatmul>("weight_quant_batchmatmul"),
                          method<rotary_axes>("rotary_axes"),
                          method<rotary_axes_cache>("rotary_axes_cache"),
+                         method<rotary_axes_quant_cache>("rotary_axes_quant_cache"),
                          method<paged_attention>("paged_attention"),
+                         method<paged_quant_attention>("paged_quant_attention"),
+                         method<paged_cache_dequant>("paged_cache_dequant"),
                          method<paged_prompt_attention>("paged_prompt_attention"),
                          {nullptr, nullptr, 0, nullptr}};
 

@@ -148,6 +148,50 @@ def npu_paged_prompt_attention(query, key_cache, value_cache, block_table, seq_l
                                            scale_value=scale_value, window=window, sinks=sinks)
 
 
+def npu_rotary_axes_quant_cache(query, key, value, positions, inv_freq, key_cache, value_cache, key_scale, value_scale, slots, *,
+                                sections=(), rotary_mode="half", axis_order="blocked"):
+    """npu_rotary_axes_cache with an int8 cache: each row (token, head) is quantized by its largest magnitude as it is written.
+
+    key_cache, value_cache int8 [pages, page size, kv heads, dim]; key_scale, value_scale fp32 [pages, kv heads, page size]: a row
+    stands for its codes times its scale.
+    """
+    if not _compiling():
+        out = _calls.rotary_axes_quant_cache(query, key, value, positions, inv_freq, key_cache, value_cache, key_scale, value_scale,
+                                             slots, sections, rotary_mode, axis_order)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_rotary_axes_quant_cache(query, key, value, positions, inv_freq, key_cache, value_cache, key_scale, value_scale,
+                                            slots, sections=sections, rotary_mode=rotary_mode, axis_order=axis_order)
+
+
+def npu_paged_quant_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, *, scale_value=None,
+                              window=0, sinks=0):
+    """npu_paged_attention over the int8 cache that npu_rotary_axes_quant_cache fills."""
+    if not _compiling():
+        out = _calls.paged_quant_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, scale_value,
+                                           window, sinks)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_paged_quant_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens,
+                                          scale_value=scale_value, window=window, sinks=sinks)
+
+
+def npu_paged_cache_dequant(key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, key_out, value_out, out_table, *,
+                            first_places=None):
+    """Reads an int8 cache back into pages of bf16, f16 or fp32, for npu_paged_prompt_attention and other readers of those.
+
+    Place j of sequence b, max(0, first_places[b]) <= j < seq_lens[b], goes to place j % n of page out_table[b, j // n] of key_out and
+    value_out [out pages, n, kv heads, dim]; nothing else of them is written.
+    """
+    if not _compiling():
+        out = _calls.paged_cache_dequant(key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, key_out, value_out,
+                                         out_table, first_places)
+        if out is not NotImplemented:
+            return out
+    return _ops.npu_paged_cache_dequant(key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, key_out, value_out,
+                                        out_table, first_places=first_places)
+
+
 def npu_mm_all_reduce_base(x1, x2, hcom, *, reduce_op="sum", bias=None, antiquant_scale=None, antiquant_offset=None,
                            x3=None, dequant_scale=None, pertoken_scale=None, antiquant_group_size=0, comm_turn=0):
     if comm_turn == 0 and x1.is_cuda:

@@ -448,6 +448,66 @@ QMM_API int qmm_paged_prompt_attention(const void *query, int dtype, int64_t tok
                                        int64_t sinks, void *out, float *lse, void *workspace, size_t workspace_bytes,
                                        void *stream);
 
+/*
+ * An int8 paged key-value cache: a qmm_kv_cache of int8 codes (strides in bytes) with an fp32 scale for each row of it; the row
+ * (page, place, head) of the keys stands for code * key[page * key_stride_page + place * key_stride_place + head * key_stride_head].
+ * Scales of a head's places that lie one behind the other (heads in front of places) are read in whole sectors.
+ */
+typedef struct qmm_kv_scales {
+    const float *key;
+    const float *value;
+    int64_t key_stride_page, key_stride_place, key_stride_head;
+    int64_t value_stride_page, value_stride_place, value_stride_head;
+} qmm_kv_scales;
+
+/*
+ * qmm_rotary_axes_cache with an int8 cache (torch op `npu_rotary_axes_quant_cache`; no counterpart in the reference).  The query comes out as from
+ * qmm_rotary_axes.  Each row y (token, head) of the turned key and of the value is quantized as it is written, in 64 bits:
+ *   scale = fp32(max |y| / 127)     code = y / scale, to the nearest whole number, ties to even
+ * (codes are 0 where the scale is 0 or not finite; a NaN in a row makes its scale NaN, an infinity, infinite).  Slots, and what is
+ * refused, as there; scales begin at 4-byte boundaries, keys' and values' at addresses of their own.
+ */
+QMM_API int qmm_rotary_axes_quant_cache(const void *query, int64_t query_stride_token, int64_t query_stride_head, const void *key,
+                                        int64_t key_stride_token, int64_t key_stride_head, const void *value,
+                                        int64_t value_stride_token, int64_t value_stride_head, int dtype, int64_t tokens,
+                                        int64_t heads, const void *positions, int position_dtype, int64_t position_stride_axis,
+                                        int64_t position_stride_token, const float *inv_freq, int64_t pairs,
+                                        const int64_t *sections, int64_t axes, int interleaved, int cyclic,
+                                        const qmm_kv_cache *cache, const qmm_kv_scales *scales, const void *slots, int slot_dtype,
+                                        int64_t slot_stride, void *query_out, void *stream);
+
+/*
+ * qmm_paged_attention over an int8 cache (torch op `npu_paged_quant_attention`; no counterpart in the reference): keys and values are what codes and
+ * scales stand for, all else is said there.  Scores, softmax and sums are fp32; query and weights enter the products in f16, the
+ * weights times the values' scales and a power of two for each row (half a step, 2^-11, of each, or 2^-33 of the largest; a bf16
+ * query is exact but for elements below 2^-21 of its row's largest, off by 2^-32 of that).
+ * The head dimension is a multiple of 16 up to 256; caches begin at 16-byte boundaries, their strides are multiples of 16;
+ * scales begin at 4-byte boundaries.  The largest |query| of a row times |scale_value| * log2(e), and 2^8 over it times a
+ * key's row, are to be in fp32's range, as the scores are.
+ */
+QMM_API int qmm_paged_quant_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_places,
+                                                     size_t *bytes);
+QMM_API int qmm_paged_quant_attention(const void *query, int dtype, int64_t batch, int64_t heads, int64_t query_stride_token,
+                                      int64_t query_stride_head, const qmm_kv_cache *cache, const qmm_kv_scales *scales,
+                                      const int32_t *block_table, int64_t table_stride, int64_t max_pages, const int32_t *seq_lens,
+                                      double scale_value, int64_t window, int64_t sinks, void *out, float *lse, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+
+/*
+ * An int8 cache read back (torch op `npu_paged_cache_dequant`; no counterpart in the reference): for every sequence b and place j,
+ * max(0, first_places[b]) <= j < seq_lens[b] (first_places NULL: from place 0 on),
+ *   out[out_table[b][j / out page size]][j % out page size] = code * scale     of place j of b in `cache`, keys and values,
+ * the fp32 product rounded to out_dtype (bf16, f16, f32).  Places that either table does not cover, or whose entry there names
+ * no page, are left out; of `out` nothing else is written.  For qmm_paged_prompt_attention over an int8 cache, and for what reads
+ * pages of 16 or 32 bits.  Places of `out` that are written are to differ, and lie outside `cache`.  Any head dimension up to 256, any
+ * strides; vectors where the dimension is a multiple of 8, the cache begins at 8-byte boundaries with strides of
+ * multiples of 8 and out at 16-byte boundaries with strides of multiples of 16 bytes.
+ */
+QMM_API int qmm_paged_cache_dequant(const qmm_kv_cache *cache, const qmm_kv_scales *scales, const int32_t *block_table,
+                                    int64_t table_stride, int64_t max_pages, const int32_t *seq_lens, const int32_t *first_places,
+                                    int64_t batch, const qmm_kv_cache *out, int out_dtype, const int32_t *out_table,
+                                    int64_t out_table_stride, int64_t out_max_pages, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
