@@ -3,8 +3,8 @@
 //
 // Bound by HBM: a code is read once, its value written once; the scales are a thirty-second of that or less.  The places of all
 // sequences are one list, cut into equal ranges for the warps, wherever sequences begin and end, so ragged lengths load the GPU
-// alike.  A lane has the same vectors of eight codes in all places of its range: their head, and where they lie in a place's rows, are
-// found once.
+// alike.  A warp's lanes are dealt out to the vectors of eight codes of a row, then to the heads, then to places, so that few or
+// small heads fill it too.
 #include "paged_common.cuh"
 
 namespace qmm {
@@ -44,18 +44,6 @@ __device__ __forceinline__ bool find_page(const Side &s, int b, int j, int64_t *
     return id >= 0 && id < s.pages;
 }
 
-// V: codes of a vector, 8 or 1.
-template <typename T, int V>
-__device__ __forceinline__ void write_values(T *dst, const int8_t *src, float scale);
-template <>
-__device__ __forceinline__ void write_values<float, 1>(float *dst, const int8_t *src, float scale) { *dst = static_cast<float>(*src) * scale; }
-template <>
-__device__ __forceinline__ void write_values<__half, 1>(__half *dst, const int8_t *src, float scale) { *dst = from_float<__half>(static_cast<float>(*src) * scale); }
-template <>
-__device__ __forceinline__ void write_values<__nv_bfloat16, 1>(__nv_bfloat16 *dst, const int8_t *src, float scale) {
-    *dst = from_float<__nv_bfloat16>(static_cast<float>(*src) * scale);
-}
-
 // Four codes as floats.
 __device__ __forceinline__ void unpack4(uint32_t w, float *f) {
     w ^= 0x80808080u;  // u = code + 128; 0x4b0000uu is 2^23 + u
@@ -63,82 +51,128 @@ __device__ __forceinline__ void unpack4(uint32_t w, float *f) {
     for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
 }
 
-// A vector of eight values.
-template <typename T>
-__device__ __forceinline__ void store8(T *dst, const float (&f)[8]) {
-    *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-}
+// A vector of codes, V of them (8, or 1 for any alignment).
+template <int V>
+struct Codes;
 template <>
-__device__ __forceinline__ void store8<float>(float *dst, const float (&f)[8]) {
-    reinterpret_cast<float4 *>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4 *>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
+struct Codes<8> {
+    uint2 w;
+    __device__ __forceinline__ void load(const int8_t *src) { w = __ldg(reinterpret_cast<const uint2 *>(src)); }
+    template <typename T>
+    __device__ __forceinline__ void store(T *dst, float scale) const {
+        float f[8];
+        unpack4(w.x, f);
+        unpack4(w.y, f + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= scale;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4 *>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4 *>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+        }
+    }
+};
+template <>
+struct Codes<1> {
+    int8_t w;
+    __device__ __forceinline__ void load(const int8_t *src) { w = __ldg(src); }
+    template <typename T>
+    __device__ __forceinline__ void store(T *dst, float scale) const { *dst = from_float<T>(static_cast<float>(w) * scale); }
+};
 
-constexpr int kVectors = 4;  // of a lane, at once
+// Rows (keys and values) that a lane has under way at once.
+constexpr int kAhead = 2;
+
+// How a warp's lanes are dealt out: 2^log_row to a row, 2^log_heads rows side by side of a place, what is left to places.
+struct Lanes {
+    int log_row, log_heads;
+};
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32) dequant_kernel(const __grid_constant__ Copy c) {
+__global__ void __launch_bounds__(kWarps * 32, kCtas) dequant_kernel(const __grid_constant__ Copy c, const __grid_constant__ Lanes lanes) {
     const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t workers = static_cast<int64_t>(gridDim.x) * kWarps, worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
     int64_t total = 0;
+    int lo = 0, hi = 0;  // of sequence `lane`, of up to 32
     for (int b = lane; b < c.batch; b += 32) {
-        int lo, hi;
         places_of(c, b, &lo, &hi);
         total += hi - lo;
     }
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int64_t range = (total + workers - 1) / workers;
-    const int64_t begin = min(total, worker * range), end = min(total, begin + range);
+    const int places_at_once = 32 >> (lanes.log_row + lanes.log_heads), step = kWarps * places_at_once;
+    const int64_t range = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t end = min(total, (blockIdx.x + 1) * range), begin = blockIdx.x * range + warp * places_at_once;
     if (begin >= end) return;
     // the sequence and place where the range begins
-    int b = 0, lo = 0, hi = 0;
+    int first = 0;
     int64_t before = 0;
-    for (;; ++b) {
-        places_of(c, b, &lo, &hi);
-        if (before + (hi - lo) > begin) break;
-        before += hi - lo;
-    }
-    const int row = c.dim / V, vectors = 2 * c.kv_heads * row;  // of a head's row, of a place's keys and values
-    for (int base = 0; base < vectors; base += 32 * kVectors) {
-        const int8_t *src[kVectors];
-        const float *scale[kVectors];
-        T *dst[kVectors];
-        bool value[kVectors];
-#pragma unroll
-        for (int i = 0; i < kVectors; ++i) {
-            const int n = base + 32 * i + lane;
-            const int head_of = min(n, vectors - 1) / row, e = (min(n, vectors - 1) - head_of * row) * V;
-            value[i] = head_of >= c.kv_heads;
-            const int head = value[i] ? head_of - c.kv_heads : head_of;
-            src[i] = n >= vectors ? nullptr : static_cast<const int8_t *>(value[i] ? c.from.v : c.from.k) + head * (value[i] ? c.from.v_sh : c.from.k_sh) + e;
-            scale[i] = (value[i] ? c.scales.v : c.scales.k) + head * (value[i] ? c.scales.v_sh : c.scales.k_sh);
-            dst[i] = static_cast<T *>(value[i] ? c.to.v : c.to.k) + head * (value[i] ? c.to.v_sh : c.to.k_sh) + e;
+    for (int b0 = 0;; b0 += 32) {
+        if (c.batch > 32) {
+            lo = hi = 0;
+            if (b0 + lane < c.batch) places_of(c, b0 + lane, &lo, &hi);
         }
-        int s = b, s_hi = hi;
-        int j = lo + static_cast<int>(begin - before);
-        for (int64_t n = begin; n < end; ++n, ++j) {
-            while (j >= s_hi) places_of(c, ++s, &j, &s_hi);
-            int64_t from, to;
-            int from_at, to_at;
-            if (!find_page(c.from, s, j, &from, &from_at) | !find_page(c.to, s, j, &to, &to_at)) continue;
+        const int64_t mine = hi - lo;
+        int64_t sum = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t left = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += left;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + sum > begin);
+        if (past != 0) {
+            const int at = __ffs(past) - 1;
+            first = b0 + at;
+            before += __shfl_sync(0xffffffffu, sum - mine, at);
+            lo = __shfl_sync(0xffffffffu, lo, at);
+            hi = __shfl_sync(0xffffffffu, hi, at);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    const int heads_at_once = 1 << lanes.log_heads;
+    const int slot = lane >> lanes.log_row, head0 = slot & (heads_at_once - 1);
+    int s = first, s_hi = hi;
+    int64_t n = begin + (slot >> lanes.log_heads);
+    int j = lo + static_cast<int>(n - before);
+    for (; n < end; n += step, j += step) {
+        while (j >= s_hi) {
+            const int over = j - s_hi;
+            places_of(c, ++s, &j, &s_hi);
+            j += over;
+        }
+        int64_t page, out;
+        int at, out_at;
+        if (!find_page(c.from, s, j, &page, &at) | !find_page(c.to, s, j, &out, &out_at)) continue;
+        for (int e = (lane & ((1 << lanes.log_row) - 1)) * V; e < c.dim; e += 32 * V) {
+            const int8_t *k = static_cast<const int8_t *>(c.from.k) + page * c.from.k_sb + at * c.from.k_st + head0 * c.from.k_sh + e;
+            const int8_t *v = static_cast<const int8_t *>(c.from.v) + page * c.from.v_sb + at * c.from.v_st + head0 * c.from.v_sh + e;
+            const float *k_scale = c.scales.k + page * c.scales.k_sb + at * c.scales.k_st + head0 * c.scales.k_sh;
+            const float *v_scale = c.scales.v + page * c.scales.v_sb + at * c.scales.v_st + head0 * c.scales.v_sh;
+            T *k_out = static_cast<T *>(c.to.k) + out * c.to.k_sb + out_at * c.to.k_st + head0 * c.to.k_sh + e;
+            T *v_out = static_cast<T *>(c.to.v) + out * c.to.v_sb + out_at * c.to.v_st + head0 * c.to.v_sh + e;
+            for (int head = head0; head < c.kv_heads; head += kAhead * heads_at_once) {
+                Codes<V> x[kAhead], y[kAhead];
+                float x_scale[kAhead], y_scale[kAhead];
 #pragma unroll
-            for (int i = 0; i < kVectors; ++i) {
-                if (src[i] == nullptr) continue;
-                const int8_t *x = src[i] + from * (value[i] ? c.from.v_sb : c.from.k_sb) + from_at * (value[i] ? c.from.v_st : c.from.k_st);
-                const float by = __ldg(scale[i] + from * (value[i] ? c.scales.v_sb : c.scales.k_sb) + from_at * (value[i] ? c.scales.v_st : c.scales.k_st));
-                T *y = dst[i] + to * (value[i] ? c.to.v_sb : c.to.k_sb) + to_at * (value[i] ? c.to.v_st : c.to.k_st);
-                if constexpr (V == 8) {
-                    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(x));
-                    float f[8];
-                    unpack4(w.x, f);
-                    unpack4(w.y, f + 4);
+                for (int i = 0; i < kAhead; ++i) {
+                    if (head + i * heads_at_once >= c.kv_heads) break;
+                    x[i].load(k);
+                    y[i].load(v);
+                    x_scale[i] = __ldg(k_scale);
+                    y_scale[i] = __ldg(v_scale);
+                    k += c.from.k_sh << lanes.log_heads;
+                    v += c.from.v_sh << lanes.log_heads;
+                    k_scale += c.scales.k_sh << lanes.log_heads;
+                    v_scale += c.scales.v_sh << lanes.log_heads;
+                }
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) f[k] *= by;
-                    store8<T>(y, f);
-                } else {
-                    write_values<T, 1>(y, x, by);
+                for (int i = 0; i < kAhead; ++i) {
+                    if (head + i * heads_at_once >= c.kv_heads) break;
+                    x[i].store(k_out, x_scale[i]);
+                    y[i].store(v_out, y_scale[i]);
+                    k_out += c.to.k_sh << lanes.log_heads;
+                    v_out += c.to.v_sh << lanes.log_heads;
                 }
             }
         }
@@ -148,7 +182,11 @@ __global__ void __launch_bounds__(kWarps * 32) dequant_kernel(const __grid_const
 template <typename T>
 int launch_t(const Copy &c, bool vectors, cudaStream_t stream) {
     auto kern = vectors ? dequant_kernel<T, 8> : dequant_kernel<T, 1>;
-    QMM_CUDA_OK(launch_pdl(kern, dim3(kCtas * sm_count()), dim3(kWarps * 32), 0, stream, c));
+    const int row = c.dim / (vectors ? 8 : 1);
+    Lanes lanes = {0, 0};
+    while (lanes.log_row < 5 && 1 << lanes.log_row < row) ++lanes.log_row;
+    while (lanes.log_row + lanes.log_heads < 5 && 1 << lanes.log_heads < c.kv_heads) ++lanes.log_heads;
+    QMM_CUDA_OK(launch_pdl(kern, dim3(kCtas * sm_count()), dim3(kWarps * 32), 0, stream, c, lanes));
     return QMM_OK;
 }
 

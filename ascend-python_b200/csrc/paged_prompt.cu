@@ -596,19 +596,6 @@ __device__ __forceinline__ void mma_ts_x4(uint32_t d, uint32_t a, uint32_t b_lo,
         "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 4-D tiled load global -> shared: columns, places of a page, heads, pages; by one lane of a converged warp.  (16 lanes with a box
-// each took 90 clocks a box: the instruction takes uniform operands, so lanes that differ go one by one.)
-__device__ __forceinline__ void tma_load_4d_warp(uint32_t dst, const CUtensorMap *m, int32_t column, int32_t place, int32_t head, int32_t page,
-                                            uint32_t bar) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred e;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t"
-        "}\n" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(column), "r"(place), "r"(head), "r"(page)
-        : "memory");
-}
 // Asks for a block of the grid that has not begun, in its place; the answer, 16 bytes, is counted on the barrier.
 __device__ __forceinline__ void ask_next_block(uint32_t answer, uint32_t bar) {
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar)
@@ -1495,7 +1482,7 @@ bool cache_map(CUtensorMap *map, const Problem &p, const void *base, int64_t sb,
         if (strides[i] <= 0 || strides[i] >= 1ll << 38) return false;
     }
     const int box[4] = {64, rows, 1, 1};
-    return make_tmap_4d(map, base, sizes, strides, box);
+    return make_tmap_4d(map, base, 2, sizes, strides, box, 128);
 }
 
 // The query: columns, heads of a group, groups, tokens.
@@ -1507,7 +1494,7 @@ bool query_map(CUtensorMap *map, const Problem &p) {
         if (strides[i] <= 0 || strides[i] >= 1ll << 38) return false;
     }
     const int box[4] = {64, p.group, 1, 128 / p.group};
-    return make_tmap_4d(map, p.q, sizes, strides, box);
+    return make_tmap_4d(map, p.q, 2, sizes, strides, box, 128);
 }
 
 template <typename T, int DP>

@@ -52,9 +52,10 @@ int sm_count();
 int make_tmap_2d(CUtensorMap *map, const void *base, int elem_bytes, uint64_t inner, uint64_t outer,
                  uint64_t ld, uint32_t box_inner, uint32_t box_outer, bool swizzle128);
 
-// Tensor map of 16-bit elements with four dimensions, the first dense: boxes of `box` elements, 128-byte swizzle,
+// Tensor map of 8- or 16-bit elements with four dimensions, the first dense: boxes of `box` elements, `swizzle` of 64 or 128 bytes,
 // zeros out of range.  `strides`: of dimensions 1 to 3, in elements.  False (and no error text): it cannot be made.
-bool make_tmap_4d(CUtensorMap *map, const void *base, const int64_t sizes[4], const int64_t strides[3], const int box[4]);
+bool make_tmap_4d(CUtensorMap *map, const void *base, int elem_bytes, const int64_t sizes[4], const int64_t strides[3], const int box[4],
+                  int swizzle);
 
 // ---------------------------------------------------------------------------
 // Device side
@@ -161,6 +162,20 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+// 4-D tiled load global -> shared (of a paged cache: columns, places of a page, heads, pages), by one lane of a converged warp.  (16 lanes
+// with a box each took 90 clocks a box: the instruction takes uniform operands, so lanes that differ go one by one.)
+__device__ __forceinline__ void tma_load_4d_warp(uint32_t dst, const CUtensorMap *m, int32_t column, int32_t place, int32_t head, int32_t page,
+                                            uint32_t bar) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t"
+        "}\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(column), "r"(place), "r"(head), "r"(page)
         : "memory");
 }
 

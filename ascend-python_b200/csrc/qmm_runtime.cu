@@ -117,16 +117,18 @@ int make_tmap_2d(CUtensorMap *map, const void *base, int elem_bytes, uint64_t in
     return QMM_OK;
 }
 
-bool make_tmap_4d(CUtensorMap *map, const void *base, const int64_t sizes[4], const int64_t strides[3], const int box[4]) {
+bool make_tmap_4d(CUtensorMap *map, const void *base, int elem_bytes, const int64_t sizes[4], const int64_t strides[3], const int box[4],
+                  int swizzle) {
     auto fn = get_encode_fn();
     if (fn == nullptr) return false;
     cuuint64_t dims[4], bytes[3];
     for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(sizes[i]);
-    for (int i = 0; i < 3; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+    for (int i = 0; i < 3; ++i) bytes[i] = static_cast<cuuint64_t>(strides[i]) * static_cast<cuuint64_t>(elem_bytes);
     cuuint32_t extent[4], step[4] = {1, 1, 1, 1};
     for (int i = 0; i < 4; ++i) extent[i] = static_cast<cuuint32_t>(box[i]);
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, bytes, extent, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return fn(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, bytes,
+              extent, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+              elem_bytes == 1 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace qmm

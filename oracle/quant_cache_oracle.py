@@ -23,9 +23,9 @@ def values(codes, scale):
 def attention(q, k_codes, v_codes, k_scale, v_scale, table, lens, scale=None, window=0, sinks=0):
     """(out, lse, out's bound, lse's bound) of one new token a sequence.
 
-    As paged_oracle.attention_bounds, but for the weights and the query.  d: a score is a sum of `dim` products of f16 (exact in fp32), times
-    the key's scale, times the row's power of two and scale_value: (dim + 5) * 2^-24 of its terms' absolute sum; a bf16 query's elements
-    far below their row's largest are off by up to 2^-32 of that one.  A weight, exp times the value's scale, is rounded to f16: 2^-11 of it, or
+    As paged_oracle.attention_bounds, but for the weights and the query.  d: a query's element is a whole number, of a step of at most 2^-21
+    of its row's largest, off by half a step, 2^-22 of that one.  A score's sum of products with codes is exact, but for its parts'
+    roundings, and then multiplied by the key's scale, the row's power of two and scale_value: (dim + 5) * 2^-24 of its terms' absolute sum is more.  A weight, exp times the value's scale, is rounded to f16: 2^-11 of it, or
     half of f16's smallest step, 2^-25, where the row's largest weight is 2^8 or more: 2^-33 of that.  So with w_j = p_j * value scale
 
         |out - ref| <= u |ref| + (2^-11 + 2 d + 2^-20) sum p |v| + 2^-33 max w sum |code|,   |lse - ref| <= d + 2^-20 + 2^-22 |lse|,
@@ -53,9 +53,7 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, table, lens, scale=None, wi
         spread[t] = v_codes[ids, js % page].double().abs().sum(0).repeat_interleave(H // KV, 0)
         most[t] = (p * v_scale[ids, :, js % page].double().abs().t().repeat_interleave(H // KV, 0)).amax(1)
         far[t] = (keys.abs().sum(2).t() * abs(by)).amax(1) * q[t].double().abs().amax(1)
-    d = (D + 5) * 2.0 ** -24 * reach
-    if q.dtype == torch.bfloat16:
-        d = d + 2.0 ** -32 * far
+    d = (D + 5) * 2.0 ** -24 * reach + 2.0 ** -22 * far
     bound = torch.finfo(q.dtype).eps / 2 * out.abs() + (2.0 ** -11 + 2 * d[..., None] + 2.0 ** -20) * weight + 2.0 ** -33 * most[..., None] * spread
     bound = bound + torch.finfo(q.dtype).smallest_normal * (torch.finfo(q.dtype).eps / 2)
     return out, lse, bound, d + 2.0 ** -20 + 2.0 ** -22 * lse.abs().nan_to_num(posinf=0.0)
