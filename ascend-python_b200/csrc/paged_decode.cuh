@@ -439,7 +439,7 @@ int launch_join(const Problem &p, const Plan &plan, const Scratch &scratch, cuda
     // all sequences are short whatever their lengths are, and no head tile is cut
     if (p.capacity <= kShort && plan.items <= 2 * plan.workers) return QMM_OK;
     const int64_t indices = scratch.by_item ? plan.items : plan.workers;
-    const bool share_parts = indices * plan.rows <= 4 * plan.workers;
+    const bool share_parts = indices * plan.rows <= 8 * sm_count();
     QMM_CUDA_OK(launch_pdl(join_kernel<T>, dim3(static_cast<unsigned>(indices), share_parts ? plan.rows : 1), dim3(kJoinWarps * 32), 0,
                            stream, p, scratch, share_parts));
     return QMM_OK;
