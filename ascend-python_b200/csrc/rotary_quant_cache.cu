@@ -10,7 +10,8 @@
 // reciprocal, corrected by its remainder, so that one that is a tie comes out as one; codes come out of its sum with 1.5 * 2^52, which has
 // them in its low bits.
 //
-// Bound by HBM: every element is read once and written once.
+// HBM bounds it (28 us for 8192 tokens, 32 + 8 heads of 128) less than its instructions do: 44.5 us, of which 30 without the rows that are
+// quantized, each 8 lanes' work of some 400 instructions in 64 bits for keys and 250 for values.
 #include "rotary_axes.cuh"
 
 namespace qmm {
@@ -22,10 +23,14 @@ struct QuantParams {
     int64_t ks_sb, ks_st, ks_sh, vs_sb, vs_st, vs_sh;
 };
 
-// The cosine and sine of a token's pair in 64 bits.
-__device__ __forceinline__ void make_turn_64(const RotaryParams &p, int64_t token, int pair, double *c, double *s) {
+// The cosine and sine of a token's pair, in 32 bits as make_turn has them, and in 64.  For these the half turns are made of two
+// numbers: the product with 1 / pi in 64 bits, and what it was rounded by together with the next 53 bits of 1 / pi.
+__device__ __forceinline__ void make_turns(const RotaryParams &p, int64_t token, int pair, float *c, float *s, double *c64, double *s64) {
     const int64_t place = load_index(p.positions, axis_of(p, pair) * p.pos_sa + token * p.pos_st, p.wide_positions);
-    sincos(static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + pair)), s, c);
+    const double angle = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + pair));
+    const double half_turns = angle * 0.31830988618379067154, rest = half_turns - 2.0 * rint(0.5 * half_turns);
+    sincospif(static_cast<float>(rest), s, c);
+    sincospi(rest + fma(angle, -1.9678676675182486e-17, fma(angle, 0.31830988618379067154, -half_turns)), s64, c64);
 }
 
 __device__ __forceinline__ double turned_first_64(double a, double b, double c, double s) { return fma(a, c, -(b * s)); }
@@ -39,6 +44,7 @@ __device__ __forceinline__ unsigned long long magnitude(double x) {
 struct RowScale {
     float scale;
     double inverse;  // 0: all codes are 0
+    double rest;     // of the inverse, beyond its 53 bits (of usual scales)
 };
 // From the largest magnitudes of the lanes of a row: `lanes` of them, a power of two.
 __device__ __forceinline__ RowScale make_scale(unsigned long long most, int lanes, uint32_t mask) {
@@ -46,6 +52,19 @@ __device__ __forceinline__ RowScale make_scale(unsigned long long most, int lane
     RowScale r;
     r.scale = static_cast<float>(__longlong_as_double(static_cast<long long>(most)) / 127.0);
     r.inverse = r.scale > 0.0f && r.scale <= 3.402823466e38f ? 1.0 / static_cast<double>(r.scale) : 0.0;
+    return r;
+}
+// From a row's largest magnitude, for scales that are neither near 0 nor very large (usual): the same by products.
+__device__ __forceinline__ bool is_usual(float most) { return most >= 0x1p-90f && most <= 0x1p90f; }
+__device__ __forceinline__ RowScale usual_scale(double most) {
+    const double about = most * (1.0 / 127.0);
+    RowScale r;
+    r.scale = static_cast<float>(fma(fma(-about, 127.0, most), 1.0 / 127.0, about));
+    const double scale = static_cast<double>(r.scale);
+    double inverse = static_cast<double>(__frcp_rn(r.scale));
+    inverse = fma(fma(-scale, inverse, 1.0), inverse, inverse);
+    r.inverse = fma(fma(-scale, inverse, 1.0), inverse, inverse);
+    r.rest = fma(-scale, r.inverse, 1.0) * r.inverse;
     return r;
 }
 
@@ -63,10 +82,7 @@ __global__ void __launch_bounds__(kThreads) rotary_quant_kernel(const __grid_con
     pdl_launch_dependents();
     pdl_wait();
     const int64_t token = blockIdx.x;
-    for (int i = threadIdx.x; i < p.pairs; i += kThreads) {
-        make_turn(p, token, i, s_cos + i, s_sin + i);
-        make_turn_64(p, token, i, s_cos64 + i, s_sin64 + i);
-    }
+    for (int i = threadIdx.x; i < p.pairs; i += kThreads) make_turns(p, token, i, s_cos + i, s_sin + i, s_cos64 + i, s_sin64 + i);
     __syncthreads();
     for (int item = threadIdx.x; item < p.heads * p.dim; item += kThreads) {
         const int row = item / p.dim, e = item - row * p.dim;
@@ -128,9 +144,28 @@ struct Eight {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
     __device__ __forceinline__ void store(T *dst) const {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(dst)[i] = w[i];
+    }
+    // The largest magnitude, as the bits of a float: magnitudes have the order of whole numbers.
+    __device__ __forceinline__ uint32_t largest() const {
+        const uint32_t *x = reinterpret_cast<const uint32_t *>(w);
+        uint32_t m = 0;
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) m = max(m, x[i] & 0x7fffffffu);
+            return m;
+        }
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) m = __vmaxu2(m, x[i] & 0x7fff7fffu);
+        m = max(m & 0xffffu, m >> 16);
+        const unsigned short one = static_cast<unsigned short>(m);
+        return __float_as_uint(to_float(*reinterpret_cast<const T *>(&one)));
     }
     __device__ __forceinline__ void unpack(float (&f)[8]) const {
         const T *x = reinterpret_cast<const T *>(w);
@@ -144,164 +179,245 @@ struct Eight {
     }
 };
 
-__device__ __forceinline__ uint2 codes_of(const double (&y)[8], const RowScale &r) {
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i >> 2] |= static_cast<uint32_t>(code_of(y[i], r) & 255) << 8 * (i & 3);
-    return make_uint2(w[0], w[1]);
-}
-
 // Vectors of eight elements.  A part of a row is, with halves, the vector of the first elements of its pairs and that of the second
 // ones, or one vector behind the pairs; interleaved, one vector.  2^log_lanes lanes of a warp, as many as parts or
-// more, have a row, and find its maximum together.  The first kAhead rows of a lane are under way while the sines and cosines are made.
-constexpr int kAhead = 3;
-template <typename T, bool INTERLEAVED, int TOKENS>
+// more, have a row, and find its maximum together.
+template <bool INTERLEAVED>
+struct Parts {
+    int lanes, part, e0, e1, pair0;  // lanes of a row, the lane's part, where its vectors begin, and its pairs
+    bool active, turns, two;
+    uint32_t mask;  // the row's lanes in the warp
+    __device__ __forceinline__ Parts(const RotaryParams &p, int log_lanes) {
+        const int turning = INTERLEAVED ? 2 * p.pairs / 8 : p.pairs / 8;  // parts of a row that turn
+        lanes = 1 << log_lanes;
+        part = threadIdx.x & (lanes - 1);
+        active = part < (INTERLEAVED ? p.dim / 8 : turning + (p.dim - 2 * p.pairs) / 8);
+        turns = part < turning;
+        two = !INTERLEAVED && turns;
+        e0 = (INTERLEAVED || turns ? part : part + turning) * 8;
+        e1 = e0 + p.pairs;
+        pair0 = INTERLEAVED ? e0 / 2 : e0;
+        mask = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
+    }
+};
+template <typename T, bool INTERLEAVED>
+__device__ __forceinline__ void load_part(const Parts<INTERLEAVED> &parts, const T *src, Eight<T> &x, Eight<T> &y) {
+    x.clear();
+    y.clear();
+    if (parts.active) x.load(src + parts.e0);
+    if (parts.two) y.load(src + parts.e1);
+}
+// A query's part, turned (`turns`) by the cosines and sines of its pairs.
+template <typename T, bool INTERLEAVED>
+__device__ __forceinline__ void turn_part(const Parts<INTERLEAVED> &parts, Eight<T> &x, Eight<T> &y, const float *cosine, const float *sine, T *dst) {
+    if (parts.turns) {
+        float a[8], b[8];
+        x.unpack(a);
+        if (INTERLEAVED) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                b[j] = turned_first(a[j], a[j + 1], cosine[j / 2], sine[j / 2]);
+                b[j + 1] = turned_second(a[j], a[j + 1], cosine[j / 2], sine[j / 2]);
+            }
+            x.pack(b);
+        } else {
+            y.unpack(b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float one = a[j];
+                a[j] = turned_first(one, b[j], cosine[j], sine[j]);
+                b[j] = turned_second(one, b[j], cosine[j], sine[j]);
+            }
+            x.pack(a);
+            y.pack(b);
+        }
+    }
+    if (parts.active) x.store(dst + parts.e0);
+    if (parts.two) y.store(dst + parts.e1);
+}
+
+__device__ __forceinline__ uint32_t low_bytes(int a, int b, int c, int d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); }
+__device__ __forceinline__ uint2 codes_of(const double (&y)[8], const RowScale &r) {
+    int c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = code_of(y[i], r);
+    return make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
+}
+// The same for usual scales, which no quotient passes 127 with: the inverse has 106 bits, so that a tie comes out as one here too.
+__device__ __forceinline__ uint2 usual_codes_of(const double (&y)[8], const RowScale &r) {
+    int c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = __double2loint(fma(y[i], r.inverse, y[i] * r.rest) + 6755399441055744.0);
+    return make_uint2(low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7]));
+}
+
+// (fmax, which looks for NaN, is twice as many instructions)
+__device__ __forceinline__ double larger(double a, double b) { return b > a ? b : a; }
+
+// A part of a key's or a value's row, as it is written: the codes, and the scale by the first of the row's lanes.
+template <typename T, bool INTERLEAVED>
+__device__ __forceinline__ void quantize_part(const Eight<T> &x, const Eight<T> &y, const Parts<INTERLEAVED> &parts, bool key, const double *cosine,
+                                              const double *sine, int8_t *dst, float *scale_at) {
+    float f[8], g[8];
+    x.unpack(f);
+    y.unpack(g);
+    uint32_t bits = x.largest();  // in which NaN is above infinity
+    if (!INTERLEAVED) bits = max(bits, y.largest());
+    double a[8], b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        a[j] = static_cast<double>(f[j]);
+        b[j] = INTERLEAVED ? 0.0 : static_cast<double>(g[j]);
+    }
+    if (key && parts.turns) {
+#pragma unroll
+        for (int j = 0; j < 8; j += INTERLEAVED ? 2 : 1) {
+            const double c = cosine[INTERLEAVED ? j / 2 : j], s = sine[INTERLEAVED ? j / 2 : j], one = a[j], other = INTERLEAVED ? a[j + 1] : b[j];
+            a[j] = turned_first_64(one, other, c, s);
+            (INTERLEAVED ? a[j + 1] : b[j]) = turned_second_64(one, other, c, s);
+        }
+    }
+    double most = __uint_as_float(bits);
+    if (key) {
+        most = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = larger(most, fabs(a[j]));
+        if (!INTERLEAVED) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = larger(most, fabs(b[j]));
+        }
+    }
+    for (int o = parts.lanes >> 1; o > 0; o >>= 1) {
+        bits = max(bits, __shfl_xor_sync(parts.mask, bits, o));
+        most = larger(most, __shfl_xor_sync(parts.mask, most, o));
+    }
+    RowScale scale;
+    uint2 codes[2];
+    if (__builtin_expect(bits < 0x7f800000u && is_usual(static_cast<float>(most)), 1)) {
+        scale = usual_scale(most);
+        codes[0] = usual_codes_of(a, scale);
+        if (!INTERLEAVED) codes[1] = usual_codes_of(b, scale);
+    } else {
+        unsigned long long all = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) all = max(all, max(magnitude(a[j]), magnitude(b[j])));
+        scale = make_scale(all, parts.lanes, parts.mask);
+        codes[0] = codes_of(a, scale);
+        if (!INTERLEAVED) codes[1] = codes_of(b, scale);
+    }
+    if (parts.active) *reinterpret_cast<uint2 *>(dst + parts.e0) = codes[0];
+    if (parts.two) *reinterpret_cast<uint2 *>(dst + parts.e1) = codes[1];
+    if (parts.part == 0) *scale_at = scale.scale;
+}
+
+// Few tokens: a CTA a token.  A lane's first rows of the query and the first one that is quantized are under way while the sines and cosines are made.
+template <typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
+rotary_quant_cta_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ QuantParams out, int log_lanes) {
+    __shared__ __align__(16) float s_cos[kMostPairs], s_sin[kMostPairs];
+    __shared__ __align__(16) double s_cos64[kMostPairs], s_sin64[kMostPairs];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t token = blockIdx.x;
+    const Parts<INTERLEAVED> parts(p, log_lanes);
+    const int row0 = threadIdx.x >> log_lanes, step = kThreads >> log_lanes;
+    const T *q = static_cast<const T *>(p.q) + token * p.q_st;
+    // of the rows that are quantized: the keys, then the values
+    auto kept = [&](int row) {
+        return row < p.kv_heads ? static_cast<const T *>(p.k) + token * p.k_st + row * p.k_sh : static_cast<const T *>(p.v) + token * p.v_st + (row - p.kv_heads) * p.v_sh;
+    };
+    Eight<T> x, y, kept_x, kept_y;
+    if (row0 < p.heads) load_part(parts, q + row0 * p.q_sh, x, y);
+    if (row0 < 2 * p.kv_heads) load_part(parts, kept(row0), kept_x, kept_y);
+    int64_t block = 0, at = 0;
+    const bool write = find_slot(p, token, &block, &at);
+    for (int i = threadIdx.x; i < p.pairs; i += kThreads) make_turns(p, token, i, s_cos + i, s_sin + i, s_cos64 + i, s_sin64 + i);
+    __syncthreads();
+    for (int row = row0; row < p.heads; row += step) {
+        if (row != row0) load_part(parts, q + row * p.q_sh, x, y);
+        turn_part(parts, x, y, s_cos + parts.pair0, s_sin + parts.pair0, static_cast<T *>(p.q_out) + (token * p.heads + row) * p.dim);
+    }
+    if (!write) return;
+    for (int row = row0; row < 2 * p.kv_heads; row += step) {
+        if (row != row0) load_part(parts, kept(row), kept_x, kept_y);
+        const bool key = row < p.kv_heads;
+        const int head = key ? row : row - p.kv_heads;
+        int8_t *dst = key ? static_cast<int8_t *>(p.k_cache) + block * p.kc_sb + at * p.kc_st + head * p.kc_sh
+                          : static_cast<int8_t *>(p.v_cache) + block * p.vc_sb + at * p.vc_st + head * p.vc_sh;
+        float *scale = key ? out.k_scale + block * out.ks_sb + at * out.ks_st + head * out.ks_sh
+                           : out.v_scale + block * out.vs_sb + at * out.vs_st + head * out.vs_sh;
+        quantize_part<T, INTERLEAVED>(kept_x, kept_y, parts, key, s_cos64 + parts.pair0, s_sin64 + parts.pair0, dst, scale);
+    }
+}
+
+// TOKENS a CTA: two where there are enough (8192 tokens, 32 + 8 heads of 128, bf16: one token 59 us, two 44.5, three 51; a warp a token, without
+// a barrier, 50).  The first row of the query for each token and the first one that is quantized are under way while the sines and
+// cosines are made.  Four CTAs an SM for two tokens (three: 47.5); few tokens need no more than one (64 registers cost 64 tokens 0.3 of 3.4 us).
+template <typename T, bool INTERLEAVED, int TOKENS>
+__global__ void __launch_bounds__(kThreads, TOKENS == 1 ? 1 : 4)
 rotary_quant_vec_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ QuantParams out, int64_t tokens, int log_lanes) {
     __shared__ __align__(16) float s_cos[TOKENS][kMostPairs], s_sin[TOKENS][kMostPairs];
     __shared__ __align__(16) double s_cos64[TOKENS][kMostPairs], s_sin64[TOKENS][kMostPairs];
-    __shared__ int64_t s_block[TOKENS], s_at[TOKENS];  // where a token goes in the cache; block < 0: nowhere
+    // where a token's keys and values go in the cache (null: nowhere), and their scales
+    __shared__ int8_t *s_codes[TOKENS][2];
+    __shared__ float *s_scales[TOKENS][2];
     pdl_launch_dependents();
     pdl_wait();
     const int64_t token0 = static_cast<int64_t>(blockIdx.x) * TOKENS;
     const int here = static_cast<int>(min(static_cast<int64_t>(TOKENS), tokens - token0));
-    const int turning = INTERLEAVED ? 2 * p.pairs / 8 : p.pairs / 8;  // parts of a row that turn
-    const int parts = INTERLEAVED ? p.dim / 8 : turning + (p.dim - 2 * p.pairs) / 8;
-    const int rows = p.heads + 2 * p.kv_heads;  // of a token
-    const int all = rows * here << log_lanes;
-    const int lanes = 1 << log_lanes;
-    const int part = threadIdx.x & (lanes - 1);  // the same in every row
-    const bool active = part < parts, turns = part < turning, two = !INTERLEAVED && turns;
-    const int e0 = (INTERLEAVED || turns ? part : part + turning) * 8, e1 = e0 + p.pairs;  // first vector, second one
-    const uint32_t mask = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
-    struct Spot {
-        int token, row;
+    const Parts<INTERLEAVED> parts(p, log_lanes);
+    const int row0 = threadIdx.x >> log_lanes, step = kThreads >> log_lanes;
+    Eight<T> x[TOKENS], y[TOKENS], kept_x, kept_y;
+    const T *q = static_cast<const T *>(p.q) + token0 * p.q_st + row0 * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i)
+        if (i < here && row0 < p.heads) load_part(parts, q + i * p.q_st, x[i], y[i]);
+    const int kept = 2 * p.kv_heads;
+    // rows that are quantized: of each token its keys, then its values
+    auto kept_row = [&](int token, int head) {
+        return head < p.kv_heads ? static_cast<const T *>(p.k) + (token0 + token) * p.k_st + head * p.k_sh : static_cast<const T *>(p.v) + (token0 + token) * p.v_st + (head - p.kv_heads) * p.v_sh;
     };
-    auto spot_of = [&](int item) {
-        Spot s;
-        const int row = item >> log_lanes;
-        s.token = 0;
+    auto token_of = [&](int row) {
+        int token = 0;
 #pragma unroll
-        for (int i = 1; i < TOKENS; ++i) s.token += row >= i * rows;
-        s.row = row - s.token * rows;
-        return s;
+        for (int i = 1; i < TOKENS; ++i) token += row >= i * kept;
+        return token;
     };
-    bool made = false;
-    for (int item0 = threadIdx.x; !made || item0 < all; item0 += kAhead * kThreads) {
-        Eight<T> x[kAhead], y[kAhead];
+    if (row0 < kept * here) load_part(parts, kept_row(token_of(row0), row0 - token_of(row0) * kept), kept_x, kept_y);
+    if (threadIdx.x < here) {
+        int64_t block = 0, at = 0;
+        const bool some = find_slot(p, token0 + threadIdx.x, &block, &at);
+        s_codes[threadIdx.x][0] = some ? static_cast<int8_t *>(p.k_cache) + block * p.kc_sb + at * p.kc_st : nullptr;
+        s_codes[threadIdx.x][1] = static_cast<int8_t *>(p.v_cache) + block * p.vc_sb + at * p.vc_st;
+        s_scales[threadIdx.x][0] = out.k_scale + block * out.ks_sb + at * out.ks_st;
+        s_scales[threadIdx.x][1] = out.v_scale + block * out.vs_sb + at * out.vs_st;
+    }
+    for (int i = threadIdx.x; i < p.pairs * here; i += kThreads) {
+        const int token = i / p.pairs, pair = i - token * p.pairs;
+        make_turns(p, token0 + token, pair, &s_cos[token][pair], &s_sin[token][pair], &s_cos64[token][pair], &s_sin64[token][pair]);
+    }
+    __syncthreads();
+    for (int row = row0; row < p.heads; row += step) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (item0 + i * kThreads >= all) break;
-            const Spot at = spot_of(item0 + i * kThreads);
-            const int64_t token = token0 + at.token;
-            const T *src = at.row < p.heads                ? static_cast<const T *>(p.q) + token * p.q_st + at.row * p.q_sh
-                           : at.row < p.heads + p.kv_heads ? static_cast<const T *>(p.k) + token * p.k_st + (at.row - p.heads) * p.k_sh
-                                                           : static_cast<const T *>(p.v) + token * p.v_st + (at.row - p.heads - p.kv_heads) * p.v_sh;
-            if (active) x[i].load(src + e0);
-            if (two) y[i].load(src + e1);
-        }
-        if (!made) {
-            if (threadIdx.x < here) {
-                int64_t block = -1, at = 0;
-                if (!find_slot(p, token0 + threadIdx.x, &block, &at)) block = -1;
-                s_block[threadIdx.x] = block;
-                s_at[threadIdx.x] = at;
-            }
-            for (int i = threadIdx.x; i < p.pairs * here; i += kThreads) {
-                const int token = i / p.pairs, pair = i - token * p.pairs;
-                make_turn(p, token0 + token, pair, &s_cos[token][pair], &s_sin[token][pair]);
-                make_turn_64(p, token0 + token, pair, &s_cos64[token][pair], &s_sin64[token][pair]);
-            }
-            __syncthreads();
-            made = true;
+        for (int i = 0; i < TOKENS; ++i) {
+            if (i >= here) break;
+            if (row != row0) load_part(parts, q + i * p.q_st, x[i], y[i]);
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (item0 + i * kThreads >= all) break;
-            const Spot at = spot_of(item0 + i * kThreads);
-            if (at.row < p.heads) {
-                if (!active) continue;
-                T *dst = static_cast<T *>(p.q_out) + ((token0 + at.token) * p.heads + at.row) * p.dim;
-                if (turns) {
-                    const float *cosine = s_cos[at.token], *sine = s_sin[at.token];
-                    float a[8], b[8];
-                    x[i].unpack(a);
-                    if (INTERLEAVED) {
-#pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            const float c = cosine[(e0 + j) >> 1], s = sine[(e0 + j) >> 1];
-                            b[j] = turned_first(a[j], a[j + 1], c, s);
-                            b[j + 1] = turned_second(a[j], a[j + 1], c, s);
-                        }
-                        x[i].pack(b);
-                    } else {
-                        y[i].unpack(b);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float c = cosine[e0 + j], s = sine[e0 + j], first = a[j];
-                            a[j] = turned_first(first, b[j], c, s);
-                            b[j] = turned_second(first, b[j], c, s);
-                        }
-                        x[i].pack(a);
-                        y[i].pack(b);
-                    }
-                }
-                x[i].store(dst + e0);
-                if (two) y[i].store(dst + e1);
-                continue;
-            }
-            const int64_t block = s_block[at.token], place = s_at[at.token];
-            if (block < 0) continue;
-            const bool key = at.row < p.heads + p.kv_heads;
-            const int head = at.row - p.heads - (key ? 0 : p.kv_heads);
-            double a[8], b[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.0;
-            if (active) {
-                float f[8];
-                x[i].unpack(f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) a[j] = static_cast<double>(f[j]);
-            }
-            if (two) {
-                float f[8];
-                y[i].unpack(f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) b[j] = static_cast<double>(f[j]);
-            }
-            if (key && turns) {
-                const double *cosine = s_cos64[at.token], *sine = s_sin64[at.token];
-                if (INTERLEAVED) {
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        const double c = cosine[(e0 + j) >> 1], s = sine[(e0 + j) >> 1], first = a[j];
-                        a[j] = turned_first_64(first, a[j + 1], c, s);
-                        a[j + 1] = turned_second_64(first, a[j + 1], c, s);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const double c = cosine[e0 + j], s = sine[e0 + j], first = a[j];
-                        a[j] = turned_first_64(first, b[j], c, s);
-                        b[j] = turned_second_64(first, b[j], c, s);
-                    }
-                }
-            }
-            unsigned long long most = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = max(most, max(magnitude(a[j]), magnitude(b[j])));
-            const RowScale scale = make_scale(most, lanes, mask);
-            int8_t *dst = key ? static_cast<int8_t *>(p.k_cache) + block * p.kc_sb + place * p.kc_st + head * p.kc_sh
-                              : static_cast<int8_t *>(p.v_cache) + block * p.vc_sb + place * p.vc_st + head * p.vc_sh;
-            if (active) *reinterpret_cast<uint2 *>(dst + e0) = codes_of(a, scale);
-            if (two) *reinterpret_cast<uint2 *>(dst + e1) = codes_of(b, scale);
-            if (part == 0) {
-                if (key)
-                    out.k_scale[block * out.ks_sb + place * out.ks_st + head * out.ks_sh] = scale.scale;
-                else
-                    out.v_scale[block * out.vs_sb + place * out.vs_st + head * out.vs_sh] = scale.scale;
-            }
+        for (int i = 0; i < TOKENS; ++i) {
+            if (i >= here) break;
+            turn_part(parts, x[i], y[i], s_cos[i] + parts.pair0, s_sin[i] + parts.pair0, static_cast<T *>(p.q_out) + ((token0 + i) * p.heads + row) * p.dim);
         }
+        q += step * p.q_sh;
+    }
+    for (int row = row0; row < kept * here; row += step) {
+        const int token = token_of(row), at = row - token * kept;
+        if (row != row0) load_part(parts, kept_row(token, at), kept_x, kept_y);
+        if (s_codes[token][0] == nullptr) continue;
+        const bool key = at < p.kv_heads;
+        const int head = key ? at : at - p.kv_heads;
+        quantize_part<T, INTERLEAVED>(kept_x, kept_y, parts, key, s_cos64[token] + parts.pair0, s_sin64[token] + parts.pair0,
+                                      s_codes[token][!key] + head * (key ? p.kc_sh : p.vc_sh), s_scales[token][!key] + head * (key ? out.ks_sh : out.vs_sh));
     }
 }
 
@@ -329,8 +445,7 @@ int launch_quant(const RotaryParams &p, const QuantParams &out, int64_t tokens, 
     const bool many = tokens >= 2ll * kTokens * sm_count();
     auto kern = p.interleaved ? (many ? rotary_quant_vec_kernel<T, true, kTokens> : rotary_quant_vec_kernel<T, true, 1>)
                               : (many ? rotary_quant_vec_kernel<T, false, kTokens> : rotary_quant_vec_kernel<T, false, 1>);
-    QMM_CUDA_OK(launch_pdl(kern, many ? dim3(static_cast<unsigned>((tokens + kTokens - 1) / kTokens)) : grid, dim3(kThreads), 0, stream, p, out, tokens,
-                           log_lanes));
+    QMM_CUDA_OK(launch_pdl(kern, many ? dim3(static_cast<unsigned>((tokens + kTokens - 1) / kTokens)) : grid, dim3(kThreads), 0, stream, p, out, tokens, log_lanes));
     return QMM_OK;
 }
 
