@@ -111,7 +111,7 @@ int qmm_paged_quant_attention_workspace_size(int64_t batch, int64_t heads, int64
     QMM_REQUIRE(bytes != nullptr, "qmm_paged_quant_attention_workspace_size: no result given");
     QMM_REQUIRE(batch >= 0 && heads >= 0 && kv_heads >= 1 && dim >= 0 && max_places >= 0,
                 "qmm_paged_quant_attention_workspace_size: sizes must be non-negative");
-    *bytes = qmm::paged::quant_decode_workspace(batch, heads, kv_heads, dim, max_places);
+    *bytes = qmm::paged::quant_decode_workspace(batch, heads, kv_heads, dim);
     return QMM_OK;
 }
 

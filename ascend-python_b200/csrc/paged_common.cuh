@@ -213,7 +213,7 @@ __device__ __forceinline__ void empty_row(const Problem &p, int64_t token, int h
 
 size_t decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
 int launch_decode(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
-size_t quant_decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places);
+size_t quant_decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim);
 int launch_quant_decode(const Problem &p, const QuantScales &scales, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 size_t prompt_workspace(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places);
 int launch_prompt(const Problem &p, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream);

@@ -26,8 +26,8 @@
 // the end of a piece).  So a box of TMA, a look-up of a page and the mask of what is seen serve four warps: by each warp for itself they were 340 of
 // 890 instructions on 32 keys (98 us).  The work of a call is the list of all (sequence, heads, tile of places), cut into equal contiguous ranges for
 // the CTAs, wherever sequences begin and end.  Of what is cut a CTA leaves its sums in the workspace, and a second kernel adds them in
-// their order.  Where every sequence is short and heads are few, CTAs have whole ones in turn.  Nothing depends on timing, and
-// nothing has to be zero before a call.
+// their order.  (CTAs that have whole heads of short sequences in turn, without that kernel: one of 200 places 10.0 us, this way 7.8.)  Nothing depends
+// on timing, and nothing has to be zero before a call.
 #include "paged_decode.cuh"
 
 namespace qmm {
@@ -48,17 +48,18 @@ constexpr float kSlack = 3.0f;  // how far, in powers of two, scores may pass th
 template <int DP, int NT>
 struct Shape {
     static constexpr int kKeys = kTileBytes / DP;  // of a warp's tile
-    static constexpr bool kKept = NT * DP < 512;   // the query in registers, else as operands in shared memory
-    static constexpr int kCtas = kKept ? 2 : 1;  // an SM
+    // The query in registers, else as operands in shared memory (32 sequences of 500 to 8000 places, 8/4 heads of 256: in registers 54 us, else 46; 128/8 of
+    // 128: 117 and 71).
+    static constexpr bool kKept = NT == 1 && DP < 256;
+    static constexpr int kCtas = NT * DP < 512 ? 2 : 1;  // an SM
     static constexpr int kStage = kWarps * 2 * (kTileBytes + kKeys * 4);    // keys, values, and their scales
     static constexpr int kSums = 8 * NT * DP * 4 + NT * 64;                 // what a warp hands to another
     static constexpr int kOperands = kKept ? 0 : kWarps * 8 * NT * DP * kDigits;
 };
 
-// How the work is dealt out: 2^log_heads key-value heads and 2^log_parts parts of a tile's places to the four warps; whole: CTAs
-// have whole head tiles in turn.  A cache comes in boxes of `rows` places of a page (TMA), or where rows is 0, row by row (cp.async).
+// How the work is dealt out: 2^log_heads key-value heads and 2^log_parts parts of a tile's places to the four warps.  A cache comes in boxes of `rows` places of a page (TMA), or where rows is 0, row by row (cp.async).
 struct Deal {
-    int log_heads, log_parts, whole, rows, stages;
+    int log_heads, log_parts, rows, stages;
     int scale_vectors;  // four places' scales lie together, at 16-byte boundaries
     uint32_t *status;  // the device status word
 };
@@ -72,7 +73,7 @@ struct QuantPlan {
 // Groups of up to 8 heads take one column tile.
 bool is_narrow(int64_t heads, int64_t kv_heads) { return heads <= 8 * kv_heads; }
 
-QuantPlan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places) {
+QuantPlan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
     QuantPlan q;
     const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
     const int ctas = is_narrow(heads, kv_heads) ? (dim > 128 ? Shape<256, 1>::kCtas : Shape<128, 1>::kCtas)
@@ -82,8 +83,7 @@ QuantPlan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim,
     plan.rows = static_cast<int>(group < kRows ? group : kRows);
     plan.tiles = static_cast<int>((group + kRows - 1) / kRows);
     plan.items = batch * kv_heads * plan.tiles;
-    q.deal.whole = places <= kShort && plan.items <= 2 * q.ctas;
-    q.deal.log_heads = q.deal.whole || kv_heads % 2 != 0 ? 0 : kv_heads % 4 != 0 ? 1 : 2;
+    q.deal.log_heads = kv_heads % 2 != 0 ? 0 : kv_heads % 4 != 0 ? 1 : 2;
     q.deal.log_parts = 2 - q.deal.log_heads;
     q.deal.rows = q.deal.stages = q.deal.scale_vectors = 0;
     q.deal.status = nullptr;
@@ -184,24 +184,12 @@ __device__ __forceinline__ Sequence sequence_of(const Problem &p, int b, int log
 
 // A CTA's share of the list of all (sequence, item, tile): an item is a head tile of 2^log_heads key-value heads.
 struct Share {
-    int items, log_keys, whole;
+    int items, log_keys;
     int64_t end, range;
 };
 
 // Steps to the CTA's next piece; false: there is none.
 __device__ __forceinline__ bool next_piece(const Problem &p, const Share &share, Piece &piece) {
-    if (share.whole) {
-        do {
-            piece.at += gridDim.x;
-            if (piece.at >= share.end) return false;
-            piece.b = static_cast<int>(piece.at / share.items);
-            piece.item = static_cast<int>(piece.at - static_cast<int64_t>(piece.b) * share.items);
-            piece.s = sequence_of(p, piece.b, share.log_keys);
-        } while (piece.s.tiles == 0);
-        piece.from = 0;
-        piece.to = piece.s.tiles;
-        return true;
-    }
     piece.at += piece.to - piece.from;
     if (piece.at >= share.end) return false;
     if (++piece.item == share.items) {
@@ -221,7 +209,6 @@ __device__ __forceinline__ bool first_piece(const Problem &p, const Scratch &scr
     const int lane = threadIdx.x & 31, worker = blockIdx.x, ctas = gridDim.x;
     share.items = (p.kv_heads >> deal.log_heads) * tiles;
     share.log_keys = log_keys;
-    share.whole = deal.whole;
     int64_t total = 0;
     int last_n = 0;  // tiles of sequence `lane`, of up to 32
     for (int b = lane; b < p.batch; b += 32) {
@@ -262,11 +249,6 @@ __device__ __forceinline__ bool first_piece(const Problem &p, const Scratch &scr
         found = true;
         piece.b = b0 + __ffs(past) - 1;
         before += __shfl_sync(0xffffffffu, sum - mine, __ffs(past) - 1);
-    }
-    if (deal.whole) {
-        share.end = static_cast<int64_t>(p.batch) * share.items;
-        piece.at = worker - ctas;
-        return next_piece(p, share, piece);
     }
     if (!found) return false;
     piece.s = sequence_of(p, piece.b, log_keys);
@@ -456,7 +438,7 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
         const float scale = factor == 0.0f ? 1.0f : fabsf(factor), sign = factor == 0.0f ? 0.0f : factor < 0.0f ? -1.0f : 1.0f;
         // the index of the CTA's head among all, for the parts and the cut items
         const int64_t worker = static_cast<int64_t>(head) * gridDim.x + blockIdx.x;
-        if (!deal.whole && !scratch.by_item && part == 0 && lane == 0) scratch.cut[worker] = make_int4(-1, 0, 0, 0);
+        if (!scratch.by_item && part == 0 && lane == 0) scratch.cut[worker] = make_int4(-1, 0, 0, 0);
 
         // A lane's place in an operand: row (or column) lane / 4, elements 2 * (lane % 4) and the next.  Of a product's sums it has rows
         // lane / 4 and 8 more, columns c0 and c0 + 1.
@@ -850,7 +832,7 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
                         }
                     }
                 }
-                if (lane == 0 && begins && !deal.whole && (!ends || scratch.by_item)) {
+                if (lane == 0 && begins && (!ends || scratch.by_item)) {
                     const int item = kvh * tiles + head_tile;
                     const int64_t last = (piece.at - piece.from + piece.s.tiles - 1) / share.range;  // the CTA that has the item's last tile
                     scratch.cut[scratch.by_item ? static_cast<int64_t>(piece.b) * p.kv_heads * tiles + item : worker] =
@@ -863,6 +845,96 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
     }
     __syncthreads();
     if (threadIdx.x == 0 && control->abort != 0) *deal.status = control->abort;
+}
+
+// Adds the parts of the head tiles that are cut, in the order of the CTAs: a warp, or with `share` the CTA's warps together, a row.  Statistics and
+// sums of kAtOnce parts are under way together.  DP: 128 or 256.
+constexpr int kJoinWarps = 8, kShareWarps = 16;
+template <typename T, int DP>
+__global__ void __launch_bounds__(kShareWarps * 32)
+quant_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, int64_t indices, bool share) {
+    __shared__ __align__(16) float s_sum[kShareWarps][DP];
+    __shared__ float2 s_stat[kShareWarps];
+    constexpr int kAtOnce = 1024 / DP;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
+    const int64_t at = share ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp, index = at / scratch.rows;
+    const int row = static_cast<int>(at - index * scratch.rows);
+    if (index >= indices) return;
+    const int4 cut = scratch.cut[index];
+    if (cut.x < 0) return;
+    const int tiles = (p.group + kRows - 1) / kRows;
+    const int kvh = cut.w / tiles, tile = cut.w - kvh * tiles;
+    if (row >= min(kRows, p.group - tile * kRows)) return;
+    const int parts = cut.y - cut.x + 1;
+    const int from = share ? parts * warp / kShareWarps : 0, to = share ? parts * (warp + 1) / kShareWarps : parts;
+    auto place = [&](int i) { return (scratch.cta_parts + static_cast<int64_t>(cut.x + i) * 2 + (i == 0)) * scratch.rows + row; };
+    float top = -INFINITY, sum = 0.0f, acc[8] = {};
+    for (int i0 = from; i0 < to; i0 += kAtOnce) {
+        float2 stat[kAtOnce];
+        float4 v[kAtOnce][2];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            stat[i] = make_float2(-INFINITY, 0.0f);
+            v[i][0] = v[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i0 + i >= to) continue;
+            stat[i] = __ldcg(scratch.stat + place(i0 + i));
+            const float *src = scratch.part + place(i0 + i) * p.dim + lane * 4;
+#pragma unroll
+            for (int c = 0; c < DP / 128; ++c)
+                if (c * 128 + lane * 4 < p.dim) v[i][c] = __ldcg(reinterpret_cast<const float4 *>(src + c * 128));
+        }
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) now = fmaxf(now, stat[i].x);
+        const float base = now == -INFINITY ? 0.0f : now, keep = exp2_fast(top - base);
+        sum *= keep;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] *= keep;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const float w = exp2_fast(stat[i].x - base);
+            sum = fmaf(stat[i].y, w, sum);
+#pragma unroll
+            for (int c = 0; c < DP / 128; ++c) {
+                acc[4 * c] = fmaf(v[i][c].x, w, acc[4 * c]);
+                acc[4 * c + 1] = fmaf(v[i][c].y, w, acc[4 * c + 1]);
+                acc[4 * c + 2] = fmaf(v[i][c].z, w, acc[4 * c + 2]);
+                acc[4 * c + 3] = fmaf(v[i][c].w, w, acc[4 * c + 3]);
+            }
+        }
+        top = now;
+    }
+    if (share) {
+#pragma unroll
+        for (int c = 0; c < DP / 128; ++c)
+            *reinterpret_cast<float4 *>(&s_sum[warp][c * 128 + lane * 4]) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+        if (lane == 0) s_stat[warp] = make_float2(top, sum);
+        __syncthreads();
+        if (warp != 0) return;
+        for (int w = 0; w < kShareWarps; ++w) top = fmaxf(top, s_stat[w].x);
+        const float all = top == -INFINITY ? 0.0f : top;
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+        for (int w = 0; w < kShareWarps; ++w) {
+            const float weight = exp2_fast(s_stat[w].x - all);
+            sum = fmaf(s_stat[w].y, weight, sum);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) acc[i] = fmaf(s_sum[w][(i >> 2) * 128 + lane * 4 + (i & 3)], weight, acc[i]);
+        }
+    }
+    const int64_t out = static_cast<int64_t>(cut.z) * p.heads + kvh * p.group + tile * kRows + row;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T *dst = static_cast<T *>(p.out) + out * p.dim;
+#pragma unroll
+    for (int c = 0; c < DP / 128; ++c) {
+        const int d = c * 128 + lane * 4;
+        if (d < p.dim)
+            *reinterpret_cast<uint2 *>(dst + d) = make_uint2(pack2<T>(acc[4 * c] * inv, acc[4 * c + 1] * inv), pack2<T>(acc[4 * c + 2] * inv, acc[4 * c + 3] * inv));
+    }
+    if (lane == 0) p.lse[out] = sum == 0.0f ? -INFINITY : top * kLn2 + logf(sum);
 }
 
 // A cache as TMA sees it: boxes of `rows` places of one page and `heads` heads by up to 128 columns (zeros behind the head dimension).  False: its
@@ -914,7 +986,13 @@ int launch(const Problem &p, const QuantScales &scales, const QuantPlan &plan, c
     const int64_t items = plan.plan.items >> plan.deal.log_heads;
     const bool far = seen > kNear && seen > kNear * plan.ctas / items;
     const int rc = far ? launch_decode_kernel<T, DP, NT, true>(p, scales, plan, scratch, stream) : launch_decode_kernel<T, DP, NT, false>(p, scales, plan, scratch, stream);
-    return rc != QMM_OK || plan.deal.whole ? rc : launch_join<T>(p, plan.plan, scratch, stream);
+    if (rc != QMM_OK) return rc;
+    // a CTA a row where rows are so few that each has many parts
+    const int64_t indices = scratch.by_item ? plan.plan.items : plan.plan.workers, all = indices * scratch.rows;
+    const bool share = all <= 2 * sm_count();
+    QMM_CUDA_OK(launch_pdl(quant_join_kernel<T, DP < 256 ? 128 : 256>, dim3(static_cast<unsigned>(share ? all : (all + kJoinWarps - 1) / kJoinWarps)), dim3((share ? kShareWarps : kJoinWarps) * 32), 0, stream, p,
+                           scratch, indices, share));
+    return QMM_OK;
 }
 
 template <typename T, int NT>
@@ -931,12 +1009,12 @@ int launch_t(const Problem &p, const QuantScales &scales, const QuantPlan &plan,
 
 }  // namespace
 
-size_t quant_decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t places) {
-    return batch == 0 || heads == 0 ? 0 : make_plan(batch, heads, kv_heads, dim, places).plan.bytes;
+size_t quant_decode_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
+    return batch == 0 || heads == 0 ? 0 : make_plan(batch, heads, kv_heads, dim).plan.bytes;
 }
 
 int launch_quant_decode(const Problem &p, const QuantScales &scales, int dtype, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
-    const QuantPlan plan = make_plan(p.batch, p.heads, p.kv_heads, p.dim, static_cast<int64_t>(p.max_pages) * p.page);
+    const QuantPlan plan = make_plan(p.batch, p.heads, p.kv_heads, p.dim);
     if (workspace_bytes < plan.plan.bytes || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
         return fail(QMM_ERR_WORKSPACE, "qmm_paged_quant_attention: needs a workspace of " + std::to_string(plan.plan.bytes) + " bytes, 16-byte aligned");
     const Scratch scratch = lay_out(plan.plan, workspace);
