@@ -25,11 +25,18 @@ static std::mutex g_mutex;
 static uint32_t *g_status_host = nullptr;
 static uint32_t *g_status_dev = nullptr;
 
+// The word is made by the first call that needs it, which may be one that a graph captures.  A capture that is not
+// relaxed forbids allocations to its thread (in its global mode, to every thread) and ends with an error at the first
+// one; this allocation belongs to no stream and stays, so it is made in the relaxed mode, whichever the thread has.
 uint32_t *device_status_word() {
     std::lock_guard<std::mutex> lock(g_mutex);
     if (g_status_dev == nullptr) {
         void *h = nullptr;
-        if (cudaHostAlloc(&h, 64, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool exchanged = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+        const cudaError_t made = cudaHostAlloc(&h, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+        if (exchanged) (void)cudaThreadExchangeStreamCaptureMode(&mode);
+        if (made != cudaSuccess) {
             (void)cudaGetLastError();
             return nullptr;
         }
