@@ -520,7 +520,7 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
                 for (int t = 0; t < NT; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.0f;
             }
             // top: what scores are relative to, within kSlack below the largest; ceiling: a score beyond it moves that; base: top times the row's
-            // scale; lift: the power of two of a head's weights; big: the largest of the lane's, so lifted
+            // scale; lift: the power of two of a head's weights; big: the lane's largest, not lifted
             float top[NT][2], ceiling[NT][2], base[NT][2], sum[NT][2], lift[NT][2], big[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -678,15 +678,15 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 float &x = s[m][t][2 * h + i];
-                                x *= by * lift[t][i];
+                                x *= by;
                                 big[t][i] = fmaxf(big[t][i], fabsf(x));
                             }
                         }
                     }
                 }
-                float largest = big[0][0];
+                float largest = 0.0f;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) largest = fmaxf(largest, fmaxf(big[t][0], big[t][1]));
+                for (int t = 0; t < NT; ++t) largest = fmaxf(largest, fmaxf(big[t][0] * lift[t][0], big[t][1] * lift[t][1]));
                 if (__builtin_expect(moves || __any_sync(0xffffffffu, largest > 60000.0f), 0)) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
@@ -696,20 +696,14 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 4));
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
                             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                            float more_lift = 1.0f;
-                            if (most > 60000.0f || (most < 256.0f && most > 0.0f)) {
-                                // to [2^11, 2^12), as far as lift stays finite
-                                const int e = 138 - static_cast<int>(__float_as_uint(most) >> 23);
+                            big[t][i] = most;
+                            const float lifted = most * lift[t][i];
+                            if (lifted > 60000.0f || (lifted < 256.0f && most > 0.0f)) {
+                                // to [2^11, 2^12), as far as lift and its step stay finite; sums that a step below 2^-126 leaves count no more
                                 const int has = static_cast<int>(__float_as_uint(lift[t][i]) >> 23) - 127;
-                                more_lift = __uint_as_float(static_cast<uint32_t>(127 + max(-126 - has, min(min(e, 127), 127 - has))) << 23);
-                            }
-                            lift[t][i] *= more_lift;
-                            big[t][i] = most * more_lift;
-                            keep[t][i] *= more_lift;
-#pragma unroll
-                            for (int m = 0; m < kTiles; ++m) {
-                                s[m][t][i] *= more_lift;
-                                s[m][t][i + 2] *= more_lift;
+                                const int e = max(-126, min(min(138 - static_cast<int>(__float_as_uint(most) >> 23), 127), 127 + has));
+                                lift[t][i] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                                keep[t][i] *= e - has < -126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + e - has) << 23);
                             }
 #pragma unroll
                             for (int n = 0; n < kSteps; ++n) {
@@ -725,7 +719,7 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
 #pragma unroll
                     for (int m = 0; m < kTiles; ++m) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) b[t][m][h] = transposed(pack2<__half>(s[m][t][2 * h], s[m][t][2 * h + 1]));
+                        for (int h = 0; h < 2; ++h) b[t][m][h] = transposed(pack2<__half>(s[m][t][2 * h] * lift[t][0], s[m][t][2 * h + 1] * lift[t][1]));
                     }
                 }
 #pragma unroll

@@ -139,6 +139,17 @@ def test_order_of_value_scales(npu, dev):
         check(npu, q, k, v, ks, vs, table, lens)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_values_far_above_those_before(npu, dev, dim):
+    """A power of two that suits values of 2^-104 would take weights of values of 2^16 beyond fp32; and the other way round."""
+    for small, large in ((range(0, 500), range(500, 900)), (range(500, 900), range(0, 500))):
+        q, k, v, ks, vs, table, lens = make(dev, [900], dim=dim, page=1024, heads=2, kv=1, spare=0, seed=20, dtype=torch.bfloat16)
+        vs[0, :, list(small)] = 2.0 ** -110
+        vs[0, :, list(large)] = 2.0 ** 10
+        # so many sequences, all of this page, that a CTA has whole ones
+        check(npu, q.repeat(400, 1, 1), k, v, ks, vs, table.repeat(400, 1), lens.repeat(400))
+
+
 def test_first_values_are_outweighed(npu, dev):
     """A key of a large value whose weight vanishes when the maximum moves; what counts lies 2^60 below it."""
     q, k, v, ks, vs, table, lens = make(dev, [300], dim=64, page=512, heads=1, kv=1, spare=0, seed=11)
