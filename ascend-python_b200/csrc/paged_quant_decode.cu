@@ -14,7 +14,7 @@
 // 0x64 (f16: 1024 + u), two subtract 1152.  Bytes of two keys that ldmatrix transposes together are rows of even and of odd dimensions,
 // so nothing is shuffled; the weights change from rows of keys to rows of heads by movmatrix.
 //
-// The weights, exp(score - base) * value scale, are multiplied by a power of two for each head that keeps the largest so far below
+// The weights, exp(score - base) * value scale, are multiplied, as they are rounded, by a power of two for each head that keeps the largest so far below
 // f16's largest number and above 2^8; it moves with the base, or when a weight would pass that.  Rounding a weight is half a step of
 // f16, 2^-11 of it, or 2^-33 of the largest one for those far below it.  The sum of the softmax takes them unrounded.  The base
 // follows the largest score only when that is 2^3 above it, so that sums are rescaled rarely.
@@ -28,6 +28,12 @@
 // the CTAs, wherever sequences begin and end.  Of what is cut a CTA leaves its sums in the workspace, and a second kernel adds them in
 // their order.  (CTAs that have whole heads of short sequences in turn, without that kernel: one of 200 places 10.0 us, this way 7.8.)  Nothing depends
 // on timing, and nothing has to be zero before a call.
+//
+// Measured (bf16, 64/8 heads of 128, 64 sequences of 500 to 8000 places; 364 MB, 55.6 us at the copy rate): 71.7 us, 66.9 of them without the second kernel, and
+// 63.8 for the copies with no products: memory, the start and the joining bound it.  Two CTAs an SM with three stages; three with two
+// 94 us, stages of keys and of values of their own 80.  One sequence of 131071 places, 32/8 heads: 51.6 us (0.82 of the copy rate).  Groups of 9
+// to 16 heads are bound by instructions on two column tiles (128/8 heads: 71 us, 0.41), pages whose size is no multiple of 8 by
+// copies row by row (5 places: 66 us, 28.6 at the copy rate).
 #include "paged_decode.cuh"
 
 namespace qmm {

@@ -478,12 +478,16 @@ QMM_API int qmm_rotary_axes_quant_cache(const void *query, int64_t query_stride_
 
 /*
  * qmm_paged_attention over an int8 cache (torch op `npu_paged_quant_attention`; no counterpart in the reference): keys and values are what codes and
- * scales stand for, all else is said there.  Scores, softmax and sums are fp32; query and weights enter the products in f16, the
- * weights times the values' scales and a power of two for each row (half a step, 2^-11, of each, or 2^-33 of the largest; a bf16
- * query is exact but for elements below 2^-21 of its row's largest, off by 2^-32 of that).
+ * scales stand for; sequences, masks, lse and workspace are as there.  An element of the query is taken as a whole number of at most 22 bits
+ * times a power of two of its row (off by 2^-22 of the row's largest at most), sums of its products with codes are exact; scales of
+ * keys, softmax and sums are fp32.  For the product with the values a weight times its value's scale is rounded to f16, after a power of two that its
+ * row has (half a step, 2^-11, of each, or 2^-33 of the largest); the sum that it is divided by takes the weight unrounded.
+ * A query's row that holds NaN or an infinity comes out as NaN; a scale that is not finite reaches the rows that see it, and no other.
+ * Scores are to be in fp32's range, and a row's largest |query| times |scale_value| * log2(e) 0 or at least 2^-104 (a smaller row counts as up to that).
+ * Of a page that holds a place that is seen, up to 31 places beside it may be read as well; whatever their codes and scales, the results are
+ * those of the places that are seen.
  * The head dimension is a multiple of 16 up to 256; caches begin at 16-byte boundaries, their strides are multiples of 16;
- * scales begin at 4-byte boundaries.  The largest |query| of a row times |scale_value| * log2(e), and 2^8 over it times a
- * key's row, are to be in fp32's range, as the scores are.
+ * scales begin at 4-byte boundaries.
  */
 QMM_API int qmm_paged_quant_attention_workspace_size(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_places,
                                                      size_t *bytes);
