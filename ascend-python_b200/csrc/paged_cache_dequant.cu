@@ -30,10 +30,11 @@ struct Copy {
     int batch, kv_heads, dim;
 };
 
-// Places [lo, hi) of sequence b are copied.
+// Places [lo, hi) of sequence b are copied; both are at most a capacity, 2^31 - 256, so that a step past them is below 2^31.
 __device__ __forceinline__ void places_of(const Copy &c, int b, int *lo, int *hi) {
-    *lo = c.first != nullptr ? max(0, __ldg(c.first + b)) : 0;
-    *hi = max(*lo, min(__ldg(c.lens + b), min(c.from.capacity, c.to.capacity)));
+    const int capacity = min(c.from.capacity, c.to.capacity);
+    *lo = c.first != nullptr ? min(max(0, __ldg(c.first + b)), capacity) : 0;
+    *hi = max(*lo, min(__ldg(c.lens + b), capacity));
 }
 
 __device__ __forceinline__ bool find_page(const Side &s, int b, int j, int64_t *block, int *at) {
@@ -231,7 +232,7 @@ extern "C" int qmm_paged_cache_dequant(const qmm_kv_cache *cache, const qmm_kv_s
     QMM_REQUIRE(batch >= 0 && max_pages >= 0 && out_max_pages >= 0 && cache->pages >= 0 && out->pages >= 0, name + ": sizes must be non-negative");
     QMM_REQUIRE(cache->page_size >= 1 && cache->page_size <= 0x7fffffff && out->page_size >= 1 && out->page_size <= 0x7fffffff,
                 name + ": the page sizes must be positive");
-    QMM_REQUIRE(batch < 0x7fffffff && max_pages <= 0x7fffffff && out_max_pages <= 0x7fffffff && cache->pages <= 0x7fffffff && out->pages <= 0x7fffffff,
+    QMM_REQUIRE(batch <= 0x7fffff00 && max_pages <= 0x7fffffff && out_max_pages <= 0x7fffffff && cache->pages <= 0x7fffffff && out->pages <= 0x7fffffff,
                 name + ": sizes out of range");
     QMM_REQUIRE(cache->kv_heads >= 1 && cache->kv_heads <= 65535 && cache->dim >= 1 && cache->dim <= 256,
                 name + ": between 1 and 65535 heads, of a dimension up to 256");

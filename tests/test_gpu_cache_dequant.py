@@ -81,6 +81,15 @@ def test_first_places(npu, dev):
     check(npu, *make(dev, [40, 40], seed=9), first=torch.tensor([2**31 - 1, -2**31], dtype=torch.int32, device=dev))
 
 
+def test_first_places_beyond_all_capacities(npu, dev):
+    """Empty sequences of the largest first places, crossed on the way from the one before to the one behind."""
+    args = make(dev, [3000, 100, 0, 3001, 50, 2999], kv=1, dim=16, seed=19)
+    check(npu, *args, first=torch.tensor([0, 2**31 - 1, 2**31 - 2, 1, 2**31 - 1, 0], dtype=torch.int32, device=dev))
+    args = make(dev, [3000, 100, 3001], kv=1, dim=16, seed=20)
+    args[5] = torch.full_like(args[5], 2**31 - 1)
+    check(npu, *args, first=torch.tensor([0, 2**31 - 1, 1], dtype=torch.int32, device=dev))
+
+
 def test_tables(npu, dev):
     """Lengths beyond either table, entries that name no page in either."""
     args = make(dev, [200, 300, 100], seed=10)
