@@ -310,46 +310,6 @@ __device__ __forceinline__ void quantize_part(const Eight<T> &x, const Eight<T> 
     if (parts.part == 0) *scale_at = scale.scale;
 }
 
-// Few tokens: a CTA a token.  A lane's first rows of the query and the first one that is quantized are under way while the sines and cosines are made.
-template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads)
-rotary_quant_cta_kernel(const __grid_constant__ RotaryParams p, const __grid_constant__ QuantParams out, int log_lanes) {
-    __shared__ __align__(16) float s_cos[kMostPairs], s_sin[kMostPairs];
-    __shared__ __align__(16) double s_cos64[kMostPairs], s_sin64[kMostPairs];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int64_t token = blockIdx.x;
-    const Parts<INTERLEAVED> parts(p, log_lanes);
-    const int row0 = threadIdx.x >> log_lanes, step = kThreads >> log_lanes;
-    const T *q = static_cast<const T *>(p.q) + token * p.q_st;
-    // of the rows that are quantized: the keys, then the values
-    auto kept = [&](int row) {
-        return row < p.kv_heads ? static_cast<const T *>(p.k) + token * p.k_st + row * p.k_sh : static_cast<const T *>(p.v) + token * p.v_st + (row - p.kv_heads) * p.v_sh;
-    };
-    Eight<T> x, y, kept_x, kept_y;
-    if (row0 < p.heads) load_part(parts, q + row0 * p.q_sh, x, y);
-    if (row0 < 2 * p.kv_heads) load_part(parts, kept(row0), kept_x, kept_y);
-    int64_t block = 0, at = 0;
-    const bool write = find_slot(p, token, &block, &at);
-    for (int i = threadIdx.x; i < p.pairs; i += kThreads) make_turns(p, token, i, s_cos + i, s_sin + i, s_cos64 + i, s_sin64 + i);
-    __syncthreads();
-    for (int row = row0; row < p.heads; row += step) {
-        if (row != row0) load_part(parts, q + row * p.q_sh, x, y);
-        turn_part(parts, x, y, s_cos + parts.pair0, s_sin + parts.pair0, static_cast<T *>(p.q_out) + (token * p.heads + row) * p.dim);
-    }
-    if (!write) return;
-    for (int row = row0; row < 2 * p.kv_heads; row += step) {
-        if (row != row0) load_part(parts, kept(row), kept_x, kept_y);
-        const bool key = row < p.kv_heads;
-        const int head = key ? row : row - p.kv_heads;
-        int8_t *dst = key ? static_cast<int8_t *>(p.k_cache) + block * p.kc_sb + at * p.kc_st + head * p.kc_sh
-                          : static_cast<int8_t *>(p.v_cache) + block * p.vc_sb + at * p.vc_st + head * p.vc_sh;
-        float *scale = key ? out.k_scale + block * out.ks_sb + at * out.ks_st + head * out.ks_sh
-                           : out.v_scale + block * out.vs_sb + at * out.vs_st + head * out.vs_sh;
-        quantize_part<T, INTERLEAVED>(kept_x, kept_y, parts, key, s_cos64 + parts.pair0, s_sin64 + parts.pair0, dst, scale);
-    }
-}
-
 // TOKENS a CTA: two where there are enough (8192 tokens, 32 + 8 heads of 128, bf16: one token 59 us, two 44.5, three 51; a warp a token, without
 // a barrier, 50).  The first row of the query for each token and the first one that is quantized are under way while the sines and
 // cosines are made.  Four CTAs an SM for two tokens (three: 47.5); few tokens need no more than one (64 registers cost 64 tokens 0.3 of 3.4 us).
