@@ -126,6 +126,7 @@ int qmm_paged_quant_attention(const void *query, int dtype, int64_t batch, int64
                                         scale_value, window, sinks, out, lse, 16);
     if (rc != QMM_OK) return rc;
     QMM_REQUIRE(scales != nullptr, "qmm_paged_quant_attention: no scales given");
+    QMM_REQUIRE(batch <= 0x7fffff00, "qmm_paged_quant_attention: sizes out of range");  // a warp counts sequences in steps of 32
     QMM_REQUIRE(qmm::paged::words(scales->key) && qmm::paged::words(scales->value), "qmm_paged_quant_attention: scales must begin at 4-byte boundaries");
     const qmm::paged::QuantScales s = {scales->key, scales->value, scales->key_stride_page, scales->key_stride_place, scales->key_stride_head,
                                        scales->value_stride_page, scales->value_stride_place, scales->value_stride_head};

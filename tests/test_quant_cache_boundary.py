@@ -233,3 +233,11 @@ def test_oracle_against_loops():
                                     first=torch.tensor([1, 0]))
     assert torch.equal(k_out[1, 2], k[2, 2].float() * ks[2, :, 2, None]) and torch.equal(v_out[0, 0], v[0, 1].float() * vs[0, :, 1, None])
     assert not k_out[1, 0].any() and bool((v_out[2, 3] == 1).all()) and torch.equal(k_out[2, 2], k[4, 2].float() * ks[4, :, 2, None])
+
+
+def test_batches_near_32_bits(capi):
+    """A warp's count of sequences goes up to 32 beyond the last one."""
+    for batch in (2**31 - 256 + 1, 2**31 - 2):
+        for call in (_attention, _read):
+            rc, message = call(capi, batch=batch)
+            assert rc == 1 and "out of range" in message
