@@ -29,7 +29,7 @@
 // their order.  (CTAs that have whole heads of short sequences in turn, without that kernel: one of 200 places 10.0 us, this way 7.8.)  Nothing depends
 // on timing, and nothing has to be zero before a call.
 //
-// Measured (bf16, 64/8 heads of 128, 64 sequences of 500 to 8000 places; 364 MB, 55.6 us at the copy rate): 71.7 us, 66.9 of them without the second kernel, and
+// Measured (bf16, 64/8 heads of 128, 64 sequences of 500 to 8000 places; 364 MB, 55.6 us at the copy rate): 70.6 us, 66.5 of them without the second kernel, and
 // 63.8 for the copies with no products: memory, the start and the joining bound it.  Two CTAs an SM with three stages; three with two
 // 94 us, stages of keys and of values of their own 80.  One sequence of 131071 places, 32/8 heads: 51.6 us (0.82 of the copy rate).  Groups of 9
 // to 16 heads are bound by instructions on two column tiles (128/8 heads: 71 us, 0.41), pages whose size is no multiple of 8 by
@@ -847,19 +847,20 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
     if (threadIdx.x == 0 && control->abort != 0) *deal.status = control->abort;
 }
 
-// Adds the parts of the head tiles that are cut, in the order of the CTAs: a warp, or with `share` the CTA's warps together, a row.  Statistics and
-// sums of kAtOnce parts are under way together.  DP: 128 or 256.
-constexpr int kJoinWarps = 8, kShareWarps = 16;
-template <typename T, int DP>
-__global__ void __launch_bounds__(kShareWarps * 32)
-quant_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, int64_t indices, bool share) {
-    __shared__ __align__(16) float s_sum[kShareWarps][DP];
-    __shared__ float2 s_stat[kShareWarps];
-    constexpr int kAtOnce = 1024 / DP;
+// Adds the parts of the head tiles that are cut, in the order of the CTAs: SHARE warps a row.  Statistics and sums of kAtOnce parts are under way
+// together.  DP: 128 or 256.
+template <int SHARE>
+constexpr int kJoinWarps = SHARE < 8 ? 8 : SHARE;  // of a CTA
+template <typename T, int DP, int SHARE>
+__global__ void __launch_bounds__(kJoinWarps<SHARE> * 32, SHARE == 8 ? 2 : 1)
+quant_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch scratch, int64_t indices) {
+    constexpr int kRowsOfCta = kJoinWarps<SHARE> / SHARE, kAtOnce = 1024 / DP;
+    __shared__ __align__(16) float s_sums[SHARE > 1 ? kRowsOfCta : 1][SHARE][DP];
+    __shared__ float2 s_stats[kRowsOfCta][SHARE];
     pdl_launch_dependents();
     pdl_wait();
-    const int warp = warp_id_uniform(), lane = threadIdx.x & 31;
-    const int64_t at = share ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kJoinWarps + warp, index = at / scratch.rows;
+    const int lane = threadIdx.x & 31, here = warp_id_uniform() / SHARE, warp = warp_id_uniform() % SHARE;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kRowsOfCta + here, index = at / scratch.rows;
     const int row = static_cast<int>(at - index * scratch.rows);
     if (index >= indices) return;
     const int4 cut = scratch.cut[index];
@@ -868,7 +869,7 @@ quant_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scr
     const int kvh = cut.w / tiles, tile = cut.w - kvh * tiles;
     if (row >= min(kRows, p.group - tile * kRows)) return;
     const int parts = cut.y - cut.x + 1;
-    const int from = share ? parts * warp / kShareWarps : 0, to = share ? parts * (warp + 1) / kShareWarps : parts;
+    const int from = parts * warp / SHARE, to = parts * (warp + 1) / SHARE;
     auto place = [&](int i) { return (scratch.cta_parts + static_cast<int64_t>(cut.x + i) * 2 + (i == 0)) * scratch.rows + row; };
     float top = -INFINITY, sum = 0.0f, acc[8] = {};
     for (int i0 = from; i0 < to; i0 += kAtOnce) {
@@ -906,19 +907,21 @@ quant_join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scr
         }
         top = now;
     }
-    if (share) {
+    if (SHARE > 1) {
+        auto &s_sum = s_sums[here];
+        auto &s_stat = s_stats[here];
 #pragma unroll
         for (int c = 0; c < DP / 128; ++c)
             *reinterpret_cast<float4 *>(&s_sum[warp][c * 128 + lane * 4]) = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
         if (lane == 0) s_stat[warp] = make_float2(top, sum);
-        __syncthreads();
+        asm volatile("bar.sync %0, %1;" ::"r"(here + 1), "n"(SHARE * 32) : "memory");  // the row's warps
         if (warp != 0) return;
-        for (int w = 0; w < kShareWarps; ++w) top = fmaxf(top, s_stat[w].x);
+        for (int w = 0; w < SHARE; ++w) top = fmaxf(top, s_stat[w].x);
         const float all = top == -INFINITY ? 0.0f : top;
         sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-        for (int w = 0; w < kShareWarps; ++w) {
+        for (int w = 0; w < SHARE; ++w) {
             const float weight = exp2_fast(s_stat[w].x - all);
             sum = fmaf(s_stat[w].y, weight, sum);
 #pragma unroll
@@ -987,11 +990,23 @@ int launch(const Problem &p, const QuantScales &scales, const QuantPlan &plan, c
     const bool far = seen > kNear && seen > kNear * plan.ctas / items;
     const int rc = far ? launch_decode_kernel<T, DP, NT, true>(p, scales, plan, scratch, stream) : launch_decode_kernel<T, DP, NT, false>(p, scales, plan, scratch, stream);
     if (rc != QMM_OK) return rc;
-    // a CTA a row where rows are so few that each has many parts
+    constexpr int kDims = DP < 256 ? 128 : 256;
     const int64_t indices = scratch.by_item ? plan.plan.items : plan.plan.workers, all = indices * scratch.rows;
-    const bool share = all <= 2 * sm_count();
-    QMM_CUDA_OK(launch_pdl(quant_join_kernel<T, DP < 256 ? 128 : 256>, dim3(static_cast<unsigned>(share ? all : (all + kJoinWarps - 1) / kJoinWarps)), dim3((share ? kShareWarps : kJoinWarps) * 32), 0, stream, p,
-                           scratch, indices, share));
+    auto join = [&](auto kern, int warps, int share) {
+        const int of_cta = warps / share;
+        return launch_pdl(kern, dim3(static_cast<unsigned>((all + of_cta - 1) / of_cta)), dim3(warps * 32), 0, stream, p, scratch, indices);
+    };
+    // Few rows have many parts each (us, by 8, 2 and 1 warps a row: 256 rows of 4 sequences of 500 to 8000 places 14.2, -, 24.6; 1024 rows, window of 4096, heads of 64, 23.4,
+    // 19.2, 20.5; 8192 rows of 128 sequences 44.2, 24.1, 19.3), a single sequence up to one of each CTA (131071 places, 148 parts: 16 warps 51.3, 8 52.3; 200 places 7.9, 7.7).
+    const int64_t parts = std::min<int64_t>(plan.plan.workers / plan.plan.items, seen / Shape<DP, NT>::kKeys);
+    if (all <= 2 * sm_count() && parts > 64)
+        QMM_CUDA_OK(join(quant_join_kernel<T, kDims, 16>, 16, 16));
+    else if (all <= 2 * sm_count())
+        QMM_CUDA_OK(join(quant_join_kernel<T, kDims, 8>, 8, 8));
+    else if (all <= 8 * sm_count())
+        QMM_CUDA_OK(join(quant_join_kernel<T, kDims, 2>, 8, 2));
+    else
+        QMM_CUDA_OK(join(quant_join_kernel<T, kDims, 1>, 8, 1));
     return QMM_OK;
 }
 
