@@ -40,14 +40,14 @@ def test_two_graphs_at_once(npu, dev):  # noqa: F811
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             got = step()
-        runs.append((graph, got, want, torch.cuda.Stream()))
+        runs.append((graph, got, want, torch.cuda.Stream(), step))  # (step has the inputs, which the graph does not keep)
     torch.cuda.synchronize()
     for _ in range(20):
-        for graph, got, _, stream in runs:
+        for graph, got, _, stream, _ in runs:
             with torch.cuda.stream(stream):
                 for x in got:
                     x.zero_()
                 graph.replay()
     torch.cuda.synchronize()
-    for _, got, want, _ in runs:
+    for _, got, want, _, _ in runs:
         assert all(torch.equal(x, y) for x, y in zip(got, want))
