@@ -15,8 +15,8 @@
 // so nothing is shuffled; the weights change from rows of keys to rows of heads by movmatrix.
 //
 // The weights, exp(score - base) * value scale, are multiplied, as they are rounded, by a power of two for each head that keeps the largest so far below
-// f16's largest number and above 2^8; it moves with the base, or when a weight would pass that.  Rounding a weight is half a step of
-// f16, 2^-11 of it, or 2^-33 of the largest one for those far below it.  The sum of the softmax takes them unrounded.  The base
+// f16's largest number and above 2^8; it moves with the base, or when a weight would pass that, as the first one above 0 always does.  Rounding a
+// weight is half a step of f16, 2^-11 of it, or 2^-33 of the largest one for those far below it.  The sum of the softmax takes them unrounded.  The base
 // follows the largest score only when that is 2^3 above it, so that sums are rescaled rarely.
 //
 // Places that are not seen have no part in a sum: their scores are -inf and their scales 0, whatever their codes are, which are finite.
@@ -710,6 +710,10 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
                                 const int e = max(-126, min(min(138 - static_cast<int>(__float_as_uint(most) >> 23), 127), 127 + has));
                                 lift[t][i] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                                 keep[t][i] *= e - has < -126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + e - has) << 23);
+                            } else if (most == 0.0f) {
+                                // none above 0: the first one passes 60000 and comes here; the sums are 0, or below what fp32 has beside the new base
+                                lift[t][i] = 0x1p127f;
+                                keep[t][i] = 0.0f;
                             }
 #pragma unroll
                             for (int n = 0; n < kSteps; ++n) {
