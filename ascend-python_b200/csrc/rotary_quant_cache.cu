@@ -10,7 +10,7 @@
 // reciprocal, corrected by its remainder, so that one that is a tie comes out as one; codes come out of its sum with 1.5 * 2^52, which has
 // them in its low bits.
 //
-// HBM bounds it (28 us for 8192 tokens, 32 + 8 heads of 128) less than its instructions do: 44.5 us, of which 30 without the rows that are
+// HBM bounds it (28 us for 8192 tokens, 32 + 8 heads of 128) less than its instructions do: 45.8 us, of which 30 without the rows that are
 // quantized, each 8 lanes' work of some 400 instructions in 64 bits for keys and 250 for values.
 #include "rotary_axes.cuh"
 
@@ -24,13 +24,15 @@ struct QuantParams {
 };
 
 // The cosine and sine of a token's pair, in 32 bits as make_turn has them, and in 64.  For these the half turns are made of two
-// numbers: the product with 1 / pi in 64 bits, and what it was rounded by together with the next 53 bits of 1 / pi.
-__device__ __forceinline__ void make_turns(const RotaryParams &p, int64_t token, int pair, float *c, float *s, double *c64, double *s64) {
+// numbers: the product with 1 / pi in 64 bits, and what it was rounded by together with the next 53 bits of 1 / pi.  False: the frequency is not
+// finite, and all four are NaN.
+__device__ __forceinline__ bool make_turns(const RotaryParams &p, int64_t token, int pair, float *c, float *s, double *c64, double *s64) {
     const int64_t place = load_index(p.positions, axis_of(p, pair) * p.pos_sa + token * p.pos_st, p.wide_positions);
     const double angle = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + pair));
     const double half_turns = angle * 0.31830988618379067154, rest = half_turns - 2.0 * rint(0.5 * half_turns);
     sincospif(static_cast<float>(rest), s, c);
     sincospi(rest + fma(angle, -1.9678676675182486e-17, fma(angle, 0.31830988618379067154, -half_turns)), s64, c64);
+    return rest == rest;
 }
 
 __device__ __forceinline__ double turned_first_64(double a, double b, double c, double s) { return fma(a, c, -(b * s)); }
@@ -254,15 +256,17 @@ __device__ __forceinline__ uint2 usual_codes_of(const double (&y)[8], const RowS
 // (fmax, which looks for NaN, is twice as many instructions)
 __device__ __forceinline__ double larger(double a, double b) { return b > a ? b : a; }
 
-// A part of a key's or a value's row, as it is written: the codes, and the scale by the first of the row's lanes.
+// A part of a key's or a value's row, as it is written: the codes, and the scale by the first of the row's lanes.  `finite`: the sines and cosines are, so
+// that NaN comes from the row's own elements alone, in whose bits it shows (`larger` passes over it).
 template <typename T, bool INTERLEAVED>
-__device__ __forceinline__ void quantize_part(const Eight<T> &x, const Eight<T> &y, const Parts<INTERLEAVED> &parts, bool key, const double *cosine,
+__device__ __forceinline__ void quantize_part(const Eight<T> &x, const Eight<T> &y, const Parts<INTERLEAVED> &parts, bool key, bool finite, const double *cosine,
                                               const double *sine, int8_t *dst, float *scale_at) {
     float f[8], g[8];
     x.unpack(f);
     y.unpack(g);
     uint32_t bits = x.largest();  // in which NaN is above infinity
     if (!INTERLEAVED) bits = max(bits, y.largest());
+    if (!finite) bits = 0x7fffffffu;
     double a[8], b[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -310,8 +314,9 @@ __device__ __forceinline__ void quantize_part(const Eight<T> &x, const Eight<T> 
     if (parts.part == 0) *scale_at = scale.scale;
 }
 
-// TOKENS a CTA: two where there are enough (8192 tokens, 32 + 8 heads of 128, bf16: one token 59 us, two 44.5, three 51; a warp a token, without
-// a barrier, 50).  The first row of the query for each token and the first one that is quantized are under way while the sines and
+// TOKENS a CTA: two where there are enough (8192 tokens, 32 + 8 heads of 128, bf16: one token 59 us, two 45.8, three 51; a warp a token, without
+// a barrier, 50).  The barrier finds out whether all turns are finite (44.5 without that; the rows' lanes looking at their own cosines 46.2, CTAs
+// that have others going another way 47 and more).  The first row of the query for each token and the first one that is quantized are under way while the sines and
 // cosines are made.  Four CTAs an SM for two tokens (three: 47.5); few tokens need no more than one (64 registers cost 64 tokens 0.3 of 3.4 us).
 template <typename T, bool INTERLEAVED, int TOKENS>
 __global__ void __launch_bounds__(kThreads, TOKENS == 1 ? 1 : 4)
@@ -352,11 +357,12 @@ rotary_quant_vec_kernel(const __grid_constant__ RotaryParams p, const __grid_con
         s_scales[threadIdx.x][0] = out.k_scale + block * out.ks_sb + at * out.ks_st;
         s_scales[threadIdx.x][1] = out.v_scale + block * out.vs_sb + at * out.vs_st;
     }
+    bool finite = true;
     for (int i = threadIdx.x; i < p.pairs * here; i += kThreads) {
         const int token = i / p.pairs, pair = i - token * p.pairs;
-        make_turns(p, token0 + token, pair, &s_cos[token][pair], &s_sin[token][pair], &s_cos64[token][pair], &s_sin64[token][pair]);
+        finite &= make_turns(p, token0 + token, pair, &s_cos[token][pair], &s_sin[token][pair], &s_cos64[token][pair], &s_sin64[token][pair]);
     }
-    __syncthreads();
+    finite = __syncthreads_and(finite);
     for (int row = row0; row < p.heads; row += step) {
 #pragma unroll
         for (int i = 0; i < TOKENS; ++i) {
@@ -376,7 +382,7 @@ rotary_quant_vec_kernel(const __grid_constant__ RotaryParams p, const __grid_con
         if (s_codes[token][0] == nullptr) continue;
         const bool key = at < p.kv_heads;
         const int head = key ? at : at - p.kv_heads;
-        quantize_part<T, INTERLEAVED>(kept_x, kept_y, parts, key, s_cos64[token] + parts.pair0, s_sin64[token] + parts.pair0,
+        quantize_part<T, INTERLEAVED>(kept_x, kept_y, parts, key, finite, s_cos64[token] + parts.pair0, s_sin64[token] + parts.pair0,
                                       s_codes[token][!key] + head * (key ? p.kc_sh : p.vc_sh), s_scales[token][!key] + head * (key ? out.ks_sh : out.vs_sh));
     }
 }
