@@ -976,12 +976,12 @@ int launch_decode_kernel(const Problem &p, const QuantScales &scales, const Quan
     if (p.page % 8 != 0 || p.pages == 0 || !cache_map(&k_map, p, p.k, p.k_sb, p.k_st, p.k_sh, heads, deal.rows, kColumns) ||
         !cache_map(&v_map, p, p.v, p.v_sb, p.v_st, p.v_sh, heads, deal.rows, kColumns))
         deal.rows = 0;
-    // as many stages as fit
+    // as many stages as fit.  The kernel's limit is one for all calls, whatever each takes of it: threads that call at the same time set it to the same.
+    constexpr int kMostSmem = kSmemOfSm / S::kCtas - 1024;
     const int fixed = (deal.log_parts > 0 ? heads * S::kSums : 0) + S::kOperands + kControlBytes;
-    const int room = kSmemOfSm / S::kCtas - 1024 - fixed;
-    deal.stages = std::min(kMostStages, room / S::kStage);
+    deal.stages = std::min(kMostStages, (kMostSmem - fixed) / S::kStage);
     const int smem = fixed + deal.stages * S::kStage;
-    QMM_CUDA_OK(cudaFuncSetAttribute(quant_decode_kernel<T, DP, NT, FAR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    QMM_CUDA_OK(cudaFuncSetAttribute(quant_decode_kernel<T, DP, NT, FAR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
     QMM_CUDA_OK(launch_pdl(quant_decode_kernel<T, DP, NT, FAR>, dim3(plan.ctas), dim3(kThreads), smem, stream, p, scales, scratch, deal, k_map, v_map));
     return QMM_OK;
 }
