@@ -527,13 +527,15 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
             }
             // top: what scores are relative to, within kSlack below the largest; ceiling: a score beyond it moves that; base: top times the row's
             // scale; lift: the power of two of a head's weights; big: the lane's largest, not lifted
-            float top[NT][2], ceiling[NT][2], base[NT][2], sum[NT][2], lift[NT][2], big[NT][2];
+            // sum: of the lane's weights; lost: what its additions rounded away, to be taken off (Kahan's summation: a chain of 65536 equal
+            // weights is off by up to 2^-10 without)
+            float top[NT][2], ceiling[NT][2], base[NT][2], sum[NT][2], lost[NT][2], lift[NT][2], big[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     top[t][i] = ceiling[t][i] = -INFINITY;
-                    sum[t][i] = big[t][i] = base[t][i] = 0.0f;
+                    sum[t][i] = lost[t][i] = big[t][i] = base[t][i] = 0.0f;
                     lift[t][i] = 1.0f;
                 }
             }
@@ -656,20 +658,29 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
                                 top[t][i] = now;
                                 ceiling[t][i] = now + kSlack / row_scale[t][i];
                                 sum[t][i] *= keep[t][i];
+                                lost[t][i] *= keep[t][i];
                                 big[t][i] *= keep[t][i];
                             }
                         }
                     }
                 }
 #pragma unroll
-                for (int m = 0; m < kTiles; ++m) {
+                for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
+                    for (int i = 0; i < 2; ++i) {
+                        float all = -lost[t][i];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            s[m][t][i] = exp2_fast(fmaf(s[m][t][i], row_scale[t][i & 1], -base[t][i & 1]));
-                            sum[t][i & 1] += s[m][t][i];
+                        for (int m = 0; m < kTiles; ++m) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float &x = s[m][t][2 * h + i];
+                                x = exp2_fast(fmaf(x, row_scale[t][i], -base[t][i]));
+                                all += x;
+                            }
                         }
+                        const float more = sum[t][i] + all;
+                        lost[t][i] = (more - sum[t][i]) - all;
+                        sum[t][i] = more;
                     }
                 }
                 tile += kSide;
@@ -758,7 +769,7 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    all[t][i] = sum[t][i];
+                    all[t][i] = sum[t][i] - lost[t][i];
                     all[t][i] += __shfl_xor_sync(0xffffffffu, all[t][i], 4);
                     all[t][i] += __shfl_xor_sync(0xffffffffu, all[t][i], 8);
                     all[t][i] += __shfl_xor_sync(0xffffffffu, all[t][i], 16);

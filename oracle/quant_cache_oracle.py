@@ -30,7 +30,8 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, table, lens, scale=None, wi
 
         |out - ref| <= u |ref| + (2^-11 + 2 d + 2^-20) sum p |v| + 2^-33 max w sum |code|,   |lse - ref| <= d + 2^-20 + 2^-22 |lse|,
 
-    u half a step of the output's type, and half of its smallest step more for an output below its full steps (f16 2^-25, bf16 2^-134).
+    whatever the number of places: a lane's weights of a tile are up to 8, what adding them to those before rounds away is kept, and that of the lanes, warps and
+    parts is within 2^-20, too; u half a step of the output's type, and half of its smallest step more for an output below its full steps (f16 2^-25, bf16 2^-134).
     """
     k, v = values(k_codes, k_scale), values(v_codes, v_scale)
     out, lse, weight, _, reach = paged_oracle.attention(q, k, v, table, lens, scale=scale, window=window, sinks=sinks)
