@@ -167,6 +167,12 @@ __device__ __forceinline__ void expect_bytes_warp(uint32_t bar, uint32_t bytes) 
         : "memory");
 }
 
+// A whole warp's wait: false for all of its lanes if one has given up.
+__device__ __forceinline__ bool mbar_wait_whole_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t where) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, mbar_wait_slow(bar, parity, abort_flag, where));
+}
+
 // The warps for products alone.
 __device__ __forceinline__ void product_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 // The lane's copies by cp.async so far, as one of a barrier's arrivals.
@@ -346,7 +352,10 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
         while (working) {
             const int head0 = piece.item / tiles << deal.log_heads;
             for (int g = piece.from; g < piece.to;) {
-                mbar_wait(smem_u32(&control->empty[stage]), phase ^ 1, &control->abort, 0xa0);
+                if (!mbar_wait_whole_warp(smem_u32(&control->empty[stage]), phase ^ 1, &control->abort, 0xa0)) {
+                    working = false;
+                    break;
+                }
                 const uint32_t full = smem_u32(&control->full[stage]);
 #pragma unroll 1
                 for (int l = 0; l < groups; ++l) {
@@ -518,6 +527,7 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
             if (lane == 0) mbar_arrive(smem_u32(&control->empty[stage]));
             advance();
         };
+        bool ok = true;  // a warp that has given up takes no more tiles, but its part in the exchange of sums
         while (working) {
             float o[kSteps][NT][4];  // dimensions 16 ks + 2 r0 (and the next: + 2) of heads c0, c0 + 1 (+ 1)
 #pragma unroll
@@ -573,7 +583,8 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
             take_query(kvh, head_tile, rows);
             for (int g = piece.from; g < piece.to; ++g) {
                 if (FAR && g != piece.from && (g - piece.from) % (kRun / KEYS) == 0) put_by(g - piece.from == kRun / KEYS, false);
-                mbar_wait(smem_u32(&control->full[stage]), phase, &control->abort, 0xa1);
+                ok = ok && mbar_wait_whole_warp(smem_u32(&control->full[stage]), phase, &control->abort, 0xa1);
+                if (!ok) break;
                 uint32_t tile = ring + stage * (2 * kSide) + lane_tile, scale_at = lane_scale + stage * (kWarps * KEYS * 8);
                 constexpr int kLooks = KEYS > 32 ? KEYS / 32 : 1;
                 uint32_t seen[kLooks];
@@ -859,7 +870,12 @@ quant_decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Q
         }
     }
     __syncthreads();
-    if (threadIdx.x == 0 && control->abort != 0) *deal.status = control->abort;
+    if (control->abort != 0) {
+        // what is still on its way comes before the CTA's shared memory goes
+        uint32_t late = 0;
+        for (int i = 0; warp == kWarps && i < deal.stages; ++i) mbar_wait(smem_u32(&control->full[i]), i < stage ? phase : phase ^ 1, &late, 0xa2);
+        if (threadIdx.x == 0 && deal.status != nullptr) atomicMax(deal.status, control->abort);
+    }
 }
 
 // Adds the parts of the head tiles that are cut, in the order of the CTAs: SHARE warps a row.  Statistics and sums of kAtOnce parts are under way
