@@ -482,8 +482,10 @@ QMM_API int qmm_rotary_axes_quant_cache(const void *query, int64_t query_stride_
  * times a power of two of its row (off by 2^-22 of the row's largest at most), sums of its products with codes are exact; scales of
  * keys, softmax and sums are fp32.  For the product with the values a weight times its value's scale is rounded to f16, after a power of two that its
  * row has (half a step, 2^-11, of each, or 2^-33 of the largest); the sum that it is divided by takes the weight unrounded.
- * A query's row that holds NaN or an infinity comes out as NaN; a scale that is not finite reaches the rows that see it, and no other.
- * Scores are to be in fp32's range, and a row's largest |query| times |scale_value| * log2(e) 0 or at least 2^-104 (a smaller row counts as up to that).
+ * A query's row that holds NaN or an infinity comes out as NaN; a scale that is not finite reaches the rows that see it, and no other (a key
+ * whose score is -inf by it has no weight; a row of such scores alone is one that sees nothing).
+ * Scores are to be in fp32's range, keys' finite scales at most 2^90, and a row's largest |query| times |scale_value| * log2(e) 0 or at least 2^-104 (a smaller row
+ * counts as up to that) and below 2^127.
  * Of a page that holds a place that is seen, up to 31 places beside it may be read as well; whatever their codes and scales, the results are
  * those of the places that are seen.
  * The head dimension is a multiple of 16 up to 256; caches begin at 16-byte boundaries, their strides are multiples of 16;
