@@ -45,6 +45,10 @@ uint64_t device_status_generation();
 // Number of SMs of the current device (cached per device).
 int sm_count();
 
+// The limit of dynamic shared memory for kernels whose calls take different amounts: all there is but 1 KiB (for what a kernel has beside it).  Each call sets it before its
+// launch, so it is one for all of them: a thread that set its own call's amount would lower it under a launch of another thread.
+constexpr int kDynamicSmemLimit = 226 * 1024;
+
 // Encode a 2-D tiled tensor map for a row-major byte matrix.
 //   inner: contiguous extent (elements), outer: number of rows, ld: row pitch in elements,
 //   elem_bytes: 1 or 2 or 4; box_inner/box_outer: tile extents in elements/rows;

@@ -48,6 +48,8 @@
 // election with uniform operands; with the role index not known to be warp-uniform the MMA warp spent
 // 75 clocks on each (45 / 51 us).  Wide: the tensor pipe and the power cap: 256 tokens 100 us, 2048
 // tokens 733 us = 1.31 PFLOP/s of a measured 1.41 sustained.
+#include <algorithm>
+
 #include "qmm_common.cuh"
 #include "w4a16_gemv.cuh"
 #include "w4a16_simt.cuh"
@@ -1693,7 +1695,8 @@ int launch_gemv_t(const uint8_t *packed, const void *x, int64_t ld_x, const void
     const size_t smem = static_cast<size_t>(pl.max_run) * M * (256 + 8);
     auto launch = [&](auto kern) -> int {
         if (smem > 48 * 1024)
-            QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+            QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             std::max(static_cast<int>(smem), kDynamicSmemLimit)));
         QMM_CUDA_OK(launch_pdl(kern, dim3(static_cast<unsigned>(pl.grid)), dim3(kGvThreads), smem, stream, p));
         return QMM_OK;
     };
@@ -1737,12 +1740,12 @@ int launch_prepacked_t(const uint8_t *packed, const void *x, int64_t ld_x, const
     static_assert(sizeof(PSmemTail) <= 1024 && sizeof(BSmemTail) <= 1024, "the tail has 1 KiB");
     if (tables != nullptr && M <= kBTok) {
         auto kern = w4a16_block_kernel<T>;
-        QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pl.smem)));
+        QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynamicSmemLimit));
         QMM_CUDA_OK(launch_pdl(kern, dim3(static_cast<unsigned>(pl.grid)), dim3(kPThreads), pl.smem, stream, tx, p, *tables));
         return QMM_OK;
     }
     auto kern = M <= kPMaxM ? w4a16_prepacked_kernel<T, false> : w4a16_prepacked_kernel<T, true>;
-    QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pl.smem)));
+    QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynamicSmemLimit));
     QMM_CUDA_OK(launch_pdl(kern, dim3(static_cast<unsigned>(pl.grid)), dim3(kPThreads), pl.smem, stream, tx, p));
     return QMM_OK;
 }

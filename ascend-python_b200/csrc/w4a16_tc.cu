@@ -213,7 +213,7 @@ int launch_w4a16_tc_t(const W4Params &w, void *workspace, cudaStream_t stream) {
     const size_t smem = 1024 + kWABufs * kWABytes + kWStages * kWPackedBytes +
                         static_cast<size_t>(kWXStages) * p.x_bytes + sizeof(WSmemTail) + kWXsSmemBytes;
     auto kern = pl.mpad <= 32 ? w4a16_tc_kernel<T, 32> : w4a16_tc_kernel<T, 64>;
-    QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    QMM_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynamicSmemLimit));
     kern<<<pl.grid, kWThreads, smem, stream>>>(tw, tx, p);
     QMM_CUDA_OK(cudaGetLastError());
     return QMM_OK;
