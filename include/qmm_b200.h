@@ -481,7 +481,8 @@ QMM_API int qmm_rotary_axes_quant_cache(const void *query, int64_t query_stride_
  * scales stand for; sequences, masks, lse and workspace are as there.  An element of the query is taken as a whole number of at most 22 bits
  * times a power of two of its row (off by 2^-22 of the row's largest at most), sums of its products with codes are exact; scales of
  * keys, softmax and sums are fp32.  For the product with the values a weight times its value's scale is rounded to f16, after a power of two that its
- * row has (half a step, 2^-11, of each, or 2^-33 of the largest); the sum that it is divided by takes the weight unrounded.
+ * row has (half a step, 2^-11, of each, or 2^-33 of the largest), for an f16 query to the
+ * sum of two f16 numbers (2^-22 of each, or 2^-33 of the largest); the sum that it is divided by takes the weight unrounded.
  * A query's row that holds NaN or an infinity comes out as NaN; a scale that is not finite reaches the rows that see it, and no other (a key
  * whose score is -inf by it has no weight; a row of such scores alone is one that sees nothing).
  * Scores are to be in fp32's range, keys' finite scales at most 2^90, and a row's largest |query| times |scale_value| * log2(e) 0 or at least 2^-104 (a smaller row

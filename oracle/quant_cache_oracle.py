@@ -25,10 +25,11 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, table, lens, scale=None, wi
 
     As paged_oracle.attention_bounds, but for the weights and the query.  d: a query's element is a whole number, of a step of at most 2^-21
     of its row's largest, off by half a step, 2^-22 of that one.  A score's sum of products with codes is exact, but for its parts'
-    roundings, and then multiplied by the key's scale, the row's power of two and scale_value: (dim + 5) * 2^-24 of its terms' absolute sum is more.  A weight, exp times the value's scale, is rounded to f16: 2^-11 of it, or
-    half of f16's smallest step, 2^-25, where the row's largest weight is 2^8 or more: 2^-33 of that.  So with w_j = p_j * value scale
+    roundings, and then multiplied by the key's scale, the row's power of two and scale_value: (dim + 5) * 2^-24 of its terms' absolute sum is more.  A weight, exp times the value's scale, is rounded to r of it, or
+    half of f16's smallest step, 2^-25, where the row's largest weight is 2^8 or more: 2^-33 of that; r is half a step of f16, 2^-11, and for an f16 query, where a weight is the sum of two f16 numbers, 2^-22.
+    So with w_j = p_j * value scale
 
-        |out - ref| <= u |ref| + (2^-11 + 2 d + 2^-20) sum p |v| + 2^-33 max w sum |code|,   |lse - ref| <= d + 2^-20 + 2^-22 |lse|,
+        |out - ref| <= u |ref| + (r + 2 d + 2^-20) sum p |v| + 2^-33 max w sum |code|,   |lse - ref| <= d + 2^-20 + 2^-22 |lse|,
 
     whatever the number of places: a lane's weights of a tile are up to 8, what adding them to those before rounds away is kept, and that of the lanes, warps and
     parts is within 2^-20, too; u half a step of the output's type, and half of its smallest step more for an output below its full steps (f16 2^-25, bf16 2^-134).
@@ -55,7 +56,8 @@ def attention(q, k_codes, v_codes, k_scale, v_scale, table, lens, scale=None, wi
         most[t] = (p * v_scale[ids, :, js % page].double().abs().t().repeat_interleave(H // KV, 0)).amax(1)
         far[t] = (keys.abs().sum(2).t() * abs(by)).amax(1) * q[t].double().abs().amax(1)
     d = (D + 5) * 2.0 ** -24 * reach + 2.0 ** -22 * far
-    bound = torch.finfo(q.dtype).eps / 2 * out.abs() + (2.0 ** -11 + 2 * d[..., None] + 2.0 ** -20) * weight + 2.0 ** -33 * most[..., None] * spread
+    r = 2.0 ** -22 if q.dtype == torch.float16 else 2.0 ** -11
+    bound = torch.finfo(q.dtype).eps / 2 * out.abs() + (r + 2 * d[..., None] + 2.0 ** -20) * weight + 2.0 ** -33 * most[..., None] * spread
     bound = bound + torch.finfo(q.dtype).smallest_normal * (torch.finfo(q.dtype).eps / 2)
     return out, lse, bound, d + 2.0 ** -20 + 2.0 ** -22 * lse.abs().nan_to_num(posinf=0.0)
 
