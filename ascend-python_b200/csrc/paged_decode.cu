@@ -37,7 +37,30 @@ struct Shape {
 };
 
 Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim) {
-    return make_plan(batch, heads, kv_heads, dim, 2, dim > 128 ? Shape<256>::kWarps : Shape<128>::kWarps);
+    Plan plan;
+    const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
+    plan.workers = 2 * sm_count();  // CTAs
+    plan.rows = static_cast<int>(group < kRows ? group : kRows);
+    plan.tiles = static_cast<int>((group + kRows - 1) / kRows);
+    plan.items = batch * kv_heads * plan.tiles;
+    plan.cta_parts = 2ll * plan.workers * (dim > 128 ? Shape<256>::kWarps : Shape<128>::kWarps);
+    const size_t rows = static_cast<size_t>(plan.cta_parts + 2 * plan.workers) * plan.rows;
+    plan.part_bytes = rows * dim * sizeof(float);
+    plan.stat_bytes = (rows * sizeof(float2) + 15) / 16 * 16;
+    plan.bytes = plan.part_bytes + plan.stat_bytes + static_cast<size_t>(plan.workers) * sizeof(int4);
+    return plan;
+}
+
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Powers of two by which weights are larger than exp(score - maximum) until the log-sum: f16 has no full step below 2^-14 and

@@ -37,22 +37,6 @@ struct Plan {
     size_t part_bytes, stat_bytes, bytes;
 };
 
-// `ctas` an SM of `warps` warps each.
-inline Plan make_plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int ctas, int warps) {
-    Plan plan;
-    const int64_t group = kv_heads > 0 ? heads / kv_heads : 0;
-    plan.workers = ctas * sm_count();
-    plan.rows = static_cast<int>(group < kRows ? group : kRows);
-    plan.tiles = static_cast<int>((group + kRows - 1) / kRows);
-    plan.items = batch * kv_heads * plan.tiles;
-    plan.cta_parts = 2ll * plan.workers * warps;
-    const size_t rows = static_cast<size_t>(plan.cta_parts + 2 * plan.workers) * plan.rows;
-    plan.part_bytes = rows * dim * sizeof(float);
-    plan.stat_bytes = (rows * sizeof(float2) + 15) / 16 * 16;
-    plan.bytes = plan.part_bytes + plan.stat_bytes + static_cast<size_t>(plan.workers) * sizeof(int4);
-    return plan;
-}
-
 inline Scratch lay_out(const Plan &plan, void *workspace) {
     Scratch scratch;
     uint8_t *base = static_cast<uint8_t *>(workspace);
@@ -80,11 +64,6 @@ struct Piece {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -100,12 +79,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
-__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
 __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -118,7 +91,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
 
 }  // namespace
 

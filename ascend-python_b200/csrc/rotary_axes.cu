@@ -20,6 +20,36 @@ namespace qmm {
 
 namespace {
 
+// The cosine and sine of a token's pair.
+__device__ __forceinline__ void make_turn(const RotaryParams &p, int64_t token, int pair, float *c, float *s) {
+    const int64_t place = load_index(p.positions, axis_of(p, pair) * p.pos_sa + token * p.pos_st, p.wide_positions);
+    const double half_turns = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + pair)) * 0.31830988618379067154;
+    sincospif(static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns)), s, c);
+}
+
+template <typename T>
+struct Vec {
+    static constexpr int kElems = 16 / sizeof(T);
+    static __device__ __forceinline__ void unpack(const uint4 &w, float (&f)[kElems]) {
+        const T *x = reinterpret_cast<const T *>(&w);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) f[i] = to_float(x[i]);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[kElems]) {
+        uint4 w;
+        T *x = reinterpret_cast<T *>(&w);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) x[i] = from_float<T>(f[i]);
+        return w;
+    }
+};
+
+// Whether rows `stride` elements apart begin at 16-byte boundaries.
+template <typename T>
+bool aligned(const void *base, int64_t a, int64_t b, int64_t c = 0) {
+    return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ((a | b | c) & (Vec<T>::kElems - 1)) == 0;
+}
+
 // Row `row` of a token: first the query's heads, then the key's, then the value's.
 template <typename T>
 __device__ __forceinline__ void find_row(const RotaryParams &p, int64_t token, int row, int64_t block, int64_t at, const T **src, T **dst) {

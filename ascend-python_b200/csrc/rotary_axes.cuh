@@ -1,5 +1,5 @@
 // What the rotary kernels share (rotary_axes.cu: outputs and caches of the tensors' type, rotary_quant_cache.cu: an int8 cache): the
-// problem's description, angles, where a token goes in the cache, and the checks of sizes.
+// problem's description, the axes of pairs, where a token goes in the cache, and the checks of sizes.
 #pragma once
 
 #include "qmm_common.cuh"
@@ -44,13 +44,6 @@ __device__ __forceinline__ int64_t load_index(const void *base, int64_t at, int 
     return wide ? __ldg(static_cast<const long long *>(base) + at) : __ldg(static_cast<const int *>(base) + at);
 }
 
-// The cosine and sine of a token's pair.
-__device__ __forceinline__ void make_turn(const RotaryParams &p, int64_t token, int pair, float *c, float *s) {
-    const int64_t place = load_index(p.positions, axis_of(p, pair) * p.pos_sa + token * p.pos_st, p.wide_positions);
-    const double half_turns = static_cast<double>(place) * static_cast<double>(__ldg(p.inv_freq + pair)) * 0.31830988618379067154;
-    sincospif(static_cast<float>(half_turns - 2.0 * rint(0.5 * half_turns)), s, c);
-}
-
 // Where the token goes in the cache; false: nowhere.
 __device__ __forceinline__ bool find_slot(const RotaryParams &p, int64_t token, int64_t *block, int64_t *at) {
     const int64_t slot = load_index(p.slots, token * p.slot_st, p.wide_slots);
@@ -62,29 +55,6 @@ __device__ __forceinline__ bool find_slot(const RotaryParams &p, int64_t token, 
 
 __device__ __forceinline__ float turned_first(float a, float b, float c, float s) { return fmaf(a, c, -(b * s)); }
 __device__ __forceinline__ float turned_second(float a, float b, float c, float s) { return fmaf(b, c, a * s); }
-
-template <typename T>
-struct Vec {
-    static constexpr int kElems = 16 / sizeof(T);
-    static __device__ __forceinline__ void unpack(const uint4 &w, float (&f)[kElems]) {
-        const T *x = reinterpret_cast<const T *>(&w);
-#pragma unroll
-        for (int i = 0; i < kElems; ++i) f[i] = to_float(x[i]);
-    }
-    static __device__ __forceinline__ uint4 pack(const float (&f)[kElems]) {
-        uint4 w;
-        T *x = reinterpret_cast<T *>(&w);
-#pragma unroll
-        for (int i = 0; i < kElems; ++i) x[i] = from_float<T>(f[i]);
-        return w;
-    }
-};
-
-// Whether rows `stride` elements apart begin at 16-byte boundaries.
-template <typename T>
-bool aligned(const void *base, int64_t a, int64_t b, int64_t c = 0) {
-    return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && ((a | b | c) & (Vec<T>::kElems - 1)) == 0;
-}
 
 // The arguments that the entries share, checked and taken over.
 inline int take_sizes(const char *op, RotaryParams &p, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t pairs,

@@ -7,8 +7,9 @@
 // The keys' rotation, the maximum and the quotient are in 64 bits: a value next to the border of two codes then has the code of
 // the definition, whichever kernel or order of operations made it, where fp32 angles alone (off by 2^-25 half turns) move a code in
 // some 2^16.  Positions times frequencies are exact there up to positions of 2^29.  The quotient is a product with the
-// reciprocal, corrected by its remainder, so that one that is a tie comes out as one; codes come out of its sum with 1.5 * 2^52, which has
-// them in its low bits.
+// reciprocal, corrected by its remainder, which an fma gives without a rounding, so that one that is a tie comes out as one (P. Markstein, Computation of
+// elementary functions on the IBM RISC System/6000 processor, 1990); reciprocals come from fp32 ones by Newton's iteration, r + r (1 - s r), whose last
+// step's correction is kept beside the rounded sum.  Codes come out of the quotient's sum with 1.5 * 2^52, which has them in its low bits.
 //
 // HBM bounds it (28 us for 8192 tokens, 32 + 8 heads of 128) less than its instructions do: 45.8 us, of which 30 without the rows that are
 // quantized, each 8 lanes' work of some 400 instructions in 64 bits for keys and 250 for values.
@@ -23,8 +24,8 @@ struct QuantParams {
     int64_t ks_sb, ks_st, ks_sh, vs_sb, vs_st, vs_sh;
 };
 
-// The cosine and sine of a token's pair, in 32 bits as make_turn has them, and in 64.  For these the half turns are made of two
-// numbers: the product with 1 / pi in 64 bits, and what it was rounded by together with the next 53 bits of 1 / pi.  False: the frequency is not
+// The cosine and sine of a token's pair, in 32 bits as npu_rotary_axes has them, and in 64.  For these the half turns are made of two
+// numbers: the product with 1 / pi in 64 bits, and what it was rounded by (T. Dekker's exact product, 1971, with an fma) together with the next 53 bits of 1 / pi.  False: the frequency is not
 // finite, and all four are NaN.
 __device__ __forceinline__ bool make_turns(const RotaryParams &p, int64_t token, int pair, float *c, float *s, double *c64, double *s64) {
     const int64_t place = load_index(p.positions, axis_of(p, pair) * p.pos_sa + token * p.pos_st, p.wide_positions);
