@@ -462,7 +462,9 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             float o[DP / 8][4];
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+            // sum: of the lane's weights; lost: what its additions rounded away, to be taken off (Kahan's summation: a chain of 65536 equal weights is
+            // off by up to 2^-10 without)
+            float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, lost[2] = {0.0f, 0.0f};
             // A long piece adds what it has to fp32 sums in its part of the workspace and begins again from 0 (back: the other way round).
             auto put_by = [&](bool first, bool back) {
                 const int rows = min(kRows, p.group - piece.item % tiles * kRows);
@@ -566,6 +568,8 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     }
                     sum[0] *= keep[0];
                     sum[1] *= keep[1];
+                    lost[0] *= keep[0];
+                    lost[1] *= keep[1];
                 }
                 // the weights, rounded to the type of the values, as they lie are the second product's first operand.  That is half a
                 // step, 2^-8 or 2^-11, of each weight (of f16 weights below 2^-29 of the largest: 2^-40 of that one).  The sum
@@ -575,14 +579,21 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
                     base[0] -= kLift<T>;
                     base[1] -= kLift<T>;
                 }
+                float all[2] = {-lost[0], -lost[1]};
 #pragma unroll
                 for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float e0 = exp2_fast(fmaf(s[n][2 * r], scale, -base[r])), e1 = exp2_fast(fmaf(s[n][2 * r + 1], scale, -base[r]));
-                        sum[r] += e0 + e1;
+                        all[r] += e0 + e1;
                         a[n >> 1][(n & 1) * 2 + r] = pack2<T>(e0, e1);
                     }
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float more = sum[r] + all[r];
+                    lost[r] = (more - sum[r]) - all[r];
+                    sum[r] = more;
                 }
                 cp_async_wait<kSlots - 2>();
                 __syncwarp();
@@ -613,6 +624,7 @@ decode_kernel(const __grid_constant__ Problem p, const __grid_constant__ Scratch
             const int64_t part0 = ((static_cast<int64_t>(worker) * S::kWarps + warp) * 2 + begins) * scratch.rows;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
+                sum[r] -= lost[r];
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
                 top[r] = fmaf(top[r], scale, -kLift<T>);  // the sums are 2^kLift times those of exp(score - maximum)
