@@ -413,7 +413,8 @@ QMM_API int qmm_rotary_axes_cache(const void *query, int64_t query_stride_token,
  *   out[b,h] = sum_j softmax_j(scale_value * query[b,h] . key[j, h / group]) * value[j, h / group],  group = heads / kv_heads
  *   lse[b,h] = log(sum_j exp(scale_value * query[b,h] . key[j, h / group]))
  * A row that sees nothing (seq_lens[b] <= 0: padding) has out 0 and lse -inf.  Entries of the table for places that are not
- * seen are not followed, and the places not read.  Scores, softmax and sums are fp32; for the product with the values a weight is
+ * seen are not followed, and the places not read.  Scores, softmax and sums are fp32; scores (of finite keys) are to be at most 2^21 in magnitude, and a weight
+ * below some 2^-125 of the row's largest counts as 0; for the product with the values a weight is
  * rounded to the query's type (half a step: bf16 2^-8, f16 2^-11 of each, of f16 weights far below the largest up to 2^-33 of that one),
  * while the sum that it is divided by takes it unrounded.
  * query: bf16 or f16 like the cache, [batch, heads, dim]; out: dense; lse: [batch, heads]; block_table: int32 [batch, max_pages],
@@ -485,7 +486,7 @@ QMM_API int qmm_rotary_axes_quant_cache(const void *query, int64_t query_stride_
  * sum of two f16 numbers (2^-22 of each, or 2^-33 of the largest); the sum that it is divided by takes the weight unrounded.
  * A query's row that holds NaN or an infinity comes out as NaN; a scale that is not finite reaches the rows that see it, and no other (a key
  * whose score is -inf by it has no weight; a row of such scores alone is one that sees nothing).
- * Scores are to be in fp32's range, keys' finite scales at most 2^90, and a row's largest |query| times |scale_value| * log2(e) 0 or at least 2^-104 (a smaller row
+ * Scores (of finite keys) are to be at most 2^21 in magnitude, keys' finite scales at most 2^90, and a row's largest |query| times |scale_value| * log2(e) 0 or at least 2^-104 (a smaller row
  * counts as up to that) and below 2^127.
  * Of a page that holds a place that is seen, up to 31 places beside it may be read as well; whatever their codes and scales, the results are
  * those of the places that are seen.
