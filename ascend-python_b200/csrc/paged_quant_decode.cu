@@ -31,10 +31,10 @@
 // their order.  (CTAs that have whole heads of short sequences in turn, without that kernel: one of 200 places 10.0 us, this way 7.8.)  Nothing depends
 // on timing, and nothing has to be zero before a call.
 //
-// Measured (bf16, 64/8 heads of 128, 64 sequences of 500 to 8000 places; 364 MB, 55.6 us at the copy rate): 70.6 us, 66.5 of them without the second kernel, and
-// 63.8 for the copies with no products: memory, the start and the joining bound it.  Two CTAs an SM with three stages; three with two
-// 94 us, stages of keys and of values of their own 80.  One sequence of 131071 places, 32/8 heads: 51.6 us (0.82 of the copy rate).  Groups of 9
-// to 16 heads are bound by instructions on two column tiles (128/8 heads: 71 us, 0.41), pages whose size is no multiple of 8 by
+// Measured (bf16, 64/8 heads of 128, 64 sequences of 500 to 8000 places; 364 MB, 55.6 us at the copy rate): 71.5 us, some 67 of them without the second kernel, and
+// 64 for the copies with no products: memory, the start and the joining bound it.  Two CTAs an SM with three stages; three with two
+// 94 us, stages of keys and of values of their own 80.  One sequence of 131071 places, 32/8 heads: 52.1 us (0.81 of the copy rate).  Groups of 9
+// to 16 heads, two column tiles, wait for loads and results with two stages and three warps a scheduler (32 sequences, 128/8 heads: 72 us, 0.40), pages whose size is no multiple of 8 by
 // copies row by row (5 places: 66 us, 28.6 at the copy rate).
 #include "paged_decode.cuh"
 

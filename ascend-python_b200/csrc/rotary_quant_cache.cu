@@ -11,7 +11,7 @@
 // elementary functions on the IBM RISC System/6000 processor, 1990); reciprocals come from fp32 ones by Newton's iteration, r + r (1 - s r), whose last
 // step's correction is kept beside the rounded sum.  Codes come out of the quotient's sum with 1.5 * 2^52, which has them in its low bits.
 //
-// HBM bounds it (28 us for 8192 tokens, 32 + 8 heads of 128) less than its instructions do: 45.8 us, of which 30 without the rows that are
+// HBM bounds it (28 us for 8192 tokens, 32 + 8 heads of 128) less than its instructions do: 45.8 us (two thirds of the issue slots; then the barrier between sines and rows), of which 30 without the rows that are
 // quantized, each 8 lanes' work of some 400 instructions in 64 bits for keys and 250 for values.
 #include "rotary_axes.cuh"
 
